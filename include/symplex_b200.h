@@ -509,6 +509,32 @@ typedef struct symplex_gemm_plan {
 } symplex_gemm_plan;
 int symplex_b200_gemm_plan(const symplex_gemm_desc* desc, int num_sms, symplex_gemm_plan* out);
 
+/* ---- a model's output end: layer norm, the loss of a linear head, products with 4-bit weights -------
+ *
+ * All three take device pointers, are asynchronous on `stream`, allocate nothing (scratch is the caller's, 256-byte
+ * aligned; two calls that may run at the same time need two workspaces) and may be captured into CUDA graphs. The
+ * reference has no counterpart of them; they stand before and behind its matmul path. */
+
+/* Layer norm over rows of `cols` values: y = (x - mean) * rstd * weight + bias with rstd = 1 / sqrt(var + eps), var the
+ * mean squared deviation. x and y have element type dtype (SYMPLEX_DT_F32 / SYMPLEX_DT_BF16) and leading dimensions
+ * ldx, ldy in elements (0 = cols); weight and bias have param_dtype (either dtype or SYMPLEX_DT_F32) and may be NULL
+ * (1 and 0), as may mean and rstd (float[rows], the statistics the backward pass takes). Statistics and arithmetic are
+ * 32-bit, y is rounded once. y may be x. rows == 0 is a no-op. */
+int symplex_b200_layer_norm(const void* x, const void* weight, const void* bias, void* y, float* mean, float* rstd,
+                            int64_t rows, int64_t cols, int64_t ldx, int64_t ldy, int32_t dtype, int32_t param_dtype,
+                            double eps, void* stream);
+
+/* Its backward pass. With xh = (x - mean) * rstd and g = dy * weight:
+ *   dx = rstd * (g - mean_cols(g) - xh * mean_cols(g * xh)),  dweight = sum_rows dy * xh,  dbias = sum_rows dy.
+ * dx (of type dtype, may be dy), dweight and dbias (of type param_dtype) may each be NULL: then they are not computed.
+ * The sums over rows are 32-bit and taken in an order that does not change from call to call. rows == 0 sets dweight
+ * and dbias to zero. The workspace is used only where dweight or dbias is asked for. */
+size_t symplex_b200_layer_norm_backward_workspace_bytes(int64_t rows, int64_t cols);
+int symplex_b200_layer_norm_backward(const void* dy, const void* x, const float* mean, const float* rstd,
+                                     const void* weight, void* dx, void* dweight, void* dbias, int64_t rows,
+                                     int64_t cols, int64_t lddy, int64_t ldx, int64_t lddx, int32_t dtype,
+                                     int32_t param_dtype, void* workspace, size_t workspace_bytes, void* stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif

@@ -8,6 +8,7 @@ validates arguments the way the reference does and forwards raw addresses.
 * ``_symplex_core`` (sub-module)             — the pyo3 functions of ``python/src/lib.rs`` for this path
 * ``engine`` (sub-module)                    — the pyclasses of ``rust-engine/src/lib.rs`` for this path
 * ``gemm`` / ``gemm_host``                   — the general fused GEMM (bf16 or fp32 inputs, epilogues)
+* ``layer_norm`` ... (``nn`` sub-module)    — operators at a model's output end, on CUDA tensors
 * ``sharding`` (sub-module)                  — ShardPlan vocabulary + the row-sharded multi-GPU GEMM
 
 There is no CPU fallback: every compute call raises (or returns the reference's error code) when the
@@ -26,7 +27,19 @@ from ._capi import (ACT_GELU, ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_SILU, ACT_TAN
 __all__ = [
     "matmul_jit", "matmul_tiled", "matmul", "fused_matmul_bias_relu", "gemm", "gemm_host", "make_desc",
     "cuda_available", "launch_count", "SymplexB200Error", "fused_elementwise",
+    "layer_norm", "layer_norm_backward",
 ]
+
+_NN = ("layer_norm", "layer_norm_backward")  # live in the nn sub-module, which imports torch
+
+
+def __getattr__(name):
+    if name in _NN:
+        from . import nn
+        for n in _NN:
+            globals()[n] = getattr(nn, n)
+        return globals()[name]
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
 def make_desc(M, N, K, in_dtype=DT_F32, out_dtype=DT_F32, *, batch=1, b_layout=ROW_MAJOR, alpha=1.0, beta=0.0,

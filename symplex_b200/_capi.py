@@ -200,6 +200,10 @@ SIGNATURES = {
                                                     ctypes.POINTER(c_int32 * 3), ctypes.POINTER(c_int32)]),
     "symplex_b200_hardware_target": (c_int, [ctypes.POINTER(Target)]),
     "symplex_b200_micro_kernel_config": (None, [c_uint8, c_size_t] + [ctypes.POINTER(c_size_t)] * 5),
+    "symplex_b200_layer_norm": (c_int, [c_void_p] * 6 + [c_int64] * 4 + [c_int32, c_int32, c_double, c_void_p]),
+    "symplex_b200_layer_norm_backward_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "symplex_b200_layer_norm_backward": (c_int, [c_void_p] * 8 + [c_int64] * 5 + [c_int32, c_int32, c_void_p, c_size_t,
+                                                                                 c_void_p]),
     "symplex_b200_gemm_plan": (c_int, [ctypes.POINTER(GemmDesc), c_int, ctypes.POINTER(GemmPlan)]),
 }
 

@@ -69,6 +69,22 @@ static int cuda_fail(cudaError_t e, const char* what) {
   return fail(code, "%s: %s", what, cudaGetErrorString(e));
 }
 
+int fail_fmt(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_err, sizeof(g_err), fmt, ap);
+  va_end(ap);
+  return code;
+}
+int launch_failed(cudaError_t e, const char* what) {
+  cudaGetLastError();
+  return cuda_fail(e, what);
+}
+void count_launches(int n) { g_launches += (uint64_t)n; }
+unsigned long long wait_limit_ns_option() {
+  return (unsigned long long)options().wait_limit_ms.load(std::memory_order_relaxed) * 1000000ull;
+}
+
 #define SX_CUDA(call)                                   \
   do {                                                  \
     cudaError_t e__ = (call);                           \
@@ -173,6 +189,32 @@ static int device_state(DeviceState** out) {
     st.ready = true;
   }
   *out = &st;
+  return SX_OK;
+}
+
+int current_device(DeviceInfo* out) {
+  DeviceState* st = nullptr;
+  const int rc = device_state(&st);
+  if (rc != SX_OK) return rc;
+  out->num_sms = st->num_sms;
+  out->status = st->status;
+  return SX_OK;
+}
+
+int current_device_sms(int* num_sms) {
+  static std::atomic<int> known[16];
+  int dev = 0;
+  SX_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 16) return fail(SX_ERR_INVALID, "device ordinal %d out of range", dev);
+  int n = known[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    int major = 0;
+    SX_CUDA(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev));
+    if (major != 10) return fail(SX_ERR_DRIVER, "device %d is sm_%d0, this library needs sm_100", dev, major);
+    SX_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+    known[dev].store(n, std::memory_order_relaxed);
+  }
+  *num_sms = n;
   return SX_OK;
 }
 

@@ -128,6 +128,20 @@ int launch_gemm_tf32x3(const TcGemmArgs& a, cudaStream_t stream);
 // Records `msg` as the calling thread's last error and returns `code`.
 int set_last_error(int code, const char* msg);
 
+// For the translation units that define their own C entry points: the current device (checked to be an sm_100 part,
+// its status word allocated on first use), the printf form of set_last_error, the class of a failed launch, and the
+// launch counter behind symplex_b200_launch_count.
+struct DeviceInfo {
+  int num_sms = 0;
+  int* status = nullptr;  // device word that receives KernelStatus from kernels that unwind
+};
+int current_device(DeviceInfo* out);
+int current_device_sms(int* num_sms);  // the same check and SM count without the status word: allocates nothing
+int fail_fmt(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+int launch_failed(cudaError_t e, const char* what);
+void count_launches(int n);
+unsigned long long wait_limit_ns_option();  // the "wait_limit_ms" option
+
 // fp32 GEMM with the tf32 hi/lo split done in shared memory (no pre-pass, no scratch): raw fp32 operands,
 // 128 x 64 tiles. For small and batched problems; operands must satisfy f32_fused_operands_ok.
 int launch_gemm_f32_fused(const TcGemmArgs& a, cudaStream_t stream);
