@@ -535,6 +535,29 @@ int symplex_b200_layer_norm_backward(const void* dy, const void* x, const float*
                                      int64_t cols, int64_t lddy, int64_t ldx, int64_t lddx, int32_t dtype,
                                      int32_t param_dtype, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Weights in 4 bits with a scale per group of consecutive k: W[n][k] = (code[n][k] - zero[n][k / group]) *
+ * scale[n][k / group]. Two codes a byte, the low half is the even k; rows of codes are ldq bytes apart (0 = ceil(K / 2)),
+ * scales and zeros are [N][ceil(K / group)] packed, group a positive multiple of 32 (the last group of a row may be
+ * shorter). scales have type scale_dtype (SYMPLEX_DT_F32 / SYMPLEX_DT_BF16); zeros are one byte each (0..15), or NULL for 8
+ * everywhere. */
+
+/* C[M, N] = act(A[M, K] . W^T + bias) for a few rows of A (M <= SYMPLEX_B200_INT4_MAX_M): the product of single tokens,
+ * bound by reading the codes. A is bf16 with leading dimension lda, C has out_dtype (F32 / BF16) and leading dimension ldc
+ * (elements, 0 = packed), bias is fp32[N] or NULL, activation one of SYMPLEX_ACT_*. code - zero enters the product as the
+ * whole number it is, sums are 32-bit, the scale is applied to each group's sum. */
+#define SYMPLEX_B200_INT4_MAX_M 64
+int symplex_b200_int4_matvec(const void* A, const uint8_t* codes, const void* scales, const uint8_t* zeros,
+                             const float* bias, void* C, int64_t M, int64_t N, int64_t K, int64_t group, int64_t lda,
+                             int64_t ldq, int64_t ldc, int32_t scale_dtype, int32_t out_dtype, int32_t activation,
+                             void* stream);
+
+/* Lay out W[N, K] (dtype F32 / BF16, leading dimension ldw) once: codes, scales and, if zeros is not NULL, zeros as above.
+ * Without zeros: scale = max|w| / 7, code = round(w / scale) + 8. With zeros: lo = min(w, 0), hi = max(w, 0), scale =
+ * (hi - lo) / 15, zero = round(-lo / scale), code = round(w / scale) + zero, all limited to 0..15. Ties go to even. The scale is
+ * rounded to scale_dtype first and the codes are taken against the rounded one; a group of zeros has scale 1. */
+int symplex_b200_int4_quantize(const void* W, uint8_t* codes, void* scales, uint8_t* zeros, int64_t N, int64_t K,
+                               int64_t group, int64_t ldw, int32_t dtype, int32_t scale_dtype, void* stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif

@@ -11,9 +11,11 @@ from __future__ import annotations
 import torch
 
 from . import _capi
-from ._capi import DT_BF16, DT_F32
+from ._capi import ACTIVATIONS, DT_BF16, DT_F32
 
-__all__ = ["layer_norm", "layer_norm_backward"]
+__all__ = ["layer_norm", "layer_norm_backward", "int4_quantize", "int4_matvec"]
+
+INT4_MAX_ROWS = 64
 
 _DT = {torch.float32: DT_F32, torch.bfloat16: DT_BF16}
 
@@ -130,5 +132,95 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, *, param_grads=None, str
             dyr.data_ptr(), xr.data_ptr(), m.data_ptr(), r.data_ptr(), _ptr(w), dx.data_ptr(), _ptr(dw), _ptr(db), rows, cols,
             lddy, ldx, cols, _DT[x.dtype], _DT[pdt], _ptr(ws), size, s))
         return dx, dw, db
+
+    return _run(x.device, stream, call)
+
+
+# ----------------------------------------------------------------------------- products with 4-bit weights
+
+def _group_count(k, group_size, who):
+    if not isinstance(group_size, int) or group_size <= 0 or group_size % 32:
+        raise ValueError(f"{who}: group_size must be a positive multiple of 32, got {group_size!r}")
+    return -(-k // group_size)
+
+
+def int4_quantize(weight, group_size=128, *, symmetric=True, scale_dtype=torch.bfloat16, stream=None):
+    """Lay out a ``[N, K]`` weight (float32 or bfloat16) in 4 bits: ``(codes, scales, zeros)`` for ``int4_matvec``.
+
+    ``codes``: uint8 ``[N, ceil(K / 2)]``, the low half of a byte is the even k. ``scales``: ``scale_dtype``
+    ``[N, ceil(K / group_size)]``. ``zeros``: None (symmetric: 8 everywhere, scale = max|w| / 7) or uint8 like ``scales``
+    (scale = range / 15). A group with a weight that is not finite gets the scale NaN. (``symplex_b200_int4_quantize``)
+    """
+    if not weight.is_cuda or weight.dtype not in _DT or weight.dim() != 2:
+        raise ValueError("int4_quantize() takes a 2-D float32 or bfloat16 CUDA tensor")
+    if scale_dtype not in _DT:
+        raise ValueError("scale_dtype must be float32 or bfloat16")
+    n, k = weight.shape
+    if k == 0:
+        raise ValueError("K == 0 is not supported")
+    groups = _group_count(k, group_size, "int4_quantize()")
+
+    def call(s):
+        w, ldw = _rows(weight)
+        codes = torch.empty(n, (k + 1) // 2, dtype=torch.uint8, device=weight.device)
+        scales = torch.empty(n, groups, dtype=scale_dtype, device=weight.device)
+        zeros = None if symmetric else torch.empty(n, groups, dtype=torch.uint8, device=weight.device)
+        _capi.check(_capi.load().symplex_b200_int4_quantize(w.data_ptr(), codes.data_ptr(), scales.data_ptr(), _ptr(zeros), n, k,
+                                                            group_size, ldw, _DT[weight.dtype], _DT[scale_dtype], s))
+        return codes, scales, zeros
+
+    return _run(weight.device, stream, call)
+
+
+def int4_matvec(x, codes, scales, zeros=None, *, group_size=128, bias=None, activation=None, out=None, out_dtype=None,
+                stream=None):
+    """``act(x @ W.T + bias)`` for a few rows of ``x`` (at most 64), ``W[n, k] = (codes[n, k] - zeros[n, k // group_size]) *
+    scales[n, k // group_size]`` held as ``int4_quantize`` lays it out (``symplex_b200_int4_matvec``).
+
+    ``x``: bfloat16 ``[K]`` or ``[M, K]``; ``zeros`` None means 8 everywhere; ``bias``: float32 ``[N]``; ``activation`` as in
+    ``gemm``. ``codes`` may be a view with unit stride in its rows. Returns ``[N]`` / ``[M, N]`` in ``out_dtype`` (bfloat16 or
+    float32). More rows than 64 are a product for ``gemm``.
+    """
+    if not x.is_cuda or x.dtype != torch.bfloat16 or x.dim() not in (1, 2):
+        raise ValueError("int4_matvec() takes a 1-D or 2-D bfloat16 CUDA tensor")
+    k = x.shape[-1]
+    m = x.shape[0] if x.dim() == 2 else 1
+    if m > INT4_MAX_ROWS:
+        raise ValueError(f"int4_matvec() takes at most {INT4_MAX_ROWS} rows, got {m}: use gemm()")
+    if k == 0:
+        raise ValueError("K == 0 is not supported")
+    groups = _group_count(k, group_size, "int4_matvec()")
+    if codes.dtype != torch.uint8 or codes.dim() != 2 or codes.shape[1] != (k + 1) // 2 or codes.device != x.device:
+        raise ValueError(f"codes must be uint8 of shape [N, {(k + 1) // 2}] on {x.device}, got {codes.dtype} {tuple(codes.shape)}")
+    n = codes.shape[0]
+    if scales.dtype not in _DT or scales.shape != (n, groups) or scales.device != x.device:
+        raise ValueError(f"scales must be float32 or bfloat16 of shape ({n}, {groups}) on {x.device}")
+    if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != (n, groups) or zeros.device != x.device):
+        raise ValueError(f"zeros must be uint8 of shape ({n}, {groups}) on {x.device}")
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or bias.device != x.device):
+        raise ValueError(f"bias must be float32 of shape ({n},) on {x.device}")
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"unknown activation {activation!r}; expected one of {sorted(a for a in ACTIVATIONS if a)}")
+    shape = (n,) if x.dim() == 1 else (m, n)
+    if out is not None:
+        if out.shape != shape or out.dtype not in _DT or out.device != x.device or not out.is_contiguous() or \
+                out_dtype not in (None, out.dtype):
+            raise ValueError(f"out must be a contiguous float32 or bfloat16 tensor of shape {shape} on {x.device}")
+        out_dtype = out.dtype
+    elif out_dtype is None:
+        out_dtype = torch.bfloat16
+    elif out_dtype not in _DT:
+        raise ValueError("out dtype must be float32 or bfloat16")
+
+    def call(s):
+        y = out if out is not None else torch.empty(shape, dtype=out_dtype, device=x.device)
+        (a, lda), (c, ldq) = _rows(x), _rows(codes)
+        sc = scales.contiguous()
+        z = zeros.contiguous() if zeros is not None else None
+        b = bias.contiguous() if bias is not None else None
+        _capi.check(_capi.load().symplex_b200_int4_matvec(
+            a.data_ptr(), c.data_ptr(), sc.data_ptr(), _ptr(z), _ptr(b), y.data_ptr(), m, n, k, group_size, lda, ldq, n,
+            _DT[sc.dtype], _DT[out_dtype], ACTIVATIONS[activation], s))
+        return y
 
     return _run(x.device, stream, call)
