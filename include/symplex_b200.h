@@ -558,6 +558,36 @@ int symplex_b200_int4_matvec(const void* A, const uint8_t* codes, const void* sc
 int symplex_b200_int4_quantize(const void* W, uint8_t* codes, void* scales, uint8_t* zeros, int64_t N, int64_t K,
                                int64_t group, int64_t ldw, int32_t dtype, int32_t scale_dtype, void* stream);
 
+/* Softmax cross entropy of a linear head, the logits never kept: l = x[T, H] . W[V, H]^T,
+ *   lse[t] = log sum_v exp l[t][v],  loss[t] = lse[t] - l[t][targets[t]], 0 where targets[t] == ignore_index.
+ * x and W have type dtype (F32: 3xTF32 products, BF16: fp32 accumulation) and leading dimensions ldx, ldw (elements, 0 = H).
+ * reduction NONE writes loss[T]; MEAN divides the sum by the number of rows that are not ignored (NaN if there are none), SUM
+ * does not: loss[1]. lse[T] is what the backward pass takes. A target that is neither ignore_index nor in 0..V-1 makes its
+ * loss NaN. The vocabulary is worked through in tiles (BF16) or pieces (F32) whose row maxima and sums, 32-bit, are joined at
+ * the end. F32 operands must be finite (an infinity has no split into tf32 parts: NaN); a BF16 logit may be -inf, a word without
+ * probability. The first call on a device must not be inside a stream capture (it sets up the device's status word); a device-side
+ * wait that ran out is reported by symplex_b200_sync_status. */
+#define SYMPLEX_LOSS_NONE 0
+#define SYMPLEX_LOSS_MEAN 1
+#define SYMPLEX_LOSS_SUM 2
+size_t symplex_b200_linear_cross_entropy_workspace_bytes(int64_t T, int64_t H, int64_t V, int32_t dtype);
+int symplex_b200_linear_cross_entropy(const void* x, const void* W, const int64_t* targets, float* loss, float* lse,
+                                      int64_t T, int64_t H, int64_t V, int64_t ldx, int64_t ldw, int32_t dtype,
+                                      int64_t ignore_index, int32_t reduction, void* workspace, size_t workspace_bytes,
+                                      void* stream);
+
+/* Its gradients: with p = exp(l - lse) and G[t][v] = (p[t][v] - [v == targets[t]]) * s[t],
+ *   dx[T, H] = G . W,  dW[V, H] = G^T . x     (packed, of type dtype)
+ * where s[t] is dloss[t] (NONE), dloss[0] (SUM) or dloss[0] / number of counted rows (MEAN), and 0 for ignored rows. The
+ * logits are computed again, a piece of the vocabulary at a time; G is held in dtype, sums are 32-bit, in an order that does
+ * not change from call to call. Rows of x that are ignored still meet G's zeros in the product: they must be finite. A target
+ * out of range makes its row of dx and all of dW NaN. T == 0 sets dW to zero. */
+size_t symplex_b200_linear_cross_entropy_backward_workspace_bytes(int64_t T, int64_t H, int64_t V, int32_t dtype);
+int symplex_b200_linear_cross_entropy_backward(const float* dloss, const void* x, const void* W, const int64_t* targets,
+                                               const float* lse, void* dx, void* dW, int64_t T, int64_t H, int64_t V,
+                                               int64_t ldx, int64_t ldw, int32_t dtype, int64_t ignore_index,
+                                               int32_t reduction, void* workspace, size_t workspace_bytes, void* stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif

@@ -27,10 +27,11 @@ from ._capi import (ACT_GELU, ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_SILU, ACT_TAN
 __all__ = [
     "matmul_jit", "matmul_tiled", "matmul", "fused_matmul_bias_relu", "gemm", "gemm_host", "make_desc",
     "cuda_available", "launch_count", "SymplexB200Error", "fused_elementwise",
-    "layer_norm", "layer_norm_backward", "int4_quantize", "int4_matvec",
+    "layer_norm", "layer_norm_backward", "linear_cross_entropy", "linear_cross_entropy_backward", "int4_quantize", "int4_matvec",
 ]
 
-_NN = ("layer_norm", "layer_norm_backward", "int4_quantize", "int4_matvec")  # live in the nn sub-module, which imports torch
+# live in the nn sub-module, which imports torch
+_NN = ("layer_norm", "layer_norm_backward", "linear_cross_entropy", "linear_cross_entropy_backward", "int4_quantize", "int4_matvec")
 
 
 def __getattr__(name):

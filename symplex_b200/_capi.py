@@ -131,6 +131,7 @@ COMM_FLAG_WORDS = 16
 DT_F64 = 10
 
 REDUCE_SUM, REDUCE_MAX, REDUCE_MIN, REDUCE_NONE = 0, 1, 2, 255
+LOSS_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 _F32P = c_void_p  # raw addresses; callers pass ints (numpy ``.ctypes.data`` / torch ``.data_ptr()``)
 
@@ -206,6 +207,12 @@ SIGNATURES = {
                                                                                  c_void_p]),
     "symplex_b200_int4_matvec": (c_int, [c_void_p] * 6 + [c_int64] * 7 + [c_int32] * 3 + [c_void_p]),
     "symplex_b200_int4_quantize": (c_int, [c_void_p] * 4 + [c_int64] * 4 + [c_int32] * 2 + [c_void_p]),
+    "symplex_b200_linear_cross_entropy_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int32]),
+    "symplex_b200_linear_cross_entropy": (c_int, [c_void_p] * 5 + [c_int64] * 5 + [c_int32, c_int64, c_int32, c_void_p, c_size_t,
+                                                                               c_void_p]),
+    "symplex_b200_linear_cross_entropy_backward_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int32]),
+    "symplex_b200_linear_cross_entropy_backward": (c_int, [c_void_p] * 7 + [c_int64] * 5 + [c_int32, c_int64, c_int32, c_void_p,
+                                                                                        c_size_t, c_void_p]),
     "symplex_b200_gemm_plan": (c_int, [ctypes.POINTER(GemmDesc), c_int, ctypes.POINTER(GemmPlan)]),
 }
 

@@ -11,9 +11,10 @@ from __future__ import annotations
 import torch
 
 from . import _capi
-from ._capi import ACTIVATIONS, DT_BF16, DT_F32
+from ._capi import ACTIVATIONS, DT_BF16, DT_F32, LOSS_REDUCTIONS
 
-__all__ = ["layer_norm", "layer_norm_backward", "int4_quantize", "int4_matvec"]
+__all__ = ["layer_norm", "layer_norm_backward", "linear_cross_entropy", "linear_cross_entropy_backward",
+           "int4_quantize", "int4_matvec"]
 
 INT4_MAX_ROWS = 64
 
@@ -132,6 +133,84 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, *, param_grads=None, str
             dyr.data_ptr(), xr.data_ptr(), m.data_ptr(), r.data_ptr(), _ptr(w), dx.data_ptr(), _ptr(dw), _ptr(db), rows, cols,
             lddy, ldx, cols, _DT[x.dtype], _DT[pdt], _ptr(ws), size, s))
         return dx, dw, db
+
+    return _run(x.device, stream, call)
+
+
+# ----------------------------------------------------------------------------- softmax cross entropy of a linear head
+
+def _loss_checks(who, x, weight, targets, ignore_index, reduction):
+    if not x.is_cuda or x.dtype not in _DT or x.dim() != 2:
+        raise ValueError(f"{who} takes a 2-D float32 or bfloat16 CUDA tensor")
+    if weight.dtype != x.dtype or weight.dim() != 2 or weight.shape[1] != x.shape[1] or weight.device != x.device:
+        raise ValueError(f"weight must be {x.dtype} of shape [V, {x.shape[1]}] on {x.device}, got {weight.dtype} {tuple(weight.shape)}")
+    if x.shape[1] == 0 or weight.shape[0] == 0:
+        raise ValueError("the hidden size and the vocabulary must not be empty")
+    if targets.dtype != torch.int64 or targets.shape != x.shape[:1] or targets.device != x.device:
+        raise ValueError(f"targets must be int64 of shape ({x.shape[0]},) on {x.device}")
+    if reduction not in LOSS_REDUCTIONS:
+        raise ValueError(f"reduction must be one of {sorted(LOSS_REDUCTIONS)}, got {reduction!r}")
+    if not isinstance(ignore_index, int) or not -2 ** 63 <= ignore_index < 2 ** 63:
+        raise ValueError("ignore_index must be a 64-bit integer")
+
+
+def linear_cross_entropy(x, weight, targets, *, ignore_index=-100, reduction="mean", stream=None):
+    """Softmax cross entropy of the logits ``x @ weight.T``, which are never kept (``symplex_b200_linear_cross_entropy``).
+
+    ``x``: float32 or bfloat16 ``[T, H]``; ``weight``: ``[V, H]`` of the same dtype (both may be views with unit stride in
+    their rows); ``targets``: int64 ``[T]``, rows equal to ``ignore_index`` have no loss. ``reduction``: ``"mean"`` over the rows
+    that count (NaN if none does), ``"sum"`` or ``"none"``. Returns ``(loss, lse)`` in float32: a 0-d tensor or ``[T]``, and the
+    rows' log-sum-exp, which the backward pass takes. A target outside ``0..V-1`` gives its row the loss NaN;
+    so does an infinity among float32 operands (their products are split into tf32 parts).
+    """
+    _loss_checks("linear_cross_entropy()", x, weight, targets, ignore_index, reduction)
+
+    def call(s):
+        lib = _capi.load()
+        (xr, ldx), (w, ldw) = _rows(x), _rows(weight)
+        t, h = x.shape
+        v = weight.shape[0]
+        loss = torch.empty(t if reduction == "none" else (), dtype=torch.float32, device=x.device)
+        lse = torch.empty(t, dtype=torch.float32, device=x.device)
+        size = lib.symplex_b200_linear_cross_entropy_workspace_bytes(t, h, v, _DT[x.dtype])
+        ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+        tg = targets.contiguous()
+        _capi.check(lib.symplex_b200_linear_cross_entropy(
+            xr.data_ptr(), w.data_ptr(), tg.data_ptr(), loss.data_ptr(), lse.data_ptr(), t, h, v, ldx, ldw, _DT[x.dtype], ignore_index,
+            LOSS_REDUCTIONS[reduction], ws.data_ptr(), size, s))
+        return loss, lse
+
+    return _run(x.device, stream, call)
+
+
+def linear_cross_entropy_backward(dloss, x, weight, targets, lse, *, ignore_index=-100, reduction="mean", stream=None):
+    """Gradients ``(dx, dweight)`` of ``linear_cross_entropy`` (``symplex_b200_linear_cross_entropy_backward``).
+
+    ``dloss``: float32, one value (``"mean"``, ``"sum"``) or ``[T]`` (``"none"``); ``lse`` from the forward pass; the other arguments
+    as there. The logits are computed again a piece of the vocabulary at a time. ``dx`` and ``dweight`` have the dtype of ``x``.
+    Ignored rows of ``x`` must be finite (their zero gradient meets them in ``dweight``).
+    """
+    _loss_checks("linear_cross_entropy_backward()", x, weight, targets, ignore_index, reduction)
+    t, h = x.shape
+    v = weight.shape[0]
+    if dloss.dtype != torch.float32 or dloss.device != x.device or \
+            (dloss.shape != (t,) if reduction == "none" else dloss.numel() != 1):
+        raise ValueError(f"dloss must be float32 on {x.device}: shape ({t},) for 'none', one value otherwise")
+    if lse.dtype != torch.float32 or lse.shape != (t,) or lse.device != x.device:
+        raise ValueError(f"lse must be float32 of shape ({t},) on {x.device}")
+
+    def call(s):
+        lib = _capi.load()
+        (xr, ldx), (w, ldw) = _rows(x), _rows(weight)
+        dx = torch.empty(t, h, dtype=x.dtype, device=x.device)
+        dw = torch.empty(v, h, dtype=x.dtype, device=x.device)
+        size = lib.symplex_b200_linear_cross_entropy_backward_workspace_bytes(t, h, v, _DT[x.dtype])
+        ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+        tg, ls, dl = targets.contiguous(), lse.contiguous(), dloss.contiguous()
+        _capi.check(lib.symplex_b200_linear_cross_entropy_backward(
+            dl.data_ptr(), xr.data_ptr(), w.data_ptr(), tg.data_ptr(), ls.data_ptr(), dx.data_ptr(), dw.data_ptr(), t, h, v, ldx, ldw,
+            _DT[x.dtype], ignore_index, LOSS_REDUCTIONS[reduction], ws.data_ptr(), size, s))
+        return dx, dw
 
     return _run(x.device, stream, call)
 
