@@ -566,11 +566,13 @@ int symplex_b200_int4_quantize(const void* W, uint8_t* codes, void* scales, uint
  * loss NaN. The vocabulary is worked through in tiles (BF16) or pieces (F32) whose row maxima and sums, 32-bit, are joined at
  * the end. F32 operands must be finite (an infinity has no split into tf32 parts: NaN); a BF16 logit may be -inf, a word without
  * probability. The first call on a device must not be inside a stream capture (it sets up the device's status word); a device-side
- * wait that ran out is reported by symplex_b200_sync_status. */
+ * wait that ran out is reported by symplex_b200_sync_status. The workspace query looks at x and W for their alignment only (BF16
+ * operands whose base or rows are not 16-byte aligned are copied into the workspace first). */
 #define SYMPLEX_LOSS_NONE 0
 #define SYMPLEX_LOSS_MEAN 1
 #define SYMPLEX_LOSS_SUM 2
-size_t symplex_b200_linear_cross_entropy_workspace_bytes(int64_t T, int64_t H, int64_t V, int32_t dtype);
+size_t symplex_b200_linear_cross_entropy_workspace_bytes(const void* x, const void* W, int64_t T, int64_t H, int64_t V,
+                                                         int64_t ldx, int64_t ldw, int32_t dtype);
 int symplex_b200_linear_cross_entropy(const void* x, const void* W, const int64_t* targets, float* loss, float* lse,
                                       int64_t T, int64_t H, int64_t V, int64_t ldx, int64_t ldw, int32_t dtype,
                                       int64_t ignore_index, int32_t reduction, void* workspace, size_t workspace_bytes,
@@ -579,10 +581,11 @@ int symplex_b200_linear_cross_entropy(const void* x, const void* W, const int64_
 /* Its gradients: with p = exp(l - lse) and G[t][v] = (p[t][v] - [v == targets[t]]) * s[t],
  *   dx[T, H] = G . W,  dW[V, H] = G^T . x     (packed, of type dtype)
  * where s[t] is dloss[t] (NONE), dloss[0] (SUM) or dloss[0] / number of counted rows (MEAN), and 0 for ignored rows. The
- * logits are computed again, a piece of the vocabulary at a time; G is held in dtype, sums are 32-bit, in an order that does
- * not change from call to call. Rows of x that are ignored still meet G's zeros in the product: they must be finite. A target
+ * logits are computed again, a piece of the vocabulary at a time; G is held in dtype (BF16: rounded, without the factor all
+ * rows share), sums are 32-bit, in an order that does not change from call to call. Rows of x that are ignored still meet G's zeros in the product: they must be finite. A target
  * out of range makes its row of dx and all of dW NaN. T == 0 sets dW to zero. */
-size_t symplex_b200_linear_cross_entropy_backward_workspace_bytes(int64_t T, int64_t H, int64_t V, int32_t dtype);
+size_t symplex_b200_linear_cross_entropy_backward_workspace_bytes(const void* x, const void* W, int64_t T, int64_t H,
+                                                                  int64_t V, int64_t ldx, int64_t ldw, int32_t dtype);
 int symplex_b200_linear_cross_entropy_backward(const float* dloss, const void* x, const void* W, const int64_t* targets,
                                                const float* lse, void* dx, void* dW, int64_t T, int64_t H, int64_t V,
                                                int64_t ldx, int64_t ldw, int32_t dtype, int64_t ignore_index,

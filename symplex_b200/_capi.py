@@ -207,10 +207,10 @@ SIGNATURES = {
                                                                                  c_void_p]),
     "symplex_b200_int4_matvec": (c_int, [c_void_p] * 6 + [c_int64] * 7 + [c_int32] * 3 + [c_void_p]),
     "symplex_b200_int4_quantize": (c_int, [c_void_p] * 4 + [c_int64] * 4 + [c_int32] * 2 + [c_void_p]),
-    "symplex_b200_linear_cross_entropy_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int32]),
+    "symplex_b200_linear_cross_entropy_workspace_bytes": (c_size_t, [c_void_p, c_void_p] + [c_int64] * 5 + [c_int32]),
     "symplex_b200_linear_cross_entropy": (c_int, [c_void_p] * 5 + [c_int64] * 5 + [c_int32, c_int64, c_int32, c_void_p, c_size_t,
                                                                                c_void_p]),
-    "symplex_b200_linear_cross_entropy_backward_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int32]),
+    "symplex_b200_linear_cross_entropy_backward_workspace_bytes": (c_size_t, [c_void_p, c_void_p] + [c_int64] * 5 + [c_int32]),
     "symplex_b200_linear_cross_entropy_backward": (c_int, [c_void_p] * 7 + [c_int64] * 5 + [c_int32, c_int64, c_int32, c_void_p,
                                                                                         c_size_t, c_void_p]),
     "symplex_b200_gemm_plan": (c_int, [ctypes.POINTER(GemmDesc), c_int, ctypes.POINTER(GemmPlan)]),

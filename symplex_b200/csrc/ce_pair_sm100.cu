@@ -1,0 +1,696 @@
+// Tensor-core kernels of the linear head's loss, bf16: logits on CTA pairs (tcgen05.mma.cta_group::2) that never leave the
+// SM, and the two products of the gradient.
+//
+//   CE_LSE     l = x W^T tile by tile; the epilogue turns each row's stretch of a tile into (largest, sum of exponentials)
+//              straight from tensor memory and picks out the target's logit. Nothing of size T x V is written.
+//   CE_GRAD    the same product again for a piece of the vocabulary; the epilogue writes G = (exp(l - lse) - 1hot) s in bf16.
+//   CE_PROD    dx += G W (A = G as stored) and dW = G^T x (A = G read MN-major, no transpose pass) as ONE list of tiles:
+//              both need G alone, their tiles differ in length (n against T k-blocks), and together they fill the pairs of the
+//              chip where dx by itself would leave the last wave mostly idle.
+//
+// Roles, barriers and tile shapes are those of the general pair kernel (gemm_pair_sm100.cu): warp 0 TMA, warp 1 MMA issue (leader CTA
+// only), then the epilogue warps; kMB = 1: 256 x 256 tiles with two alternating accumulators, kMB = 2: 512 x 256 tiles. All waits are
+// bounded; on a timeout every role unwinds and the status word says so.
+//
+// What bounds it: the tensor pipe (2 T V H flops forward, 6 T V H backward with the logits computed again).
+#include <cuda_bf16.h>
+
+#include <algorithm>
+
+#include "ce_params.h"
+#include "epilogue.cuh"
+#include "gemm_params.h"
+#include "host_api.h"
+#include "sm100_ptx.cuh"
+
+namespace sx {
+namespace {
+
+enum CeMode : int { CE_LSE = 0, CE_GRAD = 1, CE_PROD = 2 };
+
+template <int kMB>
+struct CeCfg {
+  static constexpr int ROWS = 128 * kMB;  // rows of A per CTA
+  static constexpr int BM = 2 * ROWS;
+  static constexpr int BN = 256;
+  static constexpr int BK = 64;
+  static constexpr int A_BYTES = ROWS * 128;
+  static constexpr int B_BYTES = 128 * 128;  // this CTA's 128 of the 256 columns
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int STAGES = kMB == 1 ? 6 : 4;
+  static constexpr int EPI_WARPS = 4 * kMB;
+  static constexpr int THREADS = 64 + 32 * EPI_WARPS;
+  static constexpr int TMEM_COLS = 512;
+  static constexpr int STAGING_BYTES = 32 * 128;
+  static constexpr int DYN_SMEM = STAGES * STAGE_BYTES + EPI_WARPS * STAGING_BYTES + 1024;
+};
+
+// One product: tiles of [M, N] over K.
+struct CeJob {
+  int M, N, K, m_tiles, n_tiles, group_m;
+};
+
+struct CeKernelParams {
+  CeJob job[2];     // job 1: CE_PROD only
+  int first_extra;  // CE_PROD: job-1 tiles given ahead to the pairs that got one job-0 tile fewer
+  int* status;
+  unsigned long long wait_limit_ns;
+  const long long* targets;
+  long long v0, V, ignore;
+  float2* part;
+  float* target_logit;
+  const float* lse;
+  const float* dloss;
+  const float* scale;
+  const float* acc_in;
+  int dx_bf16;      // CE_PROD: job 0 writes bf16 dx (last piece), else the fp32 accumulator
+  int tma_out[2];   // outputs written by TMA (16-byte aligned rows), else element by element
+  void* out[2];
+};
+
+struct CeTile {
+  int job, m0, n0, kb;
+};
+
+// The tiles of one pair, in order. CE_LSE / CE_GRAD: every pairs-th tile. CE_PROD: every pairs-th tile of job 0 (dx); the pairs that
+// got one fewer of those take `extra` tiles of job 1 (dW) each instead, and the rest of job 1 is dealt out evenly.
+template <int kMode, int kMB>
+struct CeWork {
+  using Cfg = CeCfg<kMB>;
+  const CeKernelParams& p;
+  int pair, pairs, stage, next, end, stride;
+
+  __host__ __device__ CeWork(const CeKernelParams& p_, int pair_, int pairs_) : p(p_), pair(pair_), pairs(pairs_), stage(0) {
+    next = pair;
+    end = p.job[0].m_tiles * p.job[0].n_tiles;
+    stride = pairs;
+  }
+  __host__ __device__ bool get(CeTile* t) {
+    if constexpr (kMode == CE_PROD) {
+      while (next >= end) {
+        const int t0 = p.job[0].m_tiles * p.job[0].n_tiles, t1 = p.job[1].m_tiles * p.job[1].n_tiles;
+        const int full = t0 % pairs;  // pairs 0 .. full-1 have one job-0 tile more
+        if (stage == 0) {
+          stage = 1;
+          next = pair >= full ? pair - full : p.first_extra;
+          end = p.first_extra;
+          stride = pairs - full;
+        } else if (stage == 1) {
+          stage = 2;
+          next = p.first_extra + pair;
+          end = t1;
+          stride = pairs;
+        } else {
+          return false;
+        }
+      }
+    } else if (next >= end) {
+      return false;
+    }
+    const int job = kMode == CE_PROD && stage > 0 ? 1 : 0;
+    const CeJob& j = p.job[job];
+    const int band = j.group_m * j.n_tiles;  // bands of group_m tile rows, column by column: operands of a band stay in L2
+    const int g = next / band;
+    const int first_m = g * j.group_m;
+    const int gsz = j.m_tiles - first_m < j.group_m ? j.m_tiles - first_m : j.group_m;
+    const int in_band = next - g * band;
+    t->job = job;
+    t->m0 = (first_m + in_band % gsz) * Cfg::BM;
+    t->n0 = (in_band / gsz) * Cfg::BN;
+    t->kb = (j.K + Cfg::BK - 1) / Cfg::BK;
+    next += stride;
+    return true;
+  }
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 32 values of one row into a 128-byte-swizzled staging tile of 32 rows x 128 bytes, one row per lane (the layout of a
+// SWIZZLE_128B tensor map): bf16 fills four of the eight 16-byte chunks from `chunk` on, fp32 all eight.
+__device__ __forceinline__ void stage_bf16(const float (&v)[32], uint8_t* tile, int lane, int chunk) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    *reinterpret_cast<uint4*>(tile + lane * 128 + (((chunk + c) ^ (lane & 7)) << 4)) = EpilogueCtx<__nv_bfloat16>::pack8_bf16(v + 8 * c);
+}
+__device__ __forceinline__ void stage_f32(const float (&v)[32], uint8_t* tile, int lane) {
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+    *reinterpret_cast<float4*>(tile + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+}
+
+template <int kMode, int kMB>
+__global__ void __launch_bounds__(CeCfg<kMB>::THREADS, 1)
+ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmB0,
+               const __grid_constant__ CUtensorMap tmA1, const __grid_constant__ CUtensorMap tmB1,
+               const __grid_constant__ CUtensorMap out0, const __grid_constant__ CUtensorMap out1,
+               const __grid_constant__ CeKernelParams p) {
+  using Cfg = CeCfg<kMB>;
+  using Work = CeWork<kMode, kMB>;
+  constexpr int BN = Cfg::BN, BK = Cfg::BK, STAGES = Cfg::STAGES;
+
+  extern __shared__ uint8_t dyn_smem[];
+  __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2];
+  __shared__ uint32_t tmem_base_slot;
+  __shared__ int abort_flag;
+
+  uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn_smem) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t cta_rank = cluster_ctarank();  // 0 = leader
+  const uint64_t wait_ns = p.wait_limit_ns;
+  const int pair_id = blockIdx.x >> 1;
+  const int num_pairs = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);   // leader: its producer's arrive.expect_tx (bytes of both CTAs)
+      mbar_init(&empty_bar[s], 1);  // one tcgen05.commit per use
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&acc_full[a], 1);
+      mbar_init(&acc_empty[a], 8 * kMB);  // every epilogue warp of both CTAs
+    }
+    abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc<2>(&tmem_base_slot, Cfg::TMEM_COLS);
+    tmem_relinquish<2>();
+  }
+  tc_fence_before_sync();
+  __syncwarp();
+  cluster_sync_all();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = tmem_base_slot;
+  pdl_launch_dependents();
+  pdl_wait_prior_grids();
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer (both CTAs)
+    if (lane == 0) {
+      tma_prefetch_desc(&tmA0);
+      tma_prefetch_desc(&tmB0);
+      if constexpr (kMode == CE_PROD) {
+        tma_prefetch_desc(&tmA1);
+        tma_prefetch_desc(&tmB1);
+      }
+      int stage = 0;
+      uint32_t phase = 0;
+      uint32_t armed = 0, armed_phase = 0;  // leader: stages whose copies (of both CTAs) may still be in flight
+      bool ok = true;
+      CeTile t;
+      for (Work w(p, pair_id, num_pairs); ok && w.get(&t);) {
+        const int my_m0 = t.m0 + int(cta_rank) * Cfg::ROWS;
+        const int my_n0 = t.n0 + int(cta_rank) * 128;
+        for (int kb = 0; kb < t.kb; ++kb) {
+          if (!mbar_wait(&empty_bar[stage], phase ^ 1, &abort_flag, wait_ns)) { ok = false; break; }
+          uint8_t* sa = tiles + stage * Cfg::STAGE_BYTES;
+          uint8_t* sb = sa + Cfg::A_BYTES;
+          if (cta_rank == 0) {
+            mbar_arrive_expect_tx(&full_bar[stage], 2 * Cfg::STAGE_BYTES);
+            armed |= 1u << stage;
+            armed_phase = (armed_phase & ~(1u << stage)) | (phase << stage);
+          }
+          const uint32_t leader_full = mapa_u32(smem_u32(&full_bar[stage]), 0);
+          if constexpr (kMode != CE_PROD) {
+            tma_load_3d_pair(sa, &tmA0, leader_full, kb * BK, my_m0, 0);
+            tma_load_3d_pair(sb, &tmB0, leader_full, kb * BK, my_n0, 0);
+          } else {
+            if (t.job == 0) {
+              tma_load_3d_pair(sa, &tmA0, leader_full, kb * BK, my_m0, 0);
+            } else {  // MN-major: boxes of [64 k][64 m], 8192 bytes each
+#pragma unroll
+              for (int c = 0; c < Cfg::ROWS / 64; ++c)
+                tma_load_3d_pair(sa + c * (BK * 128), &tmA1, leader_full, my_m0 + c * 64, kb * BK, 0);
+            }
+            const CUtensorMap* tb = t.job == 0 ? &tmB0 : &tmB1;
+            tma_load_3d_pair(sb, tb, leader_full, my_n0, kb * BK, 0);
+            tma_load_3d_pair(sb + BK * 128, tb, leader_full, my_n0 + 64, kb * BK, 0);
+          }
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+      }
+      if (!ok) {
+        // Unwinding: copies in flight get a bounded time to land (the partner, which has no barrier of its own to watch, a
+        // fixed grace period) before the CTAs meet at the cluster barrier below.
+        const uint64_t t0 = globaltimer_ns();
+        if (cta_rank == 0) {
+          for (int s = 0; s < STAGES; ++s) {
+            if (!(armed & (1u << s))) continue;
+            while (!mbar_try_wait(&full_bar[s], (armed_phase >> s) & 1u)) {
+              if (globaltimer_ns() - t0 > 2000000ull) break;
+            }
+          }
+        } else {
+          while (globaltimer_ns() - t0 < 100000ull) __nanosleep(1000);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer (leader CTA only)
+    if (lane == 0 && cta_rank == 0) {
+      constexpr uint64_t k_major = make_smem_desc_hi(16, 1024);
+      constexpr uint64_t mn_major = make_smem_desc_hi(BK * 128, 1024);  // chunks of 64 columns 8192 bytes apart
+      constexpr int KSTEPS = BK / 16;
+      constexpr bool kBmn = kMode == CE_PROD;
+      constexpr uint64_t b_hi = kBmn ? mn_major : k_major;
+      constexpr uint32_t b_kstep = kBmn ? 16 * 128 : 32;
+      int stage = 0;
+      uint32_t phase = 0;
+      int slot = 0;
+      uint32_t acc_phase = 0;
+      bool ok = true;
+      auto advance = [&](int& s, uint32_t& ph) {
+        if (++s == STAGES) { s = 0; ph ^= 1; }
+      };
+      CeTile t;
+      for (Work w(p, pair_id, num_pairs); ok && w.get(&t);) {
+        const bool a_mn = kMode == CE_PROD && t.job == 1;
+        const uint32_t idesc = a_mn ? make_idesc(1, true, kBmn, 256, BN) : make_idesc(1, false, kBmn, 256, BN);
+        const uint64_t a_hi = a_mn ? mn_major : k_major;
+        const uint32_t a_kstep = a_mn ? 16 * 128 : 32;
+        const int nk = t.kb;
+        // four MMAs (one 64-wide k-block) of row block `mb` into accumulator `acc`
+        auto issue = [&](int acc, int mb, int s, uint32_t accumulate) {
+          const uint32_t a_addr = smem_u32(tiles + s * Cfg::STAGE_BYTES) + mb * (128 * 128);
+          const uint32_t b_addr = smem_u32(tiles + s * Cfg::STAGE_BYTES) + Cfg::A_BYTES;
+#pragma unroll
+          for (int k = 0; k < KSTEPS; ++k)
+            umma<2, 0>(tmem_base + acc * BN, smem_desc(a_hi, a_addr + k * a_kstep), smem_desc(b_hi, b_addr + k * b_kstep), idesc,
+                       accumulate | (k != 0 ? 1u : 0u));
+        };
+        if constexpr (kMB == 1) {
+          if (!mbar_wait<true>(&acc_empty[slot], acc_phase ^ 1, &abort_flag, wait_ns)) break;
+          tc_fence_after_sync();
+          for (int kb = 0; kb < nk; ++kb) {
+            if (!mbar_wait(&full_bar[stage], phase, &abort_flag, wait_ns)) { ok = false; break; }
+            tc_fence_after_sync();
+            issue(slot, 0, stage, kb != 0 ? 1u : 0u);
+            umma_commit_pair(&empty_bar[stage], 3);
+            advance(stage, phase);
+          }
+          if (!ok) break;
+          umma_commit_pair(&acc_full[slot], 3);
+          if (++slot == 2) { slot = 0; acc_phase ^= 1; }
+        } else {
+          // The tile's two row blocks share every B stage; the first and last SKEW k-blocks are issued block-major, so block 0
+          // is done 4 SKEW MMAs early and the next tile starts on it while block 1 is still being drained.
+          constexpr int SKEW = 2;
+          const int head_end = min(SKEW, nk);
+          const int tail_begin = max(head_end, nk - SKEW);
+          auto group = [&](int g0, int g1) {
+            for (int mb = 0; mb < 2 && ok; ++mb) {
+              if (g0 == 0) {
+                if (!mbar_wait<true>(&acc_empty[mb], acc_phase ^ 1, &abort_flag, wait_ns)) { ok = false; break; }
+                tc_fence_after_sync();
+              }
+              int s = stage;
+              uint32_t ph = phase;
+              for (int kb = g0; kb < g1; ++kb) {
+                if (mb == 0) {
+                  if (!mbar_wait(&full_bar[s], ph, &abort_flag, wait_ns)) { ok = false; break; }
+                  tc_fence_after_sync();
+                }
+                issue(mb, mb, s, kb != 0 ? 1u : 0u);
+                if (mb == 1) umma_commit_pair(&empty_bar[s], 3);
+                advance(s, ph);
+              }
+              if (ok && g1 == nk) umma_commit_pair(&acc_full[mb], 3);
+            }
+            for (int kb = g0; kb < g1; ++kb) advance(stage, phase);
+          };
+          group(0, head_end);
+          for (int kb = head_end; ok && kb < tail_begin; ++kb) {
+            if (!mbar_wait(&full_bar[stage], phase, &abort_flag, wait_ns)) { ok = false; break; }
+            tc_fence_after_sync();
+            const uint32_t a_addr = smem_u32(tiles + stage * Cfg::STAGE_BYTES);
+            const uint32_t b_addr = a_addr + Cfg::A_BYTES;
+#pragma unroll
+            for (int k = 0; k < KSTEPS; ++k) {
+#pragma unroll
+              for (int mb = 0; mb < 2; ++mb)
+                umma<2, 0>(tmem_base + mb * BN, smem_desc(a_hi, a_addr + mb * (128 * 128) + k * a_kstep),
+                           smem_desc(b_hi, b_addr + k * b_kstep), idesc, 1u);
+            }
+            umma_commit_pair(&empty_bar[stage], 3);
+            advance(stage, phase);
+          }
+          if (ok && tail_begin < nk) group(tail_begin, nk);
+          if (!ok) break;
+          acc_phase ^= 1;
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue (both CTAs)
+    const int q = warp & 3;  // TMEM lane quarter this warp may read
+    const int half = kMB == 1 ? 0 : (warp - 2) >> 2;
+    constexpr int STRIPS = (BN / 32) / kMB;  // 32-column strips per warp and accumulator
+    uint8_t* staging = tiles + STAGES * Cfg::STAGE_BYTES + (warp - 2) * Cfg::STAGING_BYTES;
+    int slot = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    const float scale = kMode == CE_PROD && p.scale != nullptr ? *p.scale : 1.0f;
+    bool stored = false;  // this warp has TMA stores that may be reading its staging tile
+    CeTile t;
+    for (Work w(p, pair_id, num_pairs); ok && w.get(&t);) {
+      const CeJob& job = p.job[t.job];
+#pragma unroll 1
+      for (int blk = 0; blk < kMB; ++blk) {
+        if constexpr (kMB == 2) slot = blk;
+        const int row0 = t.m0 + int(cta_rank) * Cfg::ROWS + blk * 128 + q * 32;  // this warp's first row
+        const int row = row0 + lane;
+        const bool row_ok = row < job.M;
+        // What the row needs besides its logits, fetched while the accumulator is still being computed.
+        int at = -1;  // the target's column in this product
+        float lse = 0.0f, rs = 1.0f;
+        bool counted = true;
+        if constexpr (kMode != CE_PROD) {
+          const long long tg = row_ok ? p.targets[row] : -1;
+          if (tg >= p.v0 && tg < p.v0 + job.N) at = int(tg - p.v0);
+          if constexpr (kMode == CE_GRAD) {
+            counted = row_ok && tg != p.ignore;
+            if (row_ok) {
+              lse = p.lse[row];
+              if (p.dloss != nullptr) rs = p.dloss[row];
+              if (tg < 0 || tg >= p.V) rs = __int_as_float(0x7fc00000);
+            }
+          }
+        }
+        if (!mbar_wait(&acc_full[slot], acc_phase, &abort_flag, wait_ns)) { ok = false; break; }
+        tc_fence_after_sync();
+        float m = -INFINITY, s = 0.0f;
+#pragma unroll 1
+        for (int c = half * STRIPS; c < (half + 1) * STRIPS; c += 2) {
+          uint32_t r0[32], r1[32];
+          const uint32_t taddr = tmem_base + (uint32_t(q * 32) << 16) + slot * BN + c * 32;
+          tmem_ld_32x32(taddr, r0);
+          tmem_ld_32x32(taddr + 32, r1);
+          tmem_ld_wait();
+          const int col0 = t.n0 + c * 32;
+          if (col0 >= job.N) continue;
+          const bool second = col0 + 32 < job.N;
+          float v[32];
+
+          if constexpr (kMode == CE_LSE) {
+            auto strip = [&](const uint32_t (&r)[32], int cb) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+              if (cb + 32 > job.N) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                  if (cb + j >= job.N) v[j] = -INFINITY;
+              }
+              const int a = at - cb;
+              if (a >= 0 && a < 32) {
+                float l = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 32; ++j) l = a == j ? v[j] : l;
+                p.target_logit[row] = l;
+              }
+              float top = v[0];
+#pragma unroll
+              for (int j = 1; j < 32; ++j) top = fmaxf(top, v[j]);  // a NaN is passed over here and meets the sum below
+              const float nm = fmaxf(m, top);
+              if (nm == -INFINITY) {  // no mass so far: -inf - -inf must not become NaN, a NaN must stay one
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                  if (v[j] != v[j]) s = v[j];
+              } else {
+                float add = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 32; ++j) add += ex2((v[j] - nm) * CE_LOG2E);
+                s = fmaf(s, ex2((m - nm) * CE_LOG2E), add);
+                m = nm;
+              }
+            };
+            strip(r0, col0);
+            if (second) strip(r1, col0 + 32);
+          } else if constexpr (kMode == CE_GRAD) {
+            auto strip = [&](const uint32_t (&r)[32], int cb) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = ex2((__uint_as_float(r[j]) - lse) * CE_LOG2E) * rs;
+              const int a = at - cb;
+              if (a >= 0 && a < 32) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                  if (a == j) v[j] = (ex2((__uint_as_float(r[j]) - lse) * CE_LOG2E) - 1.0f) * rs;
+              }
+              if (!counted) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+              }
+            };
+            strip(r0, col0);
+            if (stored && lane == 0) bulk_wait_group_read<0>();  // the previous block has left the staging tile
+            __syncwarp();
+            stage_bf16(v, staging, lane, 0);
+            if (second) {
+              strip(r1, col0 + 32);
+              stage_bf16(v, staging, lane, 4);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_3d(&out0, staging, col0, row0, 0);
+              bulk_commit_group();
+            }
+            stored = true;
+          } else {
+            const bool f32 = t.job == 0 && !p.dx_bf16;
+            const CUtensorMap* om = t.job == 0 ? &out0 : &out1;
+            const bool tma = p.tma_out[t.job] != 0;
+            auto strip = [&](const uint32_t (&r)[32], int cb) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+              if (t.job == 0 && p.acc_in != nullptr && row_ok) {
+                const float* a = p.acc_in + (long long)row * job.N + cb;
+                if (cb + 32 <= job.N && (job.N & 3) == 0) {
+#pragma unroll
+                  for (int j = 0; j < 8; ++j) {
+                    const float4 x = *reinterpret_cast<const float4*>(a + 4 * j);
+                    v[4 * j] += x.x; v[4 * j + 1] += x.y; v[4 * j + 2] += x.z; v[4 * j + 3] += x.w;
+                  }
+                } else {
+#pragma unroll
+                  for (int j = 0; j < 32; ++j)
+                    if (cb + j < job.N) v[j] += a[j];
+                }
+              }
+              if (!f32) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] *= scale;
+              }
+            };
+            auto plain = [&](int cb) {  // rows that a TMA store cannot take
+              if (!row_ok) return;
+              const long long off = (long long)row * job.N + cb;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                if (cb + j >= job.N) break;
+                if (f32) static_cast<float*>(p.out[0])[off + j] = v[j];
+                else static_cast<__nv_bfloat16*>(p.out[t.job])[off + j] = __nv_bfloat16(v[j]);
+              }
+            };
+            strip(r0, col0);
+            if (!tma) {
+              plain(col0);
+              if (second) {
+                strip(r1, col0 + 32);
+                plain(col0 + 32);
+              }
+              continue;
+            }
+            if (stored && lane == 0) bulk_wait_group_read<0>();
+            __syncwarp();
+            if (f32) {  // one 128-byte block per strip
+              stage_f32(v, staging, lane);
+              if (second) {
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                  tma_store_3d(om, staging, col0, row0, 0);
+                  bulk_commit_group();
+                }
+                strip(r1, col0 + 32);
+                if (lane == 0) bulk_wait_group_read<0>();
+                __syncwarp();
+                stage_f32(v, staging, lane);
+              }
+            } else {
+              stage_bf16(v, staging, lane, 0);
+              if (second) {
+                strip(r1, col0 + 32);
+                stage_bf16(v, staging, lane, 4);
+              }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_3d(om, staging, f32 && second ? col0 + 32 : col0, row0, 0);
+              bulk_commit_group();
+            }
+            stored = true;
+          }
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(mapa_u32(smem_u32(&acc_empty[slot]), 0));  // leader's barrier
+        if constexpr (kMode == CE_LSE) {
+          if (row_ok) p.part[(long long)(t.n0 / BN * kMB + half) * job.M + row] = make_float2(m, s);
+        }
+      }
+      if constexpr (kMB == 1) {
+        if (++slot == 2) { slot = 0; acc_phase ^= 1; }
+      } else {
+        acc_phase ^= 1;
+      }
+    }
+    if (stored && lane == 0) bulk_wait_group<0>();  // every store of this warp has been performed
+  }
+
+  // Both CTAs stay until every remote barrier signal and paired MMA has landed.
+  tc_fence_before_sync();
+  __syncwarp();
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc<2>(tmem_base, Cfg::TMEM_COLS);
+  }
+  if (threadIdx.x == 0 && abort_flag != 0 && p.status != nullptr) atomicExch(p.status, int(ST_WAIT_TIMEOUT));
+}
+
+// ------------------------------------------------------------------ host side
+
+int map_of(CUtensorMap* out, const CeMatrix& m, uint32_t box_cols, uint32_t box_rows) {
+  const uint64_t dims[3] = {(uint64_t)m.cols, (uint64_t)m.rows, 1};
+  const uint64_t strides[2] = {(uint64_t)m.ld * 2, (uint64_t)m.rows * m.ld * 2};
+  const uint32_t box[3] = {box_cols, box_rows, 1};
+  return encode_tensor_map_3d(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, m.p, dims, strides, box);
+}
+
+int out_map(CUtensorMap* out, const void* p, long long rows, long long cols, long long ld, bool f32) {
+  const int eb = f32 ? 4 : 2;
+  const uint64_t dims[3] = {(uint64_t)cols, (uint64_t)rows, 1};
+  const uint64_t strides[2] = {(uint64_t)ld * eb, (uint64_t)rows * ld * eb};
+  const uint32_t box[3] = {(uint32_t)(128 / eb), 32, 1};
+  return encode_tensor_map_3d(out, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p, dims, strides, box);
+}
+
+// 512-row tiles or 256-row ones: fewer waves x area per tile over the tensor-pipe share each shape reaches on large products
+// (0.875 and 0.80, measured for the general pair kernel).
+int row_blocks(long long M, long long N, int num_sms) {
+  if (M <= 256) return 1;
+  const long long pairs = num_sms / 2, nt = (N + 255) / 256;
+  const long long w1 = ((M + 255) / 256 * nt + pairs - 1) / pairs, w2 = ((M + 511) / 512 * nt + pairs - 1) / pairs;
+  return (double)w2 * 2 / 0.875 <= (double)w1 / 0.80 ? 2 : 1;
+}
+
+CeJob job_of(long long M, long long N, long long K, int mb) {
+  CeJob j;
+  j.M = (int)M; j.N = (int)N; j.K = (int)K;
+  j.m_tiles = (int)((M + 256 * mb - 1) / (256 * mb));
+  j.n_tiles = (int)((N + 255) / 256);
+  j.group_m = mb == 2 ? 4 : 8;
+  return j;
+}
+
+template <int kMode, int kMB>
+int launch(const CUtensorMap (&in)[4], const CUtensorMap (&out)[2], const CeKernelParams& p, long long tiles, int num_sms, cudaStream_t stream) {
+  using Cfg = CeCfg<kMB>;
+  auto kern = ce_pair_kernel<kMode, kMB>;
+  SX_ENSURE_DYN_SMEM(kern, Cfg::DYN_SMEM);
+  const unsigned pairs = (unsigned)std::min<long long>(tiles, num_sms / 2);
+  const cudaError_t e = launch_kernel_ex(kern, 2 * pairs, Cfg::THREADS, Cfg::DYN_SMEM, stream, 2, pdl_enabled(), in[0], in[1], in[2], in[3],
+                                         out[0], out[1], p);
+  if (e != cudaSuccess) return launch_failed(e, "loss kernel launch failed");
+  count_launches(1);
+  return SX_OK;
+}
+
+CeKernelParams common(const CeCommon& c) {
+  CeKernelParams p{};
+  p.status = c.status;
+  p.wait_limit_ns = c.wait_limit_ns;
+  return p;
+}
+
+}  // namespace
+
+int ce_forward_parts(long long T, long long V, int num_sms) { return (int)((V + 255) / 256) * row_blocks(T, V, num_sms); }
+int ce_forward_parts_most(long long V) { return (int)((V + 255) / 256) * 2; }
+
+int launch_ce_forward(const CeCommon& c, const CeForward& a, cudaStream_t stream) {
+  const int mb = row_blocks(a.x.rows, a.W.rows, c.num_sms);
+  CUtensorMap in[4] = {}, out[2] = {};
+  int rc = map_of(&in[0], a.x, 64, 128 * mb);
+  if (rc == SX_OK) rc = map_of(&in[1], a.W, 64, 128);
+  if (rc != SX_OK) return rc;
+  CeKernelParams p = common(c);
+  p.job[0] = job_of(a.x.rows, a.W.rows, a.x.cols, mb);
+  p.targets = a.targets;
+  p.V = a.W.rows;
+  p.part = a.part;
+  p.target_logit = a.target_logit;
+  const long long tiles = (long long)p.job[0].m_tiles * p.job[0].n_tiles;
+  if (tiles > 0x7fffffffLL) return set_last_error(SX_ERR_INVALID, "the problem has more than 2^31-1 tiles");
+  return mb == 2 ? launch<CE_LSE, 2>(in, out, p, tiles, c.num_sms, stream) : launch<CE_LSE, 1>(in, out, p, tiles, c.num_sms, stream);
+}
+
+int launch_ce_grad(const CeCommon& c, const CeGrad& a, cudaStream_t stream) {
+  const int mb = row_blocks(a.x.rows, a.W.rows, c.num_sms);
+  CUtensorMap in[4] = {}, out[2] = {};
+  int rc = map_of(&in[0], a.x, 64, 128 * mb);
+  if (rc == SX_OK) rc = map_of(&in[1], a.W, 64, 128);
+  if (rc == SX_OK) rc = out_map(&out[0], a.G, a.x.rows, a.W.rows, a.ldg, false);
+  if (rc != SX_OK) return rc;
+  CeKernelParams p = common(c);
+  p.job[0] = job_of(a.x.rows, a.W.rows, a.x.cols, mb);
+  p.targets = a.targets;
+  p.lse = a.lse;
+  p.dloss = a.dloss;
+  p.v0 = a.v0;
+  p.V = a.V;
+  p.ignore = a.ignore;
+  const long long tiles = (long long)p.job[0].m_tiles * p.job[0].n_tiles;
+  if (tiles > 0x7fffffffLL) return set_last_error(SX_ERR_INVALID, "the problem has more than 2^31-1 tiles");
+  return mb == 2 ? launch<CE_GRAD, 2>(in, out, p, tiles, c.num_sms, stream) : launch<CE_GRAD, 1>(in, out, p, tiles, c.num_sms, stream);
+}
+
+int launch_ce_products(const CeCommon& c, const CeProducts& a, cudaStream_t stream) {
+  const long long T = a.x.rows, H = a.x.cols, n = a.W.rows;
+  const int mb = std::min(T, n) <= 256 ? 1 : 2;
+  CUtensorMap in[4], out[2] = {};
+  int rc = map_of(&in[0], a.G, 64, 128 * mb);          // dx: A = G, k = vocabulary
+  if (rc == SX_OK) rc = map_of(&in[1], a.W, 64, 64);   //     B = W, MN-major
+  if (rc == SX_OK) rc = map_of(&in[2], a.G, 64, 64);   // dW: A = G^T, MN-major, k = tokens
+  if (rc == SX_OK) rc = map_of(&in[3], a.x, 64, 64);   //     B = x, MN-major
+  if (rc != SX_OK) return rc;
+  CeKernelParams p = common(c);
+  p.job[0] = job_of(T, H, n, mb);
+  p.job[1] = job_of(n, H, T, mb);
+  p.scale = a.scale;
+  p.acc_in = a.acc_in;
+  p.dx_bf16 = a.acc_out == nullptr;
+  p.out[0] = p.dx_bf16 ? a.dx : a.acc_out;
+  p.out[1] = a.dW;
+  for (int j = 0; j < 2; ++j) {
+    const bool f32 = j == 0 && !p.dx_bf16;
+    p.tma_out[j] = (H * (f32 ? 4 : 2)) % 16 == 0 && reinterpret_cast<uintptr_t>(p.out[j]) % 16 == 0;
+    if (p.tma_out[j] && (rc = out_map(&out[j], p.out[j], j == 0 ? T : n, H, H, f32)) != SX_OK) return rc;
+  }
+  const long long t0 = (long long)p.job[0].m_tiles * p.job[0].n_tiles, t1 = (long long)p.job[1].m_tiles * p.job[1].n_tiles;
+  if (t0 + t1 > 0x3fffffffLL) return set_last_error(SX_ERR_INVALID, "the problem has more than 2^30-1 tiles");
+  const long long pairs = std::min<long long>(t0 + t1, c.num_sms / 2);
+  if (t0 % pairs != 0) {
+    const long long each = (n + T / 2) / T;  // dW tiles that take as long as one dx tile
+    p.first_extra = (int)std::min<long long>(t1, each * (pairs - t0 % pairs));
+  }
+  return mb == 2 ? launch<CE_PROD, 2>(in, out, p, t0 + t1, c.num_sms, stream) : launch<CE_PROD, 1>(in, out, p, t0 + t1, c.num_sms, stream);
+}
+
+}  // namespace sx

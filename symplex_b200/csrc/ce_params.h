@@ -1,0 +1,58 @@
+// Interface between the C entry points of the linear head's loss (linear_cross_entropy.cu) and its tensor-core kernels
+// (ce_pair_sm100.cu).
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace sx {
+
+constexpr float CE_LOG2E = 1.4426950408889634f;
+
+// A bf16 matrix of `rows` rows of `cols` values, `ld` values apart; base 16-byte aligned, ld a multiple of 8.
+struct CeMatrix {
+  const void* p;
+  long long rows, cols, ld;
+};
+
+struct CeCommon {
+  int num_sms;
+  int* status;
+  unsigned long long wait_limit_ns;
+};
+
+// Forward: every row's part (largest logit, sum of exp(l - largest)) of every tile column, and the targets' logits.
+struct CeForward {
+  CeMatrix x, W;  // [T, H], [V, H]
+  const long long* targets;
+  float2* part;  // [ce_forward_parts][T]
+  float* target_logit;
+};
+int ce_forward_parts(long long T, long long V, int num_sms);
+int ce_forward_parts_most(long long V);  // upper bound over T and SM counts
+int launch_ce_forward(const CeCommon& c, const CeForward& a, cudaStream_t stream);
+
+// G[t][v] = (exp(x W^T - lse) - [v0 + v = target]) * (dloss ? dloss[t] : 1), 0 in ignored rows, NaN where the target is none.
+struct CeGrad {
+  CeMatrix x, W;  // [T, H], the piece of W: [n, H]
+  void* G;        // bf16 [T, ldg], ldg a multiple of 8, 16-byte aligned
+  long long ldg;
+  const long long* targets;
+  const float* lse;
+  const float* dloss;  // per row, or null
+  long long v0, V, ignore;
+};
+int launch_ce_grad(const CeCommon& c, const CeGrad& a, cudaStream_t stream);
+
+// dx (+)= G W and dW = G^T x of one piece, times *scale where scale is not null. dx goes to acc (fp32 [T, H]) until the last
+// piece, which writes bf16 dx = (acc + G W) * scale; acc_in is null for the first piece.
+struct CeProducts {
+  CeMatrix G, x, W;  // [T, n], [T, H], [n, H]
+  const float* acc_in;
+  float* acc_out;  // null: last piece, dx is written
+  void* dx;
+  void* dW;        // [n, H] packed
+  const float* scale;
+};
+int launch_ce_products(const CeCommon& c, const CeProducts& a, cudaStream_t stream);
+
+}  // namespace sx

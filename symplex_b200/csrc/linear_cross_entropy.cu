@@ -7,19 +7,24 @@
 // are taken as 2^((l - m) log2 e) of the difference, not as one multiply-add of l and a scaled m: that would round m log2 e
 // once, an error that grows with |m| and, where a part's logits are all near the type's lowest value, overflows.
 //
-// This file: the row-wise kernels, the pieces of the vocabulary through the general GEMM, and the C entry points.
+// bf16 runs on the kernels of ce_pair_sm100.cu: the forward pass reduces each tile of logits where it is computed, the backward
+// pass writes G for a piece of the vocabulary and multiplies it with W and x in one launch. fp32 takes pieces of the vocabulary
+// through the 3xTF32 product with the operands split once (W's pieces as they come), logits of one piece at a time in scratch.
+//
+// This file: the row-wise kernels, the passes put together, and the C entry points.
 #include <cuda_bf16.h>
 
 #include <algorithm>
 
 #include "../../include/symplex_b200.h"
+#include "ce_params.h"
 #include "host_api.h"
 #include "sm100_ptx.cuh"
 
 namespace sx {
 namespace {
 
-constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LOG2E = CE_LOG2E;
 constexpr float LN2 = 0.6931471805599453f;
 
 struct RowPart {
@@ -126,25 +131,36 @@ ce_reduce_kernel(const float* __restrict__ row_loss, const long long* __restrict
   if (threadIdx.x == 0) *loss = (float)(mean ? s / (double)n : s);
 }
 
-// One CTA: 1 / counted rows (0 where there are none: no row has a gradient then).
+// One CTA: what every counted row's gradient is multiplied with, dloss or dloss / counted rows (0 where no row counts: there is
+// no gradient then).
 __global__ void __launch_bounds__(1024)
-ce_count_kernel(const long long* __restrict__ targets, float* __restrict__ inv_count, long long T, long long ignore) {
+ce_scale_kernel(const long long* __restrict__ targets, const float* __restrict__ dloss, float* __restrict__ scale, long long T,
+                long long ignore, int mean) {
   __shared__ long long cred[32];
   pdl_launch_dependents();
   pdl_wait_prior_grids();
   long long n = 0;
-  for (long long t = threadIdx.x; t < T; t += 1024) n += targets[t] != ignore ? 1 : 0;
-  n = cta_total(n, cred);
-  if (threadIdx.x == 0) *inv_count = n > 0 ? (float)(1.0 / (double)n) : 0.0f;
+  if (mean) {
+    for (long long t = threadIdx.x; t < T; t += 1024) n += targets[t] != ignore ? 1 : 0;
+    n = cta_total(n, cred);
+  }
+  if (threadIdx.x == 0) *scale = !mean ? *dloss : n > 0 ? (float)((double)*dloss / (double)n) : 0.0f;
 }
 
-// G and its transpose from a piece of logits: 32 x 32 tiles, the transpose through shared memory.
-template <typename T>
+__device__ __forceinline__ float tf32_part(float x) {
+  uint32_t r;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+  return __uint_as_float(r);
+}
+
+// fp32: G and its transpose from a piece of logits, both as the {hi, lo} tf32 planes the products read (hi = tf32(g), lo =
+// tf32(g - hi); planes plane_g / plane_t values apart). 32 x 32 tiles, the transpose through shared memory.
 __global__ void __launch_bounds__(256)
 ce_piece_grad_kernel(const float* __restrict__ L, long long ld, int cols, long long v0, const long long* __restrict__ targets,
-                     const float* __restrict__ lse, const float* __restrict__ dloss, int per_row, const float* __restrict__ inv_count,
-                     T* __restrict__ G, long long ldg, T* __restrict__ GT, long long ldt, long long rows, long long V, long long ignore) {
-  __shared__ T tile[32][33];
+                     const float* __restrict__ lse, const float* __restrict__ dloss, const float* __restrict__ scale,
+                     float* __restrict__ G, long long ldg, long long plane_g, float* __restrict__ GT, long long ldt, long long plane_t,
+                     long long rows, long long V, long long ignore) {
+  __shared__ float tile[32][33];
   pdl_launch_dependents();
   pdl_wait_prior_grids();
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
@@ -160,33 +176,29 @@ ce_piece_grad_kernel(const float* __restrict__ L, long long ld, int cols, long l
       if (r < rows && c < cols) {
         const long long at = targets[r];
         if (at != ignore) {
-          float s = dloss[per_row ? r : 0];
-          if (inv_count != nullptr) s *= *inv_count;
+          const float s = scale != nullptr ? *scale : dloss[r];
           g = (exp2f((L[r * ld + c] - lse[r]) * LOG2E) - (at == v0 + c ? 1.0f : 0.0f)) * s;
-          // The fp32 products round operands to tf32 by adding to their bits, which carries the NaN that arithmetic
-          // makes (all mantissa bits set) into the sign: a quiet NaN with a short mantissa survives.
-          if (at < 0 || at >= V || g != g) g = __int_as_float(0x7fc00000);
+          if (at < 0 || at >= V) g = __int_as_float(0x7fc00000);
         }
-        G[r * ldg + c] = T(g);
+        const float hi = tf32_part(g);
+        G[r * ldg + c] = hi;
+        G[plane_g + r * ldg + c] = tf32_part(g - hi);
       }
-      tile[y + 8 * j][x] = T(g);
+      tile[y + 8 * j][x] = g;
     }
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int c = c0 + y + 8 * j;
       const long long r = r0 + x;
-      if (r < rows && c < cols) GT[c * ldt + r] = tile[x][y + 8 * j];
+      if (r < rows && c < cols) {
+        const float g = tile[x][y + 8 * j], hi = tf32_part(g);
+        GT[c * ldt + r] = hi;
+        GT[plane_t + c * ldt + r] = tf32_part(g - hi);
+      }
     }
     __syncthreads();
   }
-}
-
-__global__ void __launch_bounds__(256)
-ce_round_kernel(const float* __restrict__ in, __nv_bfloat16* __restrict__ out, long long n) {
-  pdl_launch_dependents();
-  pdl_wait_prior_grids();
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) out[i] = __nv_bfloat16(in[i]);
 }
 
 // ------------------------------------------------------------------ host side
@@ -194,82 +206,85 @@ size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 long long up(long long x, long long m) { return (x + m - 1) / m * m; }
 
 struct Problem {
+  const void *x, *W;  // looked at for their alignment only where a workspace is sized
   long long T, H, V, ldx, ldw;
   bool bf16;
   int eb;
   long long ignore;
   int reduction;
+
+  // bf16 operands that TMA cannot read in place go through a padded copy.
+  bool copy(const void* p, long long ld) const { return bf16 && (ld % 8 != 0 || reinterpret_cast<uintptr_t>(p) % 16 != 0); }
+  bool copy_x() const { return copy(x, ldx); }
+  bool copy_w() const { return copy(W, ldw); }
 };
 
-// Columns of one piece: T x piece fp32 logits of about PIECE_BYTES.
-constexpr long long PIECE_BYTES = 256ll << 20;
-long long piece_columns(long long T, long long V) {
-  const long long c = PIECE_BYTES / 4 / std::max<long long>(T, 1) / 256 * 256;
-  return std::min(up(V, 8), std::max<long long>(256, c));
+// Columns of the vocabulary worked through at a time.
+// bf16 backward: G [T, piece] in bf16 of about 128 MB, so that most of it is still in L2 (126 MB) when the products read it,
+// but at least 8192 columns: dx makes a round trip through its fp32 accumulator once a piece, 8 T H bytes beside 6 T H piece
+// flops. fp32: logits of a piece of about 64 MB, with G and its transpose in two planes each four times that.
+long long piece_columns(const Problem& p, bool backward) {
+  const long long T = std::max<long long>(p.T, 1);
+  if (p.bf16) return backward ? std::min(up(p.V, 8), std::max<long long>(8192, (64ll << 20) / T / 256 * 256)) : up(p.V, 8);
+  return std::min(up(p.V, 8), std::max<long long>(256, (16ll << 20) / T / 256 * 256));
 }
 
-symplex_gemm_desc product(const Problem& p, long long M, long long N, long long K, bool out_f32, int b_layout, long long lda,
-                          long long ldb, long long ldc) {
-  symplex_gemm_desc d;
-  symplex_b200_gemm_desc_init(&d, M, N, K, p.bf16 ? SYMPLEX_DT_BF16 : SYMPLEX_DT_F32,
-                              out_f32 || !p.bf16 ? SYMPLEX_DT_F32 : SYMPLEX_DT_BF16);
-  d.b_layout = b_layout;
-  d.lda = lda;
-  d.ldb = ldb;
-  d.ldc = ldc;
-  return d;
-}
-
-// Everything the two passes keep in the workspace.
+// Everything the two passes keep in the workspace (offsets in bytes).
 struct Layout {
-  long long piece, ldl, ldt;
-  int parts;
-  size_t logits, part, target_logit, row_loss, inv_count, G, GT, acc[2], gemm, gemm_bytes, total;
+  long long hp, tp, piece;  // padded H and T, columns of a piece (a multiple of 8)
+  int pieces, parts;
+  size_t xcopy, wcopy, part, target_logit, row_loss, scale, G, acc[2];
+  size_t xs, xts, ws, wts, logits, GT;  // fp32: operand planes, a piece's logits, G^T
+  size_t total;
 };
 
 Layout layout(const Problem& p, bool backward) {
   Layout w{};
-  w.piece = piece_columns(p.T, p.V);
-  w.ldl = up(w.piece, 8);
-  w.ldt = up(p.T, 8);
-  w.parts = (int)((p.V + w.piece - 1) / w.piece);
+  w.hp = up(p.H, 8);
+  w.tp = up(p.T, 8);
+  w.piece = piece_columns(p, backward);
+  w.pieces = (int)((p.V + w.piece - 1) / w.piece);
+  w.parts = p.bf16 ? ce_forward_parts_most(p.V) : w.pieces;
   size_t off = 0;
   auto take = [&](size_t bytes) {
     const size_t at = off;
     off = up256(off + bytes);
     return at;
   };
-  w.logits = take((size_t)p.T * w.ldl * 4);
+  if (p.copy_x()) w.xcopy = take((size_t)p.T * w.hp * 2);
+  if (p.copy_w()) w.wcopy = take((size_t)w.piece * w.hp * 2);
+  if (!p.bf16) {
+    w.xs = take((size_t)2 * p.T * w.hp * 4);
+    w.ws = take((size_t)2 * w.piece * w.hp * 4);
+    w.logits = take((size_t)p.T * w.piece * 4);
+  }
   if (!backward) {
     w.part = take((size_t)w.parts * p.T * sizeof(float2));
     w.target_logit = take((size_t)p.T * 4);
     w.row_loss = take((size_t)p.T * 4);
   } else {
-    w.inv_count = take(4);
-    w.G = take((size_t)p.T * w.ldl * p.eb);
-    w.GT = take((size_t)w.piece * w.ldt * p.eb);
-    w.acc[0] = take((size_t)p.T * p.H * 4);
-    w.acc[1] = take((size_t)p.T * p.H * 4);
+    w.scale = take(4);
+    w.G = take((size_t)p.T * w.piece * (p.bf16 ? 2 : 8));
+    if (w.pieces > 1) w.acc[0] = take((size_t)p.T * p.H * 4);
+    if (!p.bf16) {
+      if (w.pieces > 2) w.acc[1] = take((size_t)p.T * p.H * 4);
+      w.xts = take((size_t)2 * p.H * w.tp * 4);
+      w.wts = take((size_t)2 * p.H * w.piece * 4);
+      w.GT = take((size_t)2 * w.piece * w.tp * 4);
+    }
   }
-  // The products' own scratch, at the size of a full piece.
-  auto need = [&](const symplex_gemm_desc& d) { w.gemm_bytes = std::max(w.gemm_bytes, symplex_b200_gemm_workspace_bytes(&d)); };
-  need(product(p, p.T, w.piece, p.H, true, SYMPLEX_COL_MAJOR, p.ldx, p.ldw, w.ldl));
-  if (backward) {
-    need(product(p, p.T, p.H, w.piece, true, SYMPLEX_ROW_MAJOR, w.ldl, p.ldw, p.H));
-    need(product(p, w.piece, p.H, p.T, false, SYMPLEX_ROW_MAJOR, w.ldt, p.ldx, p.H));
-  }
-  w.gemm = take(w.gemm_bytes);
   w.total = off;
   return w;
 }
 
-int check(Problem* p, int64_t T, int64_t H, int64_t V, int64_t ldx, int64_t ldw, int32_t dtype, int64_t ignore, int32_t reduction) {
+int check(Problem* p, const void* x, const void* W, int64_t T, int64_t H, int64_t V, int64_t ldx, int64_t ldw, int32_t dtype, int64_t ignore,
+          int32_t reduction) {
   if (T < 0 || H <= 0 || V <= 0) return fail_fmt(SX_ERR_INVALID, "the loss needs T >= 0, H >= 1 and V >= 1");
   if (T > 0x3fffffffLL || H > 0x3fffffffLL || V > 0x3fffffffLL) return fail_fmt(SX_ERR_INVALID, "dimension exceeds 2^30-1");
   if (dtype != SYMPLEX_DT_F32 && dtype != SYMPLEX_DT_BF16)
     return fail_fmt(SX_ERR_INVALID, "dtype %d not supported (F32=9, BF16=11)", dtype);
   if (reduction < SYMPLEX_LOSS_NONE || reduction > SYMPLEX_LOSS_SUM) return fail_fmt(SX_ERR_INVALID, "reduction %d not supported", reduction);
-  *p = Problem{T, H, V, ldx ? ldx : H, ldw ? ldw : H, dtype == SYMPLEX_DT_BF16, dtype == SYMPLEX_DT_BF16 ? 2 : 4, ignore, reduction};
+  *p = Problem{x, W, T, H, V, ldx ? ldx : H, ldw ? ldw : H, dtype == SYMPLEX_DT_BF16, dtype == SYMPLEX_DT_BF16 ? 2 : 4, ignore, reduction};
   if (p->ldx < H || p->ldw < H) return fail_fmt(SX_ERR_INVALID, "leading dimension too small");
   return SX_OK;
 }
@@ -289,69 +304,148 @@ bool aligned_to(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p
     count_launches(1);                                                                                                \
   } while (0)
 
-int forward(const Problem& p, const void* x, const void* W, const long long* targets, float* loss, float* lse, uint8_t* ws,
-            cudaStream_t stream) {
+int prep(int rc) {
+  if (rc != SX_OK) return launch_failed(cudaGetLastError(), "operand preparation launch failed");
+  count_launches(1);
+  return SX_OK;
+}
+#define CE_TRY(call)                  \
+  do {                                \
+    const int rc__ = (call);          \
+    if (rc__ != SX_OK) return rc__;   \
+  } while (0)
+
+// x, or rows [v0, v0 + n) of W, where TMA can read it.
+int readable(bool copy, const void* p, long long rows, long long cols, long long ld, uint8_t* to, cudaStream_t stream, CeMatrix* out) {
+  if (!copy) {
+    *out = CeMatrix{p, rows, cols, ld};
+    return SX_OK;
+  }
+  const long long ldc = up(cols, 8);
+  CE_TRY(prep(launch_repack_16(p, ld, 0, to, ldc, (int)rows, (int)cols, 1, stream)));
+  *out = CeMatrix{to, rows, cols, ldc};
+  return SX_OK;
+}
+
+// fp32: C[M, N] = A B^T + R from operands in {hi, lo} planes, both K contiguous.
+int split_product(const CeCommon& c, const float* A, long long lda, long long plane_a, const float* B, long long ldb, long long plane_b, float* C,
+                  long long ldc, const float* R, long long M, long long N, long long K, cudaStream_t stream) {
+  TcGemmArgs g{};
+  g.M = M; g.N = N; g.K = K;
+  g.batch = 1;
+  g.A = A; g.lda = lda; g.a_plane_stride = plane_a;
+  g.B = B; g.ldb = ldb; g.b_plane_stride = plane_b;
+  g.C = C; g.ldc = ldc; g.c_batch_stride = M * ldc;
+  g.alpha = 1.0f;
+  g.beta = R != nullptr ? 1.0f : 0.0f;
+  g.residual = R;
+  g.status = c.status;
+  g.num_sms = c.num_sms;
+  g.wait_limit_ns = c.wait_limit_ns;
+  // the general product's rule: 128-column tiles where they fill the chip
+  g.bn = N > 64 && ((M + 127) / 128) * ((N + 127) / 128) >= c.num_sms ? 128 : 64;
+  const int rc = launch_gemm_tf32x3(g, stream);
+  if (rc == SX_ERR_EXEC) return launch_failed(cudaGetLastError(), "loss product launch failed");
+  if (rc == SX_OK) count_launches(1);
+  return rc;
+}
+
+int forward(const Problem& p, const CeCommon& dev, const long long* targets, float* loss, float* lse, uint8_t* ws, cudaStream_t stream) {
   const Layout w = layout(p, false);
-  float* logits = reinterpret_cast<float*>(ws + w.logits);
   float2* part = reinterpret_cast<float2*>(ws + w.part);
   float* target_logit = reinterpret_cast<float*>(ws + w.target_logit);
   float* row_loss = p.reduction == SYMPLEX_LOSS_NONE ? loss : reinterpret_cast<float*>(ws + w.row_loss);
-  for (int i = 0; i < w.parts; ++i) {
-    const long long v0 = i * w.piece, n = std::min(w.piece, p.V - v0);
-    const symplex_gemm_desc d = product(p, p.T, n, p.H, true, SYMPLEX_COL_MAJOR, p.ldx, p.ldw, w.ldl);
-    const int rc = symplex_b200_gemm_ws(&d, x, static_cast<const uint8_t*>(W) + (size_t)v0 * p.ldw * p.eb, logits, nullptr, nullptr,
-                                        ws + w.gemm, w.gemm_bytes, stream);
-    if (rc != SX_OK) return rc;
-    CE_LAUNCH(ce_piece_rows_kernel, p.T, 256, (const float*)logits, w.ldl, (int)n, v0, targets, part + i * p.T, target_logit);
+  int parts = w.parts;
+  if (p.bf16) {
+    CeForward f{};
+    CE_TRY(readable(p.copy_x(), p.x, p.T, p.H, p.ldx, ws + w.xcopy, stream, &f.x));
+    CE_TRY(readable(p.copy_w(), p.W, p.V, p.H, p.ldw, ws + w.wcopy, stream, &f.W));
+    f.targets = targets;
+    f.part = part;
+    f.target_logit = target_logit;
+    parts = ce_forward_parts(p.T, p.V, dev.num_sms);
+    CE_TRY(launch_ce_forward(dev, f, stream));
+  } else {
+    float *xs = reinterpret_cast<float*>(ws + w.xs), *wsp = reinterpret_cast<float*>(ws + w.ws), *logits = reinterpret_cast<float*>(ws + w.logits);
+    CE_TRY(prep(launch_split_tf32(static_cast<const float*>(p.x), p.ldx, 0, xs, (int)p.T, (int)p.H, (int)w.hp, 1, stream)));
+    for (int i = 0; i < w.pieces; ++i) {
+      const long long v0 = i * w.piece, n = std::min(w.piece, p.V - v0);
+      CE_TRY(prep(launch_split_tf32(static_cast<const float*>(p.W) + v0 * p.ldw, p.ldw, 0, wsp, (int)n, (int)p.H, (int)w.hp, 1, stream)));
+      CE_TRY(split_product(dev, xs, w.hp, p.T * w.hp, wsp, w.hp, n * w.hp, logits, w.piece, nullptr, p.T, n, p.H, stream));
+      CE_LAUNCH(ce_piece_rows_kernel, p.T, 256, (const float*)logits, w.piece, (int)n, v0, targets, part + i * p.T, target_logit);
+    }
   }
-  CE_LAUNCH(ce_finish_kernel, (p.T + 7) / 8, 256, (const float2*)part, w.parts, (const float*)target_logit, targets, row_loss, lse, p.T, p.V,
+  CE_LAUNCH(ce_finish_kernel, (p.T + 7) / 8, 256, (const float2*)part, parts, (const float*)target_logit, targets, row_loss, lse, p.T, p.V,
             p.ignore);
   if (p.reduction != SYMPLEX_LOSS_NONE)
     CE_LAUNCH(ce_reduce_kernel, 1, 1024, (const float*)row_loss, targets, loss, p.T, p.ignore, p.reduction == SYMPLEX_LOSS_MEAN ? 1 : 0);
   return SX_OK;
 }
 
-int backward(const Problem& p, const float* dloss, const void* x, const void* W, const long long* targets, const float* lse, void* dx,
-             void* dW, uint8_t* ws, int num_sms, cudaStream_t stream) {
+int backward(const Problem& p, const CeCommon& dev, const float* dloss, const long long* targets, const float* lse, void* dx, void* dW,
+             uint8_t* ws, cudaStream_t stream) {
   const Layout w = layout(p, true);
-  float* logits = reinterpret_cast<float*>(ws + w.logits);
-  float* inv_count = nullptr;
-  if (p.reduction == SYMPLEX_LOSS_MEAN) {
-    inv_count = reinterpret_cast<float*>(ws + w.inv_count);
-    CE_LAUNCH(ce_count_kernel, 1, 1024, targets, inv_count, p.T, p.ignore);
+  const bool per_row = p.reduction == SYMPLEX_LOSS_NONE;
+  float* scale = nullptr;
+  if (!per_row) {
+    scale = reinterpret_cast<float*>(ws + w.scale);
+    CE_LAUNCH(ce_scale_kernel, 1, 1024, targets, dloss, scale, p.T, p.ignore, p.reduction == SYMPLEX_LOSS_MEAN ? 1 : 0);
   }
-  const int per_row = p.reduction == SYMPLEX_LOSS_NONE ? 1 : 0;
-  float* acc[2] = {reinterpret_cast<float*>(ws + w.acc[0]), reinterpret_cast<float*>(ws + w.acc[1])};
-  for (int i = 0; i < w.parts; ++i) {
+  if (p.bf16) {
+    CeMatrix x;
+    CE_TRY(readable(p.copy_x(), p.x, p.T, p.H, p.ldx, ws + w.xcopy, stream, &x));
+    float* acc = reinterpret_cast<float*>(ws + w.acc[0]);
+    for (int i = 0; i < w.pieces; ++i) {
+      const long long v0 = i * w.piece, n = std::min(w.piece, p.V - v0);
+      CeMatrix Wp;
+      CE_TRY(readable(p.copy_w(), static_cast<const uint8_t*>(p.W) + (size_t)v0 * p.ldw * 2, n, p.H, p.ldw, ws + w.wcopy, stream, &Wp));
+      CeGrad g{};
+      g.x = x;
+      g.W = Wp;
+      g.G = ws + w.G;
+      g.ldg = w.piece;
+      g.targets = targets;
+      g.lse = lse;
+      g.dloss = per_row ? dloss : nullptr;
+      g.v0 = v0;
+      g.V = p.V;
+      g.ignore = p.ignore;
+      CE_TRY(launch_ce_grad(dev, g, stream));
+      // One factor for all rows is left out of G, where rounding it would move every large entry (the targets', close to
+      // -factor) the same way, and multiplied into the results' fp32 sums instead.
+      CeProducts d{};
+      d.G = CeMatrix{ws + w.G, p.T, n, w.piece};
+      d.x = x;
+      d.W = Wp;
+      d.acc_in = i > 0 ? acc : nullptr;
+      d.acc_out = i < w.pieces - 1 ? acc : nullptr;
+      d.dx = dx;
+      d.dW = static_cast<uint8_t*>(dW) + (size_t)v0 * p.H * 2;
+      d.scale = scale;
+      CE_TRY(launch_ce_products(dev, d, stream));
+    }
+    return SX_OK;
+  }
+  auto at = [&](size_t off) { return reinterpret_cast<float*>(ws + off); };
+  float *xs = at(w.xs), *xts = at(w.xts), *wsp = at(w.ws), *wts = at(w.wts), *logits = at(w.logits), *G = at(w.G), *GT = at(w.GT);
+  float* acc[2] = {at(w.acc[0]), at(w.acc[1])};
+  const float* x = static_cast<const float*>(p.x);
+  CE_TRY(prep(launch_split_tf32(x, p.ldx, 0, xs, (int)p.T, (int)p.H, (int)w.hp, 1, stream)));
+  CE_TRY(prep(launch_split_tf32_transpose(x, p.ldx, 0, xts, (int)p.T, (int)p.H, (int)w.tp, 1, stream)));
+  for (int i = 0; i < w.pieces; ++i) {
     const long long v0 = i * w.piece, n = std::min(w.piece, p.V - v0);
-    const uint8_t* Wp = static_cast<const uint8_t*>(W) + (size_t)v0 * p.ldw * p.eb;
-    symplex_gemm_desc d = product(p, p.T, n, p.H, true, SYMPLEX_COL_MAJOR, p.ldx, p.ldw, w.ldl);
-    int rc = symplex_b200_gemm_ws(&d, x, Wp, logits, nullptr, nullptr, ws + w.gemm, w.gemm_bytes, stream);
-    if (rc != SX_OK) return rc;
+    const float* Wp = static_cast<const float*>(p.W) + v0 * p.ldw;
+    CE_TRY(prep(launch_split_tf32(Wp, p.ldw, 0, wsp, (int)n, (int)p.H, (int)w.hp, 1, stream)));
+    CE_TRY(prep(launch_split_tf32_transpose(Wp, p.ldw, 0, wts, (int)n, (int)p.H, (int)w.piece, 1, stream)));
+    CE_TRY(split_product(dev, xs, w.hp, p.T * w.hp, wsp, w.hp, n * w.hp, logits, w.piece, nullptr, p.T, n, p.H, stream));
     const long long tiles = (p.T + 31) / 32 * ((n + 31) / 32);
-    const unsigned grid = (unsigned)std::min<long long>(tiles, num_sms * 8LL);
-    if (p.bf16)
-      CE_LAUNCH(ce_piece_grad_kernel<__nv_bfloat16>, grid, 256, (const float*)logits, w.ldl, (int)n, v0, targets, lse, dloss, per_row,
-                (const float*)inv_count, reinterpret_cast<__nv_bfloat16*>(ws + w.G), w.ldl, reinterpret_cast<__nv_bfloat16*>(ws + w.GT),
-                w.ldt, p.T, p.V, p.ignore);
-    else
-      CE_LAUNCH(ce_piece_grad_kernel<float>, grid, 256, (const float*)logits, w.ldl, (int)n, v0, targets, lse, dloss, per_row,
-                (const float*)inv_count, reinterpret_cast<float*>(ws + w.G), w.ldl, reinterpret_cast<float*>(ws + w.GT), w.ldt, p.T,
-                p.V, p.ignore);
-    // dx: pieces add up in 32 bits, from one accumulator into the other; fp32 ends in dx itself
-    d = product(p, p.T, p.H, n, true, SYMPLEX_ROW_MAJOR, w.ldl, p.ldw, p.H);
-    d.beta = i ? 1.0f : 0.0f;
-    float* to = !p.bf16 && i == w.parts - 1 ? static_cast<float*>(dx) : acc[i & 1];
-    rc = symplex_b200_gemm_ws(&d, ws + w.G, Wp, to, nullptr, i ? acc[(i & 1) ^ 1] : nullptr, ws + w.gemm, w.gemm_bytes, stream);
-    if (rc != SX_OK) return rc;
-    d = product(p, n, p.H, p.T, false, SYMPLEX_ROW_MAJOR, w.ldt, p.ldx, p.H);
-    rc = symplex_b200_gemm_ws(&d, ws + w.GT, x, static_cast<uint8_t*>(dW) + (size_t)v0 * p.H * p.eb, nullptr, nullptr, ws + w.gemm,
-                              w.gemm_bytes, stream);
-    if (rc != SX_OK) return rc;
+    CE_LAUNCH(ce_piece_grad_kernel, std::min<long long>(tiles, dev.num_sms * 8LL), 256, (const float*)logits, w.piece, (int)n, v0, targets, lse,
+              dloss, (const float*)scale, G, w.piece, p.T * w.piece, GT, w.tp, n * w.tp, p.T, p.V, p.ignore);
+    // dx: pieces add up in 32 bits, from one accumulator into the other and at last into dx
+    float* to = i == w.pieces - 1 ? static_cast<float*>(dx) : acc[i & 1];
+    CE_TRY(split_product(dev, G, w.piece, p.T * w.piece, wts, w.piece, p.H * w.piece, to, p.H, i ? acc[(i & 1) ^ 1] : nullptr, p.T, p.H, n, stream));
+    CE_TRY(split_product(dev, GT, w.tp, n * w.tp, xts, w.tp, p.H * w.tp, static_cast<float*>(dW) + v0 * p.H, p.H, nullptr, n, p.H, p.T, stream));
   }
-  if (p.bf16)
-    CE_LAUNCH(ce_round_kernel, std::min<long long>((p.T * p.H + 255) / 256, num_sms * 16LL), 256, (const float*)acc[(w.parts - 1) & 1],
-              static_cast<__nv_bfloat16*>(dx), p.T * p.H);
   return SX_OK;
 }
 
@@ -362,9 +456,10 @@ using namespace sx;
 
 extern "C" {
 
-size_t symplex_b200_linear_cross_entropy_workspace_bytes(int64_t T, int64_t H, int64_t V, int32_t dtype) {
+size_t symplex_b200_linear_cross_entropy_workspace_bytes(const void* x, const void* W, int64_t T, int64_t H, int64_t V, int64_t ldx,
+                                                         int64_t ldw, int32_t dtype) {
   Problem p;
-  if (check(&p, T, H, V, 0, 0, dtype, 0, 0) != SX_OK || T == 0) return 0;
+  if (check(&p, x, W, T, H, V, ldx, ldw, dtype, 0, 0) != SX_OK || T == 0) return 0;
   return layout(p, false).total;
 }
 
@@ -373,16 +468,17 @@ int symplex_b200_linear_cross_entropy(const void* x, const void* W, const int64_
                                       int64_t ignore_index, int32_t reduction, void* workspace, size_t workspace_bytes,
                                       void* stream) {
   Problem p;
-  int rc = check(&p, T, H, V, ldx, ldw, dtype, ignore_index, reduction);
+  int rc = check(&p, x, W, T, H, V, ldx, ldw, dtype, ignore_index, reduction);
   if (rc != SX_OK) return rc;
   if (T == 0 && reduction == SYMPLEX_LOSS_NONE) return SX_OK;
   if (loss == nullptr || (T > 0 && (x == nullptr || W == nullptr || targets == nullptr || lse == nullptr)))
     return fail_fmt(SX_ERR_INVALID, "null pointer");
   if (!aligned_to(x, p.eb) || !aligned_to(W, p.eb) || !aligned_to(targets, 8) || !aligned_to(loss, 4) || !aligned_to(lse, 4))
     return fail_fmt(SX_ERR_INVALID, "a pointer is not aligned to its element type");
-  if ((rc = check_workspace(symplex_b200_linear_cross_entropy_workspace_bytes(T, H, V, dtype), workspace, workspace_bytes)) != SX_OK) return rc;
-  DeviceInfo dev;
-  if ((rc = current_device(&dev)) != SX_OK) return rc;
+  if ((rc = check_workspace(symplex_b200_linear_cross_entropy_workspace_bytes(x, W, T, H, V, ldx, ldw, dtype), workspace, workspace_bytes)) != SX_OK) return rc;
+  DeviceInfo info;
+  if ((rc = current_device(&info)) != SX_OK) return rc;
+  const CeCommon dev{info.num_sms, info.status, wait_limit_ns_option()};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const long long* tg = reinterpret_cast<const long long*>(targets);
   if (T == 0) {
@@ -390,12 +486,13 @@ int symplex_b200_linear_cross_entropy(const void* x, const void* W, const int64_
     CE_LAUNCH(ce_reduce_kernel, 1, 1024, (const float*)nullptr, tg, loss, 0LL, (long long)ignore_index, reduction == SYMPLEX_LOSS_MEAN ? 1 : 0);
     return SX_OK;
   }
-  return forward(p, x, W, tg, loss, lse, static_cast<uint8_t*>(workspace), st);
+  return forward(p, dev, tg, loss, lse, static_cast<uint8_t*>(workspace), st);
 }
 
-size_t symplex_b200_linear_cross_entropy_backward_workspace_bytes(int64_t T, int64_t H, int64_t V, int32_t dtype) {
+size_t symplex_b200_linear_cross_entropy_backward_workspace_bytes(const void* x, const void* W, int64_t T, int64_t H, int64_t V,
+                                                                  int64_t ldx, int64_t ldw, int32_t dtype) {
   Problem p;
-  if (check(&p, T, H, V, 0, 0, dtype, 0, 0) != SX_OK || T == 0) return 0;
+  if (check(&p, x, W, T, H, V, ldx, ldw, dtype, 0, 0) != SX_OK || T == 0) return 0;
   return layout(p, true).total;
 }
 
@@ -404,23 +501,24 @@ int symplex_b200_linear_cross_entropy_backward(const float* dloss, const void* x
                                                int64_t ldx, int64_t ldw, int32_t dtype, int64_t ignore_index,
                                                int32_t reduction, void* workspace, size_t workspace_bytes, void* stream) {
   Problem p;
-  int rc = check(&p, T, H, V, ldx, ldw, dtype, ignore_index, reduction);
+  int rc = check(&p, x, W, T, H, V, ldx, ldw, dtype, ignore_index, reduction);
   if (rc != SX_OK) return rc;
   if (dW == nullptr || (T > 0 && (dloss == nullptr || x == nullptr || W == nullptr || targets == nullptr || lse == nullptr || dx == nullptr)))
     return fail_fmt(SX_ERR_INVALID, "null pointer");
   if (!aligned_to(x, p.eb) || !aligned_to(W, p.eb) || !aligned_to(targets, 8) || !aligned_to(dloss, 4) || !aligned_to(lse, 4) ||
       !aligned_to(dx, p.eb) || !aligned_to(dW, p.eb))
     return fail_fmt(SX_ERR_INVALID, "a pointer is not aligned to its element type");
-  if ((rc = check_workspace(symplex_b200_linear_cross_entropy_backward_workspace_bytes(T, H, V, dtype), workspace, workspace_bytes)) != SX_OK)
+  if ((rc = check_workspace(symplex_b200_linear_cross_entropy_backward_workspace_bytes(x, W, T, H, V, ldx, ldw, dtype), workspace, workspace_bytes)) != SX_OK)
     return rc;
-  DeviceInfo dev;
-  if ((rc = current_device(&dev)) != SX_OK) return rc;
+  DeviceInfo info;
+  if ((rc = current_device(&info)) != SX_OK) return rc;
+  const CeCommon dev{info.num_sms, info.status, wait_limit_ns_option()};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (T == 0) {
     const cudaError_t e = cudaMemsetAsync(dW, 0, (size_t)V * H * p.eb, st);
     return e == cudaSuccess ? SX_OK : launch_failed(e, "cudaMemsetAsync");
   }
-  return backward(p, dloss, x, W, reinterpret_cast<const long long*>(targets), lse, dx, dW, static_cast<uint8_t*>(workspace), dev.num_sms, st);
+  return backward(p, dev, dloss, reinterpret_cast<const long long*>(targets), lse, dx, dW, static_cast<uint8_t*>(workspace), st);
 }
 
 }  // extern "C"

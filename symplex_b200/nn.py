@@ -172,7 +172,7 @@ def linear_cross_entropy(x, weight, targets, *, ignore_index=-100, reduction="me
         v = weight.shape[0]
         loss = torch.empty(t if reduction == "none" else (), dtype=torch.float32, device=x.device)
         lse = torch.empty(t, dtype=torch.float32, device=x.device)
-        size = lib.symplex_b200_linear_cross_entropy_workspace_bytes(t, h, v, _DT[x.dtype])
+        size = lib.symplex_b200_linear_cross_entropy_workspace_bytes(xr.data_ptr(), w.data_ptr(), t, h, v, ldx, ldw, _DT[x.dtype])
         ws = torch.empty(size, dtype=torch.uint8, device=x.device)
         tg = targets.contiguous()
         _capi.check(lib.symplex_b200_linear_cross_entropy(
@@ -204,7 +204,7 @@ def linear_cross_entropy_backward(dloss, x, weight, targets, lse, *, ignore_inde
         (xr, ldx), (w, ldw) = _rows(x), _rows(weight)
         dx = torch.empty(t, h, dtype=x.dtype, device=x.device)
         dw = torch.empty(v, h, dtype=x.dtype, device=x.device)
-        size = lib.symplex_b200_linear_cross_entropy_backward_workspace_bytes(t, h, v, _DT[x.dtype])
+        size = lib.symplex_b200_linear_cross_entropy_backward_workspace_bytes(xr.data_ptr(), w.data_ptr(), t, h, v, ldx, ldw, _DT[x.dtype])
         ws = torch.empty(size, dtype=torch.uint8, device=x.device)
         tg, ls, dl = targets.contiguous(), lse.contiguous(), dloss.contiguous()
         _capi.check(lib.symplex_b200_linear_cross_entropy_backward(

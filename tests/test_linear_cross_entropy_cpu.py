@@ -48,12 +48,19 @@ def test_refuses_its_own_pointers(lib):
 
 def test_workspace_bytes(lib):
     f, b = lib.symplex_b200_linear_cross_entropy_workspace_bytes, lib.symplex_b200_linear_cross_entropy_backward_workspace_bytes
-    for w in (f, b):
+    for fn in (f, b):
+        def w(T, H, V, dt, x=256, W=512, ldx=0, ldw=0):
+            return fn(x, W, T, H, V, ldx, ldw, dt)
         assert w(0, 64, 100, BF16) == 0 and w(4, 0, 100, BF16) == 0 and w(4, 64, 0, BF16) == 0 and w(4, 64, 100, 3) == 0
         for dt in (BF16, F32):
             assert w(1, 64, 100, dt) > 0
             # the logits of the whole problem never fit in it
             assert w(8192, 4096, 1 << 17, dt) < 8192 * (1 << 17) * 4
+        # operands that are copied first need room for it
+        aligned = w(100, 64, 1000, BF16)
+        for bad in (dict(x=258), dict(ldx=65), dict(W=520), dict(ldw=68)):
+            assert w(100, 64, 1000, BF16, **bad) > aligned
+        assert w(100, 64, 1000, BF16, ldx=72, ldw=128) == aligned
 
 
 @pytest.mark.skipif(torch.cuda.is_available(), reason="needs a box without a GPU")
