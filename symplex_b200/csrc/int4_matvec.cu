@@ -2,7 +2,15 @@
 //
 //   C[m][n] = act(sum_g scale[n][g] * sum_{k in g} (code[n][k] - zero[n][g]) * A[m][k] + bias[n])
 //
-// Bound by HBM: N K / 2 bytes of codes, read once whatever M is, up to about a hundred rows.
+// Bound by HBM: N K / 2 bytes of codes, read once for every 16 rows of A.
+//
+// int4_mma_kernel: the rows of W are the M side of mma.sync m16n8k16, the rows of A (up to 8 per fragment) its N side. A code
+// becomes bf16 exactly - four masked bits under the exponent of 128 read 128 + code, minus (128 + zero) - so the products are
+// exact and each group's sum is scaled once, in fp32. Which k a fragment slot stands for is free as long as both operands agree:
+// a lane takes 8 consecutive k of its row (one 32-bit word), whose nibbles j and j + 4 fall into the halves of one register
+// (pairs (k0,k4), (k1,k5), ...), and the same pairs of A are put together with byte permutes. No shuffle, no shared memory on
+// the way in. 4-bit products are far below what even the warp-level tensor path delivers, so the tcgen05 path has nothing to
+// add here: what has to be fast is the dequantisation, 11 instructions for 8 codes.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -34,11 +42,264 @@ struct Int4Args {
   const uint8_t* zeros;
   const float* bias;
   void* C;
-  int M, N, K, group, groups;
+  int M, N, K, group, groups, group_log2;  // group_log2: -1 where group is no power of two
   long long lda, ldq, ldc;
   int act;
 };
 
+// ------------------------------------------------------------------ fast path
+constexpr int MV_WARPS = 8;
+constexpr int MV_TILE = 32;  // rows of W per warp: two m16 tiles share every fragment of A
+constexpr int MV_K = 128;    // k of one step
+constexpr int MV_AHEAD = 2;  // steps in flight per warp: 2 KB of codes each, and 16 warps an SM
+
+__device__ __forceinline__ uint32_t ldg_stream_32(const void* p) {
+  uint32_t v;
+  asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint2 ldg_stream_64(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint4 ldg_stream_128(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+// Eight codes -> four registers (k0,k4), (k1,k5), (k2,k6), (k3,k7) of code - zero; zero2 = (128 + zero) twice.
+__device__ __forceinline__ void dequant8(uint32_t w, uint32_t zero2, uint32_t (&out)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) out[j] = sub_bf16x2(((w >> (4 * j)) & 0x000f000fu) | 0x43004300u, zero2);
+}
+
+// What a warp holds of one step of 128 k for its 32 rows: per row slot (g, g + 8, g + 16, g + 24) four words of codes and the
+// scales (and zeros) of the step's groups, packed as they lie in memory. kGW = 128, 64 or 32 is how many k share a scale within
+// a step: a lane's words are laid out so that the four lanes of a row stay inside one group for every pair of MMAs.
+template <int kGW, typename ST, bool kZeros>
+struct MvStep {
+  static constexpr int GROUPS = MV_K / kGW;
+  static constexpr int SCALE_WORDS = (GROUPS * int(sizeof(ST)) + 3) / 4;
+  uint32_t c[4][4];
+  uint32_t s[4][SCALE_WORDS];
+  uint32_t z[4];
+
+  __device__ __forceinline__ float scale(int r, int j) const {
+    if constexpr (sizeof(ST) == 4) return __uint_as_float(s[r][j]);
+    return __uint_as_float(j & 1 ? s[r][j / 2] & 0xffff0000u : s[r][j / 2] << 16);  // bf16: the high half of a float
+  }
+  // 128 + zero, twice, in bf16
+  __device__ __forceinline__ uint32_t zero2(int r, int j) const {
+    if constexpr (!kZeros) return 0x43084308u;
+    return 0x43004300u | (((z[r] >> (8 * j)) & 0xffu) * 0x00010001u);
+  }
+
+  // k0: first k of the step, t: lane in the quad. Everything past K reads as nothing: codes 0 and, later, A 0. s_vec: the step's
+  // groups are GROUPS whole scales in a row, aligned.
+  __device__ __forceinline__ void load(const Int4Args& p, const uint8_t* const (&row)[4], const long long (&srow)[4], int k0, int t, int s_vec) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if constexpr (kGW == 128) {
+        const int k = k0 + 32 * t;
+        const uint4 v = k < p.K ? ldg_stream_128(row[r] + (k >> 1)) : make_uint4(0, 0, 0, 0);
+        c[r][0] = v.x; c[r][1] = v.y; c[r][2] = v.z; c[r][3] = v.w;
+      } else if constexpr (kGW == 64) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int k = k0 + 64 * h + 16 * t;
+          const uint2 v = k < p.K ? ldg_stream_64(row[r] + (k >> 1)) : make_uint2(0, 0);
+          c[r][2 * h] = v.x; c[r][2 * h + 1] = v.y;
+        }
+      } else {
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const int k = k0 + 32 * h + 8 * t;
+          c[r][h] = k < p.K ? ldg_stream_32(row[r] + (k >> 1)) : 0u;
+        }
+      }
+    }
+    const ST* scales = static_cast<const ST*>(p.scales);
+    if (GROUPS > 1 && s_vec) {
+      const int g = k0 / kGW;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if constexpr (SCALE_WORDS == 1) {
+          s[r][0] = __ldg(reinterpret_cast<const uint32_t*>(scales + srow[r] + g));
+        } else if constexpr (SCALE_WORDS == 2) {
+          const uint2 v = __ldg(reinterpret_cast<const uint2*>(scales + srow[r] + g));
+          s[r][0] = v.x; s[r][1] = v.y;
+        } else {
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(scales + srow[r] + g));
+          s[r][0] = v.x; s[r][1] = v.y; s[r][2] = v.z; s[r][3] = v.w;
+        }
+        if constexpr (kZeros && GROUPS == 2) z[r] = __ldg(reinterpret_cast<const uint16_t*>(p.zeros + srow[r] + g));
+        if constexpr (kZeros && GROUPS == 4) z[r] = __ldg(reinterpret_cast<const uint32_t*>(p.zeros + srow[r] + g));
+      }
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < GROUPS; ++j) {
+      const int k = min(k0 + j * kGW, p.K - 1);
+      const int g = p.group_log2 >= 0 ? k >> p.group_log2 : k / p.group;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if constexpr (sizeof(ST) == 4) {
+          s[r][j] = __ldg(reinterpret_cast<const uint32_t*>(scales) + srow[r] + g);
+        } else {
+          const uint32_t v = __ldg(reinterpret_cast<const uint16_t*>(scales) + srow[r] + g);
+          s[r][j / 2] = j & 1 ? s[r][j / 2] | (v << 16) : v;
+        }
+        if constexpr (kZeros) {
+          const uint32_t v = __ldg(p.zeros + srow[r] + g);
+          z[r] = j ? z[r] | (v << (8 * j)) : v;
+        }
+      }
+    }
+  }
+};
+
+template <int kGW, int kNB, typename ST, bool kZeros>
+__global__ void __launch_bounds__(MV_WARPS * 32, 2)
+int4_mma_kernel(const Int4Args p, int kw_log2, int out_bf16, int a_vec, int s_vec) {
+  using Step = MvStep<kGW, ST, kZeros>;
+  constexpr int WPG = kGW / 32;  // words of a lane per group of a step
+  __shared__ float red[MV_WARPS][MV_TILE][8 * kNB + 1];
+  pdl_launch_dependents();
+  pdl_wait_prior_grids();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int kw = 1 << kw_log2;             // warps that share a row tile, each with every kw-th step
+  const int my_k = warp & (kw - 1), my_r = warp >> kw_log2;
+  const int rows_cta = (MV_WARPS >> kw_log2) * MV_TILE;
+  const long long n0 = (long long)blockIdx.x * rows_cta + my_r * MV_TILE;
+  const int m0 = blockIdx.y * (8 * kNB);
+
+  const uint8_t* row[4];
+  long long srow[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const long long n = min(n0 + g + 8 * r, (long long)p.N - 1);  // rows past the end repeat the last one and are not written
+    row[r] = p.codes + n * p.ldq;
+    srow[r] = n * p.groups;
+  }
+  const __nv_bfloat16* arow[kNB];
+  bool a_ok[kNB];
+#pragma unroll
+  for (int b = 0; b < kNB; ++b) {
+    a_ok[b] = m0 + 8 * b + g < p.M;
+    arow[b] = p.A + (long long)(a_ok[b] ? m0 + 8 * b + g : 0) * p.lda;
+  }
+
+  float acc[kNB][2][4] = {};
+  auto compute = [&](const Step& st, int k0) {
+#pragma unroll
+    for (int j = 0; j < Step::GROUPS; ++j) {
+      float part[kNB][2][4] = {};
+      uint32_t zero2[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) zero2[r] = st.zero2(r, j);
+#pragma unroll
+      for (int i = 0; i < WPG; ++i) {
+        const int w = j * WPG + i;
+        const int k = k0 + j * kGW + t * (kGW / 4) + i * 8;
+        uint32_t b[kNB][4];
+#pragma unroll
+        for (int nb = 0; nb < kNB; ++nb) {
+          uint4 x = make_uint4(0, 0, 0, 0);
+          if (a_ok[nb] && k < p.K) {
+            if (a_vec) {
+              x = __ldg(reinterpret_cast<const uint4*>(arow[nb] + k));
+            } else {
+              const uint16_t* a = reinterpret_cast<const uint16_t*>(arow[nb] + k);
+              x.x = a[0] | (uint32_t(a[1]) << 16);
+              x.y = a[2] | (uint32_t(a[3]) << 16);
+              x.z = a[4] | (uint32_t(a[5]) << 16);
+              x.w = a[6] | (uint32_t(a[7]) << 16);
+            }
+          }
+          b[nb][0] = __byte_perm(x.x, x.z, 0x5410);
+          b[nb][1] = __byte_perm(x.x, x.z, 0x7632);
+          b[nb][2] = __byte_perm(x.y, x.w, 0x5410);
+          b[nb][3] = __byte_perm(x.y, x.w, 0x7632);
+        }
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+          uint32_t lo[4], hi[4];  // rows g and g + 8 of this m16 tile
+          dequant8(st.c[2 * mt][w], zero2[2 * mt], lo);
+          dequant8(st.c[2 * mt + 1][w], zero2[2 * mt + 1], hi);
+#pragma unroll
+          for (int nb = 0; nb < kNB; ++nb) {
+            mma_bf16(part[nb][mt], lo[0], hi[0], lo[1], hi[1], b[nb][0], b[nb][1]);
+            mma_bf16(part[nb][mt], lo[2], hi[2], lo[3], hi[3], b[nb][2], b[nb][3]);
+          }
+        }
+      }
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        const float s0 = st.scale(2 * mt, j), s1 = st.scale(2 * mt + 1, j);
+#pragma unroll
+        for (int nb = 0; nb < kNB; ++nb) {
+          // past K the codes and A are 0 but the scale repeats the last group's, which may be anything: 0 * inf must not count
+          if (k0 + j * kGW < p.K) {
+            acc[nb][mt][0] = fmaf(s0, part[nb][mt][0], acc[nb][mt][0]);
+            acc[nb][mt][1] = fmaf(s0, part[nb][mt][1], acc[nb][mt][1]);
+            acc[nb][mt][2] = fmaf(s1, part[nb][mt][2], acc[nb][mt][2]);
+            acc[nb][mt][3] = fmaf(s1, part[nb][mt][3], acc[nb][mt][3]);
+          }
+        }
+      }
+    }
+  };
+
+  const int steps = (p.K + MV_K - 1) / MV_K;
+  Step buf[MV_AHEAD];
+#pragma unroll
+  for (int i = 0; i < MV_AHEAD; ++i)
+    if (my_k + i * kw < steps) buf[i].load(p, row, srow, (my_k + i * kw) * MV_K, t, s_vec);
+  for (int u = my_k; u < steps; u += MV_AHEAD * kw) {
+#pragma unroll
+    for (int i = 0; i < MV_AHEAD; ++i) {
+      const int v = u + i * kw;
+      if (v < steps) {
+        compute(buf[i], v * MV_K);
+        if (v + MV_AHEAD * kw < steps) buf[i].load(p, row, srow, (v + MV_AHEAD * kw) * MV_K, t, s_vec);
+      }
+    }
+  }
+
+#pragma unroll
+  for (int nb = 0; nb < kNB; ++nb)
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) red[warp][16 * mt + g + 8 * (i >> 1)][8 * nb + 2 * t + (i & 1)] = acc[nb][mt][i];
+  __syncthreads();
+  const int cols = min(8 * kNB, p.M - m0);
+  for (int e = threadIdx.x; e < cols * rows_cta; e += MV_WARPS * 32) {
+    const int m = e / rows_cta, r = e - m * rows_cta;
+    const long long n = (long long)blockIdx.x * rows_cta + r;
+    if (n >= p.N) continue;
+    float v = 0.0f;
+    for (int i = 0; i < kw; ++i) v += red[(r / MV_TILE) * kw + i][r % MV_TILE][m];  // a fixed order
+    if (p.bias != nullptr) v += p.bias[n];
+    v = activate(v, p.act);
+    const long long at = (m0 + m) * p.ldc + n;
+    if (out_bf16) static_cast<__nv_bfloat16*>(p.C)[at] = __nv_bfloat16(v);
+    else static_cast<float*>(p.C)[at] = v;
+  }
+}
+
+// ------------------------------------------------------------------ any K, stride and alignment
 constexpr int MV_ROWS = 8;  // rows of A of one warp's accumulators
 
 // One warp per row of W, codes byte by byte: any K, stride and alignment.
@@ -149,9 +410,53 @@ int check_int4(int64_t N, int64_t K, int64_t group, int32_t scale_dtype) {
 bool aligned_to(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 int bytes_of(int32_t dtype) { return dtype == SYMPLEX_DT_F32 ? 4 : 2; }
 
-template <typename ST, typename OutT>
-int matvec(const Int4Args& a, cudaStream_t stream) {
-  cudaError_t e = launch_kernel_ex(int4_matvec_any_kernel<ST, OutT>, (unsigned)((a.N + 7) / 8), 256, 0, stream, 1, pdl_enabled(), a);
+template <int kGW, int kNB, typename ST, bool kZeros>
+int matvec_mma(const Int4Args& a, bool out_bf16, int sms, cudaStream_t stream) {
+  // Warps per row tile: enough warps for the chip's loads in flight (12 a SM with 6 KB each), never more than there are steps.
+  const long long tiles = (a.N + MV_TILE - 1) / MV_TILE;
+  const int steps = (a.K + MV_K - 1) / MV_K;
+  int kw = 0;
+  while (kw < 3 && (2 << kw) <= steps && (tiles << kw) < sms * 12LL) ++kw;
+  const int rows_cta = (MV_WARPS >> kw) * MV_TILE;
+  const int a_vec = a.lda % 8 == 0 && reinterpret_cast<uintptr_t>(a.A) % 16 == 0;
+  constexpr int GROUPS = MV_K / kGW;
+  const int s_vec = a.group == kGW && a.groups % GROUPS == 0 && reinterpret_cast<uintptr_t>(a.scales) % (GROUPS * sizeof(ST)) == 0 &&
+                    reinterpret_cast<uintptr_t>(a.zeros) % GROUPS == 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((a.N + rows_cta - 1) / rows_cta), (unsigned)((a.M + 8 * kNB - 1) / (8 * kNB)), 1);
+  cfg.blockDim = dim3(MV_WARPS * 32, 1, 1);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, int4_mma_kernel<kGW, kNB, ST, kZeros>, a, kw, out_bf16 ? 1 : 0, a_vec, s_vec);
+  if (e != cudaSuccess) return launch_failed(e, "4-bit product launch failed");
+  count_launches(1);
+  return SX_OK;
+}
+
+template <int kGW, typename ST>
+int matvec_gw(const Int4Args& a, bool out_bf16, int sms, cudaStream_t stream) {
+  if (a.M <= 8)
+    return a.zeros ? matvec_mma<kGW, 1, ST, true>(a, out_bf16, sms, stream) : matvec_mma<kGW, 1, ST, false>(a, out_bf16, sms, stream);
+  return a.zeros ? matvec_mma<kGW, 2, ST, true>(a, out_bf16, sms, stream) : matvec_mma<kGW, 2, ST, false>(a, out_bf16, sms, stream);
+}
+
+template <typename ST>
+int matvec(const Int4Args& a, bool out_bf16, int sms, cudaStream_t stream) {
+  // The widest load whose lanes' shares stay inside one group, as far as the rows' alignment allows.
+  const uintptr_t at = reinterpret_cast<uintptr_t>(a.codes) | (uintptr_t)a.ldq;
+  if (a.K % 32 == 0 && at % 4 == 0) {
+    if (a.group % 128 == 0 && at % 16 == 0) return matvec_gw<128, ST>(a, out_bf16, sms, stream);
+    if (a.group % 64 == 0 && at % 8 == 0) return matvec_gw<64, ST>(a, out_bf16, sms, stream);
+    return matvec_gw<32, ST>(a, out_bf16, sms, stream);
+  }
+  const cudaError_t e = out_bf16 ? launch_kernel_ex(int4_matvec_any_kernel<ST, __nv_bfloat16>, (unsigned)((a.N + 7) / 8), 256, 0, stream, 1,
+                                                    pdl_enabled(), a)
+                                 : launch_kernel_ex(int4_matvec_any_kernel<ST, float>, (unsigned)((a.N + 7) / 8), 256, 0, stream, 1,
+                                                    pdl_enabled(), a);
   if (e != cudaSuccess) return launch_failed(e, "4-bit product launch failed");
   count_launches(1);
   return SX_OK;
@@ -193,6 +498,7 @@ int symplex_b200_int4_matvec(const void* A, const uint8_t* codes, const void* sc
   a.M = (int)M; a.N = (int)N; a.K = (int)K;
   a.group = (int)group;
   a.groups = (int)((K + group - 1) / group);
+  a.group_log2 = (group & (group - 1)) == 0 ? __builtin_ctzll((unsigned long long)group) : -1;
   a.lda = lda ? lda : K;
   a.ldq = ldq ? ldq : (K + 1) / 2;
   a.ldc = ldc ? ldc : N;
@@ -211,9 +517,8 @@ int symplex_b200_int4_matvec(const void* A, const uint8_t* codes, const void* sc
   int sms = 0;
   if ((rc = current_device_sms(&sms)) != SX_OK) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (scale_dtype == SYMPLEX_DT_F32)
-    return out_dtype == SYMPLEX_DT_F32 ? matvec<float, float>(a, st) : matvec<float, __nv_bfloat16>(a, st);
-  return out_dtype == SYMPLEX_DT_F32 ? matvec<__nv_bfloat16, float>(a, st) : matvec<__nv_bfloat16, __nv_bfloat16>(a, st);
+  const bool out_bf16 = out_dtype == SYMPLEX_DT_BF16;
+  return scale_dtype == SYMPLEX_DT_F32 ? matvec<float>(a, out_bf16, sms, st) : matvec<__nv_bfloat16>(a, out_bf16, sms, st);
 }
 
 int symplex_b200_int4_quantize(const void* W, uint8_t* codes, void* scales, uint8_t* zeros, int64_t N, int64_t K,
