@@ -52,6 +52,7 @@ constexpr int MV_WARPS = 8;
 constexpr int MV_TILE = 32;  // rows of W per warp: two m16 tiles share every fragment of A
 constexpr int MV_K = 128;    // k of one step
 constexpr int MV_AHEAD = 2;  // steps in flight per warp: 2 KB of codes each, and 16 warps an SM
+constexpr int MV_STAGE_BYTES = 88 * 1024;  // shared memory of a CTA for A, if all of A fits: two CTAs an SM
 
 __device__ __forceinline__ uint32_t ldg_stream_32(const void* p) {
   uint32_t v;
@@ -69,9 +70,14 @@ __device__ __forceinline__ uint4 ldg_stream_128(const void* p) {
   return v;
 }
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
   const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
@@ -101,66 +107,62 @@ struct MvStep {
   // 128 + zero, twice, in bf16
   __device__ __forceinline__ uint32_t zero2(int r, int j) const {
     if constexpr (!kZeros) return 0x43084308u;
-    return 0x43004300u | (((z[r] >> (8 * j)) & 0xffu) * 0x00010001u);
+    return __byte_perm(z[r], 0x00000043u, 0x4040u + 0x0101u * j);
   }
 
-  // k0: first k of the step, t: lane in the quad. Everything past K reads as nothing: codes 0 and, later, A 0. s_vec: the step's
-  // groups are GROUPS whole scales in a row, aligned.
-  __device__ __forceinline__ void load(const Int4Args& p, const uint8_t* const (&row)[4], const long long (&srow)[4], int k0, int t, int s_vec) {
+  // row: this lane's four rows, at the first byte of the lane's share of step 0. k0: first k of the step, t: lane in the quad. Words
+  // past K repeat the row's beginning (A is 0 there). s_vec: the step's groups are GROUPS whole scales in a row, aligned.
+  __device__ __forceinline__ void load(const Int4Args& p, const uint8_t* const (&row)[4], const uint32_t (&srow)[4], int k0, int t, int s_vec) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      if constexpr (kGW == 128) {
-        const int k = k0 + 32 * t;
-        const uint4 v = k < p.K ? ldg_stream_128(row[r] + (k >> 1)) : make_uint4(0, 0, 0, 0);
-        c[r][0] = v.x; c[r][1] = v.y; c[r][2] = v.z; c[r][3] = v.w;
-      } else if constexpr (kGW == 64) {
+    for (int h = 0; h < GROUPS; ++h) {
+      const int k = k0 + h * kGW + t * (kGW / 4);
+      const long long at = k < p.K ? k0 / 2 + h * (kGW / 2) : 0;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int k = k0 + 64 * h + 16 * t;
-          const uint2 v = k < p.K ? ldg_stream_64(row[r] + (k >> 1)) : make_uint2(0, 0);
+      for (int r = 0; r < 4; ++r) {
+        if constexpr (kGW == 128) {
+          const uint4 v = ldg_stream_128(row[r] + at);
+          c[r][0] = v.x; c[r][1] = v.y; c[r][2] = v.z; c[r][3] = v.w;
+        } else if constexpr (kGW == 64) {
+          const uint2 v = ldg_stream_64(row[r] + at);
           c[r][2 * h] = v.x; c[r][2 * h + 1] = v.y;
-        }
-      } else {
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          const int k = k0 + 32 * h + 8 * t;
-          c[r][h] = k < p.K ? ldg_stream_32(row[r] + (k >> 1)) : 0u;
+        } else {
+          c[r][h] = ldg_stream_32(row[r] + at);
         }
       }
     }
     const ST* scales = static_cast<const ST*>(p.scales);
     if (GROUPS > 1 && s_vec) {
-      const int g = k0 / kGW;
+      const uint32_t g = k0 / kGW;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         if constexpr (SCALE_WORDS == 1) {
-          s[r][0] = __ldg(reinterpret_cast<const uint32_t*>(scales + srow[r] + g));
+          s[r][0] = __ldg(reinterpret_cast<const uint32_t*>(scales + (srow[r] + g)));
         } else if constexpr (SCALE_WORDS == 2) {
-          const uint2 v = __ldg(reinterpret_cast<const uint2*>(scales + srow[r] + g));
+          const uint2 v = __ldg(reinterpret_cast<const uint2*>(scales + (srow[r] + g)));
           s[r][0] = v.x; s[r][1] = v.y;
         } else {
-          const uint4 v = __ldg(reinterpret_cast<const uint4*>(scales + srow[r] + g));
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(scales + (srow[r] + g)));
           s[r][0] = v.x; s[r][1] = v.y; s[r][2] = v.z; s[r][3] = v.w;
         }
-        if constexpr (kZeros && GROUPS == 2) z[r] = __ldg(reinterpret_cast<const uint16_t*>(p.zeros + srow[r] + g));
-        if constexpr (kZeros && GROUPS == 4) z[r] = __ldg(reinterpret_cast<const uint32_t*>(p.zeros + srow[r] + g));
+        if constexpr (kZeros && GROUPS == 2) z[r] = __ldg(reinterpret_cast<const uint16_t*>(p.zeros + (srow[r] + g)));
+        if constexpr (kZeros && GROUPS == 4) z[r] = __ldg(reinterpret_cast<const uint32_t*>(p.zeros + (srow[r] + g)));
       }
       return;
     }
 #pragma unroll
     for (int j = 0; j < GROUPS; ++j) {
       const int k = min(k0 + j * kGW, p.K - 1);
-      const int g = p.group_log2 >= 0 ? k >> p.group_log2 : k / p.group;
+      const uint32_t g = p.group_log2 >= 0 ? k >> p.group_log2 : k / p.group;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         if constexpr (sizeof(ST) == 4) {
-          s[r][j] = __ldg(reinterpret_cast<const uint32_t*>(scales) + srow[r] + g);
+          s[r][j] = __ldg(reinterpret_cast<const uint32_t*>(scales) + (srow[r] + g));
         } else {
-          const uint32_t v = __ldg(reinterpret_cast<const uint16_t*>(scales) + srow[r] + g);
+          const uint32_t v = __ldg(reinterpret_cast<const uint16_t*>(scales) + (srow[r] + g));
           s[r][j / 2] = j & 1 ? s[r][j / 2] | (v << 16) : v;
         }
         if constexpr (kZeros) {
-          const uint32_t v = __ldg(p.zeros + srow[r] + g);
+          const uint32_t v = __ldg(p.zeros + (srow[r] + g));
           z[r] = j ? z[r] | (v << (8 * j)) : v;
         }
       }
@@ -168,70 +170,96 @@ struct MvStep {
   }
 };
 
+// A in shared memory: rows of 16-byte blocks of 8 k, each block as the pairs the dequantised words have, (k0,k4) (k1,k5) (k2,k6)
+// (k3,k7); block b of a row stands at b ^ ((b >> 3) & 1), and rows are MvPad blocks longer than their k: the eight lanes of a
+// quarter warp (two rows, four shares of a group) then read eight different bank groups. Row `rows` is zeros, for lanes whose row
+// of A does not exist.
+template <int kGW> constexpr int MvPad = kGW == 128 ? 2 : kGW == 64 ? 1 : 4;
+
+__device__ __forceinline__ void stage_a(const Int4Args& p, uint4* to, int pitch, int m0, int rows, int k0, int kn, int a_vec) {
+  const int blocks = kn >> 3;
+  for (int e = threadIdx.x; e < blocks * (rows + 1); e += MV_WARPS * 32) {
+    const int m = e / blocks, b = e - m * blocks;
+    const int k = k0 + 8 * b;
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (m < rows && k < p.K) {  // K is a multiple of 8: a block is inside or outside
+      const __nv_bfloat16* a = p.A + (m0 + m) * p.lda + k;
+      if (a_vec) {
+        x = __ldg(reinterpret_cast<const uint4*>(a));
+      } else {
+        const uint16_t* u = reinterpret_cast<const uint16_t*>(a);
+        x.x = u[0] | (uint32_t(u[1]) << 16);
+        x.y = u[2] | (uint32_t(u[3]) << 16);
+        x.z = u[4] | (uint32_t(u[5]) << 16);
+        x.w = u[6] | (uint32_t(u[7]) << 16);
+      }
+    }
+    to[m * pitch + (b ^ ((b >> 3) & 1))] = make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632),
+                                                      __byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632));
+  }
+}
+
+struct MvPlan {
+  int kw_log2;      // warps that share a row tile, each with every kw-th step
+  int chunk_steps;  // steps whose A is staged at a time, a multiple of kw * MV_AHEAD; all of them where A fits
+  int pitch;        // 16-byte blocks from one staged row to the next
+  int a_vec, s_vec, out_bf16;
+};
+
 template <int kGW, int kNB, typename ST, bool kZeros>
 __global__ void __launch_bounds__(MV_WARPS * 32, 2)
-int4_mma_kernel(const Int4Args p, int kw_log2, int out_bf16, int a_vec, int s_vec) {
+int4_mma_kernel(const Int4Args p, const MvPlan plan) {
   using Step = MvStep<kGW, ST, kZeros>;
   constexpr int WPG = kGW / 32;  // words of a lane per group of a step
+  extern __shared__ uint4 a_smem[];
   __shared__ float red[MV_WARPS][MV_TILE][8 * kNB + 1];
-  pdl_launch_dependents();
-  pdl_wait_prior_grids();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  const int kw = 1 << kw_log2;             // warps that share a row tile, each with every kw-th step
-  const int my_k = warp & (kw - 1), my_r = warp >> kw_log2;
-  const int rows_cta = (MV_WARPS >> kw_log2) * MV_TILE;
+  const int kw = 1 << plan.kw_log2;
+  const int my_k = warp & (kw - 1), my_r = warp >> plan.kw_log2;
+  const int rows_cta = (MV_WARPS >> plan.kw_log2) * MV_TILE;
   const long long n0 = (long long)blockIdx.x * rows_cta + my_r * MV_TILE;
   const int m0 = blockIdx.y * (8 * kNB);
+  const int m_here = min(8 * kNB, p.M - m0);
 
   const uint8_t* row[4];
-  long long srow[4];
+  uint32_t srow[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const long long n = min(n0 + g + 8 * r, (long long)p.N - 1);  // rows past the end repeat the last one and are not written
-    row[r] = p.codes + n * p.ldq;
-    srow[r] = n * p.groups;
+    row[r] = p.codes + n * p.ldq + t * (kGW / 8);
+    srow[r] = (uint32_t)n * (uint32_t)p.groups;  // checked by the host: N * groups < 2^32
   }
-  const __nv_bfloat16* arow[kNB];
-  bool a_ok[kNB];
+  const int steps = (p.K + MV_K - 1) / MV_K;
+  pdl_launch_dependents();
+  pdl_wait_prior_grids();
+  Step buf[MV_AHEAD];
 #pragma unroll
-  for (int b = 0; b < kNB; ++b) {
-    a_ok[b] = m0 + 8 * b + g < p.M;
-    arow[b] = p.A + (long long)(a_ok[b] ? m0 + 8 * b + g : 0) * p.lda;
-  }
+  for (int i = 0; i < MV_AHEAD; ++i)
+    if (my_k + i * kw < steps) buf[i].load(p, row, srow, (my_k + i * kw) * MV_K, t, plan.s_vec);
 
+  const int buf_blocks = plan.pitch * (m_here + 1);
+  const int chunk_k = plan.chunk_steps * MV_K;
+  stage_a(p, a_smem, plan.pitch, m0, m_here, 0, chunk_k, plan.a_vec);
+  __syncthreads();
+
+  const uint4* arow[kNB];
   float acc[kNB][2][4] = {};
-  auto compute = [&](const Step& st, int k0) {
+  // one step; block: first 16-byte block of the step inside the staged rows (a multiple of 16)
+  auto compute = [&](const Step& st, int k0, int block) {
 #pragma unroll
     for (int j = 0; j < Step::GROUPS; ++j) {
-      float part[kNB][2][4] = {};
+      float part[kNB][2][4];
       uint32_t zero2[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) zero2[r] = st.zero2(r, j);
 #pragma unroll
       for (int i = 0; i < WPG; ++i) {
         const int w = j * WPG + i;
-        const int k = k0 + j * kGW + t * (kGW / 4) + i * 8;
-        uint32_t b[kNB][4];
+        const int b = j * (kGW / 8) + t * (kGW / 32) + i;  // this lane's block of the step
+        uint4 x[kNB];
 #pragma unroll
-        for (int nb = 0; nb < kNB; ++nb) {
-          uint4 x = make_uint4(0, 0, 0, 0);
-          if (a_ok[nb] && k < p.K) {
-            if (a_vec) {
-              x = __ldg(reinterpret_cast<const uint4*>(arow[nb] + k));
-            } else {
-              const uint16_t* a = reinterpret_cast<const uint16_t*>(arow[nb] + k);
-              x.x = a[0] | (uint32_t(a[1]) << 16);
-              x.y = a[2] | (uint32_t(a[3]) << 16);
-              x.z = a[4] | (uint32_t(a[5]) << 16);
-              x.w = a[6] | (uint32_t(a[7]) << 16);
-            }
-          }
-          b[nb][0] = __byte_perm(x.x, x.z, 0x5410);
-          b[nb][1] = __byte_perm(x.x, x.z, 0x7632);
-          b[nb][2] = __byte_perm(x.y, x.w, 0x5410);
-          b[nb][3] = __byte_perm(x.y, x.w, 0x7632);
-        }
+        for (int nb = 0; nb < kNB; ++nb) x[nb] = arow[nb][block + (b ^ ((b >> 3) & 1))];
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
           uint32_t lo[4], hi[4];  // rows g and g + 8 of this m16 tile
@@ -239,18 +267,19 @@ int4_mma_kernel(const Int4Args p, int kw_log2, int out_bf16, int a_vec, int s_ve
           dequant8(st.c[2 * mt + 1][w], zero2[2 * mt + 1], hi);
 #pragma unroll
           for (int nb = 0; nb < kNB; ++nb) {
-            mma_bf16(part[nb][mt], lo[0], hi[0], lo[1], hi[1], b[nb][0], b[nb][1]);
-            mma_bf16(part[nb][mt], lo[2], hi[2], lo[3], hi[3], b[nb][2], b[nb][3]);
+            if (i == 0) mma_bf16_zero(part[nb][mt], lo[0], hi[0], lo[1], hi[1], x[nb].x, x[nb].y);
+            else mma_bf16(part[nb][mt], lo[0], hi[0], lo[1], hi[1], x[nb].x, x[nb].y);
+            mma_bf16(part[nb][mt], lo[2], hi[2], lo[3], hi[3], x[nb].z, x[nb].w);
           }
         }
       }
+      // A group that lies past K whole has sums of 0 and repeats a scale, which may be anything: 0 * inf must not count.
+      if (Step::GROUPS == 1 || k0 + j * kGW < p.K) {
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        const float s0 = st.scale(2 * mt, j), s1 = st.scale(2 * mt + 1, j);
+        for (int mt = 0; mt < 2; ++mt) {
+          const float s0 = st.scale(2 * mt, j), s1 = st.scale(2 * mt + 1, j);
 #pragma unroll
-        for (int nb = 0; nb < kNB; ++nb) {
-          // past K the codes and A are 0 but the scale repeats the last group's, which may be anything: 0 * inf must not count
-          if (k0 + j * kGW < p.K) {
+          for (int nb = 0; nb < kNB; ++nb) {
             acc[nb][mt][0] = fmaf(s0, part[nb][mt][0], acc[nb][mt][0]);
             acc[nb][mt][1] = fmaf(s0, part[nb][mt][1], acc[nb][mt][1]);
             acc[nb][mt][2] = fmaf(s1, part[nb][mt][2], acc[nb][mt][2]);
@@ -261,18 +290,22 @@ int4_mma_kernel(const Int4Args p, int kw_log2, int out_bf16, int a_vec, int s_ve
     }
   };
 
-  const int steps = (p.K + MV_K - 1) / MV_K;
-  Step buf[MV_AHEAD];
+  for (int c = 0, s0 = 0; s0 < steps; ++c, s0 += plan.chunk_steps) {
+    // Behind the barrier chunk c is staged and nobody reads chunk c - 1 any more: its buffer takes chunk c + 1.
+    if (c > 0) __syncthreads();
+    if (s0 + plan.chunk_steps < steps)
+      stage_a(p, a_smem + ((c + 1) & 1) * buf_blocks, plan.pitch, m0, m_here, (s0 + plan.chunk_steps) * MV_K, chunk_k, plan.a_vec);
 #pragma unroll
-  for (int i = 0; i < MV_AHEAD; ++i)
-    if (my_k + i * kw < steps) buf[i].load(p, row, srow, (my_k + i * kw) * MV_K, t, s_vec);
-  for (int u = my_k; u < steps; u += MV_AHEAD * kw) {
+    for (int b = 0; b < kNB; ++b) arow[b] = a_smem + (c & 1) * buf_blocks + min(8 * b + g, m_here) * plan.pitch;
+    const int end = min(s0 + plan.chunk_steps, steps);
+    for (int u = s0 + my_k; u < end; u += MV_AHEAD * kw) {
 #pragma unroll
-    for (int i = 0; i < MV_AHEAD; ++i) {
-      const int v = u + i * kw;
-      if (v < steps) {
-        compute(buf[i], v * MV_K);
-        if (v + MV_AHEAD * kw < steps) buf[i].load(p, row, srow, (v + MV_AHEAD * kw) * MV_K, t, s_vec);
+      for (int i = 0; i < MV_AHEAD; ++i) {
+        const int v = u + i * kw;
+        if (v < end) {
+          compute(buf[i], v * MV_K, (v - s0) * (MV_K / 8));
+          if (v + MV_AHEAD * kw < steps) buf[i].load(p, row, srow, (v + MV_AHEAD * kw) * MV_K, t, plan.s_vec);
+        }
       }
     }
   }
@@ -284,8 +317,7 @@ int4_mma_kernel(const Int4Args p, int kw_log2, int out_bf16, int a_vec, int s_ve
 #pragma unroll
       for (int i = 0; i < 4; ++i) red[warp][16 * mt + g + 8 * (i >> 1)][8 * nb + 2 * t + (i & 1)] = acc[nb][mt][i];
   __syncthreads();
-  const int cols = min(8 * kNB, p.M - m0);
-  for (int e = threadIdx.x; e < cols * rows_cta; e += MV_WARPS * 32) {
+  for (int e = threadIdx.x; e < m_here * rows_cta; e += MV_WARPS * 32) {
     const int m = e / rows_cta, r = e - m * rows_cta;
     const long long n = (long long)blockIdx.x * rows_cta + r;
     if (n >= p.N) continue;
@@ -294,7 +326,7 @@ int4_mma_kernel(const Int4Args p, int kw_log2, int out_bf16, int a_vec, int s_ve
     if (p.bias != nullptr) v += p.bias[n];
     v = activate(v, p.act);
     const long long at = (m0 + m) * p.ldc + n;
-    if (out_bf16) static_cast<__nv_bfloat16*>(p.C)[at] = __nv_bfloat16(v);
+    if (plan.out_bf16) static_cast<__nv_bfloat16*>(p.C)[at] = __nv_bfloat16(v);
     else static_cast<float*>(p.C)[at] = v;
   }
 }
@@ -412,26 +444,40 @@ int bytes_of(int32_t dtype) { return dtype == SYMPLEX_DT_F32 ? 4 : 2; }
 
 template <int kGW, int kNB, typename ST, bool kZeros>
 int matvec_mma(const Int4Args& a, bool out_bf16, int sms, cudaStream_t stream) {
-  // Warps per row tile: enough warps for the chip's loads in flight (12 a SM with 6 KB each), never more than there are steps.
+  auto kern = int4_mma_kernel<kGW, kNB, ST, kZeros>;
+  constexpr int GROUPS = MV_K / kGW;
+  MvPlan plan{};
+  // Warps per row tile: enough warps for the chip's loads in flight (12 a SM), never more than there are steps.
   const long long tiles = (a.N + MV_TILE - 1) / MV_TILE;
   const int steps = (a.K + MV_K - 1) / MV_K;
-  int kw = 0;
-  while (kw < 3 && (2 << kw) <= steps && (tiles << kw) < sms * 12LL) ++kw;
-  const int rows_cta = (MV_WARPS >> kw) * MV_TILE;
-  const int a_vec = a.lda % 8 == 0 && reinterpret_cast<uintptr_t>(a.A) % 16 == 0;
-  constexpr int GROUPS = MV_K / kGW;
-  const int s_vec = a.group == kGW && a.groups % GROUPS == 0 && reinterpret_cast<uintptr_t>(a.scales) % (GROUPS * sizeof(ST)) == 0 &&
-                    reinterpret_cast<uintptr_t>(a.zeros) % GROUPS == 0;
+  while (plan.kw_log2 < 3 && (2 << plan.kw_log2) <= steps && (tiles << plan.kw_log2) < sms * 12LL) ++plan.kw_log2;
+  const int round = MV_AHEAD << plan.kw_log2;
+  const int rows = std::min(a.M, 8 * kNB) + 1;
+  auto bytes = [&](int n) { return (size_t)rows * (n * (MV_K / 8) + MvPad<kGW>) * 16; };
+  plan.chunk_steps = (steps + round - 1) / round * round;
+  size_t smem = bytes(plan.chunk_steps);
+  if (smem > MV_STAGE_BYTES) {  // in chunks of 8 steps (16 where 8 warps share a tile), two buffers
+    plan.chunk_steps = std::max(8, round);
+    smem = 2 * bytes(plan.chunk_steps);
+  }
+  plan.pitch = plan.chunk_steps * (MV_K / 8) + MvPad<kGW>;
+  plan.a_vec = a.lda % 8 == 0 && reinterpret_cast<uintptr_t>(a.A) % 16 == 0;
+  plan.s_vec = a.group == kGW && a.groups % GROUPS == 0 && reinterpret_cast<uintptr_t>(a.scales) % (GROUPS * sizeof(ST)) == 0 &&
+               reinterpret_cast<uintptr_t>(a.zeros) % GROUPS == 0;
+  plan.out_bf16 = out_bf16 ? 1 : 0;
+  SX_ENSURE_DYN_SMEM(kern, 160 * 1024);
+  const int rows_cta = (MV_WARPS >> plan.kw_log2) * MV_TILE;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((a.N + rows_cta - 1) / rows_cta), (unsigned)((a.M + 8 * kNB - 1) / (8 * kNB)), 1);
   cfg.blockDim = dim3(MV_WARPS * 32, 1, 1);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, int4_mma_kernel<kGW, kNB, ST, kZeros>, a, kw, out_bf16 ? 1 : 0, a_vec, s_vec);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a, plan);
   if (e != cudaSuccess) return launch_failed(e, "4-bit product launch failed");
   count_launches(1);
   return SX_OK;
@@ -448,7 +494,7 @@ template <typename ST>
 int matvec(const Int4Args& a, bool out_bf16, int sms, cudaStream_t stream) {
   // The widest load whose lanes' shares stay inside one group, as far as the rows' alignment allows.
   const uintptr_t at = reinterpret_cast<uintptr_t>(a.codes) | (uintptr_t)a.ldq;
-  if (a.K % 32 == 0 && at % 4 == 0) {
+  if (a.K % 32 == 0 && at % 4 == 0 && (long long)a.N * a.groups < (1ll << 32)) {
     if (a.group % 128 == 0 && at % 16 == 0) return matvec_gw<128, ST>(a, out_bf16, sms, stream);
     if (a.group % 64 == 0 && at % 8 == 0) return matvec_gw<64, ST>(a, out_bf16, sms, stream);
     return matvec_gw<32, ST>(a, out_bf16, sms, stream);
