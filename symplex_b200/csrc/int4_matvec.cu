@@ -48,26 +48,28 @@ struct Int4Args {
 };
 
 // ------------------------------------------------------------------ fast path
-constexpr int MV_WARPS = 8;
-constexpr int MV_TILE = 32;  // rows of W per warp: two m16 tiles share every fragment of A
+constexpr int MV_WARPS = 16;
+constexpr int MV_TILE = 32;  // rows of W per tile: two m16 tiles share every fragment of A
 constexpr int MV_K = 128;    // k of one step
-constexpr int MV_AHEAD = 2;  // steps in flight per warp: 2 KB of codes each, and 16 warps an SM
-constexpr int MV_STAGE_BYTES = 88 * 1024;  // shared memory of a CTA for A, if all of A fits: two CTAs an SM
+constexpr int MV_RING = 3;   // steps of codes in flight per warp, 2 KB each: 96 KB an SM
+constexpr int MV_STEP_BYTES = MV_TILE * MV_K / 2;
+constexpr int MV_RING_BYTES = MV_WARPS * MV_RING * MV_STEP_BYTES;
+constexpr int MV_A_BYTES = 72 * 1024;  // shared memory for A
+constexpr int MV_SLAB_STEPS = 8;       // steps of a slab where all of A does not fit; two of 16 rows fit
 
-__device__ __forceinline__ uint32_t ldg_stream_32(const void* p) {
-  uint32_t v;
-  asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(v) : "l"(p));
-  return v;
+// 16 bytes global -> shared, past L1; `bytes` 0 writes zeros without reading.
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ uint2 ldg_stream_64(const void* p) {
-  uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-  return v;
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kN>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kN) : "memory");
 }
-__device__ __forceinline__ uint4 ldg_stream_128(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
+// The warps of one group (at least two: then there are at most 8 groups, barriers 1 to 8) or the one warp.
+__device__ __forceinline__ void group_barrier(int group, int warps) {
+  if (warps == 1) __syncwarp();
+  else asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(32 * warps) : "memory");
 }
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -83,20 +85,23 @@ __device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
   const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-// Eight codes -> four registers (k0,k4), (k1,k5), (k2,k6), (k3,k7) of code - zero; zero2 = (128 + zero) twice.
-__device__ __forceinline__ void dequant8(uint32_t w, uint32_t zero2, uint32_t (&out)[4]) {
+// Eight codes -> four registers (k0,k4), (k1,k5), (k2,k6), (k3,k7) of code - zero; zero2 = (128 + zero) twice. The mask and the
+// exponent are registers: one three-input operation each, where two immediates would take two.
+__device__ __forceinline__ void dequant8(uint32_t w, uint32_t zero2, uint32_t mask, uint32_t base, uint32_t (&out)[4]) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) out[j] = sub_bf16x2(((w >> (4 * j)) & 0x000f000fu) | 0x43004300u, zero2);
+  for (int j = 0; j < 4; ++j) {
+    uint32_t v;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(v) : "r"(w >> (4 * j)), "r"(mask), "r"(base));  // (w & mask) | base
+    out[j] = sub_bf16x2(v, zero2);
+  }
 }
 
-// What a warp holds of one step of 128 k for its 32 rows: per row slot (g, g + 8, g + 16, g + 24) four words of codes and the
-// scales (and zeros) of the step's groups, packed as they lie in memory. kGW = 128, 64 or 32 is how many k share a scale within
-// a step: a lane's words are laid out so that the four lanes of a row stay inside one group for every pair of MMAs.
+// The scales (and zeros) of one step of 128 k for a lane's four rows (g, g + 8, g + 16, g + 24), packed as they lie in memory.
+// kGW = 128, 64 or 32 is how many k share a scale within a step.
 template <int kGW, typename ST, bool kZeros>
-struct MvStep {
+struct MvScales {
   static constexpr int GROUPS = MV_K / kGW;
   static constexpr int SCALE_WORDS = (GROUPS * int(sizeof(ST)) + 3) / 4;
-  uint32_t c[4][4];
   uint32_t s[4][SCALE_WORDS];
   uint32_t z[4];
 
@@ -110,26 +115,8 @@ struct MvStep {
     return __byte_perm(z[r], 0x00000043u, 0x4040u + 0x0101u * j);
   }
 
-  // row: this lane's four rows, at the first byte of the lane's share of step 0. k0: first k of the step, t: lane in the quad. Words
-  // past K repeat the row's beginning (A is 0 there). s_vec: the step's groups are GROUPS whole scales in a row, aligned.
-  __device__ __forceinline__ void load(const Int4Args& p, const uint8_t* const (&row)[4], const uint32_t (&srow)[4], int k0, int t, int s_vec) {
-#pragma unroll
-    for (int h = 0; h < GROUPS; ++h) {
-      const int k = k0 + h * kGW + t * (kGW / 4);
-      const long long at = k < p.K ? k0 / 2 + h * (kGW / 2) : 0;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        if constexpr (kGW == 128) {
-          const uint4 v = ldg_stream_128(row[r] + at);
-          c[r][0] = v.x; c[r][1] = v.y; c[r][2] = v.z; c[r][3] = v.w;
-        } else if constexpr (kGW == 64) {
-          const uint2 v = ldg_stream_64(row[r] + at);
-          c[r][2 * h] = v.x; c[r][2 * h + 1] = v.y;
-        } else {
-          c[r][h] = ldg_stream_32(row[r] + at);
-        }
-      }
-    }
+  // srow: the rows' first groups, k0: first k of the step; s_vec: its groups are GROUPS whole scales in a row, aligned.
+  __device__ __forceinline__ void load(const Int4Args& p, const uint32_t (&srow)[4], int k0, int s_vec) {
     const ST* scales = static_cast<const ST*>(p.scales);
     if (GROUPS > 1 && s_vec) {
       const uint32_t g = k0 / kGW;
@@ -170,21 +157,38 @@ struct MvStep {
   }
 };
 
+struct MvPlan {
+  int tiles;
+  int kw_log2;     // warps that share a tile, each with every kw-th step; MV_WARPS / kw tiles are worked on at a time
+  int slab_steps;  // steps whose A is in shared memory at a time: all of them where A fits, else a multiple of kw
+  int slabs;
+  int pitch;       // 16-byte blocks from one staged row of A to the next
+  int a_vec, s_vec, out_bf16;
+};
+
 // A in shared memory: rows of 16-byte blocks of 8 k, each block as the pairs the dequantised words have, (k0,k4) (k1,k5) (k2,k6)
 // (k3,k7); block b of a row stands at b ^ ((b >> 3) & 1), and rows are MvPad blocks longer than their k: the eight lanes of a
-// quarter warp (two rows, four shares of a group) then read eight different bank groups. Row `rows` is zeros, for lanes whose row
-// of A does not exist.
+// quarter warp (two rows, four shares of a group) then read eight different bank groups.
 template <int kGW> constexpr int MvPad = kGW == 128 ? 2 : kGW == 64 ? 1 : 4;
 
-__device__ __forceinline__ void stage_a(const Int4Args& p, uint4* to, int pitch, int m0, int rows, int k0, int kn, int a_vec) {
-  const int blocks = kn >> 3;
-  for (int e = threadIdx.x; e < blocks * (rows + 1); e += MV_WARPS * 32) {
-    const int m = e / blocks, b = e - m * blocks;
-    const int k = k0 + 8 * b;
+__device__ __forceinline__ uint4 pairs_of(const uint4& x) {
+  return make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632), __byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632));
+}
+
+// f(block to write, k of it relative to the slab, row of A): this thread's blocks of a slab.
+template <typename F>
+__device__ __forceinline__ void for_blocks(const MvPlan& plan, int rows, F&& f) {
+  const int blocks = plan.slab_steps * (MV_K / 8);
+  for (int m = 0; m < rows; ++m)
+    for (int b = threadIdx.x; b < blocks; b += MV_WARPS * 32) f(m * plan.pitch + (b ^ ((b >> 3) & 1)), 8 * b, m);
+}
+
+__device__ __forceinline__ void stage_a(const Int4Args& p, const MvPlan& plan, uint4* to, int m0, int rows, int k0) {
+  for_blocks(plan, rows, [&](int at, int k, int m) {
     uint4 x = make_uint4(0, 0, 0, 0);
-    if (m < rows && k < p.K) {  // K is a multiple of 8: a block is inside or outside
-      const __nv_bfloat16* a = p.A + (m0 + m) * p.lda + k;
-      if (a_vec) {
+    if (k0 + k < p.K) {  // K is a multiple of 8: a block is inside or outside
+      const __nv_bfloat16* a = p.A + (long long)(m0 + m) * p.lda + k0 + k;
+      if (plan.a_vec) {
         x = __ldg(reinterpret_cast<const uint4*>(a));
       } else {
         const uint16_t* u = reinterpret_cast<const uint16_t*>(a);
@@ -194,141 +198,233 @@ __device__ __forceinline__ void stage_a(const Int4Args& p, uint4* to, int pitch,
         x.w = u[6] | (uint32_t(u[7]) << 16);
       }
     }
-    to[m * pitch + (b ^ ((b >> 3) & 1))] = make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632),
-                                                      __byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632));
-  }
+    to[at] = pairs_of(x);
+  });
 }
 
-struct MvPlan {
-  int kw_log2;      // warps that share a row tile, each with every kw-th step
-  int chunk_steps;  // steps whose A is staged at a time, a multiple of kw * MV_AHEAD; all of them where A fits
-  int pitch;        // 16-byte blocks from one staged row to the next
-  int a_vec, s_vec, out_bf16;
-};
-
+// Work of a CTA: its tiles t0 .. t1 in rounds of MV_WARPS / kw. Where all of A is in shared memory (one slab), 16 warps share a tile:
+// the CTA's work is even whatever its number of tiles, and a tile's sums are joined at once. Where A goes through in slabs, two warps
+// hold a tile's sums in registers over all slabs, so that every slab serves 8 tiles; the next slab is copied asynchronously behind the
+// current one and brought into pairs in place by the threads that copied it.
 template <int kGW, int kNB, typename ST, bool kZeros>
-__global__ void __launch_bounds__(MV_WARPS * 32, 2)
+__global__ void __launch_bounds__(MV_WARPS * 32, 1)
 int4_mma_kernel(const Int4Args p, const MvPlan plan) {
-  using Step = MvStep<kGW, ST, kZeros>;
+  using Scales = MvScales<kGW, ST, kZeros>;
+  constexpr int GROUPS = Scales::GROUPS;
   constexpr int WPG = kGW / 32;  // words of a lane per group of a step
-  extern __shared__ uint4 a_smem[];
-  __shared__ float red[MV_WARPS][MV_TILE][8 * kNB + 1];
+  constexpr int RED_PITCH = 8 * kNB + 1;
+  extern __shared__ uint4 dyn_smem[];
+  float* const red = reinterpret_cast<float*>(dyn_smem + MV_RING_BYTES / 16);  // [warp][row of the tile][row of A]
+  uint4* const a_smem = reinterpret_cast<uint4*>(red + MV_WARPS * MV_TILE * RED_PITCH);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  const int kw = 1 << plan.kw_log2;
-  const int my_k = warp & (kw - 1), my_r = warp >> plan.kw_log2;
-  const int rows_cta = (MV_WARPS >> plan.kw_log2) * MV_TILE;
-  const long long n0 = (long long)blockIdx.x * rows_cta + my_r * MV_TILE;
+  const int kw = 1 << plan.kw_log2, RG = MV_WARPS >> plan.kw_log2;
+  const int mk = warp & (kw - 1), rg = warp >> plan.kw_log2;
   const int m0 = blockIdx.y * (8 * kNB);
   const int m_here = min(8 * kNB, p.M - m0);
-
-  const uint8_t* row[4];
-  uint32_t srow[4];
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const long long n = min(n0 + g + 8 * r, (long long)p.N - 1);  // rows past the end repeat the last one and are not written
-    row[r] = p.codes + n * p.ldq + t * (kGW / 8);
-    srow[r] = (uint32_t)n * (uint32_t)p.groups;  // checked by the host: N * groups < 2^32
-  }
   const int steps = (p.K + MV_K - 1) / MV_K;
-  pdl_launch_dependents();
-  pdl_wait_prior_grids();
-  Step buf[MV_AHEAD];
-#pragma unroll
-  for (int i = 0; i < MV_AHEAD; ++i)
-    if (my_k + i * kw < steps) buf[i].load(p, row, srow, (my_k + i * kw) * MV_K, t, plan.s_vec);
+  const int t0 = (int)((long long)plan.tiles * blockIdx.x / gridDim.x), t1 = (int)((long long)plan.tiles * (blockIdx.x + 1) / gridDim.x);
 
-  const int buf_blocks = plan.pitch * (m_here + 1);
-  const int chunk_k = plan.chunk_steps * MV_K;
-  stage_a(p, a_smem, plan.pitch, m0, m_here, 0, chunk_k, plan.a_vec);
-  __syncthreads();
+  // The warp's ring of codes: a step is 32 rows of 64 bytes, 16-byte block q of a row at q ^ f with f = the bits of row / 2 in reverse,
+  // so that every read below (16, 8 or 4 bytes a lane) meets each bank once.
+  const uint32_t ring = smem_u32(dyn_smem) + warp * (MV_RING * MV_STEP_BYTES);
+  const uint32_t f = ((g >> 2) & 1) | (g & 2);  // row / 2 = (g >> 1) mod 4 for all four rows
+  const uint32_t put = ring + g * 64 + ((t ^ f) << 4);
 
-  const uint4* arow[kNB];
-  float acc[kNB][2][4] = {};
-  // one step; block: first 16-byte block of the step inside the staged rows (a multiple of 16)
-  auto compute = [&](const Step& st, int k0, int block) {
+  // The step whose codes are fetched next runs ahead of the one being multiplied by the ring.
+  int far_tile = t0 + rg, far_step = mk;
+  const uint8_t* row[4];  // this lane's share of the fetched tile's rows
+  auto far_rows = [&]() {
 #pragma unroll
-    for (int j = 0; j < Step::GROUPS; ++j) {
-      float part[kNB][2][4];
-      uint32_t zero2[4];
+    for (int r = 0; r < 4; ++r)  // rows past the end repeat the last one and are not written
+      row[r] = p.codes + (long long)min(far_tile * MV_TILE + g + 8 * r, p.N - 1) * p.ldq + 16 * t;
+  };
+  auto fetch = [&](uint32_t slot) {
+    if (far_tile < t1) {
+      const int bytes = far_step * MV_K + 32 * t < p.K ? 16 : 0;  // K is a multiple of 32: a block is inside or outside
+      const long long at = bytes ? (long long)far_step * (MV_K / 2) : 0;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) zero2[r] = st.zero2(r, j);
-#pragma unroll
-      for (int i = 0; i < WPG; ++i) {
-        const int w = j * WPG + i;
-        const int b = j * (kGW / 8) + t * (kGW / 32) + i;  // this lane's block of the step
-        uint4 x[kNB];
-#pragma unroll
-        for (int nb = 0; nb < kNB; ++nb) x[nb] = arow[nb][block + (b ^ ((b >> 3) & 1))];
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-          uint32_t lo[4], hi[4];  // rows g and g + 8 of this m16 tile
-          dequant8(st.c[2 * mt][w], zero2[2 * mt], lo);
-          dequant8(st.c[2 * mt + 1][w], zero2[2 * mt + 1], hi);
-#pragma unroll
-          for (int nb = 0; nb < kNB; ++nb) {
-            if (i == 0) mma_bf16_zero(part[nb][mt], lo[0], hi[0], lo[1], hi[1], x[nb].x, x[nb].y);
-            else mma_bf16(part[nb][mt], lo[0], hi[0], lo[1], hi[1], x[nb].x, x[nb].y);
-            mma_bf16(part[nb][mt], lo[2], hi[2], lo[3], hi[3], x[nb].z, x[nb].w);
-          }
-        }
-      }
-      // A group that lies past K whole has sums of 0 and repeats a scale, which may be anything: 0 * inf must not count.
-      if (Step::GROUPS == 1 || k0 + j * kGW < p.K) {
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-          const float s0 = st.scale(2 * mt, j), s1 = st.scale(2 * mt + 1, j);
-#pragma unroll
-          for (int nb = 0; nb < kNB; ++nb) {
-            acc[nb][mt][0] = fmaf(s0, part[nb][mt][0], acc[nb][mt][0]);
-            acc[nb][mt][1] = fmaf(s0, part[nb][mt][1], acc[nb][mt][1]);
-            acc[nb][mt][2] = fmaf(s1, part[nb][mt][2], acc[nb][mt][2]);
-            acc[nb][mt][3] = fmaf(s1, part[nb][mt][3], acc[nb][mt][3]);
-          }
-        }
+      for (int r = 0; r < 4; ++r) cp_async_16(put + slot + r * 512, row[r] + at, bytes);
+      far_step += kw;
+      if (far_step >= steps) {
+        far_tile += RG;
+        far_step = mk;
+        if (far_tile < t1) far_rows();
       }
     }
+    cp_async_commit();
+  };
+  // So do the scales, by one step.
+  uint32_t srow[4];
+  auto scale_rows = [&](int tile) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) srow[r] = (uint32_t)min(tile * MV_TILE + g + 8 * r, p.N - 1) * (uint32_t)p.groups;  // host: N * groups < 2^32
   };
 
-  for (int c = 0, s0 = 0; s0 < steps; ++c, s0 += plan.chunk_steps) {
-    // Behind the barrier chunk c is staged and nobody reads chunk c - 1 any more: its buffer takes chunk c + 1.
-    if (c > 0) __syncthreads();
-    if (s0 + plan.chunk_steps < steps)
-      stage_a(p, a_smem + ((c + 1) & 1) * buf_blocks, plan.pitch, m0, m_here, (s0 + plan.chunk_steps) * MV_K, chunk_k, plan.a_vec);
+  pdl_launch_dependents();
+  pdl_wait_prior_grids();
+  if (far_tile < t1) far_rows();
 #pragma unroll
-    for (int b = 0; b < kNB; ++b) arow[b] = a_smem + (c & 1) * buf_blocks + min(8 * b + g, m_here) * plan.pitch;
-    const int end = min(s0 + plan.chunk_steps, steps);
-    for (int u = s0 + my_k; u < end; u += MV_AHEAD * kw) {
-#pragma unroll
-      for (int i = 0; i < MV_AHEAD; ++i) {
-        const int v = u + i * kw;
-        if (v < end) {
-          compute(buf[i], v * MV_K, (v - s0) * (MV_K / 8));
-          if (v + MV_AHEAD * kw < steps) buf[i].load(p, row, srow, (v + MV_AHEAD * kw) * MV_K, t, plan.s_vec);
-        }
-      }
-    }
+  for (int i = 0; i < MV_RING; ++i) fetch(i * MV_STEP_BYTES);
+  Scales sc;
+  if (t0 + rg < t1) {
+    scale_rows(t0 + rg);
+    sc.load(p, srow, mk * MV_K, plan.s_vec);
   }
+  stage_a(p, plan, a_smem, m0, m_here, 0);
 
+  // Where a lane finds its blocks of A in a step: two bases, for the even and odd ones among its words, because of the exchange of
+  // neighbours in every other eight blocks. Rows of A that do not exist repeat the last one; their sums are not written.
+  int a_base[kNB][2];
 #pragma unroll
   for (int nb = 0; nb < kNB; ++nb)
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
+    for (int i = 0; i < 2; ++i)
+      a_base[nb][i] = min(8 * nb + g, m_here - 1) * plan.pitch + (kGW == 128 ? 4 * t + (i ^ (t >> 1)) : kGW == 64 ? 2 * t + i : t ^ i);
+  uint32_t mask = 0x000f000fu, base128 = 0x43004300u;
+  asm volatile("" : "+r"(mask), "+r"(base128));
+
+  const int buf_blocks = m_here * plan.pitch;
+  uint32_t slot = 0;
+  int buf = 0;
+  for (int b0 = t0; b0 < t1; b0 += RG) {
+    const int tile = b0 + rg;
+    float acc[kNB][2][4] = {};
+    for (int s0 = 0; s0 < steps; s0 += plan.slab_steps) {
+      const int s1 = min(s0 + plan.slab_steps, steps);
+      const bool last = s1 == steps && b0 + RG >= t1;
+      const int next_k = s1 == steps ? 0 : s1 * MV_K;  // the slab after this one
+      if (plan.slabs > 1 || b0 == t0) __syncthreads();  // this slab is in place, and nobody reads the one before it
+      if (plan.slabs > 1 && !last) {
+        uint4* to = a_smem + (buf ^ 1) * buf_blocks;
+        if (plan.a_vec) {
+          for_blocks(plan, m_here, [&](int at, int k, int m) {
+            const bool in = next_k + k < p.K;
+            cp_async_16(smem_u32(to + at), p.A + (long long)(m0 + m) * p.lda + (in ? next_k + k : 0), in ? 16 : 0);
+          });
+        } else {
+          stage_a(p, plan, to, m0, m_here, next_k);
+        }
+        cp_async_commit();
+      }
+      if (tile < t1) {
+        const uint4* a0 = a_smem + buf * buf_blocks + mk * (MV_K / 8);
+        for (int v = s0 + mk; v < s1; v += kw, a0 += kw * (MV_K / 8)) {
+          cp_async_wait<MV_RING - 1>();
+          __syncwarp();
+          uint32_t codes[4][4];
+          const uint32_t base = ring + slot + g * 64;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) red[warp][16 * mt + g + 8 * (i >> 1)][8 * nb + 2 * t + (i & 1)] = acc[nb][mt][i];
-  __syncthreads();
-  for (int e = threadIdx.x; e < m_here * rows_cta; e += MV_WARPS * 32) {
-    const int m = e / rows_cta, r = e - m * rows_cta;
-    const long long n = (long long)blockIdx.x * rows_cta + r;
-    if (n >= p.N) continue;
-    float v = 0.0f;
-    for (int i = 0; i < kw; ++i) v += red[(r / MV_TILE) * kw + i][r % MV_TILE][m];  // a fixed order
-    if (p.bias != nullptr) v += p.bias[n];
-    v = activate(v, p.act);
-    const long long at = (m0 + m) * p.ldc + n;
-    if (plan.out_bf16) static_cast<__nv_bfloat16*>(p.C)[at] = __nv_bfloat16(v);
-    else static_cast<float*>(p.C)[at] = v;
+          for (int r = 0; r < 4; ++r) {
+            if constexpr (kGW == 128) {
+              asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(codes[r][0]), "=r"(codes[r][1]), "=r"(codes[r][2]), "=r"(codes[r][3])
+                           : "r"(base + ((t ^ f) << 4) + r * 512));
+            } else if constexpr (kGW == 64) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
+                             : "=r"(codes[r][2 * h]), "=r"(codes[r][2 * h + 1])
+                             : "r"(base + ((((2 * h) | (t >> 1)) ^ f) << 4) + ((t & 1) << 3) + r * 512));
+            } else {
+#pragma unroll
+              for (int h = 0; h < 4; ++h)
+                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(codes[r][h]) : "r"(base + ((h ^ f) << 4) + (t << 2) + r * 512));
+            }
+          }
+          const Scales cur = sc;
+          if (v + kw < steps) {
+            sc.load(p, srow, (v + kw) * MV_K, plan.s_vec);
+          } else if (tile + RG < t1) {
+            scale_rows(tile + RG);
+            sc.load(p, srow, mk * MV_K, plan.s_vec);
+          }
+#pragma unroll
+          for (int j = 0; j < GROUPS; ++j) {
+            float part[kNB][2][4];
+            uint32_t zero2[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) zero2[r] = cur.zero2(r, j);
+#pragma unroll
+            for (int i = 0; i < WPG; ++i) {
+              const int w = j * WPG + i;
+              uint4 x[kNB];
+#pragma unroll
+              for (int nb = 0; nb < kNB; ++nb) {
+                if constexpr (kGW == 128) x[nb] = a0[a_base[nb][i & 1] + (i & 2)];
+                else if constexpr (kGW == 64) x[nb] = a0[a_base[nb][i ^ j] + 8 * j];
+                else x[nb] = a0[a_base[nb][j >> 1] + 4 * j];
+              }
+#pragma unroll
+              for (int mt = 0; mt < 2; ++mt) {
+                uint32_t lo[4], hi[4];  // rows g and g + 8 of this m16 tile
+                dequant8(codes[2 * mt][w], zero2[2 * mt], mask, base128, lo);
+                dequant8(codes[2 * mt + 1][w], zero2[2 * mt + 1], mask, base128, hi);
+#pragma unroll
+                for (int nb = 0; nb < kNB; ++nb) {
+                  if (i == 0) mma_bf16_zero(part[nb][mt], lo[0], hi[0], lo[1], hi[1], x[nb].x, x[nb].y);
+                  else mma_bf16(part[nb][mt], lo[0], hi[0], lo[1], hi[1], x[nb].x, x[nb].y);
+                  mma_bf16(part[nb][mt], lo[2], hi[2], lo[3], hi[3], x[nb].z, x[nb].w);
+                }
+              }
+            }
+            // A group that lies past K whole has sums of 0 and repeats a scale, which may be anything: 0 * inf must not count.
+            if (GROUPS == 1 || v * MV_K + j * kGW < p.K) {
+#pragma unroll
+              for (int mt = 0; mt < 2; ++mt) {
+                const float sc0 = cur.scale(2 * mt, j), sc1 = cur.scale(2 * mt + 1, j);
+#pragma unroll
+                for (int nb = 0; nb < kNB; ++nb) {
+                  acc[nb][mt][0] = fmaf(sc0, part[nb][mt][0], acc[nb][mt][0]);
+                  acc[nb][mt][1] = fmaf(sc0, part[nb][mt][1], acc[nb][mt][1]);
+                  acc[nb][mt][2] = fmaf(sc1, part[nb][mt][2], acc[nb][mt][2]);
+                  acc[nb][mt][3] = fmaf(sc1, part[nb][mt][3], acc[nb][mt][3]);
+                }
+              }
+            }
+          }
+          __syncwarp();  // every lane has its words: the slot takes the step after the ring's last
+          fetch(slot);
+          slot = slot == (MV_RING - 1) * MV_STEP_BYTES ? 0 : slot + MV_STEP_BYTES;
+        }
+      }
+      if (plan.slabs > 1) {
+        buf ^= 1;
+        if (plan.a_vec && !last) {
+          // The copies of the next slab are older than this slab's fetches, if those were as many as the ring is deep.
+          if (tile < t1 && s1 - s0 >= MV_RING * kw) cp_async_wait<MV_RING - 1>();
+          else cp_async_wait<0>();
+          uint4* to = a_smem + buf * buf_blocks;
+          for_blocks(plan, m_here, [&](int at, int, int) { to[at] = pairs_of(to[at]); });
+        }
+      }
+    }
+    // The tile's sums over the warps that share it, always in the order of the warps.
+    if (tile < t1) {
+#pragma unroll
+      for (int nb = 0; nb < kNB; ++nb)
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            red[(warp * MV_TILE + 16 * mt + g + 8 * (i >> 1)) * RED_PITCH + 8 * nb + 2 * t + (i & 1)] = acc[nb][mt][i];
+      group_barrier(rg, kw);
+      for (int e = mk * 32 + lane; e < m_here * MV_TILE; e += 32 * kw) {
+        const int m = e / MV_TILE, r = e % MV_TILE;
+        float v = 0.0f;
+        for (int i = 0; i < kw; ++i) v += red[((rg * kw + i) * MV_TILE + r) * RED_PITCH + m];
+        const int n = tile * MV_TILE + r;
+        if (n >= p.N) continue;
+        if (p.bias != nullptr) v += p.bias[n];
+        v = activate(v, p.act);
+        const long long at = (m0 + m) * p.ldc + n;
+        if (plan.out_bf16) static_cast<__nv_bfloat16*>(p.C)[at] = __nv_bfloat16(v);
+        else static_cast<float*>(p.C)[at] = v;
+      }
+      group_barrier(rg, kw);  // red is free again
+    }
   }
+  cp_async_wait<0>();
 }
 
 // ------------------------------------------------------------------ any K, stride and alignment
@@ -447,28 +543,31 @@ int matvec_mma(const Int4Args& a, bool out_bf16, int sms, cudaStream_t stream) {
   auto kern = int4_mma_kernel<kGW, kNB, ST, kZeros>;
   constexpr int GROUPS = MV_K / kGW;
   MvPlan plan{};
-  // Warps per row tile: enough warps for the chip's loads in flight (12 a SM), never more than there are steps.
-  const long long tiles = (a.N + MV_TILE - 1) / MV_TILE;
+  plan.tiles = (a.N + MV_TILE - 1) / MV_TILE;
   const int steps = (a.K + MV_K - 1) / MV_K;
-  while (plan.kw_log2 < 3 && (2 << plan.kw_log2) <= steps && (tiles << plan.kw_log2) < sms * 12LL) ++plan.kw_log2;
-  const int round = MV_AHEAD << plan.kw_log2;
-  const int rows = std::min(a.M, 8 * kNB) + 1;
+  const int rows = std::min(a.M, 8 * kNB);
   auto bytes = [&](int n) { return (size_t)rows * (n * (MV_K / 8) + MvPad<kGW>) * 16; };
-  plan.chunk_steps = (steps + round - 1) / round * round;
-  size_t smem = bytes(plan.chunk_steps);
-  if (smem > MV_STAGE_BYTES) {  // in chunks of 8 steps (16 where 8 warps share a tile), two buffers
-    plan.chunk_steps = std::max(8, round);
-    smem = 2 * bytes(plan.chunk_steps);
+  // All of A where it fits, with up to 16 warps on a tile; else slabs of 8 steps in two buffers, two warps on a tile.
+  const bool whole = bytes(steps) <= MV_A_BYTES;
+  if (whole) {
+    while (plan.kw_log2 < 4 && (2 << plan.kw_log2) <= steps) ++plan.kw_log2;
+    plan.slab_steps = steps;
+    plan.slabs = 1;
+  } else {
+    plan.kw_log2 = 1;
+    plan.slab_steps = MV_SLAB_STEPS;
+    plan.slabs = (steps + MV_SLAB_STEPS - 1) / MV_SLAB_STEPS;
   }
-  plan.pitch = plan.chunk_steps * (MV_K / 8) + MvPad<kGW>;
+  plan.pitch = plan.slab_steps * (MV_K / 8) + MvPad<kGW>;
   plan.a_vec = a.lda % 8 == 0 && reinterpret_cast<uintptr_t>(a.A) % 16 == 0;
   plan.s_vec = a.group == kGW && a.groups % GROUPS == 0 && reinterpret_cast<uintptr_t>(a.scales) % (GROUPS * sizeof(ST)) == 0 &&
                reinterpret_cast<uintptr_t>(a.zeros) % GROUPS == 0;
   plan.out_bf16 = out_bf16 ? 1 : 0;
-  SX_ENSURE_DYN_SMEM(kern, 160 * 1024);
-  const int rows_cta = (MV_WARPS >> plan.kw_log2) * MV_TILE;
+  const size_t smem = MV_RING_BYTES + MV_WARPS * MV_TILE * (8 * kNB + 1) * 4 + bytes(plan.slab_steps) * (whole ? 1 : 2);
+  SX_ENSURE_DYN_SMEM(kern, 227 * 1024);
+  const int mblocks = (a.M + 8 * kNB - 1) / (8 * kNB);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((a.N + rows_cta - 1) / rows_cta), (unsigned)((a.M + 8 * kNB - 1) / (8 * kNB)), 1);
+  cfg.gridDim = dim3((unsigned)std::min(plan.tiles, std::max(1, sms / mblocks)), (unsigned)mblocks, 1);
   cfg.blockDim = dim3(MV_WARPS * 32, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -492,11 +591,11 @@ int matvec_gw(const Int4Args& a, bool out_bf16, int sms, cudaStream_t stream) {
 
 template <typename ST>
 int matvec(const Int4Args& a, bool out_bf16, int sms, cudaStream_t stream) {
-  // The widest load whose lanes' shares stay inside one group, as far as the rows' alignment allows.
+  // The fast path reads rows of codes in 16-byte blocks; which of its forms goes by the group.
   const uintptr_t at = reinterpret_cast<uintptr_t>(a.codes) | (uintptr_t)a.ldq;
-  if (a.K % 32 == 0 && at % 4 == 0 && (long long)a.N * a.groups < (1ll << 32)) {
-    if (a.group % 128 == 0 && at % 16 == 0) return matvec_gw<128, ST>(a, out_bf16, sms, stream);
-    if (a.group % 64 == 0 && at % 8 == 0) return matvec_gw<64, ST>(a, out_bf16, sms, stream);
+  if (a.K % 32 == 0 && at % 16 == 0 && (long long)a.N * a.groups < (1ll << 32)) {
+    if (a.group % 128 == 0) return matvec_gw<128, ST>(a, out_bf16, sms, stream);
+    if (a.group % 64 == 0) return matvec_gw<64, ST>(a, out_bf16, sms, stream);
     return matvec_gw<32, ST>(a, out_bf16, sms, stream);
   }
   const cudaError_t e = out_bf16 ? launch_kernel_ex(int4_matvec_any_kernel<ST, __nv_bfloat16>, (unsigned)((a.N + 7) / 8), 256, 0, stream, 1,
