@@ -14,7 +14,9 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <initializer_list>
+#include <type_traits>
 
 #include "../../include/symplex_b200.h"
 #include "host_api.h"
@@ -146,83 +148,166 @@ ln_backward_columns_kernel(const T* __restrict__ dy, const T* __restrict__ x, co
   }
 }
 
-// dweight / dbias from the partial rows, always in the same order: eight interleaved chains, then their sum.
+// dweight / dbias from the partial rows, always in the same order: 32 interleaved chains (a warp each, eight loads in flight a lane),
+// then their sum. Few columns a CTA and many warps, because what it costs is the latency of the chains.
 template <typename W>
-__global__ void __launch_bounds__(LN_THREADS)
+__global__ void __launch_bounds__(1024)
 ln_backward_finish_kernel(const float* __restrict__ part, W* __restrict__ dw, W* __restrict__ db, long long cols, int parts) {
-  __shared__ float s[2][8][LN_COL_TILE];
+  __shared__ float s[2][32][LN_COL_TILE + 1];
   pdl_launch_dependents();
   pdl_wait_prior_grids();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long c = (long long)blockIdx.x * LN_COL_TILE + lane;
   float a = 0.0f, d = 0.0f;
   if (c < cols) {
-    for (int i = warp; i < parts; i += 8) {
-      a += part[(long long)(2 * i) * cols + c];
-      d += part[(long long)(2 * i + 1) * cols + c];
+    for (int i = warp; i < parts; i += 4 * 32) {
+      float x[4], y[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool in = i + 32 * j < parts;
+        const float* p = part + (long long)(2 * (in ? i + 32 * j : i)) * cols + c;
+        x[j] = in ? p[0] : 0.0f;
+        y[j] = in ? p[cols] : 0.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        a += x[j];
+        d += y[j];
+      }
     }
   }
   s[0][warp][lane] = a;
   s[1][warp][lane] = d;
   __syncthreads();
-  if (warp < 2 && c < cols) {
-    float v = s[warp][0][lane];
-    for (int i = 1; i < 8; ++i) v += s[warp][i][lane];
-    W* dst = warp == 0 ? dw : db;
-    if (dst != nullptr) dst[c] = W(v);
+  // warp w adds up column w: 32 chains across its lanes
+  const long long col = (long long)blockIdx.x * LN_COL_TILE + warp;
+  a = warp_sum(s[0][lane][warp]);
+  d = warp_sum(s[1][lane][warp]);
+  if (lane == 0 && col < cols) {
+    if (dw != nullptr) dw[col] = W(a);
+    if (db != nullptr) db[col] = W(d);
   }
 }
 
 // ------------------------------------------------------------------ rows in registers
+// VEC values of a thread, in pairs: one instruction of the packed fp32 unit for two of them.
+template <int VEC>
+struct Fv {
+  unsigned long long p[VEC / 2];
+  static __device__ __forceinline__ unsigned long long pair(float a, float b) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+  }
+  static __device__ __forceinline__ float2 split(unsigned long long v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+  }
+  __device__ __forceinline__ void fill(float s) {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) p[i] = pair(s, s);
+  }
+  __device__ __forceinline__ void add(const Fv& o) {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) asm("add.rn.f32x2 %0, %0, %1;" : "+l"(p[i]) : "l"(o.p[i]));
+  }
+  __device__ __forceinline__ void mul(const Fv& o) {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(p[i]) : "l"(o.p[i]));
+  }
+  // this += a * b
+  __device__ __forceinline__ void fma(const Fv& a, const Fv& b) {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(p[i]) : "l"(a.p[i]), "l"(b.p[i]));
+  }
+  // sums over all values are kept in one pair
+  using Sum = unsigned long long;
+  static __device__ __forceinline__ Sum zero() { return 0ull; }
+  static __device__ __forceinline__ float total(Sum s) {
+    const float2 v = split(s);
+    return v.x + v.y;
+  }
+  __device__ __forceinline__ void sum_into(Sum& s) const {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) asm("add.rn.f32x2 %0, %0, %1;" : "+l"(s) : "l"(p[i]));
+  }
+  __device__ __forceinline__ void dot_into(Sum& s, const Fv& o) const {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(s) : "l"(p[i]), "l"(o.p[i]));
+  }
+  __device__ __forceinline__ float get(int j) const {
+    const float2 v = split(p[j / 2]);
+    return j & 1 ? v.y : v.x;
+  }
+};
+template <>
+struct Fv<1> {
+  float p;
+  __device__ __forceinline__ void fill(float s) { p = s; }
+  __device__ __forceinline__ void add(const Fv& o) { p += o.p; }
+  __device__ __forceinline__ void mul(const Fv& o) { p *= o.p; }
+  __device__ __forceinline__ void fma(const Fv& a, const Fv& b) { p = fmaf(a.p, b.p, p); }
+  using Sum = float;
+  static __device__ __forceinline__ Sum zero() { return 0.0f; }
+  static __device__ __forceinline__ float total(Sum s) { return s; }
+  __device__ __forceinline__ void sum_into(Sum& s) const { s += p; }
+  __device__ __forceinline__ void dot_into(Sum& s, const Fv& o) const { s = fmaf(p, o.p, s); }
+  __device__ __forceinline__ float get(int) const { return p; }
+};
+
 template <typename T, int VEC>
 struct LnRaw {
   uint4 v;
   __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const uint4*>(p); }
-  __device__ __forceinline__ void unpack(float (&f)[VEC]) const {
+  __device__ __forceinline__ void unpack(Fv<VEC>& f) const {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(w[i]);
+      for (int i = 0; i < 2; ++i) f.p[i] = Fv<VEC>::pair(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        f[2 * i] = __uint_as_float(w[i] << 16);
-        f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-      }
+      for (int i = 0; i < 4; ++i) f.p[i] = Fv<VEC>::pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
     }
   }
-  static __device__ __forceinline__ void store(T* p, const float (&f)[VEC]) {
+  static __device__ __forceinline__ void store(T* p, const Fv<VEC>& f) {
+    uint32_t w[4];
     if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float2 v = Fv<VEC>::split(f.p[i]);
+        w[2 * i] = __float_as_uint(v.x);
+        w[2 * i + 1] = __float_as_uint(v.y);
+      }
     } else {
-      uint32_t w[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+        const __nv_bfloat162 h = __float22bfloat162_rn(Fv<VEC>::split(f.p[i]));
         w[i] = *reinterpret_cast<const uint32_t*>(&h);
       }
-      *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
     }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 };
 template <typename T>
 struct LnRaw<T, 1> {
   T v;
   __device__ __forceinline__ void load(const T* p) { v = *p; }
-  __device__ __forceinline__ void unpack(float (&f)[1]) const { f[0] = float(v); }
-  static __device__ __forceinline__ void store(T* p, const float (&f)[1]) { *p = T(f[0]); }
+  __device__ __forceinline__ void unpack(Fv<1>& f) const { f.p = float(v); }
+  static __device__ __forceinline__ void store(T* p, const Fv<1>& f) { *p = T(f.p); }
 };
 
 // VEC consecutive parameters (of the input's type or float).
 template <typename W, int VEC>
-__device__ __forceinline__ void load_params(const W* p, float (&f)[VEC]) {
+__device__ __forceinline__ void load_params(const W* p, Fv<VEC>& f) {
   if constexpr (VEC == 1) {
-    f[0] = float(*p);
+    f.p = float(*p);
   } else if constexpr (sizeof(W) == 4) {
 #pragma unroll
     for (int i = 0; i < VEC; i += 4) {
       const float4 x = __ldg(reinterpret_cast<const float4*>(p + i));
-      f[i] = x.x; f[i + 1] = x.y; f[i + 2] = x.z; f[i + 3] = x.w;
+      f.p[i / 2] = Fv<VEC>::pair(x.x, x.y);
+      f.p[i / 2 + 1] = Fv<VEC>::pair(x.z, x.w);
     }
   } else {
     LnRaw<W, VEC> r;
@@ -231,33 +316,79 @@ __device__ __forceinline__ void load_params(const W* p, float (&f)[VEC]) {
   }
 }
 
-// kN sums over the tpr threads of a row, the same values in every thread. `red`: this row group's [32][kN] floats for this call; the
-// caller alternates between two of them, and the barrier in between keeps a use of one apart from the next use of the same.
-template <int kN>
-__device__ __forceinline__ void row_sum(float (&v)[kN], float* red, int tpr, int group) {
+// Parameters staged in shared memory as floats, the 4-float pieces of a vector nvec * 16 bytes apart (so that neighbouring lanes read
+// neighbouring 16 bytes). Persistent CTAs unpack them once instead of once a row.
+template <typename W, int VEC>
+__device__ __forceinline__ void stage_params(const W* p, float* to, int nvec) {
+  if constexpr (VEC > 1) {
+    for (int v = threadIdx.x; v < nvec; v += blockDim.x) {
+      Fv<VEC> f;
+      load_params<W, VEC>(p + (long long)v * VEC, f);
 #pragma unroll
-  for (int i = 0; i < kN; ++i) v[i] = warp_sum(v[i]);
-  if (tpr == 32) return;
-  const int lane = threadIdx.x & 31, warp = (threadIdx.x & (tpr - 1)) >> 5, warps = tpr >> 5;
-  if (lane == 0) {
-#pragma unroll
-    for (int i = 0; i < kN; ++i) red[warp * kN + i] = v[i];
+      for (int h = 0; h < VEC / 4; ++h) {
+        const float2 a = Fv<VEC>::split(f.p[2 * h]), b = Fv<VEC>::split(f.p[2 * h + 1]);
+        reinterpret_cast<float4*>(to)[h * nvec + v] = make_float4(a.x, a.y, b.x, b.y);
+      }
+    }
   }
-  asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(tpr) : "memory");  // at most 8 groups of 64 threads
+}
+template <int VEC>
+__device__ __forceinline__ void staged_params(const float* from, int nvec, int v, Fv<VEC>& f) {
+  if constexpr (VEC > 1) {
 #pragma unroll
-  for (int i = 0; i < kN; ++i) {
-    float s = lane < warps ? red[lane * kN + i] : 0.0f;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    v[i] = s;
+    for (int h = 0; h < VEC / 4; ++h) {
+      const float4 x = reinterpret_cast<const float4*>(from)[h * nvec + v];
+      f.p[2 * h] = Fv<VEC>::pair(x.x, x.y);
+      f.p[2 * h + 1] = Fv<VEC>::pair(x.z, x.w);
+    }
   }
 }
 
-template <typename T, typename W, int VEC, int NV, int BLOCK>
+// v^-1/2: the hardware's estimate and one step of Newton's method, which leaves two roundings' error; 1 / sqrt as the formula has it
+// where the step would meet an infinity (v = 0) or a NaN.
+__device__ __forceinline__ float inverse_root(float v) {
+  const float y = rsqrtf(v);
+  const float z = fmaf(fmaf(-v * y, y, 1.0f), 0.5f * y, y);
+  return y < 3.402823466e38f && v < 1e30f ? z : y;
+}
+
+// kN sums over the tpr threads of a row, the same values in every thread (kTpr: tpr where it is known, else 0). `red`: this row group's
+// kN * warps floats for this call; the caller alternates between two such places, and the barrier in between keeps a use of one
+// apart from the next use of the same.
+template <int kN, int kTpr>
+__device__ __forceinline__ void row_sum(float (&v)[kN], float* red, int tpr, int group) {
+#pragma unroll
+  for (int i = 0; i < kN; ++i) v[i] = warp_sum(v[i]);
+  if ((kTpr ? kTpr : tpr) == 32) return;
+  const int lane = threadIdx.x & 31, warp = (threadIdx.x & ((kTpr ? kTpr : tpr) - 1)) >> 5, warps = (kTpr ? kTpr : tpr) >> 5;
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) red[i * warps + warp] = v[i];
+  }
+  asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(kTpr ? kTpr : tpr) : "memory");  // at most 8 groups
+  if constexpr (kTpr == 128 || kTpr == 256) {  // four or eight values: read by everyone, shorter than another round of shuffles
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const float4 a = *reinterpret_cast<const float4*>(red + i * warps);
+      v[i] = (a.x + a.y) + (a.z + a.w);
+      if constexpr (kTpr == 256) {
+        const float4 b = *reinterpret_cast<const float4*>(red + i * warps + 4);
+        v[i] += (b.x + b.y) + (b.z + b.w);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) v[i] = warp_sum(lane < warps ? red[i * warps + lane] : 0.0f);
+  }
+}
+
+template <typename T, typename W, int VEC, int NV, int BLOCK, bool kStage, int kTpr>
 __global__ void __launch_bounds__(BLOCK)
 ln_forward_kernel(const T* x, const W* __restrict__ w, const W* __restrict__ b, T* y, float* __restrict__ mean_out,
-                  float* __restrict__ rstd_out, long long rows, int cols, long long ldx, long long ldy, float eps, int tpr) {
-  __shared__ float red[BLOCK / 32 * 2 * 2 + 64];
+                  float* __restrict__ rstd_out, long long rows, int cols, long long ldx, long long ldy, float eps, int tpr_) {
+  const int tpr = kTpr ? kTpr : tpr_;
+  extern __shared__ float4 staged[];  // kStage: the weights, the biases
+  __shared__ __align__(16) float red[BLOCK / 32 * 2];
   const int group = threadIdx.x / tpr, t = threadIdx.x & (tpr - 1);
   const long long groups = (long long)gridDim.x * (BLOCK / tpr);
   float* const my_red = red + group * (tpr >> 5) * 2;
@@ -273,53 +404,59 @@ ln_forward_kernel(const T* x, const W* __restrict__ w, const W* __restrict__ b, 
   };
   long long r = (long long)blockIdx.x * (BLOCK / tpr) + group;
   if (r < rows) fetch(r);
+  const float* const ws = reinterpret_cast<const float*>(staged);
+  const float* const bs = ws + (w != nullptr ? cols : 0);
+  if constexpr (kStage) {
+    if (w != nullptr) stage_params<W, VEC>(w, reinterpret_cast<float*>(staged), nvec);
+    if (b != nullptr) stage_params<W, VEC>(b, reinterpret_cast<float*>(staged) + (w != nullptr ? cols : 0), nvec);
+    __syncthreads();
+  }
   for (; r < rows; r += groups) {
-    float f[NV][VEC];
-    float s[1] = {0.0f};
+    Fv<VEC> f[NV], k;
+    typename Fv<VEC>::Sum sum = Fv<VEC>::zero();
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if (t + i * tpr < nvec) {
         next[i].unpack(f[i]);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) s[0] += f[i][j];
+        f[i].sum_into(sum);
       }
     }
     if (r + groups < rows) fetch(r + groups);
-    row_sum(s, my_red, tpr, group);
+    float s[1] = {Fv<VEC>::total(sum)};
+    row_sum<1, kTpr>(s, my_red, tpr, group);
     const float mean = s[0] * inv;
-    float q[1] = {0.0f};
+    k.fill(-mean);
+    sum = Fv<VEC>::zero();
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if (t + i * tpr < nvec) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          f[i][j] -= mean;
-          q[0] = fmaf(f[i][j], f[i][j], q[0]);
-        }
+        f[i].add(k);
+        f[i].dot_into(sum, f[i]);
       }
     }
-    row_sum(q, my_red + (tpr >> 5), tpr, group);
-    const float rstd = 1.0f / sqrtf(q[0] * inv + eps);
+    float q[1] = {Fv<VEC>::total(sum)};
+    row_sum<1, kTpr>(q, my_red + (tpr >> 5), tpr, group);
+    const float rstd = inverse_root(q[0] * inv + eps);
     if (t == 0) {
       if (mean_out != nullptr) mean_out[r] = mean;
       if (rstd_out != nullptr) rstd_out[r] = rstd;
     }
+    k.fill(rstd);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int v = t + i * tpr;
       if (v < nvec) {
-        float p[VEC];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) f[i][j] *= rstd;
+        Fv<VEC> p;
+        f[i].mul(k);
         if (w != nullptr) {
-          load_params<W, VEC>(w + v * VEC, p);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) f[i][j] *= p[j];
+          if constexpr (kStage) staged_params<VEC>(ws, nvec, v, p);
+          else load_params<W, VEC>(w + v * VEC, p);
+          f[i].mul(p);
         }
         if (b != nullptr) {
-          load_params<W, VEC>(b + v * VEC, p);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) f[i][j] += p[j];
+          if constexpr (kStage) staged_params<VEC>(bs, nvec, v, p);
+          else load_params<W, VEC>(b + v * VEC, p);
+          f[i].add(p);
         }
         LnRaw<T, VEC>::store(y + r * ldy + (long long)v * VEC, f[i]);
       }
@@ -328,13 +465,14 @@ ln_forward_kernel(const T* x, const W* __restrict__ w, const W* __restrict__ b, 
 }
 
 // dx, and this CTA's share of dw and db as row blockIdx.x of part[grid][2][cols] (part null: dx only; dx null: those only).
-template <typename T, typename W, int VEC, int NV, int BLOCK, bool kAhead>
-__global__ void __launch_bounds__(BLOCK)
+template <typename T, typename W, int VEC, int NV, int BLOCK, int kTpr>
+__global__ void __launch_bounds__(BLOCK, 1)
 ln_backward_kernel(const T* dy, const T* __restrict__ x, const float* __restrict__ mean_in, const float* __restrict__ rstd_in,
                    const W* __restrict__ w, T* dx, float* __restrict__ part, long long rows, int cols, long long lddy, long long ldx,
-                   long long lddx, int tpr) {
+                   long long lddx, int tpr_) {
+  const int tpr = kTpr ? kTpr : tpr_;
   extern __shared__ float joined[];  // [2][cols], where several row groups are joined
-  __shared__ float red[2][BLOCK / 32 * 2];
+  __shared__ __align__(16) float red[2][BLOCK / 32 * 2];
   const int group = threadIdx.x / tpr, t = threadIdx.x & (tpr - 1), per_cta = BLOCK / tpr;
   const long long groups = (long long)gridDim.x * per_cta;
   const int nvec = cols / VEC;
@@ -354,44 +492,54 @@ ln_backward_kernel(const T* dy, const T* __restrict__ x, const float* __restrict
     nmean = mean_in[r];
     nrstd = rstd_in[r];
   };
-  float dw[NV][VEC] = {}, db[NV][VEC] = {};
+  Fv<VEC> dw[NV], db[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    dw[i].fill(0.0f);
+    db[i].fill(0.0f);
+  }
   long long r = (long long)blockIdx.x * per_cta + group;
-  if (kAhead && r < rows) fetch(r);
+  if (r < rows) fetch(r);
   int buf = 0;
   for (; r < rows; r += groups, buf ^= 1) {
-    if (!kAhead) fetch(r);
     const float mean = nmean, rstd = nrstd;
-    float xh[NV][VEC], g[NV][VEC];
-    float s[2] = {0.0f, 0.0f};
+    Fv<VEC> xm[NV], g[NV], km, kr;  // x - mean; rstd is multiplied where it is needed: dw, the sum of g xh, and dx
+    km.fill(-mean);
+    kr.fill(rstd);
+    typename Fv<VEC>::Sum s0 = Fv<VEC>::zero(), s1 = Fv<VEC>::zero();
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int v = t + i * tpr;
       if (v < nvec) {
-        nx[i].unpack(xh[i]);
+        nx[i].unpack(xm[i]);
         nd[i].unpack(g[i]);
-        float p[VEC];
-        if (w != nullptr) load_params<W, VEC>(w + v * VEC, p);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          xh[i][j] = (xh[i][j] - mean) * rstd;
-          dw[i][j] = fmaf(g[i][j], xh[i][j], dw[i][j]);
-          db[i][j] += g[i][j];
-          if (w != nullptr) g[i][j] *= p[j];
-          s[0] += g[i][j];
-          s[1] = fmaf(g[i][j], xh[i][j], s[1]);
+        xm[i].add(km);
+        db[i].add(g[i]);
+        Fv<VEC> p = g[i];
+        p.mul(kr);
+        dw[i].fma(p, xm[i]);
+        if (w != nullptr) {
+          load_params<W, VEC>(w + v * VEC, p);
+          g[i].mul(p);
         }
+        g[i].sum_into(s0);
+        g[i].dot_into(s1, xm[i]);
       }
     }
-    if (kAhead && r + groups < rows) fetch(r + groups);
+    if (r + groups < rows) fetch(r + groups);
     if (dx == nullptr) continue;
-    row_sum(s, red[buf] + group * (tpr >> 5) * 2, tpr, group);
-    const float c1 = s[0] * inv, c2 = s[1] * inv;
+    float s[2] = {Fv<VEC>::total(s0), Fv<VEC>::total(s1)};
+    row_sum<2, kTpr>(s, red[buf] + group * (tpr >> 5) * 2, tpr, group);
+    Fv<VEC> k1, k2;
+    k1.fill(-s[0] * inv);
+    k2.fill(-(s[1] * rstd) * inv * rstd);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int v = t + i * tpr;
       if (v < nvec) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) g[i][j] = rstd * (g[i][j] - c1 - xh[i][j] * c2);
+        g[i].add(k1);
+        g[i].fma(xm[i], k2);
+        g[i].mul(kr);
         LnRaw<T, VEC>::store(dx + r * lddx + (long long)v * VEC, g[i]);
       }
     }
@@ -408,7 +556,7 @@ ln_backward_kernel(const T* dy, const T* __restrict__ x, const float* __restrict
 #pragma unroll
           for (int j = 0; j < VEC; ++j) {
             const int c = v * VEC + j;
-            float a = dw[i][j], d = db[i][j];
+            float a = dw[i].get(j), d = db[i].get(j);
             if (turn > 0) {
               a += joined[c];
               d += joined[cols + c];
@@ -446,16 +594,53 @@ bool all_aligned(std::initializer_list<const void*> ps, std::initializer_list<lo
   return a % 16 == 0;
 }
 
+// One call of f with the number of threads as a constant.
+template <typename F>
+auto with_threads(int tpr, F&& f) {
+  switch (tpr) {
+    case 32: return f(std::integral_constant<int, 32>{});
+    case 64: return f(std::integral_constant<int, 64>{});
+    case 128: return f(std::integral_constant<int, 128>{});
+    case 256: return f(std::integral_constant<int, 256>{});
+    case 512: return f(std::integral_constant<int, 512>{});
+    default: return f(std::integral_constant<int, 1024>{});
+  }
+}
+
 template <typename T, typename W, int VEC, int NV>
 cudaError_t forward_rows(const void* x, const void* w, const void* b, void* y, float* mean, float* rstd, const LnShape& s, float eps, int tpr,
                          int num_sms, cudaStream_t stream) {
-  auto go = [&](auto kern, int block, int ctas_per_sm) {
+  auto go = [&](auto kern, int block, int ctas_per_sm, size_t smem) {
     const long long per_cta = block / tpr;
     const unsigned grid = (unsigned)std::min<long long>((s.rows + per_cta - 1) / per_cta, (long long)num_sms * ctas_per_sm);
-    return launch_kernel_ex(kern, grid, block, 0, stream, 1, pdl_enabled(), static_cast<const T*>(x), static_cast<const W*>(w),
+    return launch_kernel_ex(kern, grid, block, smem, stream, 1, pdl_enabled(), static_cast<const T*>(x), static_cast<const W*>(w),
                             static_cast<const W*>(b), static_cast<T*>(y), mean, rstd, s.rows, (int)s.cols, s.ldx, s.ldy, eps, tpr);
   };
-  return tpr <= 256 ? go(ln_forward_kernel<T, W, VEC, NV, 256>, 256, 4) : go(ln_forward_kernel<T, W, VEC, NV, 1024>, 1024, 1);
+  if constexpr (VEC > 1) {
+    return with_threads(tpr, [&](auto n) -> cudaError_t {
+      constexpr int TPR = decltype(n)::value;
+      constexpr int BLOCK = TPR >= 512 ? 1024 : 512;  // at most 8 groups that need a barrier
+      // Parameters staged once per CTA where a group sees several rows (NV = 1 is the form for few rows or short ones).
+      const size_t smem = ((w != nullptr ? 1 : 0) + (b != nullptr ? 1 : 0)) * (size_t)s.cols * 4;
+      if constexpr (NV > 1) {
+        if (s.rows >= 8LL * num_sms * (1024 / TPR) && smem > 0) {
+          auto kern = ln_forward_kernel<T, W, VEC, NV, BLOCK, true, TPR>;
+          static std::atomic<uint32_t> raised{0};  // once per device and instance
+          int dev = 0;
+          cudaGetDevice(&dev);
+          if (!((raised.load(std::memory_order_relaxed) >> (dev & 31)) & 1u)) {
+            const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * 16384 * 4);
+            if (e != cudaSuccess) return e;
+            raised.fetch_or(1u << (dev & 31));
+          }
+          return go(kern, BLOCK, smem <= 100 * 1024 ? 1024 / BLOCK : 1, smem);
+        }
+      }
+      return go(ln_forward_kernel<T, W, VEC, NV, BLOCK, false, TPR>, BLOCK, 1024 / BLOCK, 0);
+    });
+  }
+  return tpr <= 256 ? go(ln_forward_kernel<T, W, VEC, NV, 256, false, 0>, 256, 4, 0)
+                    : go(ln_forward_kernel<T, W, VEC, NV, 1024, false, 0>, 1024, 1, 0);
 }
 
 template <typename T, typename W>
@@ -470,7 +655,6 @@ int forward(const void* x, const void* w, const void* b, void* y, float* mean, f
     const int tpr = threads_per_row(s.cols / VEC, MOST, 1024, few);
     const long long nv = (s.cols / VEC + tpr - 1) / tpr;
     if (nv <= 1) e = forward_rows<T, W, VEC, 1>(x, w, b, y, mean, rstd, s, eps, tpr, num_sms, stream);
-    else if (nv <= 2) e = forward_rows<T, W, VEC, 2>(x, w, b, y, mean, rstd, s, eps, tpr, num_sms, stream);
     else e = forward_rows<T, W, VEC, MOST>(x, w, b, y, mean, rstd, s, eps, tpr, num_sms, stream);
   } else if (!vec && s.cols <= 1024 * 16) {
     const int tpr = threads_per_row(s.cols, 8, 1024, few);
@@ -493,46 +677,48 @@ template <typename T, typename W, int VEC, int NV>
 int backward_rows(const void* dy, const void* x, const float* mean, const float* rstd, const void* w, void* dx, float* part, const LnShape& s,
                   int tpr, int num_sms, cudaStream_t stream, int* parts) {
   constexpr int BLOCK = 512;
-  auto kern = ln_backward_kernel<T, W, VEC, NV, BLOCK, true>;
-  const long long per_cta = BLOCK / tpr;
-  const size_t smem = per_cta > 1 && part != nullptr ? (size_t)s.cols * 8 : 0;
-  SX_ENSURE_DYN_SMEM(kern, 64 * 1024);
+  const long long per_cta = std::min(BLOCK / tpr, 8);
+  const size_t smem = BLOCK / tpr > 1 && part != nullptr ? (size_t)s.cols * 8 : 0;
   *parts = (int)std::min<long long>((s.rows + per_cta - 1) / per_cta, std::min(num_sms, LN_PARTS));
-  const cudaError_t e = launch_kernel_ex(kern, (unsigned)*parts, BLOCK, smem, stream, 1, pdl_enabled(), static_cast<const T*>(dy),
-                                         static_cast<const T*>(x), mean, rstd, static_cast<const W*>(w), static_cast<T*>(dx), part, s.rows,
-                                         (int)s.cols, s.ldd, s.ldx, s.ldy, tpr);
-  if (e != cudaSuccess) return launch_failed(e, "layer norm backward launch failed");
-  count_launches(1);
-  return SX_OK;
+  auto go = [&](auto kern) -> int {
+    SX_ENSURE_DYN_SMEM(kern, 64 * 1024);
+    const cudaError_t e = launch_kernel_ex(kern, (unsigned)*parts, BLOCK, smem, stream, 1, pdl_enabled(), static_cast<const T*>(dy),
+                                           static_cast<const T*>(x), mean, rstd, static_cast<const W*>(w), static_cast<T*>(dx), part,
+                                           s.rows, (int)s.cols, s.ldd, s.ldx, s.ldy, tpr);
+    if (e != cudaSuccess) return launch_failed(e, "layer norm backward launch failed");
+    count_launches(1);
+    return SX_OK;
+  };
+  if constexpr (VEC > 1)
+    return with_threads(tpr, [&](auto n) {
+      constexpr int TPR = decltype(n)::value <= BLOCK ? decltype(n)::value : BLOCK;
+      return go(ln_backward_kernel<T, W, VEC, NV, BLOCK, TPR>);
+    });
+  return go(ln_backward_kernel<T, W, VEC, NV, BLOCK, 0>);
 }
 
 template <typename T, typename W>
 int backward(const void* dy, const void* x, const float* mean, const float* rstd, const void* w, void* dx, void* dw,
              void* db, const LnShape& s, float* part, int num_sms, cudaStream_t stream) {
+  constexpr int VEC = 16 / sizeof(T), MOST = 16 / VEC;
   const bool pdl = pdl_enabled();
   const bool params = dw != nullptr || db != nullptr;
-  const long long tiles = (s.cols + LN_COL_TILE - 1) / LN_COL_TILE;
-  int parts = 0;
+  const long long tiles = (s.cols + LN_COL_TILE - 1) / LN_COL_TILE, eb = sizeof(T);
+  const bool few = s.rows <= num_sms;
+  const bool vec = s.cols % VEC == 0 && all_aligned({x, dy, dx, w}, {s.ldx * eb, s.ldd * eb, s.ldy * eb});
+  float* to = params ? part : nullptr;
+  int parts = 0, rc = SX_OK;
   cudaError_t e;
+  const int tpr = threads_per_row(vec ? s.cols / VEC : s.cols, vec ? MOST : 4, 512, few);
+  const long long nv = ((vec ? s.cols / VEC : s.cols) + tpr - 1) / tpr;
   if (s.rows > 0 && s.cols <= 512 * 16) {
-    constexpr int VEC = 16 / sizeof(T), MOST = 16 / VEC;
-    const long long eb = sizeof(T);
-    const bool few = s.rows <= num_sms;
-    float* to = params ? part : nullptr;
-    int rc;
-    if (s.cols % VEC == 0 && all_aligned({x, dy, dx, w}, {s.ldx * eb, s.ldd * eb, s.ldy * eb})) {
-      const int tpr = threads_per_row(s.cols / VEC, MOST, 512, few);
-      const long long nv = (s.cols / VEC + tpr - 1) / tpr;
-      rc = nv <= 1   ? backward_rows<T, W, VEC, 1>(dy, x, mean, rstd, w, dx, to, s, tpr, num_sms, stream, &parts)
-           : nv <= 2 ? backward_rows<T, W, VEC, 2>(dy, x, mean, rstd, w, dx, to, s, tpr, num_sms, stream, &parts)
-                     : backward_rows<T, W, VEC, MOST>(dy, x, mean, rstd, w, dx, to, s, tpr, num_sms, stream, &parts);
-    } else {
-      const int tpr = threads_per_row(s.cols, 4, 512, few);
-      const long long nv = (s.cols + tpr - 1) / tpr;
+    if (vec)
+      rc = nv <= 1 ? backward_rows<T, W, VEC, 1>(dy, x, mean, rstd, w, dx, to, s, tpr, num_sms, stream, &parts)
+                   : backward_rows<T, W, VEC, MOST>(dy, x, mean, rstd, w, dx, to, s, tpr, num_sms, stream, &parts);
+    else
       rc = nv <= 1   ? backward_rows<T, W, 1, 1>(dy, x, mean, rstd, w, dx, to, s, tpr, num_sms, stream, &parts)
            : nv <= 4 ? backward_rows<T, W, 1, 4>(dy, x, mean, rstd, w, dx, to, s, tpr, num_sms, stream, &parts)
                      : backward_rows<T, W, 1, 16>(dy, x, mean, rstd, w, dx, to, s, tpr, num_sms, stream, &parts);
-    }
     if (rc != SX_OK || !params) return rc;
   } else if (s.rows > 0) {
     if (params) {  // before dx: dx may overwrite dy
@@ -551,7 +737,7 @@ int backward(const void* dy, const void* x, const float* mean, const float* rstd
     }
   }
   if (params) {
-    e = launch_kernel_ex(ln_backward_finish_kernel<W>, (unsigned)tiles, LN_THREADS, 0, stream, 1, pdl, (const float*)part,
+    e = launch_kernel_ex(ln_backward_finish_kernel<W>, (unsigned)tiles, 1024u, 0, stream, 1, pdl, (const float*)part,
                          static_cast<W*>(dw), static_cast<W*>(db), s.cols, parts);
     if (e != cudaSuccess) return launch_failed(e, "layer norm backward launch failed");
     count_launches(1);

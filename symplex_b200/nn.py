@@ -21,13 +21,17 @@ INT4_MAX_ROWS = 64
 _DT = {torch.float32: DT_F32, torch.bfloat16: DT_BF16}
 
 
+# The handle of torch's current stream; the object that torch.cuda.current_stream() makes for it costs 3 us a call.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _run(device, stream, fn):
     """``fn(raw_stream)`` with ``device`` current and, where a stream is given, torch's allocations on that stream."""
     if stream is None:
         if device.index == torch.cuda.current_device():
-            return fn(torch.cuda.current_stream().cuda_stream)
+            return fn(_raw_stream(device.index))
         with torch.cuda.device(device):
-            return fn(torch.cuda.current_stream().cuda_stream)
+            return fn(_raw_stream(device.index))
     with torch.cuda.device(device), torch.cuda.stream(torch.cuda.ExternalStream(stream, device)):
         return fn(stream)
 
@@ -39,6 +43,11 @@ def _rows(t):
     if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= t.shape[1]:
         return t, t.stride(0)
     return t.contiguous(), t.shape[-1]
+
+
+def _like(t):
+    """A contiguous tensor like ``t`` (``empty_like`` takes half the time of ``empty``, but keeps other strides)."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def _ptr(t):
@@ -56,7 +65,7 @@ def _norm_checks(who, x, *params):
     for p in params:
         if p is None:
             continue
-        if tuple(p.shape) != (x.shape[-1],) or p.device != x.device:
+        if p.dim() != 1 or p.shape[0] != x.shape[-1] or p.device != x.device:
             raise ValueError(f"weight and bias must have shape ({x.shape[-1]},) on {x.device}")
         if p.dtype != x.dtype and p.dtype != torch.float32 or dtype not in (None, p.dtype):
             raise ValueError("weight and bias must both have the input's dtype or both be float32")
@@ -82,7 +91,7 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5, out=None, return_stats=Fa
 
     def call(s):
         xr, ldx = _rows(x)
-        y = out if out is not None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        y = out if out is not None else _like(x)
         mean = rstd = None
         if return_stats:
             mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
@@ -119,12 +128,12 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, *, param_grads=None, str
         (xr, ldx), (dyr, lddy) = _rows(x), _rows(dy)
         cols = x.shape[-1]
         rows = x.numel() // cols
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dx = _like(x)
         dw = db = ws = None
         size = 0
         if param_grads:
             dw = torch.empty(cols, dtype=pdt, device=x.device)
-            db = torch.empty(cols, dtype=pdt, device=x.device)
+            db = torch.empty_like(dw)
             size = lib.symplex_b200_layer_norm_backward_workspace_bytes(rows, cols)
             ws = torch.empty(size, dtype=torch.uint8, device=x.device)
         w = weight.contiguous() if weight is not None else None
@@ -170,8 +179,8 @@ def linear_cross_entropy(x, weight, targets, *, ignore_index=-100, reduction="me
         (xr, ldx), (w, ldw) = _rows(x), _rows(weight)
         t, h = x.shape
         v = weight.shape[0]
-        loss = torch.empty(t if reduction == "none" else (), dtype=torch.float32, device=x.device)
         lse = torch.empty(t, dtype=torch.float32, device=x.device)
+        loss = torch.empty_like(lse) if reduction == "none" else torch.empty((), dtype=torch.float32, device=x.device)
         size = lib.symplex_b200_linear_cross_entropy_workspace_bytes(xr.data_ptr(), w.data_ptr(), t, h, v, ldx, ldw, _DT[x.dtype])
         ws = torch.empty(size, dtype=torch.uint8, device=x.device)
         tg = targets.contiguous()
@@ -202,8 +211,7 @@ def linear_cross_entropy_backward(dloss, x, weight, targets, lse, *, ignore_inde
     def call(s):
         lib = _capi.load()
         (xr, ldx), (w, ldw) = _rows(x), _rows(weight)
-        dx = torch.empty(t, h, dtype=x.dtype, device=x.device)
-        dw = torch.empty(v, h, dtype=x.dtype, device=x.device)
+        dx, dw = _like(x), _like(weight)
         size = lib.symplex_b200_linear_cross_entropy_backward_workspace_bytes(xr.data_ptr(), w.data_ptr(), t, h, v, ldx, ldw, _DT[x.dtype])
         ws = torch.empty(size, dtype=torch.uint8, device=x.device)
         tg, ls, dl = targets.contiguous(), lse.contiguous(), dloss.contiguous()
