@@ -19,6 +19,7 @@
 #include <type_traits>
 
 #include "../../include/symplex_b200.h"
+#include "gemm_params.h"
 #include "host_api.h"
 #include "sm100_ptx.cuh"
 
@@ -216,6 +217,11 @@ struct Fv {
 #pragma unroll
     for (int i = 0; i < VEC / 2; ++i) asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(p[i]) : "l"(o.p[i]));
   }
+  // this = a * b, without a copy of a
+  __device__ __forceinline__ void product(const Fv& a, const Fv& b) {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(p[i]) : "l"(a.p[i]), "l"(b.p[i]));
+  }
   // this += a * b
   __device__ __forceinline__ void fma(const Fv& a, const Fv& b) {
 #pragma unroll
@@ -247,6 +253,7 @@ struct Fv<1> {
   __device__ __forceinline__ void fill(float s) { p = s; }
   __device__ __forceinline__ void add(const Fv& o) { p += o.p; }
   __device__ __forceinline__ void mul(const Fv& o) { p *= o.p; }
+  __device__ __forceinline__ void product(const Fv& a, const Fv& b) { p = a.p * b.p; }
   __device__ __forceinline__ void fma(const Fv& a, const Fv& b) { p = fmaf(a.p, b.p, p); }
   using Sum = float;
   static __device__ __forceinline__ Sum zero() { return 0.0f; }
@@ -471,7 +478,7 @@ ln_backward_kernel(const T* dy, const T* __restrict__ x, const float* __restrict
                    const W* __restrict__ w, T* dx, float* __restrict__ part, long long rows, int cols, long long lddy, long long ldx,
                    long long lddx, int tpr_) {
   const int tpr = kTpr ? kTpr : tpr_;
-  extern __shared__ float joined[];  // [2][cols], where several row groups are joined
+  extern __shared__ float joined[];  // [group][2][cols]: 512 threads with at most 16 columns each, 64 KB
   __shared__ __align__(16) float red[2][BLOCK / 32 * 2];
   const int group = threadIdx.x / tpr, t = threadIdx.x & (tpr - 1), per_cta = BLOCK / tpr;
   const long long groups = (long long)gridDim.x * per_cta;
@@ -515,8 +522,8 @@ ln_backward_kernel(const T* dy, const T* __restrict__ x, const float* __restrict
         nd[i].unpack(g[i]);
         xm[i].add(km);
         db[i].add(g[i]);
-        Fv<VEC> p = g[i];
-        p.mul(kr);
+        Fv<VEC> p;
+        p.product(g[i], kr);
         dw[i].fma(p, xm[i]);
         if (w != nullptr) {
           load_params<W, VEC>(w + v * VEC, p);
@@ -546,32 +553,171 @@ ln_backward_kernel(const T* dy, const T* __restrict__ x, const float* __restrict
   }
   if (part == nullptr) return;
   float* const out = part + (long long)blockIdx.x * 2 * cols;
-  for (int turn = 0; turn < per_cta; ++turn) {  // group after group, always in the same order
-    if (per_cta > 1) __syncthreads();
-    if (group == turn) {
+  // The groups' shares side by side in shared memory, then their sum, group after group.
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int v = t + i * tpr;
+    if (v < nvec) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        joined[(2 * group) * cols + v * VEC + j] = dw[i].get(j);
+        joined[(2 * group + 1) * cols + v * VEC + j] = db[i].get(j);
+      }
+    }
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < 2 * cols; c += blockDim.x) {
+    float a = joined[c];
+    for (int k = 1; k < per_cta; ++k) a += joined[2 * k * cols + c];
+    out[c] = a;
+  }
+}
+
+// The same for 16-byte aligned rows of some length, through shared memory: every row group has a ring of LN_RING rows (x and dy), filled
+// by one of its threads with bulk copies two rows ahead, and the weights stand there as floats. In registers the next row can only be
+// fetched once this one has been unpacked, which is too late for HBM. Waits are bounded: a group whose wait ran out goes on without
+// waiting (in bounds), and the status word says so.
+constexpr int LN_RING = 3;
+constexpr int LN_RING_BYTES = 220 * 1024;
+constexpr long long LN_RING_COLS = 1024;  // shorter rows: registers
+
+template <typename T, typename W, int VEC, int NV, int kTpr>
+__global__ void __launch_bounds__(512, 1)
+ln_backward_ring_kernel(const T* dy, const T* __restrict__ x, const float* __restrict__ mean_in, const float* __restrict__ rstd_in,
+                        const W* __restrict__ w, T* dx, float* __restrict__ part, long long rows, int cols, long long lddy, long long ldx,
+                        long long lddx, int* status, unsigned long long wait_ns) {
+  extern __shared__ float4 ring_smem[];  // weights [cols]; [group][LN_RING][x row, dy row], at the end [group][2][cols] floats
+  __shared__ __align__(16) float red[2][512 / 32 * 2];
+  __shared__ uint64_t full[512 / kTpr * LN_RING];
+  __shared__ int abort_flag;
+  const int group = threadIdx.x / kTpr, t = threadIdx.x & (kTpr - 1), per_cta = blockDim.x / kTpr;
+  const long long groups = (long long)gridDim.x * per_cta;
+  const int nvec = cols / VEC;
+  const int row_bytes = cols * int(sizeof(T));
+  const float inv = 1.0f / (float)cols;
+  float* const ws = reinterpret_cast<float*>(ring_smem);
+  uint8_t* const rings = reinterpret_cast<uint8_t*>(ws + (w != nullptr ? cols : 0));
+  uint64_t* const bars = full + group * LN_RING;
+  uint8_t* const ring = rings + (size_t)group * LN_RING * 2 * row_bytes;
+  if (t == 0) {
+    for (int i = 0; i < LN_RING; ++i) mbar_init(&bars[i], 1);
+    if (group == 0) abort_flag = 0;
+    fence_mbar_init();
+  }
+  pdl_launch_dependents();
+  pdl_wait_prior_grids();
+  bool ok = true;
+  auto fetch = [&](long long r, int slot) {  // thread 0 of the group
+    mbar_arrive_expect_tx(&bars[slot], 2 * row_bytes);
+    bulk_load_1d(ring + (size_t)slot * 2 * row_bytes, x + r * ldx, row_bytes, &bars[slot]);
+    bulk_load_1d(ring + (size_t)slot * 2 * row_bytes + row_bytes, dy + r * lddy, row_bytes, &bars[slot]);
+  };
+  const long long r0 = (long long)blockIdx.x * per_cta + group;
+  if (t == 0) {
+    for (int i = 0; i < LN_RING - 1; ++i)
+      if (r0 + i * groups < rows) fetch(r0 + i * groups, i);
+  }
+  if (w != nullptr) stage_params<W, VEC>(w, ws, nvec);
+  __syncthreads();
+  Fv<VEC> dw[NV], db[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    dw[i].fill(0.0f);
+    db[i].fill(0.0f);
+  }
+  int buf = 0, slot = 0;
+  uint32_t phase = 0;
+  float nmean = 0.0f, nrstd = 0.0f;
+  if (r0 < rows) {
+    nmean = mean_in[r0];
+    nrstd = rstd_in[r0];
+  }
+  for (long long r = r0; r < rows; r += groups, buf ^= 1) {
+    if (ok && !mbar_wait(&bars[slot], phase, &abort_flag, wait_ns)) ok = false;
+    const float rstd = nrstd;
+    Fv<VEC> xm[NV], g[NV], km, kr;
+    km.fill(-nmean);
+    kr.fill(nrstd);
+    if (r + groups < rows) {
+      nmean = mean_in[r + groups];
+      nrstd = rstd_in[r + groups];
+    }
+    const T* xs = reinterpret_cast<const T*>(ring + (size_t)slot * 2 * row_bytes);
+    const T* ds = reinterpret_cast<const T*>(ring + (size_t)slot * 2 * row_bytes + row_bytes);
+    typename Fv<VEC>::Sum s0 = Fv<VEC>::zero(), s1 = Fv<VEC>::zero();
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int v = t + i * kTpr;
+      if (v < nvec) {
+        LnRaw<T, VEC> rx, rd;
+        rx.load(xs + v * VEC);
+        rd.load(ds + v * VEC);
+        rx.unpack(xm[i]);
+        rd.unpack(g[i]);
+        xm[i].add(km);
+        db[i].add(g[i]);
+        Fv<VEC> p;
+        p.product(g[i], kr);
+        dw[i].fma(p, xm[i]);
+        if (w != nullptr) {
+          staged_params<VEC>(ws, nvec, v, p);
+          g[i].mul(p);
+        }
+        g[i].sum_into(s0);
+        g[i].dot_into(s1, xm[i]);
+      }
+    }
+    float s[2] = {Fv<VEC>::total(s0), Fv<VEC>::total(s1)};
+    row_sum<2, kTpr>(s, red[buf] + group * (kTpr >> 5) * 2, kTpr, group);
+    // Behind this barrier the whole group has the row in registers, and the row before it is long done with: the slot of that one
+    // takes the row after next.
+    const int free_slot = slot == 0 ? LN_RING - 1 : slot - 1;
+    if (t == 0 && ok && r + (LN_RING - 1) * groups < rows) fetch(r + (LN_RING - 1) * groups, free_slot);
+    if (dx != nullptr) {
+      Fv<VEC> k1, k2;
+      k1.fill(-s[0] * inv);
+      k2.fill(-(s[1] * rstd) * inv * rstd);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int v = t + i * tpr;
+        const int v = t + i * kTpr;
         if (v < nvec) {
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const int c = v * VEC + j;
-            float a = dw[i].get(j), d = db[i].get(j);
-            if (turn > 0) {
-              a += joined[c];
-              d += joined[cols + c];
-            }
-            if (turn == per_cta - 1) {
-              out[c] = a;
-              out[cols + c] = d;
-            } else {
-              joined[c] = a;
-              joined[cols + c] = d;
-            }
-          }
+          g[i].add(k1);
+          g[i].fma(xm[i], k2);
+          g[i].mul(kr);
+          LnRaw<T, VEC>::store(dx + r * lddx + (long long)v * VEC, g[i]);
         }
       }
     }
+    if (++slot == LN_RING) { slot = 0; phase ^= 1; }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0 && abort_flag != 0) {
+    const uint64_t from = globaltimer_ns();  // copies that were issued get a bounded time to land
+    while (globaltimer_ns() - from < 1000000ull) __nanosleep(1000);
+    if (status != nullptr) atomicExch(status, int(ST_WAIT_TIMEOUT));
+  }
+  if (part == nullptr) return;
+  float* const joined = reinterpret_cast<float*>(rings);  // the rings are not used any more
+  float* const out = part + (long long)blockIdx.x * 2 * cols;
+  // The groups' shares side by side in shared memory, then their sum, group after group.
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int v = t + i * kTpr;
+    if (v < nvec) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        joined[(2 * group) * cols + v * VEC + j] = dw[i].get(j);
+        joined[(2 * group + 1) * cols + v * VEC + j] = db[i].get(j);
+      }
+    }
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < 2 * cols; c += blockDim.x) {
+    float a = joined[c];
+    for (int k = 1; k < per_cta; ++k) a += joined[2 * k * cols + c];
+    out[c] = a;
   }
 }
 
@@ -677,11 +823,14 @@ template <typename T, typename W, int VEC, int NV>
 int backward_rows(const void* dy, const void* x, const float* mean, const float* rstd, const void* w, void* dx, float* part, const LnShape& s,
                   int tpr, int num_sms, cudaStream_t stream, int* parts) {
   constexpr int BLOCK = 512;
-  const long long per_cta = std::min(BLOCK / tpr, 8);
-  const size_t smem = BLOCK / tpr > 1 && part != nullptr ? (size_t)s.cols * 8 : 0;
+  const long long per_cta = BLOCK / tpr;
+  const size_t smem = part != nullptr ? (size_t)(BLOCK / tpr) * s.cols * 8 : 0;
   *parts = (int)std::min<long long>((s.rows + per_cta - 1) / per_cta, std::min(num_sms, LN_PARTS));
-  auto go = [&](auto kern) -> int {
-    SX_ENSURE_DYN_SMEM(kern, 64 * 1024);
+  // n: the threads of a row as a constant, 0 in the form for single values
+  auto go = [&](auto n) -> int {
+    constexpr int TPR = decltype(n)::value <= BLOCK ? decltype(n)::value : BLOCK;
+    auto kern = ln_backward_kernel<T, W, VEC, NV, BLOCK, TPR>;
+    SX_ENSURE_DYN_SMEM(kern, 128 * 1024);
     const cudaError_t e = launch_kernel_ex(kern, (unsigned)*parts, BLOCK, smem, stream, 1, pdl_enabled(), static_cast<const T*>(dy),
                                            static_cast<const T*>(x), mean, rstd, static_cast<const W*>(w), static_cast<T*>(dx), part,
                                            s.rows, (int)s.cols, s.ldd, s.ldx, s.ldy, tpr);
@@ -689,17 +838,42 @@ int backward_rows(const void* dy, const void* x, const float* mean, const float*
     count_launches(1);
     return SX_OK;
   };
-  if constexpr (VEC > 1)
-    return with_threads(tpr, [&](auto n) {
-      constexpr int TPR = decltype(n)::value <= BLOCK ? decltype(n)::value : BLOCK;
-      return go(ln_backward_kernel<T, W, VEC, NV, BLOCK, TPR>);
-    });
-  return go(ln_backward_kernel<T, W, VEC, NV, BLOCK, 0>);
+  if constexpr (VEC > 1) return with_threads(tpr, go);
+  return go(std::integral_constant<int, 0>{});
+}
+
+// Row groups of a CTA of the ring kernel (0: the rows are too long, or too short, for it).
+int ring_groups(const LnShape& s, int eb, int tpr, int num_sms) {
+  if (s.cols < LN_RING_COLS || tpr < 64) return 0;
+  const long long ring = LN_RING * 2 * s.cols * eb;
+  const long long fit = std::min<long long>(512 / tpr, (LN_RING_BYTES - 4 * s.cols) / ring);
+  return (int)std::min(fit, (s.rows + num_sms - 1) / num_sms);
+}
+
+template <typename T, typename W, int VEC, int NV>
+int backward_ring(const void* dy, const void* x, const float* mean, const float* rstd, const void* w, void* dx, float* part, const LnShape& s,
+                  int tpr, int groups, const DeviceInfo& dev, cudaStream_t stream, int* parts) {
+  // (the rings, 12 or 24 bytes a column and group, are also large enough for the sums at the end, 8 bytes)
+  const size_t smem = (size_t)groups * LN_RING * 2 * s.cols * sizeof(T) + (w != nullptr ? (size_t)s.cols * 4 : 0);
+  *parts = (int)std::min<long long>((s.rows + groups - 1) / groups, std::min(dev.num_sms, LN_PARTS));
+  return with_threads(tpr, [&](auto n) -> int {
+    constexpr int TPR = decltype(n)::value < 64 ? 64 : decltype(n)::value > 512 ? 512 : decltype(n)::value;
+    auto kern = ln_backward_ring_kernel<T, W, VEC, NV, TPR>;
+    SX_ENSURE_DYN_SMEM(kern, LN_RING_BYTES);
+    const cudaError_t e = launch_kernel_ex(kern, (unsigned)*parts, (unsigned)(groups * TPR), smem, stream, 1, pdl_enabled(),
+                                           static_cast<const T*>(dy), static_cast<const T*>(x), mean, rstd, static_cast<const W*>(w),
+                                           static_cast<T*>(dx), part, s.rows, (int)s.cols, s.ldd, s.ldx, s.ldy, dev.status,
+                                           wait_limit_ns_option());
+    if (e != cudaSuccess) return launch_failed(e, "layer norm backward launch failed");
+    count_launches(1);
+    return SX_OK;
+  });
 }
 
 template <typename T, typename W>
 int backward(const void* dy, const void* x, const float* mean, const float* rstd, const void* w, void* dx, void* dw,
-             void* db, const LnShape& s, float* part, int num_sms, cudaStream_t stream) {
+             void* db, const LnShape& s, float* part, const DeviceInfo& dev, cudaStream_t stream) {
+  const int num_sms = dev.num_sms;
   constexpr int VEC = 16 / sizeof(T), MOST = 16 / VEC;
   const bool pdl = pdl_enabled();
   const bool params = dw != nullptr || db != nullptr;
@@ -712,7 +886,11 @@ int backward(const void* dy, const void* x, const float* mean, const float* rstd
   const int tpr = threads_per_row(vec ? s.cols / VEC : s.cols, vec ? MOST : 4, 512, few);
   const long long nv = ((vec ? s.cols / VEC : s.cols) + tpr - 1) / tpr;
   if (s.rows > 0 && s.cols <= 512 * 16) {
-    if (vec)
+    const int ring = vec ? ring_groups(s, sizeof(T), tpr, num_sms) : 0;
+    if (ring > 0)
+      rc = nv <= 1 ? backward_ring<T, W, VEC, 1>(dy, x, mean, rstd, w, dx, to, s, tpr, ring, dev, stream, &parts)
+                   : backward_ring<T, W, VEC, MOST>(dy, x, mean, rstd, w, dx, to, s, tpr, ring, dev, stream, &parts);
+    else if (vec)
       rc = nv <= 1 ? backward_rows<T, W, VEC, 1>(dy, x, mean, rstd, w, dx, to, s, tpr, num_sms, stream, &parts)
                    : backward_rows<T, W, VEC, MOST>(dy, x, mean, rstd, w, dx, to, s, tpr, num_sms, stream, &parts);
     else
@@ -816,15 +994,15 @@ int symplex_b200_layer_norm_backward(const void* dy, const void* x, const float*
       return fail_fmt(SX_ERR_INVALID, "workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
     if (reinterpret_cast<uintptr_t>(workspace) % 256) return fail_fmt(SX_ERR_INVALID, "workspace must be 256-byte aligned");
   }
-  int sms = 0;
-  if ((rc = current_device_sms(&sms)) != SX_OK) return rc;
+  DeviceInfo dev;
+  if ((rc = current_device(&dev)) != SX_OK) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   float* part = static_cast<float*>(workspace);
   if (dtype == SYMPLEX_DT_F32)
-    return backward<float, float>(dy, x, mean, rstd, weight, dx, dweight, dbias, s, part, sms, st);
+    return backward<float, float>(dy, x, mean, rstd, weight, dx, dweight, dbias, s, part, dev, st);
   if (param_dtype == SYMPLEX_DT_F32)
-    return backward<__nv_bfloat16, float>(dy, x, mean, rstd, weight, dx, dweight, dbias, s, part, sms, st);
-  return backward<__nv_bfloat16, __nv_bfloat16>(dy, x, mean, rstd, weight, dx, dweight, dbias, s, part, sms, st);
+    return backward<__nv_bfloat16, float>(dy, x, mean, rstd, weight, dx, dweight, dbias, s, part, dev, st);
+  return backward<__nv_bfloat16, __nv_bfloat16>(dy, x, mean, rstd, weight, dx, dweight, dbias, s, part, dev, st);
 }
 
 }  // extern "C"
