@@ -27,6 +27,10 @@ namespace sx {
 namespace {
 
 constexpr int LN_THREADS = 256;
+// Rows of single values (no 16-byte vectors) that are held in registers: longer ones are faster in the kernels that read a row
+// several times and put more rows on an SM (bf16, device: forward of 2048 x 7777 57 us in registers, 38 so;
+// backward 128 and 80; forward of 16384 x 1001 47 us in registers, 56 so).
+constexpr long long LN_SINGLE_FORWARD = 2048, LN_SINGLE_BACKWARD = 2048;
 constexpr int LN_PARTS = 320;      // upper bound of the partial rows a column reduction is split into
 constexpr int LN_COL_TILE = 32;    // columns of one CTA of the column reductions
 
@@ -60,10 +64,12 @@ ln_forward_any_kernel(const T* x, const W* __restrict__ w, const W* __restrict__
     const T* xr = x + r * ldx;
     T* yr = y + r * ldy;
     float s = 0.0f;
-    for (long long c = threadIdx.x; c < cols; c += LN_THREADS) s += float(xr[c]);
+#pragma unroll 8
+    for (int c = threadIdx.x; c < (int)cols; c += LN_THREADS) s += float(xr[c]);
     const float mean = cta_sum(s, red) * inv;
     float q = 0.0f;
-    for (long long c = threadIdx.x; c < cols; c += LN_THREADS) {
+#pragma unroll 8
+    for (int c = threadIdx.x; c < (int)cols; c += LN_THREADS) {
       const float d = float(xr[c]) - mean;
       q = fmaf(d, d, q);
     }
@@ -72,79 +78,12 @@ ln_forward_any_kernel(const T* x, const W* __restrict__ w, const W* __restrict__
       if (mean_out != nullptr) mean_out[r] = mean;
       if (rstd_out != nullptr) rstd_out[r] = rstd;
     }
-    for (long long c = threadIdx.x; c < cols; c += LN_THREADS) {
+#pragma unroll 4
+    for (int c = threadIdx.x; c < (int)cols; c += LN_THREADS) {
       float v = (float(xr[c]) - mean) * rstd;
       if (w != nullptr) v *= float(w[c]);
       if (b != nullptr) v += float(b[c]);
       yr[c] = T(v);
-    }
-  }
-}
-
-// dx of one row per CTA, rows of any length and alignment.
-template <typename T, typename W>
-__global__ void __launch_bounds__(LN_THREADS)
-ln_backward_dx_any_kernel(const T* dy, const T* __restrict__ x, const float* __restrict__ mean_in,
-                          const float* __restrict__ rstd_in, const W* __restrict__ w, T* dx, long long rows, long long cols,
-                          long long lddy, long long ldx, long long lddx) {
-  __shared__ float red[32];
-  pdl_launch_dependents();
-  pdl_wait_prior_grids();
-  const float inv = 1.0f / (float)cols;
-  for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
-    const float mean = mean_in[r], rstd = rstd_in[r];
-    const T* xr = x + r * ldx;
-    const T* dyr = dy + r * lddy;
-    float s1 = 0.0f, s2 = 0.0f;
-    for (long long c = threadIdx.x; c < cols; c += LN_THREADS) {
-      const float g = w != nullptr ? float(dyr[c]) * float(w[c]) : float(dyr[c]);
-      s1 += g;
-      s2 = fmaf(g, (float(xr[c]) - mean) * rstd, s2);
-    }
-    const float c1 = cta_sum(s1, red) * inv;
-    const float c2 = cta_sum(s2, red) * inv;
-    for (long long c = threadIdx.x; c < cols; c += LN_THREADS) {
-      const float g = w != nullptr ? float(dyr[c]) * float(w[c]) : float(dyr[c]);
-      const float xh = (float(xr[c]) - mean) * rstd;
-      dx[r * lddx + c] = T(rstd * (g - c1 - xh * c2));
-    }
-  }
-}
-
-// Column sums of dy * xh and dy over one slab of rows: CTA (column tile, slab) -> part[slab][2][cols].
-template <typename T>
-__global__ void __launch_bounds__(LN_THREADS)
-ln_backward_columns_kernel(const T* __restrict__ dy, const T* __restrict__ x, const float* __restrict__ mean_in,
-                           const float* __restrict__ rstd_in, float* __restrict__ part, long long rows, long long cols,
-                           long long lddy, long long ldx, int slabs) {
-  __shared__ float sw[8][LN_COL_TILE], sb[8][LN_COL_TILE];
-  pdl_launch_dependents();
-  pdl_wait_prior_grids();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long tiles = (cols + LN_COL_TILE - 1) / LN_COL_TILE;
-  for (long long t = blockIdx.x; t < tiles * slabs; t += gridDim.x) {
-    const long long slab = t / tiles;
-    const long long c = (t - slab * tiles) * LN_COL_TILE + lane;
-    const long long r0 = rows * slab / slabs, r1 = rows * (slab + 1) / slabs;
-    float dw = 0.0f, db = 0.0f;
-    if (c < cols) {
-      for (long long r = r0 + warp; r < r1; r += 8) {
-        const float d = float(dy[r * lddy + c]);
-        dw = fmaf(d, (float(x[r * ldx + c]) - mean_in[r]) * rstd_in[r], dw);
-        db += d;
-      }
-    }
-    __syncthreads();  // the previous tile's sums have been read
-    sw[warp][lane] = dw;
-    sb[warp][lane] = db;
-    __syncthreads();
-    if (warp == 0 && c < cols) {
-      for (int i = 1; i < 8; ++i) {
-        dw += sw[i][lane];
-        db += sb[i][lane];
-      }
-      part[(slab * 2) * cols + c] = dw;
-      part[(slab * 2 + 1) * cols + c] = db;
     }
   }
 }
@@ -359,6 +298,118 @@ __device__ __forceinline__ float inverse_root(float v) {
   return y < 3.402823466e38f && v < 1e30f ? z : y;
 }
 
+// ---- backward for rows that do not fit into registers: dx with one CTA a row, which reads it twice (the second time from L2), and the
+// column sums by a kernel of their own, which reads x and dy again.
+template <typename T, typename W, int VEC>
+__global__ void __launch_bounds__(512)
+ln_backward_dx_any_kernel(const T* dy, const T* __restrict__ x, const float* __restrict__ mean_in,
+                          const float* __restrict__ rstd_in, const W* __restrict__ w, T* dx, long long rows, long long cols,
+                          long long lddy, long long ldx, long long lddx) {
+  __shared__ float red[32];
+  pdl_launch_dependents();
+  pdl_wait_prior_grids();
+  const float inv = 1.0f / (float)cols;
+  const long long nvec = cols / VEC;
+  for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
+    Fv<VEC> km, kr;
+    km.fill(-mean_in[r]);
+    kr.fill(rstd_in[r]);
+    const T* xr = x + r * ldx;
+    const T* dyr = dy + r * lddy;
+    auto values = [&](long long v, Fv<VEC>& xm, Fv<VEC>& g) {
+      LnRaw<T, VEC> a, d;
+      a.load(xr + v * VEC);
+      d.load(dyr + v * VEC);
+      a.unpack(xm);
+      d.unpack(g);
+      xm.add(km);
+      if (w != nullptr) {
+        Fv<VEC> p;
+        load_params<W, VEC>(w + v * VEC, p);
+        g.mul(p);
+      }
+    };
+    typename Fv<VEC>::Sum s0 = Fv<VEC>::zero(), s1 = Fv<VEC>::zero();
+#pragma unroll 4
+    for (long long v = threadIdx.x; v < nvec; v += 512) {
+      Fv<VEC> xm, g;
+      values(v, xm, g);
+      g.sum_into(s0);
+      g.dot_into(s1, xm);
+    }
+    const float rstd = rstd_in[r];
+    Fv<VEC> k1, k2;
+    k1.fill(-cta_sum(Fv<VEC>::total(s0), red) * inv);
+    k2.fill(-(cta_sum(Fv<VEC>::total(s1), red) * rstd) * inv * rstd);
+#pragma unroll 4
+    for (long long v = threadIdx.x; v < nvec; v += 512) {
+      Fv<VEC> xm, g;
+      values(v, xm, g);
+      g.add(k1);
+      g.fma(xm, k2);
+      g.mul(kr);
+      LnRaw<T, VEC>::store(dx + r * lddx + v * VEC, g);
+    }
+  }
+}
+
+// Column sums of dy * xh and dy over one slab of rows: CTA (32 vectors of columns, slab) -> part[slab][2][cols].
+template <typename T, int VEC>
+__global__ void __launch_bounds__(LN_THREADS)
+ln_backward_columns_kernel(const T* __restrict__ dy, const T* __restrict__ x, const float* __restrict__ mean_in,
+                           const float* __restrict__ rstd_in, float* __restrict__ part, long long rows, long long cols,
+                           long long lddy, long long ldx, int slabs) {
+  __shared__ float sw[8][32 * VEC + 1], sb[8][32 * VEC + 1];
+  pdl_launch_dependents();
+  pdl_wait_prior_grids();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long nvec = cols / VEC, tiles = (nvec + 31) / 32;
+  for (long long t = blockIdx.x; t < tiles * slabs; t += gridDim.x) {
+    const long long slab = t / tiles;
+    const long long v = (t - slab * tiles) * 32 + lane;
+    const long long r0 = rows * slab / slabs, r1 = rows * (slab + 1) / slabs;
+    Fv<VEC> dw, db;
+    dw.fill(0.0f);
+    db.fill(0.0f);
+    if (v < nvec) {
+#pragma unroll 4
+      for (long long r = r0 + warp; r < r1; r += 8) {
+        LnRaw<T, VEC> a, d;
+        a.load(x + r * ldx + v * VEC);
+        d.load(dy + r * lddy + v * VEC);
+        Fv<VEC> xm, g, k;
+        a.unpack(xm);
+        d.unpack(g);
+        db.add(g);
+        k.fill(-mean_in[r]);
+        xm.add(k);
+        k.fill(rstd_in[r]);
+        g.mul(k);
+        dw.fma(g, xm);
+      }
+    }
+    __syncthreads();  // the previous tile's sums have been read
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      sw[warp][j * 32 + lane] = dw.get(j);
+      sb[warp][j * 32 + lane] = db.get(j);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < 32 * VEC; e += LN_THREADS) {
+      const long long c = ((t - slab * tiles) * 32 + (e & 31)) * VEC + (e >> 5);
+      if (c >= cols) continue;
+      float a = 0.0f, d = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        a += sw[i][e];
+        d += sb[i][e];
+      }
+      part[(slab * 2) * cols + c] = a;
+      part[(slab * 2 + 1) * cols + c] = d;
+    }
+  }
+}
+
 // kN sums over the tpr threads of a row, the same values in every thread (kTpr: tpr where it is known, else 0). `red`: this row group's
 // kN * warps floats for this call; the caller alternates between two such places, and the barrier in between keeps a use of one
 // apart from the next use of the same.
@@ -478,7 +529,7 @@ ln_backward_kernel(const T* dy, const T* __restrict__ x, const float* __restrict
                    const W* __restrict__ w, T* dx, float* __restrict__ part, long long rows, int cols, long long lddy, long long ldx,
                    long long lddx, int tpr_) {
   const int tpr = kTpr ? kTpr : tpr_;
-  extern __shared__ float joined[];  // [group][2][cols]: 512 threads with at most 16 columns each, 64 KB
+  extern __shared__ float joined[];  // [group][2][cols]: 512 threads with at most 16 columns each or 1024 with 8, 64 KB
   __shared__ __align__(16) float red[2][BLOCK / 32 * 2];
   const int group = threadIdx.x / tpr, t = threadIdx.x & (tpr - 1), per_cta = BLOCK / tpr;
   const long long groups = (long long)gridDim.x * per_cta;
@@ -785,7 +836,7 @@ cudaError_t forward_rows(const void* x, const void* w, const void* b, void* y, f
       return go(ln_forward_kernel<T, W, VEC, NV, BLOCK, false, TPR>, BLOCK, 1024 / BLOCK, 0);
     });
   }
-  return tpr <= 256 ? go(ln_forward_kernel<T, W, VEC, NV, 256, false, 0>, 256, 4, 0)
+  return tpr <= 256 ? go(ln_forward_kernel<T, W, VEC, NV, 256, false, 0>, 256, 8, 0)
                     : go(ln_forward_kernel<T, W, VEC, NV, 1024, false, 0>, 1024, 1, 0);
 }
 
@@ -802,12 +853,11 @@ int forward(const void* x, const void* w, const void* b, void* y, float* mean, f
     const long long nv = (s.cols / VEC + tpr - 1) / tpr;
     if (nv <= 1) e = forward_rows<T, W, VEC, 1>(x, w, b, y, mean, rstd, s, eps, tpr, num_sms, stream);
     else e = forward_rows<T, W, VEC, MOST>(x, w, b, y, mean, rstd, s, eps, tpr, num_sms, stream);
-  } else if (!vec && s.cols <= 1024 * 16) {
-    const int tpr = threads_per_row(s.cols, 8, 1024, few);
+  } else if (!vec && s.cols <= LN_SINGLE_FORWARD) {
+    const int tpr = threads_per_row(s.cols, 4, 1024, few);
     const long long nv = (s.cols + tpr - 1) / tpr;
-    if (nv <= 1) e = forward_rows<T, W, 1, 1>(x, w, b, y, mean, rstd, s, eps, tpr, num_sms, stream);
-    else if (nv <= 8) e = forward_rows<T, W, 1, 8>(x, w, b, y, mean, rstd, s, eps, tpr, num_sms, stream);
-    else e = forward_rows<T, W, 1, 16>(x, w, b, y, mean, rstd, s, eps, tpr, num_sms, stream);
+    e = nv <= 1 ? forward_rows<T, W, 1, 1>(x, w, b, y, mean, rstd, s, eps, tpr, num_sms, stream)
+                : forward_rows<T, W, 1, 4>(x, w, b, y, mean, rstd, s, eps, tpr, num_sms, stream);
   } else {
     const unsigned grid = (unsigned)std::min<long long>(s.rows, (long long)num_sms * 64);
     e = launch_kernel_ex(ln_forward_any_kernel<T, W>, grid, LN_THREADS, 0, stream, 1, pdl_enabled(), static_cast<const T*>(x),
@@ -819,10 +869,9 @@ int forward(const void* x, const void* w, const void* b, void* y, float* mean, f
   return SX_OK;
 }
 
-template <typename T, typename W, int VEC, int NV>
+template <typename T, typename W, int VEC, int NV, int BLOCK = 512>
 int backward_rows(const void* dy, const void* x, const float* mean, const float* rstd, const void* w, void* dx, float* part, const LnShape& s,
                   int tpr, int num_sms, cudaStream_t stream, int* parts) {
-  constexpr int BLOCK = 512;
   const long long per_cta = BLOCK / tpr;
   const size_t smem = part != nullptr ? (size_t)(BLOCK / tpr) * s.cols * 8 : 0;
   *parts = (int)std::min<long long>((s.rows + per_cta - 1) / per_cta, std::min(num_sms, LN_PARTS));
@@ -883,9 +932,9 @@ int backward(const void* dy, const void* x, const float* mean, const float* rstd
   float* to = params ? part : nullptr;
   int parts = 0, rc = SX_OK;
   cudaError_t e;
-  const int tpr = threads_per_row(vec ? s.cols / VEC : s.cols, vec ? MOST : 4, 512, few);
+  const int tpr = vec ? threads_per_row(s.cols / VEC, MOST, 512, few) : std::max(128, threads_per_row(s.cols, 4, 1024, few));
   const long long nv = ((vec ? s.cols / VEC : s.cols) + tpr - 1) / tpr;
-  if (s.rows > 0 && s.cols <= 512 * 16) {
+  if (s.rows > 0 && s.cols <= (vec ? 512 * 16 : LN_SINGLE_BACKWARD)) {
     const int ring = vec ? ring_groups(s, sizeof(T), tpr, num_sms) : 0;
     if (ring > 0)
       rc = nv <= 1 ? backward_ring<T, W, VEC, 1>(dy, x, mean, rstd, w, dx, to, s, tpr, ring, dev, stream, &parts)
@@ -894,25 +943,33 @@ int backward(const void* dy, const void* x, const float* mean, const float* rstd
       rc = nv <= 1 ? backward_rows<T, W, VEC, 1>(dy, x, mean, rstd, w, dx, to, s, tpr, num_sms, stream, &parts)
                    : backward_rows<T, W, VEC, MOST>(dy, x, mean, rstd, w, dx, to, s, tpr, num_sms, stream, &parts);
     else
-      rc = nv <= 1   ? backward_rows<T, W, 1, 1>(dy, x, mean, rstd, w, dx, to, s, tpr, num_sms, stream, &parts)
-           : nv <= 4 ? backward_rows<T, W, 1, 4>(dy, x, mean, rstd, w, dx, to, s, tpr, num_sms, stream, &parts)
-                     : backward_rows<T, W, 1, 16>(dy, x, mean, rstd, w, dx, to, s, tpr, num_sms, stream, &parts);
+      rc = nv <= 1 ? backward_rows<T, W, 1, 1, 1024>(dy, x, mean, rstd, w, dx, to, s, tpr, num_sms, stream, &parts)
+                   : backward_rows<T, W, 1, 4, 1024>(dy, x, mean, rstd, w, dx, to, s, tpr, num_sms, stream, &parts);
     if (rc != SX_OK || !params) return rc;
   } else if (s.rows > 0) {
-    if (params) {  // before dx: dx may overwrite dy
-      parts = (int)std::min<long long>(std::min<long long>(LN_PARTS, (s.rows + 7) / 8), std::max<long long>(1, num_sms * 8LL / tiles));
-      e = launch_kernel_ex(ln_backward_columns_kernel<T>, (unsigned)std::min<long long>(tiles * parts, num_sms * 8LL), LN_THREADS, 0, stream,
-                           1, pdl, static_cast<const T*>(dy), static_cast<const T*>(x), mean, rstd, part, s.rows, s.cols, s.ldd, s.ldx, parts);
-      if (e != cudaSuccess) return launch_failed(e, "layer norm backward launch failed");
-      count_launches(1);
-    }
-    if (dx != nullptr) {
-      e = launch_kernel_ex(ln_backward_dx_any_kernel<T, W>, (unsigned)std::min<long long>(s.rows, (long long)num_sms * 64), LN_THREADS, 0,
-                           stream, 1, pdl, static_cast<const T*>(dy), static_cast<const T*>(x), mean, rstd, static_cast<const W*>(w),
-                           static_cast<T*>(dx), s.rows, s.cols, s.ldd, s.ldx, s.ldy);
-      if (e != cudaSuccess) return launch_failed(e, "layer norm backward launch failed");
-      count_launches(1);
-    }
+    auto any = [&](auto n) -> cudaError_t {
+      constexpr int V = decltype(n)::value;
+      cudaError_t err = cudaSuccess;
+      if (params) {  // before dx: dx may overwrite dy
+        const long long vtiles = (s.cols / V + 31) / 32;
+        parts = (int)std::min<long long>(std::min<long long>(LN_PARTS, (s.rows + 31) / 32), std::max<long long>(1, num_sms * 8LL / vtiles));
+        err = launch_kernel_ex(ln_backward_columns_kernel<T, V>, (unsigned)std::min<long long>(vtiles * parts, num_sms * 8LL), LN_THREADS, 0,
+                               stream, 1, pdl, static_cast<const T*>(dy), static_cast<const T*>(x), mean, rstd, part, s.rows, s.cols, s.ldd,
+                               s.ldx, parts);
+        if (err != cudaSuccess) return err;
+        count_launches(1);
+      }
+      if (dx != nullptr) {
+        err = launch_kernel_ex(ln_backward_dx_any_kernel<T, W, V>, (unsigned)std::min<long long>(s.rows, (long long)num_sms * 64), 512, 0, stream,
+                               1, pdl, static_cast<const T*>(dy), static_cast<const T*>(x), mean, rstd, static_cast<const W*>(w),
+                               static_cast<T*>(dx), s.rows, s.cols, s.ldd, s.ldx, s.ldy);
+        if (err != cudaSuccess) return err;
+        count_launches(1);
+      }
+      return err;
+    };
+    e = vec ? any(std::integral_constant<int, VEC>{}) : any(std::integral_constant<int, 1>{});
+    if (e != cudaSuccess) return launch_failed(e, "layer norm backward launch failed");
   }
   if (params) {
     e = launch_kernel_ex(ln_backward_finish_kernel<W>, (unsigned)tiles, 1024u, 0, stream, 1, pdl, (const float*)part,
@@ -925,7 +982,7 @@ int backward(const void* dy, const void* x, const float* mean, const float* rstd
 
 int check_shape(int64_t rows, int64_t cols, int32_t dtype, int32_t param_dtype) {
   if (rows < 0 || cols <= 0) return fail_fmt(SX_ERR_INVALID, "layer norm needs rows >= 0 and cols >= 1");
-  if (cols > 0x7fffffffLL) return fail_fmt(SX_ERR_INVALID, "dimension exceeds 2^31-1");
+  if (cols > 0x3fffffffLL) return fail_fmt(SX_ERR_INVALID, "cols exceeds 2^30-1");
   if (dtype != SYMPLEX_DT_F32 && dtype != SYMPLEX_DT_BF16)
     return fail_fmt(SX_ERR_INVALID, "dtype %d not supported (F32=9, BF16=11)", dtype);
   if (param_dtype != dtype && param_dtype != SYMPLEX_DT_F32)
