@@ -21,6 +21,7 @@
 #include "epilogue.cuh"
 #include "gemm_params.h"
 #include "host_api.h"
+#include "options.h"
 #include "sm100_ptx.cuh"
 
 namespace sx {
@@ -48,6 +49,7 @@ struct CeCfg {
 // One product: tiles of [M, N] over K.
 struct CeJob {
   int M, N, K, m_tiles, n_tiles, group_m;
+  int chunks, chunk_kb;  // k cut into parts of chunk_kb k-blocks, each a list of tiles of its own (CE_PROD's dx; else 1)
 };
 
 struct CeKernelParams {
@@ -62,14 +64,15 @@ struct CeKernelParams {
   const float* lse;
   const float* dloss;
   const float* scale;
-  const float* acc_in;
-  int dx_bf16;      // CE_PROD: job 0 writes bf16 dx (last piece), else the fp32 accumulator
+  int dx_add;       // CE_PROD: job 0 adds to what the accumulators hold
+  const float* dx_acc;
+  int dx_bf16;      // CE_PROD: job 0 writes bf16 dx (last piece, one chunk), else the fp32 accumulators
   int tma_out[2];   // outputs written by TMA (16-byte aligned rows), else element by element
   void* out[2];
 };
 
 struct CeTile {
-  int job, m0, n0, kb;
+  int job, m0, n0, chunk, kb0, kb;  // k-blocks kb0 .. kb0 + kb
 };
 
 // The tiles of one pair, in order. CE_LSE / CE_GRAD: every pairs-th tile. CE_PROD: every pairs-th tile of job 0 (dx); the pairs that
@@ -82,13 +85,13 @@ struct CeWork {
 
   __host__ __device__ CeWork(const CeKernelParams& p_, int pair_, int pairs_) : p(p_), pair(pair_), pairs(pairs_), stage(0) {
     next = pair;
-    end = p.job[0].m_tiles * p.job[0].n_tiles;
+    end = p.job[0].m_tiles * p.job[0].n_tiles * p.job[0].chunks;
     stride = pairs;
   }
   __host__ __device__ bool get(CeTile* t) {
     if constexpr (kMode == CE_PROD) {
       while (next >= end) {
-        const int t0 = p.job[0].m_tiles * p.job[0].n_tiles, t1 = p.job[1].m_tiles * p.job[1].n_tiles;
+        const int t0 = p.job[0].m_tiles * p.job[0].n_tiles * p.job[0].chunks, t1 = p.job[1].m_tiles * p.job[1].n_tiles;
         const int full = t0 % pairs;  // pairs 0 .. full-1 have one job-0 tile more
         if (stage == 0) {
           stage = 1;
@@ -109,15 +112,21 @@ struct CeWork {
     }
     const int job = kMode == CE_PROD && stage > 0 ? 1 : 0;
     const CeJob& j = p.job[job];
+    const int per_chunk = j.m_tiles * j.n_tiles;
+    const int chunk = kMode == CE_PROD ? next / per_chunk : 0;
+    const int at = kMode == CE_PROD ? next - chunk * per_chunk : next;
     const int band = j.group_m * j.n_tiles;  // bands of group_m tile rows, column by column: operands of a band stay in L2
-    const int g = next / band;
+    const int g = at / band;
     const int first_m = g * j.group_m;
     const int gsz = j.m_tiles - first_m < j.group_m ? j.m_tiles - first_m : j.group_m;
-    const int in_band = next - g * band;
+    const int in_band = at - g * band;
+    const int all = (j.K + Cfg::BK - 1) / Cfg::BK;
     t->job = job;
     t->m0 = (first_m + in_band % gsz) * Cfg::BM;
     t->n0 = (in_band / gsz) * Cfg::BN;
-    t->kb = (j.K + Cfg::BK - 1) / Cfg::BK;
+    t->chunk = chunk;
+    t->kb0 = kMode == CE_PROD ? chunk * j.chunk_kb : 0;
+    t->kb = kMode == CE_PROD ? (all - t->kb0 < j.chunk_kb ? all - t->kb0 : j.chunk_kb) : all;
     next += stride;
     return true;
   }
@@ -206,7 +215,7 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
       for (Work w(p, pair_id, num_pairs); ok && w.get(&t);) {
         const int my_m0 = t.m0 + int(cta_rank) * Cfg::ROWS;
         const int my_n0 = t.n0 + int(cta_rank) * 128;
-        for (int kb = 0; kb < t.kb; ++kb) {
+        for (int kb = t.kb0; kb < t.kb0 + t.kb; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1, &abort_flag, wait_ns)) { ok = false; break; }
           uint8_t* sa = tiles + stage * Cfg::STAGE_BYTES;
           uint8_t* sb = sa + Cfg::A_BYTES;
@@ -467,8 +476,8 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
             auto strip = [&](const uint32_t (&r)[32], int cb) {
 #pragma unroll
               for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-              if (t.job == 0 && p.acc_in != nullptr && row_ok) {
-                const float* a = p.acc_in + (long long)row * job.N + cb;
+              if (t.job == 0 && p.dx_add && row_ok) {
+                const float* a = p.dx_acc + ((long long)t.chunk * job.M + row) * job.N + cb;
                 if (cb + 32 <= job.N && (job.N & 3) == 0) {
 #pragma unroll
                   for (int j = 0; j < 8; ++j) {
@@ -488,7 +497,7 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
             };
             auto plain = [&](int cb) {  // rows that a TMA store cannot take
               if (!row_ok) return;
-              const long long off = (long long)row * job.N + cb;
+              const long long off = ((long long)t.chunk * job.M + row) * job.N + cb;
 #pragma unroll
               for (int j = 0; j < 32; ++j) {
                 if (cb + j >= job.N) break;
@@ -513,7 +522,7 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) {
-                  tma_store_3d(om, staging, col0, row0, 0);
+                  tma_store_3d(om, staging, col0, row0, t.chunk);
                   bulk_commit_group();
                 }
                 strip(r1, col0 + 32);
@@ -531,7 +540,7 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
-              tma_store_3d(om, staging, f32 && second ? col0 + 32 : col0, row0, 0);
+              tma_store_3d(om, staging, f32 && second ? col0 + 32 : col0, row0, t.chunk);
               bulk_commit_group();
             }
             stored = true;
@@ -573,17 +582,19 @@ int map_of(CUtensorMap* out, const CeMatrix& m, uint32_t box_cols, uint32_t box_
   return encode_tensor_map_3d(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, m.p, dims, strides, box);
 }
 
-int out_map(CUtensorMap* out, const void* p, long long rows, long long cols, long long ld, bool f32) {
+int out_map(CUtensorMap* out, const void* p, long long rows, long long cols, long long ld, bool f32, int planes = 1) {
   const int eb = f32 ? 4 : 2;
-  const uint64_t dims[3] = {(uint64_t)cols, (uint64_t)rows, 1};
+  const uint64_t dims[3] = {(uint64_t)cols, (uint64_t)rows, (uint64_t)planes};
   const uint64_t strides[2] = {(uint64_t)ld * eb, (uint64_t)rows * ld * eb};
   const uint32_t box[3] = {(uint32_t)(128 / eb), 32, 1};
   return encode_tensor_map_3d(out, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p, dims, strides, box);
 }
 
 // 512-row tiles or 256-row ones: fewer waves x area per tile over the tensor-pipe share each shape reaches on large products
-// (0.875 and 0.80, measured for the general pair kernel).
+// (0.875 and 0.80, measured for the general pair kernel). The option "pair_mode" decides here as it does there.
 int row_blocks(long long M, long long N, int num_sms) {
+  const int64_t mode = options().pair_mode.load(std::memory_order_relaxed);
+  if (mode == 1 || mode == 2) return (int)mode;
   if (M <= 256) return 1;
   const long long pairs = num_sms / 2, nt = (N + 255) / 256;
   const long long w1 = ((M + 255) / 256 * nt + pairs - 1) / pairs, w2 = ((M + 511) / 512 * nt + pairs - 1) / pairs;
@@ -596,6 +607,8 @@ CeJob job_of(long long M, long long N, long long K, int mb) {
   j.m_tiles = (int)((M + 256 * mb - 1) / (256 * mb));
   j.n_tiles = (int)((N + 255) / 256);
   j.group_m = mb == 2 ? 4 : 8;
+  j.chunks = 1;
+  j.chunk_kb = (int)((K + 63) / 64);
   return j;
 }
 
@@ -621,8 +634,28 @@ CeKernelParams common(const CeCommon& c) {
 
 }  // namespace
 
+int ce_dx_chunks(long long T, long long H, long long n) {
+  // dx has T / 512 x H / 256 tiles of n / 64 k-blocks each. Where these are fewer than the 74 CTA pairs, the longest of them would
+  // outlast everything else (1999 x 768 tokens: 12 tiles of 524 k-blocks, 290 us of a product of 330): as many parts as make a wave,
+  // none shorter than 16 k-blocks.
+  const long long tiles = ((T + 511) / 512) * ((H + 255) / 256), nkb = (n + 63) / 64;
+  if (tiles >= 74) return 1;
+  return (int)std::max<long long>(1, std::min((74 + tiles - 1) / tiles, nkb / 16));
+}
+long long ce_piece_of_waves(long long T, long long V, long long most) {
+  const long long m = (T + 511) / 512, columns = (V + 255) / 256;
+  auto waves = [&](long long c) { return (m * c + 73) / 74; };
+  long long best = most / 256;
+  double least = 1e30;
+  for (long long c = most / 256; c >= most / 512 && c > 0; --c) {
+    const double cost = columns / c * (waves(c) + 0.5) + (columns % c ? waves(columns % c) + 0.5 : 0);
+    if (cost < least) least = cost, best = c;
+  }
+  return best * 256;
+}
+
 int ce_forward_parts(long long T, long long V, int num_sms) { return (int)((V + 255) / 256) * row_blocks(T, V, num_sms); }
-int ce_forward_parts_most(long long V) { return (int)((V + 255) / 256) * 2; }
+int ce_forward_parts_most(long long V) { return (int)((V + 255) / 256) * 2; }  // whatever the tile shape
 
 int launch_ce_forward(const CeCommon& c, const CeForward& a, cudaStream_t stream) {
   const int mb = row_blocks(a.x.rows, a.W.rows, c.num_sms);
@@ -663,7 +696,8 @@ int launch_ce_grad(const CeCommon& c, const CeGrad& a, cudaStream_t stream) {
 
 int launch_ce_products(const CeCommon& c, const CeProducts& a, cudaStream_t stream) {
   const long long T = a.x.rows, H = a.x.cols, n = a.W.rows;
-  const int mb = std::min(T, n) <= 256 ? 1 : 2;
+  const int64_t mode = options().pair_mode.load(std::memory_order_relaxed);
+  const int mb = mode == 1 || mode == 2 ? (int)mode : std::min(T, n) <= 256 ? 1 : 2;
   CUtensorMap in[4], out[2] = {};
   int rc = map_of(&in[0], a.G, 64, 128 * mb);          // dx: A = G, k = vocabulary
   if (rc == SX_OK) rc = map_of(&in[1], a.W, 64, 64);   //     B = W, MN-major
@@ -673,21 +707,26 @@ int launch_ce_products(const CeCommon& c, const CeProducts& a, cudaStream_t stre
   CeKernelParams p = common(c);
   p.job[0] = job_of(T, H, n, mb);
   p.job[1] = job_of(n, H, T, mb);
+  // The widest piece (the first one) sets how many accumulators there are; a narrower one may fill fewer of them.
+  const long long nkb = (n + 63) / 64;
+  p.job[0].chunk_kb = (int)((nkb + a.chunks - 1) / a.chunks);
+  p.job[0].chunks = (int)((nkb + p.job[0].chunk_kb - 1) / p.job[0].chunk_kb);
   p.scale = a.scale;
-  p.acc_in = a.acc_in;
-  p.dx_bf16 = a.acc_out == nullptr;
-  p.out[0] = p.dx_bf16 ? a.dx : a.acc_out;
+  p.dx_acc = a.acc;
+  p.dx_add = a.first ? 0 : 1;
+  p.dx_bf16 = a.chunks == 1 && a.last;
+  p.out[0] = p.dx_bf16 ? a.dx : a.acc;
   p.out[1] = a.dW;
   for (int j = 0; j < 2; ++j) {
     const bool f32 = j == 0 && !p.dx_bf16;
     p.tma_out[j] = (H * (f32 ? 4 : 2)) % 16 == 0 && reinterpret_cast<uintptr_t>(p.out[j]) % 16 == 0;
-    if (p.tma_out[j] && (rc = out_map(&out[j], p.out[j], j == 0 ? T : n, H, H, f32)) != SX_OK) return rc;
+    if (p.tma_out[j] && (rc = out_map(&out[j], p.out[j], j == 0 ? T : n, H, H, f32, j == 0 ? p.job[0].chunks : 1)) != SX_OK) return rc;
   }
-  const long long t0 = (long long)p.job[0].m_tiles * p.job[0].n_tiles, t1 = (long long)p.job[1].m_tiles * p.job[1].n_tiles;
+  const long long t0 = (long long)p.job[0].m_tiles * p.job[0].n_tiles * p.job[0].chunks, t1 = (long long)p.job[1].m_tiles * p.job[1].n_tiles;
   if (t0 + t1 > 0x3fffffffLL) return set_last_error(SX_ERR_INVALID, "the problem has more than 2^30-1 tiles");
   const long long pairs = std::min<long long>(t0 + t1, c.num_sms / 2);
   if (t0 % pairs != 0) {
-    const long long each = (n + T / 2) / T;  // dW tiles that take as long as one dx tile
+    const long long tkb = (T + 63) / 64, each = (p.job[0].chunk_kb + tkb / 2) / tkb;  // dW tiles that take as long as one of dx
     p.first_extra = (int)std::min<long long>(t1, each * (pairs - t0 % pairs));
   }
   return mb == 2 ? launch<CE_PROD, 2>(in, out, p, t0 + t1, c.num_sms, stream) : launch<CE_PROD, 1>(in, out, p, t0 + t1, c.num_sms, stream);

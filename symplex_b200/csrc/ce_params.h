@@ -43,16 +43,23 @@ struct CeGrad {
 };
 int launch_ce_grad(const CeCommon& c, const CeGrad& a, cudaStream_t stream);
 
-// dx (+)= G W and dW = G^T x of one piece, times *scale where scale is not null. dx goes to acc (fp32 [T, H]) until the last
-// piece, which writes bf16 dx = (acc + G W) * scale; acc_in is null for the first piece.
+// dx (+)= G W and dW = G^T x of one piece, times *scale where scale is not null. dx goes to `chunks` fp32 accumulators [T, H] in a row
+// (its k, the vocabulary, cut into as many parts), to which pieces after the first one add. With one chunk the last piece writes
+// bf16 dx = (acc + G W) * scale instead; with several, launch_ce_join does it in the end.
 struct CeProducts {
   CeMatrix G, x, W;  // [T, n], [T, H], [n, H]
-  const float* acc_in;
-  float* acc_out;  // null: last piece, dx is written
+  float* acc;
+  int chunks;
+  bool first, last;
   void* dx;
-  void* dW;        // [n, H] packed
+  void* dW;  // [n, H] packed
   const float* scale;
 };
 int launch_ce_products(const CeCommon& c, const CeProducts& a, cudaStream_t stream);
+// Chunks for a problem whose widest piece has n columns, on a device with 148 SMs (the workspace is sized without one).
+int ce_dx_chunks(long long T, long long H, long long n);
+// Columns of a piece, at most `most` (a multiple of 256): those with which the pieces' logits take the fewest waves of tiles, half
+// a wave counted for each piece's start and end.
+long long ce_piece_of_waves(long long T, long long V, long long most);
 
 }  // namespace sx

@@ -154,42 +154,45 @@ __device__ __forceinline__ float tf32_part(float x) {
 }
 
 // fp32: G and its transpose from a piece of logits, both as the {hi, lo} tf32 planes the products read (hi = tf32(g), lo =
-// tf32(g - hi); planes plane_g / plane_t values apart). 32 x 32 tiles, the transpose through shared memory.
+// tf32(g - hi)): G in parts of `chunk` columns (a multiple of 32), [part][2][rows][chunk], the columns of the last part past the
+// piece 0; G^T [2][cols][ldt], planes plane_t values apart. 32 x 32 tiles, the transpose through shared memory.
 __global__ void __launch_bounds__(256)
 ce_piece_grad_kernel(const float* __restrict__ L, long long ld, int cols, long long v0, const long long* __restrict__ targets,
                      const float* __restrict__ lse, const float* __restrict__ dloss, const float* __restrict__ scale,
-                     float* __restrict__ G, long long ldg, long long plane_g, float* __restrict__ GT, long long ldt, long long plane_t,
+                     float* __restrict__ G, long long chunk, float* __restrict__ GT, long long ldt, long long plane_t,
                      long long rows, long long V, long long ignore) {
   __shared__ float tile[32][33];
   pdl_launch_dependents();
   pdl_wait_prior_grids();
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
-  const long long row_tiles = (rows + 31) / 32, tiles = row_tiles * ((cols + 31) / 32);
+  const long long padded = (cols + chunk - 1) / chunk * chunk;
+  const long long row_tiles = (rows + 31) / 32, tiles = row_tiles * (padded / 32);
   for (long long i = blockIdx.x; i < tiles; i += gridDim.x) {
     const long long r0 = i % row_tiles * 32;
-    const int c0 = int(i / row_tiles) * 32;
+    const long long c0 = i / row_tiles * 32, part = c0 / chunk;
+    float* const g_part = G + part * 2 * rows * chunk + (c0 - part * chunk);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const long long r = r0 + y + 8 * j;
-      const int c = c0 + x;
+      const long long c = c0 + x;
       float g = 0.0f;
-      if (r < rows && c < cols) {
+      if (r < rows) {
         const long long at = targets[r];
-        if (at != ignore) {
+        if (c < cols && at != ignore) {
           const float s = scale != nullptr ? *scale : dloss[r];
           g = (exp2f((L[r * ld + c] - lse[r]) * LOG2E) - (at == v0 + c ? 1.0f : 0.0f)) * s;
           if (at < 0 || at >= V) g = __int_as_float(0x7fc00000);
         }
         const float hi = tf32_part(g);
-        G[r * ldg + c] = hi;
-        G[plane_g + r * ldg + c] = tf32_part(g - hi);
+        g_part[r * chunk + x] = hi;
+        g_part[(rows + r) * chunk + x] = tf32_part(g - hi);
       }
       tile[y + 8 * j][x] = g;
     }
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int c = c0 + y + 8 * j;
+      const long long c = c0 + y + 8 * j;
       const long long r = r0 + x;
       if (r < rows && c < cols) {
         const float g = tile[x][y + 8 * j], hi = tf32_part(g);
@@ -198,6 +201,21 @@ ce_piece_grad_kernel(const float* __restrict__ L, long long ld, int cols, long l
       }
     }
     __syncthreads();
+  }
+}
+
+// out = (add ? out : 0) + scale * the sum of `chunks` accumulators of n values each, in their order.
+template <typename T>
+__global__ void __launch_bounds__(256)
+ce_join_kernel(const float* __restrict__ acc, int chunks, long long n, const float* __restrict__ scale, T* out, int add) {
+  pdl_launch_dependents();
+  pdl_wait_prior_grids();
+  const float f = scale != nullptr ? *scale : 1.0f;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+    float v = 0.0f;
+    for (int c = 0; c < chunks; ++c) v += acc[c * n + i];
+    v *= f;
+    out[i] = add ? T(float(out[i]) + v) : T(v);
   }
 }
 
@@ -225,7 +243,11 @@ struct Problem {
 // flops. fp32: logits of a piece of about 64 MB, with G and its transpose in two planes each four times that.
 long long piece_columns(const Problem& p, bool backward) {
   const long long T = std::max<long long>(p.T, 1);
-  if (p.bf16) return backward ? std::min(up(p.V, 8), std::max<long long>(8192, (64ll << 20) / T / 256 * 256)) : up(p.V, 8);
+  if (p.bf16 && !backward) return up(p.V, 8);
+  if (p.bf16) {
+    const long long most = std::max<long long>(8192, (64ll << 20) / T / 256 * 256);
+    return p.V <= most ? up(p.V, 8) : ce_piece_of_waves(T, p.V, most);
+  }
   return std::min(up(p.V, 8), std::max<long long>(256, (16ll << 20) / T / 256 * 256));
 }
 
@@ -233,7 +255,9 @@ long long piece_columns(const Problem& p, bool backward) {
 struct Layout {
   long long hp, tp, piece;  // padded H and T, columns of a piece (a multiple of 8)
   int pieces, parts;
-  size_t xcopy, wcopy, part, target_logit, row_loss, scale, G, acc[2];
+  int chunks;         // parts that the vocabulary is cut into for dx, each with an accumulator
+  long long chunk;    // fp32: columns of one
+  size_t xcopy, wcopy, part, target_logit, row_loss, scale, G, acc;
   size_t xs, xts, ws, wts, logits, GT;  // fp32: operand planes, a piece's logits, G^T
   size_t total;
 };
@@ -245,6 +269,22 @@ Layout layout(const Problem& p, bool backward) {
   w.piece = piece_columns(p, backward);
   w.pieces = (int)((p.V + w.piece - 1) / w.piece);
   w.parts = p.bf16 ? ce_forward_parts_most(p.V) : w.pieces;
+  w.chunks = 1;
+  w.chunk = up(w.piece, 32);
+  if (backward && p.bf16) {
+    // counted as the kernel cuts them: parts of as many k-blocks each, the last one shorter
+    const long long nkb = (std::min(w.piece, p.V) + 63) / 64, c = ce_dx_chunks(p.T, p.H, std::min(w.piece, p.V)), kb = (nkb + c - 1) / c;
+    w.chunks = (int)((nkb + kb - 1) / kb);
+  }
+  if (backward && !p.bf16) {
+    // dx = G W has T / 128 x H / 64 tiles over the whole piece: cut into parts of 512 columns or more until they fill the SMs
+    const long long tiles = ((p.T + 127) / 128) * ((p.H + 63) / 64);
+    const long long want = std::min<long long>((148 + tiles - 1) / tiles, w.piece / 512);
+    if (want > 1) {
+      w.chunk = up((w.piece + want - 1) / want, 32);
+      w.chunks = (int)((w.piece + w.chunk - 1) / w.chunk);
+    }
+  }
   size_t off = 0;
   auto take = [&](size_t bytes) {
     const size_t at = off;
@@ -264,12 +304,13 @@ Layout layout(const Problem& p, bool backward) {
     w.row_loss = take((size_t)p.T * 4);
   } else {
     w.scale = take(4);
-    w.G = take((size_t)p.T * w.piece * (p.bf16 ? 2 : 8));
-    if (w.pieces > 1) w.acc[0] = take((size_t)p.T * p.H * 4);
+    const long long cols = p.bf16 ? w.piece : w.chunks * w.chunk;
+    w.G = take((size_t)p.T * cols * (p.bf16 ? 2 : 8));
+    if (w.chunks > 1) w.acc = take((size_t)w.chunks * p.T * p.H * 4);
+    else if (w.pieces > 1) w.acc = take((size_t)p.T * p.H * 4 * (p.bf16 ? 1 : 2));  // fp32: from one accumulator into the other
     if (!p.bf16) {
-      if (w.pieces > 2) w.acc[1] = take((size_t)p.T * p.H * 4);
       w.xts = take((size_t)2 * p.H * w.tp * 4);
-      w.wts = take((size_t)2 * p.H * w.piece * 4);
+      w.wts = take((size_t)2 * p.H * cols * 4);
       w.GT = take((size_t)2 * w.piece * w.tp * 4);
     }
   }
@@ -329,10 +370,10 @@ int readable(bool copy, const void* p, long long rows, long long cols, long long
 
 // fp32: C[M, N] = A B^T + R from operands in {hi, lo} planes, both K contiguous.
 int split_product(const CeCommon& c, const float* A, long long lda, long long plane_a, const float* B, long long ldb, long long plane_b, float* C,
-                  long long ldc, const float* R, long long M, long long N, long long K, cudaStream_t stream) {
+                  long long ldc, const float* R, long long M, long long N, long long K, cudaStream_t stream, int batch = 1) {
   TcGemmArgs g{};
   g.M = M; g.N = N; g.K = K;
-  g.batch = 1;
+  g.batch = batch;
   g.A = A; g.lda = lda; g.a_plane_stride = plane_a;
   g.B = B; g.ldb = ldb; g.b_plane_stride = plane_b;
   g.C = C; g.ldc = ldc; g.c_batch_stride = M * ldc;
@@ -343,7 +384,7 @@ int split_product(const CeCommon& c, const float* A, long long lda, long long pl
   g.num_sms = c.num_sms;
   g.wait_limit_ns = c.wait_limit_ns;
   // the general product's rule: 128-column tiles where they fill the chip
-  g.bn = N > 64 && ((M + 127) / 128) * ((N + 127) / 128) >= c.num_sms ? 128 : 64;
+  g.bn = N > 64 && ((M + 127) / 128) * ((N + 127) / 128) * batch >= c.num_sms ? 128 : 64;
   const int rc = launch_gemm_tf32x3(g, stream);
   if (rc == SX_ERR_EXEC) return launch_failed(cudaGetLastError(), "loss product launch failed");
   if (rc == SX_OK) count_launches(1);
@@ -394,7 +435,7 @@ int backward(const Problem& p, const CeCommon& dev, const float* dloss, const lo
   if (p.bf16) {
     CeMatrix x;
     CE_TRY(readable(p.copy_x(), p.x, p.T, p.H, p.ldx, ws + w.xcopy, stream, &x));
-    float* acc = reinterpret_cast<float*>(ws + w.acc[0]);
+    float* acc = reinterpret_cast<float*>(ws + w.acc);
     for (int i = 0; i < w.pieces; ++i) {
       const long long v0 = i * w.piece, n = std::min(w.piece, p.V - v0);
       CeMatrix Wp;
@@ -417,18 +458,23 @@ int backward(const Problem& p, const CeCommon& dev, const float* dloss, const lo
       d.G = CeMatrix{ws + w.G, p.T, n, w.piece};
       d.x = x;
       d.W = Wp;
-      d.acc_in = i > 0 ? acc : nullptr;
-      d.acc_out = i < w.pieces - 1 ? acc : nullptr;
+      d.acc = acc;
+      d.chunks = w.chunks;
+      d.first = i == 0;
+      d.last = i == w.pieces - 1;
       d.dx = dx;
       d.dW = static_cast<uint8_t*>(dW) + (size_t)v0 * p.H * 2;
       d.scale = scale;
       CE_TRY(launch_ce_products(dev, d, stream));
     }
+    if (w.chunks > 1)
+      CE_LAUNCH(ce_join_kernel<__nv_bfloat16>, std::min<long long>((p.T * p.H + 255) / 256, dev.num_sms * 8LL), 256, (const float*)acc, w.chunks,
+                p.T * p.H, (const float*)scale, static_cast<__nv_bfloat16*>(dx), 0);
     return SX_OK;
   }
   auto at = [&](size_t off) { return reinterpret_cast<float*>(ws + off); };
   float *xs = at(w.xs), *xts = at(w.xts), *wsp = at(w.ws), *wts = at(w.wts), *logits = at(w.logits), *G = at(w.G), *GT = at(w.GT);
-  float* acc[2] = {at(w.acc[0]), at(w.acc[1])};
+  float* acc[2] = {at(w.acc), at(w.acc) + p.T * p.H};  // one chunk: accumulators of pieces
   const float* x = static_cast<const float*>(p.x);
   CE_TRY(prep(launch_split_tf32(x, p.ldx, 0, xs, (int)p.T, (int)p.H, (int)w.hp, 1, stream)));
   CE_TRY(prep(launch_split_tf32_transpose(x, p.ldx, 0, xts, (int)p.T, (int)p.H, (int)w.tp, 1, stream)));
@@ -436,14 +482,26 @@ int backward(const Problem& p, const CeCommon& dev, const float* dloss, const lo
     const long long v0 = i * w.piece, n = std::min(w.piece, p.V - v0);
     const float* Wp = static_cast<const float*>(p.W) + v0 * p.ldw;
     CE_TRY(prep(launch_split_tf32(Wp, p.ldw, 0, wsp, (int)n, (int)p.H, (int)w.hp, 1, stream)));
-    CE_TRY(prep(launch_split_tf32_transpose(Wp, p.ldw, 0, wts, (int)n, (int)p.H, (int)w.piece, 1, stream)));
     CE_TRY(split_product(dev, xs, w.hp, p.T * w.hp, wsp, w.hp, n * w.hp, logits, w.piece, nullptr, p.T, n, p.H, stream));
-    const long long tiles = (p.T + 31) / 32 * ((n + 31) / 32);
+    // dx: the piece in parts of the vocabulary, their planes one after the other (rows of W past the piece are 0)
+    const int chunks = (int)((n + w.chunk - 1) / w.chunk), whole = (int)(n / w.chunk);
+    const long long part_w = 2 * p.H * w.chunk;
+    if (whole > 0)
+      CE_TRY(prep(launch_split_tf32_transpose(Wp, p.ldw, w.chunk * p.ldw, wts, (int)w.chunk, (int)p.H, (int)w.chunk, whole, stream)));
+    if (whole < chunks)
+      CE_TRY(prep(launch_split_tf32_transpose(Wp + whole * w.chunk * p.ldw, p.ldw, 0, wts + whole * part_w, (int)(n - whole * w.chunk), (int)p.H,
+                                              (int)w.chunk, 1, stream)));
+    const long long tiles = (p.T + 31) / 32 * (chunks * w.chunk / 32 + 1);
     CE_LAUNCH(ce_piece_grad_kernel, std::min<long long>(tiles, dev.num_sms * 8LL), 256, (const float*)logits, w.piece, (int)n, v0, targets, lse,
-              dloss, (const float*)scale, G, w.piece, p.T * w.piece, GT, w.tp, n * w.tp, p.T, p.V, p.ignore);
-    // dx: pieces add up in 32 bits, from one accumulator into the other and at last into dx
-    float* to = i == w.pieces - 1 ? static_cast<float*>(dx) : acc[i & 1];
-    CE_TRY(split_product(dev, G, w.piece, p.T * w.piece, wts, w.piece, p.H * w.piece, to, p.H, i ? acc[(i & 1) ^ 1] : nullptr, p.T, p.H, n, stream));
+              dloss, (const float*)scale, G, w.chunk, GT, w.tp, n * w.tp, p.T, p.V, p.ignore);
+    if (w.chunks > 1) {
+      CE_TRY(split_product(dev, G, w.chunk, p.T * w.chunk, wts, w.chunk, p.H * w.chunk, acc[0], p.H, nullptr, p.T, p.H, w.chunk, stream, chunks));
+      CE_LAUNCH(ce_join_kernel<float>, std::min<long long>((p.T * p.H + 255) / 256, dev.num_sms * 8LL), 256, (const float*)acc[0], chunks, p.T * p.H,
+                (const float*)nullptr, static_cast<float*>(dx), i > 0 ? 1 : 0);
+    } else {
+      float* to = i == w.pieces - 1 ? static_cast<float*>(dx) : acc[i & 1];
+      CE_TRY(split_product(dev, G, w.chunk, p.T * w.chunk, wts, w.chunk, p.H * w.chunk, to, p.H, i ? acc[(i & 1) ^ 1] : nullptr, p.T, p.H, n, stream));
+    }
     CE_TRY(split_product(dev, GT, w.tp, n * w.tp, xts, w.tp, p.H * w.tp, static_cast<float*>(dW) + v0 * p.H, p.H, nullptr, n, p.H, p.T, stream));
   }
   return SX_OK;

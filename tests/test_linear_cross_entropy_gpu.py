@@ -14,6 +14,7 @@ import pytest
 import torch
 
 import symplex_b200 as sx
+from symplex_b200 import _capi
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -117,6 +118,19 @@ def test_medium(t, h, v, dtype):
 
 def test_several_pieces():
     _both(4096, 128, 65536, BF, "none", seed=5)
+
+
+@pytest.mark.parametrize("t,h,v,dtype", [(2049, 136, 40000, BF), (8192, 64, 5000, F32), (3000, 72, 12001, F32), (100, 300, 20011, F32)])
+def test_pieces_in_parts(t, h, v, dtype):
+    """Pieces of the vocabulary whose product dx is cut over the vocabulary once more, the last piece in fewer or shorter parts."""
+    _both(t, h, v, dtype, "mean", seed=v)
+
+
+@pytest.mark.parametrize("shape", [1, 2])
+@pytest.mark.parametrize("t,h,v", [(40, 64, 700), (600, 200, 3001), (1100, 512, 9000)])
+def test_both_tile_shapes(t, h, v, shape):
+    with _capi.option("pair_mode", shape):
+        _both(t, h, v, BF, "sum", seed=t)
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
