@@ -29,6 +29,7 @@ namespace {
 
 enum CeMode : int { CE_LSE = 0, CE_GRAD = 1, CE_PROD = 2 };
 
+// kMB = 1, 2: row blocks of 128 per CTA of a pair. kMB = 0: one CTA by itself, 128 rows.
 template <int kMB>
 struct CeCfg {
   static constexpr int ROWS = 128 * kMB;  // rows of A per CTA
@@ -44,6 +45,26 @@ struct CeCfg {
   static constexpr int TMEM_COLS = 512;
   static constexpr int STAGING_BYTES = 32 * 128;
   static constexpr int DYN_SMEM = STAGES * STAGE_BYTES + EPI_WARPS * STAGING_BYTES + 1024;
+};
+
+// At most 128 tokens. A pair's tile would be filled up to 256 rows with nothing, and its MMAs then take as long as W's rows take to
+// arrive (512 cycles for 16 KB per SM, 9 TB/s with no pause): one CTA has half the rows to multiply (1 x 4096 x 65536: 150 us on
+// pairs, 94 us alone, 5.7 TB/s; 61 x 1024 x 50257: 32 and 25 us). Columns of a tile, rows of A that
+// are copied and stages are set at launch: the tiles share the vocabulary out evenly, and the stages fill shared memory. The MMA
+// reads 128 rows of A from a stage whatever was copied; the rows behind the copied ones are other data, and nobody reads their sums.
+template <>
+struct CeCfg<0> {
+  static constexpr int ROWS = 128;
+  static constexpr int BM = 128;
+  static constexpr int BN = 256;  // at most
+  static constexpr int BK = 64;
+  static constexpr int STAGES = 12;  // at most
+  static constexpr int EPI_WARPS = 4;
+  static constexpr int THREADS = 64 + 32 * EPI_WARPS;
+  static constexpr int TMEM_COLS = 512;
+  static constexpr int STAGING_BYTES = 32 * 128;
+  static constexpr int STAGE_ROOM = 200 * 1024;
+  static constexpr int DYN_SMEM = STAGE_ROOM + EPI_WARPS * STAGING_BYTES + 1024;
 };
 
 // One product: tiles of [M, N] over K.
@@ -67,6 +88,7 @@ struct CeKernelParams {
   int dx_add;       // CE_PROD: job 0 adds to what the accumulators hold
   const float* dx_acc;
   int dx_bf16;      // CE_PROD: job 0 writes bf16 dx (last piece, one chunk), else the fp32 accumulators
+  int bn, a_bytes, stages;  // kMB = 0: columns of a tile, bytes of A in a stage, stages
   int tma_out[2];   // outputs written by TMA (16-byte aligned rows), else element by element
   void* out[2];
 };
@@ -123,7 +145,7 @@ struct CeWork {
     const int all = (j.K + Cfg::BK - 1) / Cfg::BK;
     t->job = job;
     t->m0 = (first_m + in_band % gsz) * Cfg::BM;
-    t->n0 = (in_band / gsz) * Cfg::BN;
+    t->n0 = (in_band / gsz) * (kMB == 0 ? p.bn : Cfg::BN);
     t->chunk = chunk;
     t->kb0 = kMode == CE_PROD ? chunk * j.chunk_kb : 0;
     t->kb = kMode == CE_PROD ? (all - t->kb0 < j.chunk_kb ? all - t->kb0 : j.chunk_kb) : all;
@@ -159,20 +181,28 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
                const __grid_constant__ CeKernelParams p) {
   using Cfg = CeCfg<kMB>;
   using Work = CeWork<kMode, kMB>;
-  constexpr int BN = Cfg::BN, BK = Cfg::BK, STAGES = Cfg::STAGES;
+  constexpr int BN = Cfg::BN, BK = Cfg::BK;
+  constexpr bool kPair = kMB > 0;
+  constexpr int kGroup = kPair ? 2 : 1;  // CTAs that share a tile
+  int STAGES, STAGE_BYTES, A_BYTES;
+  if constexpr (kPair) {
+    STAGES = Cfg::STAGES, STAGE_BYTES = Cfg::STAGE_BYTES, A_BYTES = Cfg::A_BYTES;
+  } else {
+    STAGES = p.stages, A_BYTES = p.a_bytes, STAGE_BYTES = p.a_bytes + p.bn * 128;
+  }
 
   extern __shared__ uint8_t dyn_smem[];
-  __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2];
+  __shared__ uint64_t full_bar[Cfg::STAGES], empty_bar[Cfg::STAGES], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_base_slot;
   __shared__ int abort_flag;
 
   uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn_smem) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const uint32_t cta_rank = cluster_ctarank();  // 0 = leader
+  const uint32_t cta_rank = kPair ? cluster_ctarank() : 0;  // 0 = leader
   const uint64_t wait_ns = p.wait_limit_ns;
-  const int pair_id = blockIdx.x >> 1;
-  const int num_pairs = gridDim.x >> 1;
+  const int pair_id = blockIdx.x / kGroup;
+  const int num_pairs = gridDim.x / kGroup;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -181,18 +211,19 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&acc_full[a], 1);
-      mbar_init(&acc_empty[a], 8 * kMB);  // every epilogue warp of both CTAs
+      mbar_init(&acc_empty[a], kGroup * Cfg::EPI_WARPS);  // every epilogue warp of both CTAs
     }
     abort_flag = 0;
     fence_mbar_init();
   }
   if (warp == 1) {
-    tmem_alloc<2>(&tmem_base_slot, Cfg::TMEM_COLS);
-    tmem_relinquish<2>();
+    tmem_alloc<kGroup>(&tmem_base_slot, Cfg::TMEM_COLS);
+    tmem_relinquish<kGroup>();
   }
   tc_fence_before_sync();
   __syncwarp();
-  cluster_sync_all();
+  if constexpr (kPair) cluster_sync_all();
+  else __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = tmem_base_slot;
   pdl_launch_dependents();
@@ -217,15 +248,18 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
         const int my_n0 = t.n0 + int(cta_rank) * 128;
         for (int kb = t.kb0; kb < t.kb0 + t.kb; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1, &abort_flag, wait_ns)) { ok = false; break; }
-          uint8_t* sa = tiles + stage * Cfg::STAGE_BYTES;
-          uint8_t* sb = sa + Cfg::A_BYTES;
+          uint8_t* sa = tiles + stage * STAGE_BYTES;
+          uint8_t* sb = sa + A_BYTES;
           if (cta_rank == 0) {
-            mbar_arrive_expect_tx(&full_bar[stage], 2 * Cfg::STAGE_BYTES);
+            mbar_arrive_expect_tx(&full_bar[stage], kGroup * STAGE_BYTES);
             armed |= 1u << stage;
             armed_phase = (armed_phase & ~(1u << stage)) | (phase << stage);
           }
-          const uint32_t leader_full = mapa_u32(smem_u32(&full_bar[stage]), 0);
-          if constexpr (kMode != CE_PROD) {
+          const uint32_t leader_full = kPair ? mapa_u32(smem_u32(&full_bar[stage]), 0) : 0;
+          if constexpr (!kPair) {
+            tma_load_3d(sa, &tmA0, &full_bar[stage], kb * BK, t.m0, 0);
+            tma_load_3d(sb, &tmB0, &full_bar[stage], kb * BK, t.n0, 0);
+          } else if constexpr (kMode != CE_PROD) {
             tma_load_3d_pair(sa, &tmA0, leader_full, kb * BK, my_m0, 0);
             tma_load_3d_pair(sb, &tmB0, leader_full, kb * BK, my_n0, 0);
           } else {
@@ -279,31 +313,35 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
       CeTile t;
       for (Work w(p, pair_id, num_pairs); ok && w.get(&t);) {
         const bool a_mn = kMode == CE_PROD && t.job == 1;
-        const uint32_t idesc = a_mn ? make_idesc(1, true, kBmn, 256, BN) : make_idesc(1, false, kBmn, 256, BN);
+        const uint32_t idesc = !kPair ? make_idesc(1, false, false, 128, p.bn) : a_mn ? make_idesc(1, true, kBmn, 256, BN) : make_idesc(1, false, kBmn, 256, BN);
         const uint64_t a_hi = a_mn ? mn_major : k_major;
         const uint32_t a_kstep = a_mn ? 16 * 128 : 32;
         const int nk = t.kb;
         // four MMAs (one 64-wide k-block) of row block `mb` into accumulator `acc`
         auto issue = [&](int acc, int mb, int s, uint32_t accumulate) {
-          const uint32_t a_addr = smem_u32(tiles + s * Cfg::STAGE_BYTES) + mb * (128 * 128);
-          const uint32_t b_addr = smem_u32(tiles + s * Cfg::STAGE_BYTES) + Cfg::A_BYTES;
+          const uint32_t a_addr = smem_u32(tiles + s * STAGE_BYTES) + mb * (128 * 128);
+          const uint32_t b_addr = smem_u32(tiles + s * STAGE_BYTES) + A_BYTES;
 #pragma unroll
           for (int k = 0; k < KSTEPS; ++k)
-            umma<2, 0>(tmem_base + acc * BN, smem_desc(a_hi, a_addr + k * a_kstep), smem_desc(b_hi, b_addr + k * b_kstep), idesc,
+            umma<kGroup, 0>(tmem_base + acc * BN, smem_desc(a_hi, a_addr + k * a_kstep), smem_desc(b_hi, b_addr + k * b_kstep), idesc,
                        accumulate | (k != 0 ? 1u : 0u));
         };
-        if constexpr (kMB == 1) {
+        auto commit = [&](uint64_t* bar) {
+          if constexpr (kPair) umma_commit_pair(bar, 3);
+          else umma_commit(bar);
+        };
+        if constexpr (kMB <= 1) {
           if (!mbar_wait<true>(&acc_empty[slot], acc_phase ^ 1, &abort_flag, wait_ns)) break;
           tc_fence_after_sync();
           for (int kb = 0; kb < nk; ++kb) {
             if (!mbar_wait(&full_bar[stage], phase, &abort_flag, wait_ns)) { ok = false; break; }
             tc_fence_after_sync();
             issue(slot, 0, stage, kb != 0 ? 1u : 0u);
-            umma_commit_pair(&empty_bar[stage], 3);
+            commit(&empty_bar[stage]);
             advance(stage, phase);
           }
           if (!ok) break;
-          umma_commit_pair(&acc_full[slot], 3);
+          commit(&acc_full[slot]);
           if (++slot == 2) { slot = 0; acc_phase ^= 1; }
         } else {
           // The tile's two row blocks share every B stage; the first and last SKEW k-blocks are issued block-major, so block 0
@@ -325,10 +363,10 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
                   tc_fence_after_sync();
                 }
                 issue(mb, mb, s, kb != 0 ? 1u : 0u);
-                if (mb == 1) umma_commit_pair(&empty_bar[s], 3);
+                if (mb == 1) commit(&empty_bar[s]);
                 advance(s, ph);
               }
-              if (ok && g1 == nk) umma_commit_pair(&acc_full[mb], 3);
+              if (ok && g1 == nk) commit(&acc_full[mb]);
             }
             for (int kb = g0; kb < g1; ++kb) advance(stage, phase);
           };
@@ -336,8 +374,8 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
           for (int kb = head_end; ok && kb < tail_begin; ++kb) {
             if (!mbar_wait(&full_bar[stage], phase, &abort_flag, wait_ns)) { ok = false; break; }
             tc_fence_after_sync();
-            const uint32_t a_addr = smem_u32(tiles + stage * Cfg::STAGE_BYTES);
-            const uint32_t b_addr = a_addr + Cfg::A_BYTES;
+            const uint32_t a_addr = smem_u32(tiles + stage * STAGE_BYTES);
+            const uint32_t b_addr = a_addr + A_BYTES;
 #pragma unroll
             for (int k = 0; k < KSTEPS; ++k) {
 #pragma unroll
@@ -345,7 +383,7 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
                 umma<2, 0>(tmem_base + mb * BN, smem_desc(a_hi, a_addr + mb * (128 * 128) + k * a_kstep),
                            smem_desc(b_hi, b_addr + k * b_kstep), idesc, 1u);
             }
-            umma_commit_pair(&empty_bar[stage], 3);
+            commit(&empty_bar[stage]);
             advance(stage, phase);
           }
           if (ok && tail_begin < nk) group(tail_begin, nk);
@@ -357,9 +395,10 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
   } else {
     // ------------------------------------------------------------ epilogue (both CTAs)
     const int q = warp & 3;  // TMEM lane quarter this warp may read
-    const int half = kMB == 1 ? 0 : (warp - 2) >> 2;
-    constexpr int STRIPS = (BN / 32) / kMB;  // 32-column strips per warp and accumulator
-    uint8_t* staging = tiles + STAGES * Cfg::STAGE_BYTES + (warp - 2) * Cfg::STAGING_BYTES;
+    const int half = kMB <= 1 ? 0 : (warp - 2) >> 2;
+    constexpr int kBlocks = kMB == 2 ? 2 : 1;
+    constexpr int STRIPS = (BN / 32) / kBlocks;  // 32-column strips per warp and accumulator
+    uint8_t* staging = tiles + (kPair ? STAGES * STAGE_BYTES : Cfg::DYN_SMEM - 1024 - Cfg::EPI_WARPS * Cfg::STAGING_BYTES) + (warp - 2) * Cfg::STAGING_BYTES;
     int slot = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
@@ -368,8 +407,9 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
     CeTile t;
     for (Work w(p, pair_id, num_pairs); ok && w.get(&t);) {
       const CeJob& job = p.job[t.job];
+      const int n_end = kPair ? job.N : min(job.N, t.n0 + p.bn);  // columns of this tile end here at the latest
 #pragma unroll 1
-      for (int blk = 0; blk < kMB; ++blk) {
+      for (int blk = 0; blk < kBlocks; ++blk) {
         if constexpr (kMB == 2) slot = blk;
         const int row0 = t.m0 + int(cta_rank) * Cfg::ROWS + blk * 128 + q * 32;  // this warp's first row
         const int row = row0 + lane;
@@ -380,7 +420,7 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
         bool counted = true;
         if constexpr (kMode != CE_PROD) {
           const long long tg = row_ok ? p.targets[row] : -1;
-          if (tg >= p.v0 && tg < p.v0 + job.N) at = int(tg - p.v0);
+          if (tg >= p.v0 && tg < p.v0 + n_end) at = int(tg - p.v0);
           if constexpr (kMode == CE_GRAD) {
             counted = row_ok && tg != p.ignore;
             if (row_ok) {
@@ -401,18 +441,18 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
           tmem_ld_32x32(taddr + 32, r1);
           tmem_ld_wait();
           const int col0 = t.n0 + c * 32;
-          if (col0 >= job.N) continue;
-          const bool second = col0 + 32 < job.N;
+          if (col0 >= n_end) continue;
+          const bool second = col0 + 32 < n_end;
           float v[32];
 
           if constexpr (kMode == CE_LSE) {
             auto strip = [&](const uint32_t (&r)[32], int cb) {
 #pragma unroll
               for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-              if (cb + 32 > job.N) {
+              if (cb + 32 > n_end) {
 #pragma unroll
                 for (int j = 0; j < 32; ++j)
-                  if (cb + j >= job.N) v[j] = -INFINITY;
+                  if (cb + j >= n_end) v[j] = -INFINITY;
               }
               const int a = at - cb;
               if (a >= 0 && a < 32) {
@@ -548,12 +588,15 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
         }
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(mapa_u32(smem_u32(&acc_empty[slot]), 0));  // leader's barrier
+        if (lane == 0) {
+          if constexpr (kPair) mbar_arrive_cluster(mapa_u32(smem_u32(&acc_empty[slot]), 0));  // leader's barrier
+          else mbar_arrive(&acc_empty[slot]);
+        }
         if constexpr (kMode == CE_LSE) {
-          if (row_ok) p.part[(long long)(t.n0 / BN * kMB + half) * job.M + row] = make_float2(m, s);
+          if (row_ok) p.part[(long long)(kPair ? t.n0 / BN * kMB + half : t.n0 / p.bn) * job.M + row] = make_float2(m, s);
         }
       }
-      if constexpr (kMB == 1) {
+      if constexpr (kMB <= 1) {
         if (++slot == 2) { slot = 0; acc_phase ^= 1; }
       } else {
         acc_phase ^= 1;
@@ -565,10 +608,11 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
   // Both CTAs stay until every remote barrier signal and paired MMA has landed.
   tc_fence_before_sync();
   __syncwarp();
-  cluster_sync_all();
+  if constexpr (kPair) cluster_sync_all();
+  else __syncthreads();
   if (warp == 1) {
     tc_fence_after_sync();
-    tmem_dealloc<2>(tmem_base, Cfg::TMEM_COLS);
+    tmem_dealloc<kGroup>(tmem_base, Cfg::TMEM_COLS);
   }
   if (threadIdx.x == 0 && abort_flag != 0 && p.status != nullptr) atomicExch(p.status, int(ST_WAIT_TIMEOUT));
 }
@@ -595,16 +639,29 @@ int out_map(CUtensorMap* out, const void* p, long long rows, long long cols, lon
 int row_blocks(long long M, long long N, int num_sms) {
   const int64_t mode = options().pair_mode.load(std::memory_order_relaxed);
   if (mode == 1 || mode == 2) return (int)mode;
+  if (M <= 128) return 0;
   if (M <= 256) return 1;
   const long long pairs = num_sms / 2, nt = (N + 255) / 256;
   const long long w1 = ((M + 255) / 256 * nt + pairs - 1) / pairs, w2 = ((M + 511) / 512 * nt + pairs - 1) / pairs;
   return (double)w2 * 2 / 0.875 <= (double)w1 / 0.80 ? 2 : 1;
 }
 
+// kMB = 0: columns of a tile, a multiple of `step` of at most 256, so that every CTA's tiles together have as few columns as can be.
+int columns_alone(long long N, int step, int num_sms) {
+  int best = 256;
+  long long least = 1LL << 62;
+  for (int bn = 256; bn >= 32; bn -= step) {
+    const long long tiles = (N + bn - 1) / bn, each = (tiles + num_sms - 1) / num_sms * bn;
+    if (each < least) least = each, best = bn;
+  }
+  return best;
+}
+
 CeJob job_of(long long M, long long N, long long K, int mb) {
   CeJob j;
   j.M = (int)M; j.N = (int)N; j.K = (int)K;
-  j.m_tiles = (int)((M + 256 * mb - 1) / (256 * mb));
+  const int bm = mb > 0 ? 256 * mb : 128;
+  j.m_tiles = (int)((M + bm - 1) / bm);
   j.n_tiles = (int)((N + 255) / 256);
   j.group_m = mb == 2 ? 4 : 8;
   j.chunks = 1;
@@ -617,8 +674,9 @@ int launch(const CUtensorMap (&in)[4], const CUtensorMap (&out)[2], const CeKern
   using Cfg = CeCfg<kMB>;
   auto kern = ce_pair_kernel<kMode, kMB>;
   SX_ENSURE_DYN_SMEM(kern, Cfg::DYN_SMEM);
-  const unsigned pairs = (unsigned)std::min<long long>(tiles, num_sms / 2);
-  const cudaError_t e = launch_kernel_ex(kern, 2 * pairs, Cfg::THREADS, Cfg::DYN_SMEM, stream, 2, pdl_enabled(), in[0], in[1], in[2], in[3],
+  constexpr int kGroup = kMB > 0 ? 2 : 1;
+  const unsigned groups = (unsigned)std::min<long long>(tiles, num_sms / kGroup);
+  const cudaError_t e = launch_kernel_ex(kern, kGroup * groups, Cfg::THREADS, Cfg::DYN_SMEM, stream, kGroup, pdl_enabled(), in[0], in[1], in[2], in[3],
                                          out[0], out[1], p);
   if (e != cudaSuccess) return launch_failed(e, "loss kernel launch failed");
   count_launches(1);
@@ -654,44 +712,65 @@ long long ce_piece_of_waves(long long T, long long V, long long most) {
   return best * 256;
 }
 
-int ce_forward_parts(long long T, long long V, int num_sms) { return (int)((V + 255) / 256) * row_blocks(T, V, num_sms); }
-int ce_forward_parts_most(long long V) { return (int)((V + 255) / 256) * 2; }  // whatever the tile shape
+int ce_forward_parts(long long T, long long V, int num_sms) {
+  const int mb = row_blocks(T, V, num_sms);
+  if (mb > 0) return (int)((V + 255) / 256) * mb;
+  const int bn = columns_alone(V, 16, num_sms);
+  return (int)((V + bn - 1) / bn);
+}
+int ce_forward_parts_most(long long T, long long V) {  // whatever the tile shape
+  return (int)std::max((V + 255) / 256 * 2, T <= 128 ? (V + 31) / 32 : 0);
+}
+
+// The logits' product of either pass: operands, tile shape, and the kernel for it.
+template <int kMode>
+static int launch_logits(const CeCommon& c, const CeMatrix& x, const CeMatrix& W, const CUtensorMap& to, CeKernelParams* p, cudaStream_t stream) {
+  const int mb = row_blocks(x.rows, W.rows, c.num_sms);
+  uint32_t a_rows = 128 * mb, b_rows = 128;
+  p->job[0] = job_of(x.rows, W.rows, x.cols, mb);
+  if (mb == 0) {
+    a_rows = (uint32_t)(x.rows + 15) / 16 * 16;
+    b_rows = (uint32_t)columns_alone(W.rows, kMode == CE_GRAD ? 64 : 16, c.num_sms);  // G leaves in blocks of 64 columns
+    p->bn = (int)b_rows;
+    p->a_bytes = (int)a_rows * 128;
+    p->stages = std::min(CeCfg<0>::STAGES, CeCfg<0>::STAGE_ROOM / (p->a_bytes + p->bn * 128));
+    p->job[0].n_tiles = (int)((W.rows + p->bn - 1) / p->bn);
+  }
+  CUtensorMap in[4] = {};
+  const CUtensorMap out[2] = {to, CUtensorMap{}};
+  int rc = map_of(&in[0], x, 64, a_rows);
+  if (rc == SX_OK) rc = map_of(&in[1], W, 64, b_rows);
+  if (rc != SX_OK) return rc;
+  const long long tiles = (long long)p->job[0].m_tiles * p->job[0].n_tiles;
+  if (tiles > 0x7fffffffLL) return set_last_error(SX_ERR_INVALID, "the problem has more than 2^31-1 tiles");
+  switch (mb) {
+    case 0: return launch<kMode, 0>(in, out, *p, tiles, c.num_sms, stream);
+    case 1: return launch<kMode, 1>(in, out, *p, tiles, c.num_sms, stream);
+    default: return launch<kMode, 2>(in, out, *p, tiles, c.num_sms, stream);
+  }
+}
 
 int launch_ce_forward(const CeCommon& c, const CeForward& a, cudaStream_t stream) {
-  const int mb = row_blocks(a.x.rows, a.W.rows, c.num_sms);
-  CUtensorMap in[4] = {}, out[2] = {};
-  int rc = map_of(&in[0], a.x, 64, 128 * mb);
-  if (rc == SX_OK) rc = map_of(&in[1], a.W, 64, 128);
-  if (rc != SX_OK) return rc;
   CeKernelParams p = common(c);
-  p.job[0] = job_of(a.x.rows, a.W.rows, a.x.cols, mb);
   p.targets = a.targets;
   p.V = a.W.rows;
   p.part = a.part;
   p.target_logit = a.target_logit;
-  const long long tiles = (long long)p.job[0].m_tiles * p.job[0].n_tiles;
-  if (tiles > 0x7fffffffLL) return set_last_error(SX_ERR_INVALID, "the problem has more than 2^31-1 tiles");
-  return mb == 2 ? launch<CE_LSE, 2>(in, out, p, tiles, c.num_sms, stream) : launch<CE_LSE, 1>(in, out, p, tiles, c.num_sms, stream);
+  return launch_logits<CE_LSE>(c, a.x, a.W, CUtensorMap{}, &p, stream);
 }
 
 int launch_ce_grad(const CeCommon& c, const CeGrad& a, cudaStream_t stream) {
-  const int mb = row_blocks(a.x.rows, a.W.rows, c.num_sms);
-  CUtensorMap in[4] = {}, out[2] = {};
-  int rc = map_of(&in[0], a.x, 64, 128 * mb);
-  if (rc == SX_OK) rc = map_of(&in[1], a.W, 64, 128);
-  if (rc == SX_OK) rc = out_map(&out[0], a.G, a.x.rows, a.W.rows, a.ldg, false);
+  CUtensorMap to{};
+  const int rc = out_map(&to, a.G, a.x.rows, a.W.rows, a.ldg, false);
   if (rc != SX_OK) return rc;
   CeKernelParams p = common(c);
-  p.job[0] = job_of(a.x.rows, a.W.rows, a.x.cols, mb);
   p.targets = a.targets;
   p.lse = a.lse;
   p.dloss = a.dloss;
   p.v0 = a.v0;
   p.V = a.V;
   p.ignore = a.ignore;
-  const long long tiles = (long long)p.job[0].m_tiles * p.job[0].n_tiles;
-  if (tiles > 0x7fffffffLL) return set_last_error(SX_ERR_INVALID, "the problem has more than 2^31-1 tiles");
-  return mb == 2 ? launch<CE_GRAD, 2>(in, out, p, tiles, c.num_sms, stream) : launch<CE_GRAD, 1>(in, out, p, tiles, c.num_sms, stream);
+  return launch_logits<CE_GRAD>(c, a.x, a.W, to, &p, stream);
 }
 
 int launch_ce_products(const CeCommon& c, const CeProducts& a, cudaStream_t stream) {

@@ -28,7 +28,7 @@ struct CeForward {
   float* target_logit;
 };
 int ce_forward_parts(long long T, long long V, int num_sms);
-int ce_forward_parts_most(long long V);  // upper bound over T and SM counts
+int ce_forward_parts_most(long long T, long long V);  // upper bound over SM counts
 int launch_ce_forward(const CeCommon& c, const CeForward& a, cudaStream_t stream);
 
 // G[t][v] = (exp(x W^T - lse) - [v0 + v = target]) * (dloss ? dloss[t] : 1), 0 in ignored rows, NaN where the target is none.

@@ -126,6 +126,12 @@ def test_pieces_in_parts(t, h, v, dtype):
     _both(t, h, v, dtype, "mean", seed=v)
 
 
+@pytest.mark.parametrize("t", [1, 15, 16, 17, 61, 127, 128, 129])
+@pytest.mark.parametrize("h,v", [(64, 33), (200, 4736), (136, 40009), (1024, 20000)])
+def test_few_tokens(t, h, v):
+    _both(t, h, v, BF, "none" if t % 2 else "mean", seed=t)
+
+
 @pytest.mark.parametrize("shape", [1, 2])
 @pytest.mark.parametrize("t,h,v", [(40, 64, 700), (600, 200, 3001), (1100, 512, 9000)])
 def test_both_tile_shapes(t, h, v, shape):
