@@ -82,6 +82,7 @@ struct CeKernelParams {
   long long v0, V, ignore;
   float2* part;
   float* target_logit;
+  unsigned* done;   // CE_LSE: set to 0 for the kernel behind this one
   const float* lse;
   const float* dloss;
   const float* scale;
@@ -228,6 +229,7 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
   const uint32_t tmem_base = tmem_base_slot;
   pdl_launch_dependents();
   pdl_wait_prior_grids();
+  if (kMode == CE_LSE && blockIdx.x == 0 && threadIdx.x == 0) *p.done = 0;
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer (both CTAs)
@@ -756,6 +758,7 @@ int launch_ce_forward(const CeCommon& c, const CeForward& a, cudaStream_t stream
   p.V = a.W.rows;
   p.part = a.part;
   p.target_logit = a.target_logit;
+  p.done = a.done;
   return launch_logits<CE_LSE>(c, a.x, a.W, CUtensorMap{}, &p, stream);
 }
 

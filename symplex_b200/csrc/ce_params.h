@@ -26,6 +26,7 @@ struct CeForward {
   const long long* targets;
   float2* part;  // [ce_forward_parts][T]
   float* target_logit;
+  unsigned* done;  // set to 0
 };
 int ce_forward_parts(long long T, long long V, int num_sms);
 int ce_forward_parts_most(long long T, long long V);  // upper bound over SM counts

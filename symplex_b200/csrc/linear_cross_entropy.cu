@@ -41,11 +41,12 @@ __device__ __forceinline__ RowPart join(RowPart a, RowPart b) {
 // One CTA per row of a piece of logits L[T, ld]: its part of the row, and the target's logit if it is in the piece.
 __global__ void __launch_bounds__(256)
 ce_piece_rows_kernel(const float* __restrict__ L, long long ld, int cols, long long v0, const long long* __restrict__ targets,
-                     float2* __restrict__ part, float* __restrict__ target_logit) {
+                     float2* __restrict__ part, float* __restrict__ target_logit, unsigned* __restrict__ done) {
   __shared__ float2 red[8];
   pdl_launch_dependents();
   pdl_wait_prior_grids();
   const long long t = blockIdx.x;
+  if (t == 0 && threadIdx.x == 0) *done = 0;
   const float* row = L + t * ld;
   float top = -INFINITY;
   bool nan = false;
@@ -71,40 +72,15 @@ ce_piece_rows_kernel(const float* __restrict__ L, long long ld, int cols, long l
   }
 }
 
-// One warp per row: the parts [parts][T] joined, lse and the row's loss.
-__global__ void __launch_bounds__(256)
-ce_finish_kernel(const float2* __restrict__ part, int parts, const float* __restrict__ target_logit,
-                 const long long* __restrict__ targets, float* __restrict__ loss, float* __restrict__ lse, long long T, long long V,
-                 long long ignore) {
-  pdl_launch_dependents();
-  pdl_wait_prior_grids();
-  const int lane = threadIdx.x & 31;
-  const long long t = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (t >= T) return;
-  RowPart r{-INFINITY, 0.0f};
-  for (int i = lane; i < parts; i += 32) {
-    const float2 p = part[(long long)i * T + t];
-    r = join(r, {p.x, p.y});
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) r = join(r, {__shfl_xor_sync(0xffffffffu, r.m, o), __shfl_xor_sync(0xffffffffu, r.s, o)});
-  if (lane == 0) {
-    const float l = fmaf(log2f(r.s), LN2, r.m);
-    lse[t] = l;
-    const long long at = targets[t];
-    loss[t] = at == ignore ? 0.0f : (at < 0 || at >= V) ? __int_as_float(0x7fc00000) : l - target_logit[t];
-  }
-}
-
-// Sum of v over the CTA (1024 threads), in thread 0.
-template <typename S>
+// Sum of v over the CTA's kThreads threads, in thread 0.
+template <int kThreads, typename S>
 __device__ __forceinline__ S cta_total(S v, S* red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
   if (threadIdx.x < 32) {
-    v = red[threadIdx.x];
+    v = threadIdx.x < kThreads / 32 ? red[threadIdx.x] : S(0);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   }
@@ -112,23 +88,69 @@ __device__ __forceinline__ S cta_total(S v, S* red) {
   return v;
 }
 
-// One CTA: the rows' losses summed in 64 bits, divided by the counted rows for a mean.
-__global__ void __launch_bounds__(1024)
-ce_reduce_kernel(const float* __restrict__ row_loss, const long long* __restrict__ targets, float* __restrict__ loss, long long T,
-                 long long ignore, int mean) {
+// Four rows per CTA, 64 threads on the parts [parts][T] of each (four rows make whole sectors of 32 bytes; 61 rows of 286 parts have
+// 16 CTAs at work on them): lse and the row's loss. With `sum`, the CTA that finishes last sums the rows' losses, in 64 bits and in
+// the order of the rows, and divides by the counted ones for a mean; the kernel before this one has set `done` to 0.
+__global__ void __launch_bounds__(256)
+ce_finish_kernel(const float2* __restrict__ part, int parts, const float* __restrict__ target_logit,
+                 const long long* __restrict__ targets, float* __restrict__ row_loss, float* __restrict__ lse, long long T, long long V,
+                 long long ignore, float* __restrict__ sum, int mean, unsigned* __restrict__ done) {
+  __shared__ float2 red[8][4];
+  __shared__ int last;
   __shared__ double sred[32];
   __shared__ long long cred[32];
   pdl_launch_dependents();
   pdl_wait_prior_grids();
+  const int mine = threadIdx.x & 3;
+  const long long t = (long long)blockIdx.x * 4 + mine;
+  RowPart r{-INFINITY, 0.0f};
+  if (t < T) {
+    constexpr int AHEAD = 6;
+    for (int i0 = threadIdx.x >> 2; i0 < parts; i0 += 64 * AHEAD) {
+      float2 p[AHEAD];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k)
+        p[k] = i0 + 64 * k < parts ? part[(long long)(i0 + 64 * k) * T + t] : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) r = join(r, {p[k].x, p[k].y});
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 2; o >>= 1) r = join(r, {__shfl_xor_sync(0xffffffffu, r.m, o), __shfl_xor_sync(0xffffffffu, r.s, o)});
+  if ((threadIdx.x & 31) < 4) red[threadIdx.x >> 5][mine] = make_float2(r.m, r.s);
+  __syncthreads();
+  if (threadIdx.x < 4 && t < T) {
+    for (int w = 1; w < 8; ++w) r = join(r, {red[w][mine].x, red[w][mine].y});
+    const float l = fmaf(log2f(r.s), LN2, r.m);
+    lse[t] = l;
+    const long long at = targets[t];
+    row_loss[t] = at == ignore ? 0.0f : (at < 0 || at >= V) ? __int_as_float(0x7fc00000) : l - target_logit[t];
+  }
+  if (sum == nullptr) return;
+  if (threadIdx.x < 4) __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    last = atomicAdd(done, 1u) == gridDim.x - 1;
+    __threadfence();
+  }
+  __syncthreads();
+  if (!last) return;
   double s = 0.0;
   long long n = 0;
-  for (long long t = threadIdx.x; t < T; t += 1024) {
-    s += row_loss[t];
-    n += targets[t] != ignore ? 1 : 0;
+  for (long long i = threadIdx.x; i < T; i += 256) {
+    s += __ldcg(row_loss + i);
+    n += targets[i] != ignore ? 1 : 0;
   }
-  s = cta_total(s, sred);
-  n = cta_total(n, cred);
-  if (threadIdx.x == 0) *loss = (float)(mean ? s / (double)n : s);
+  s = cta_total<256>(s, sred);
+  n = cta_total<256>(n, cred);
+  if (threadIdx.x == 0) *sum = (float)(mean ? s / (double)n : s);
+}
+
+// The sum over no rows, or their mean.
+__global__ void ce_nothing_kernel(float* loss, int mean) {
+  pdl_launch_dependents();
+  pdl_wait_prior_grids();
+  *loss = mean ? __int_as_float(0x7fc00000) : 0.0f;
 }
 
 // One CTA: what every counted row's gradient is multiplied with, dloss or dloss / counted rows (0 where no row counts: there is
@@ -142,7 +164,7 @@ ce_scale_kernel(const long long* __restrict__ targets, const float* __restrict__
   long long n = 0;
   if (mean) {
     for (long long t = threadIdx.x; t < T; t += 1024) n += targets[t] != ignore ? 1 : 0;
-    n = cta_total(n, cred);
+    n = cta_total<1024>(n, cred);
   }
   if (threadIdx.x == 0) *scale = !mean ? *dloss : n > 0 ? (float)((double)*dloss / (double)n) : 0.0f;
 }
@@ -257,7 +279,7 @@ struct Layout {
   int pieces, parts;
   int chunks;         // parts that the vocabulary is cut into for dx, each with an accumulator
   long long chunk;    // fp32: columns of one
-  size_t xcopy, wcopy, part, target_logit, row_loss, scale, G, acc;
+  size_t xcopy, wcopy, part, target_logit, row_loss, done, scale, G, acc;
   size_t xs, xts, ws, wts, logits, GT;  // fp32: operand planes, a piece's logits, G^T
   size_t total;
 };
@@ -302,6 +324,7 @@ Layout layout(const Problem& p, bool backward) {
     w.part = take((size_t)w.parts * p.T * sizeof(float2));
     w.target_logit = take((size_t)p.T * 4);
     w.row_loss = take((size_t)p.T * 4);
+    w.done = take(4);
   } else {
     w.scale = take(4);
     const long long cols = p.bf16 ? w.piece : w.chunks * w.chunk;
@@ -396,6 +419,7 @@ int forward(const Problem& p, const CeCommon& dev, const long long* targets, flo
   float2* part = reinterpret_cast<float2*>(ws + w.part);
   float* target_logit = reinterpret_cast<float*>(ws + w.target_logit);
   float* row_loss = p.reduction == SYMPLEX_LOSS_NONE ? loss : reinterpret_cast<float*>(ws + w.row_loss);
+  unsigned* done = reinterpret_cast<unsigned*>(ws + w.done);
   int parts = w.parts;
   if (p.bf16) {
     CeForward f{};
@@ -404,6 +428,7 @@ int forward(const Problem& p, const CeCommon& dev, const long long* targets, flo
     f.targets = targets;
     f.part = part;
     f.target_logit = target_logit;
+    f.done = done;
     parts = ce_forward_parts(p.T, p.V, dev.num_sms);
     CE_TRY(launch_ce_forward(dev, f, stream));
   } else {
@@ -413,13 +438,12 @@ int forward(const Problem& p, const CeCommon& dev, const long long* targets, flo
       const long long v0 = i * w.piece, n = std::min(w.piece, p.V - v0);
       CE_TRY(prep(launch_split_tf32(static_cast<const float*>(p.W) + v0 * p.ldw, p.ldw, 0, wsp, (int)n, (int)p.H, (int)w.hp, 1, stream)));
       CE_TRY(split_product(dev, xs, w.hp, p.T * w.hp, wsp, w.hp, n * w.hp, logits, w.piece, nullptr, p.T, n, p.H, stream));
-      CE_LAUNCH(ce_piece_rows_kernel, p.T, 256, (const float*)logits, w.piece, (int)n, v0, targets, part + i * p.T, target_logit);
+      CE_LAUNCH(ce_piece_rows_kernel, p.T, 256, (const float*)logits, w.piece, (int)n, v0, targets, part + i * p.T, target_logit, done);
     }
   }
-  CE_LAUNCH(ce_finish_kernel, (p.T + 7) / 8, 256, (const float2*)part, parts, (const float*)target_logit, targets, row_loss, lse, p.T, p.V,
-            p.ignore);
-  if (p.reduction != SYMPLEX_LOSS_NONE)
-    CE_LAUNCH(ce_reduce_kernel, 1, 1024, (const float*)row_loss, targets, loss, p.T, p.ignore, p.reduction == SYMPLEX_LOSS_MEAN ? 1 : 0);
+  const bool all = p.reduction != SYMPLEX_LOSS_NONE;
+  CE_LAUNCH(ce_finish_kernel, (p.T + 3) / 4, 256, (const float2*)part, parts, (const float*)target_logit, targets, row_loss, lse, p.T, p.V,
+            p.ignore, all ? loss : nullptr, p.reduction == SYMPLEX_LOSS_MEAN ? 1 : 0, done);
   return SX_OK;
 }
 
@@ -541,7 +565,7 @@ int symplex_b200_linear_cross_entropy(const void* x, const void* W, const int64_
   const long long* tg = reinterpret_cast<const long long*>(targets);
   if (T == 0) {
     cudaStream_t stream = st;
-    CE_LAUNCH(ce_reduce_kernel, 1, 1024, (const float*)nullptr, tg, loss, 0LL, (long long)ignore_index, reduction == SYMPLEX_LOSS_MEAN ? 1 : 0);
+    CE_LAUNCH(ce_nothing_kernel, 1, 1, loss, reduction == SYMPLEX_LOSS_MEAN ? 1 : 0);
     return SX_OK;
   }
   return forward(p, dev, tg, loss, lse, static_cast<uint8_t*>(workspace), st);
