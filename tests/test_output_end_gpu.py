@@ -1,0 +1,125 @@
+"""A model's output end as a program runs it: norm, loss of the head, its gradients and the norm's; norm and the 4-bit head
+for single tokens. Held to 64-bit arithmetic and captured into graphs.
+
+Bounds, u = 2^-24, on relative Frobenius norms. float32: the norm's result is off by under 16 u of |y|, a logit by at most
+dl = (2 H + 96) u sum|y w|; p and with it every gradient moves by at most 2 dl of its own size, the products add chains of
+(2 n + 128) u over n = V or T terms. At H = 256, V = 1500, sum|y w| < 40 that is under 2e-3 + 4e-4. bfloat16 is checked stage
+by stage from what the stage before it wrote, so that only the stage's own roundings count: G and the result, half a step
+(2^-8) each at the most and independent (as in the tests of the single operators).
+"""
+import math
+
+import pytest
+import torch
+
+import symplex_b200 as sx
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF, F32 = torch.bfloat16, torch.float32
+T, H, V = 333, 256, 1500
+
+
+def _model(dtype, t=T, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    x = (torch.randn(t, H, generator=g, device=DEV) * 2 + 0.5).to(dtype)
+    gain = (1 + 0.2 * torch.randn(H, generator=g, device=DEV)).to(dtype)
+    shift = (0.1 * torch.randn(H, generator=g, device=DEV)).to(dtype)
+    head = (torch.randn(V, H, generator=g, device=DEV) / math.sqrt(H)).to(dtype)
+    targets = torch.randint(0, V, (t,), generator=g, device=DEV)
+    targets[::7] = -100
+    return x, gain, shift, head, targets
+
+
+def _train_step(x, gain, shift, head, targets, stream=None):
+    y, mean, rstd = sx.layer_norm(x, gain, shift, return_stats=True, stream=stream)
+    loss, lse = sx.linear_cross_entropy(y, head, targets, stream=stream)
+    one = torch.ones((), device=DEV)
+    dy, dhead = sx.linear_cross_entropy_backward(one, y, head, targets, lse, stream=stream)
+    dx, dgain, dshift = sx.layer_norm_backward(dy, x, mean, rstd, gain, stream=stream)
+    return dict(y=y, loss=loss, dy=dy, dhead=dhead, dx=dx, dgain=dgain, dshift=dshift)
+
+
+def _exact(x, gain, shift, head, targets, y=None, dy=None):
+    """The same in 64 bits; later stages from y and dy where they are given."""
+    xd, gd, sd, hd = (a.double().requires_grad_() for a in (x, gain, shift, head))
+    yd = torch.nn.functional.layer_norm(xd, (H,), gd, sd, 1e-5)
+    yin = (yd if y is None else y.double()).detach().requires_grad_()
+    loss = torch.nn.functional.cross_entropy(yin @ hd.t(), targets, ignore_index=-100)
+    dyd, dhead = torch.autograd.grad(loss, (yin, hd))
+    dx, dgain, dshift = torch.autograd.grad(yd, (xd, gd, sd), dyd if dy is None else dy.double())
+    return dict(y=yd.detach(), loss=loss.detach(), dy=dyd, dhead=dhead, dx=dx, dgain=dgain, dshift=dshift)
+
+
+def _off(a, b):
+    return float((a.double() - b).norm() / b.norm())
+
+
+def test_a_training_step_in_32_bits():
+    got, ref = _train_step(*_model(F32)), _exact(*_model(F32))
+    sx.sync_status()
+    for k in ref:
+        assert _off(got[k], ref[k]) < 2.4e-3, k
+
+
+def test_a_training_step_in_bfloat16():
+    m = _model(BF)
+    got = _train_step(*m)
+    sx.sync_status()
+    ref = _exact(*m, y=got["y"], dy=got["dy"])
+    assert _off(got["loss"], ref["loss"]) < 1e-4
+    for k in ("y", "dy", "dhead", "dx", "dgain", "dshift"):
+        assert _off(got[k], ref[k]) < 1.5 * 2.0 ** -8, k
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_a_training_step_captured_and_on_another_stream(dtype):
+    m = _model(dtype)
+    want = _train_step(*m)
+    other = _train_step(*_model(dtype, seed=1))
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    elsewhere = _train_step(*m, stream=s.cuda_stream)
+    s.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = _train_step(*m)
+    for seed, ref in ((0, want), (1, other), (0, want)):
+        for a, b in zip(m, _model(dtype, seed=seed)):
+            a.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(got[k], ref[k]) for k in ref)
+    assert all(torch.equal(elsewhere[k], want[k]) for k in want)
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 16])
+@pytest.mark.parametrize("symmetric", [True, False])
+def test_tokens_through_a_4_bit_head(tokens, symmetric):
+    """Norm and head of a decoding step; the loss of the same rows under the weights that the codes stand for agrees with its logits."""
+    x, gain, shift, head, targets = _model(BF, t=tokens)
+    codes, scales, zeros = sx.int4_quantize(head, 64, symmetric=symmetric)
+    q = torch.stack([codes & 15, codes >> 4], 2).reshape(V, H).double()
+    z = 8.0 if zeros is None else zeros.double().repeat_interleave(64, 1)
+    w = (q - z) * scales.double().repeat_interleave(64, 1)
+
+    def step():
+        y = sx.layer_norm(x, gain, shift)
+        return y, sx.int4_matvec(y, codes, scales, zeros, group_size=64, out_dtype=F32)
+
+    y, logits = step()
+    ref = y.double() @ w.t()
+    # exact products (bf16 x 4 bits x scale in fp32): chains of H steps and the scaling, in fp32
+    bound = (2 * H + 128) * 2.0 ** -24 * (y.double().abs() @ ((q + z) * scales.double().repeat_interleave(64, 1).abs()).t())
+    assert bool(((logits.double() - ref).abs() <= bound).all())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        _, again = step()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(again, logits)
+    # w has at most 8 significant bits times a bf16 scale's 8: rounded to bf16 for the loss, half a step of each weight
+    _, lse = sx.linear_cross_entropy(y, w.to(BF), targets)
+    moved = (2.0 ** -8 + (2 * H + 64) * 2.0 ** -24) * (y.double().abs() @ w.abs().t()).max(1).values + 1e-4
+    assert bool(((lse.double() - torch.logsumexp(logits.double(), 1)).abs() <= moved).all())
