@@ -14,6 +14,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "../../include/symplex_b200.h"
 #include "epilogue.cuh"
@@ -54,8 +55,9 @@ constexpr int MV_K = 128;    // k of one step
 constexpr int MV_RING = 3;   // steps of codes in flight per warp, 2 KB each: 96 KB an SM
 constexpr int MV_STEP_BYTES = MV_TILE * MV_K / 2;
 constexpr int MV_RING_BYTES = MV_WARPS * MV_RING * MV_STEP_BYTES;
-constexpr int MV_A_BYTES = 72 * 1024;  // shared memory for A
-constexpr int MV_SLAB_STEPS = 8;       // steps of a slab where all of A does not fit; two of 16 rows fit
+constexpr int MV_SMEM = 227 * 1024;
+constexpr int MV_SLAB_STEPS = 8;  // steps of a slab where A does not fit; two of 16 rows fit
+constexpr int MV_CLUSTER_MOST = 8;
 
 // 16 bytes global -> shared, past L1; `bytes` 0 writes zeros without reading.
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, int bytes) {
@@ -66,10 +68,16 @@ template <int kN>
 __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(kN) : "memory");
 }
-// The warps of one group (at least two: then there are at most 8 groups, barriers 1 to 8) or the one warp.
-__device__ __forceinline__ void group_barrier(int group, int warps) {
-  if (warps == 1) __syncwarp();
-  else asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(32 * warps) : "memory");
+// The warps of one of `groups` groups (1, 2, 4 or 8: barriers `groups` to 2 groups - 1, so that no barrier ever has two sizes).
+__device__ __forceinline__ void group_barrier(int group, int groups) {
+  asm volatile("bar.sync %0, %1;" ::"r"(groups + group), "r"(32 * MV_WARPS / groups) : "memory");
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_u32(addr, rank)) : "memory");
+  return v;
 }
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -160,8 +168,9 @@ struct MvScales {
 struct MvPlan {
   int tiles;
   int kw_log2;     // warps that share a tile, each with every kw-th step; MV_WARPS / kw tiles are worked on at a time
-  int slab_steps;  // steps whose A is in shared memory at a time: all of them where A fits, else a multiple of kw
-  int slabs;
+  int cluster;     // CTAs that share tiles, each with slab_steps of their steps
+  int slab_steps;  // steps whose A is in shared memory at a time
+  int slabs;       // 1, or (cluster 1 only) how often A is replaced in a tile's way through k
   int pitch;       // 16-byte blocks from one staged row of A to the next
   int a_vec, s_vec, out_bf16;
 };
@@ -202,10 +211,16 @@ __device__ __forceinline__ void stage_a(const Int4Args& p, const MvPlan& plan, u
   });
 }
 
-// Work of a CTA: its tiles t0 .. t1 in rounds of MV_WARPS / kw. Where all of A is in shared memory (one slab), 16 warps share a tile:
-// the CTA's work is even whatever its number of tiles, and a tile's sums are joined at once. Where A goes through in slabs, two warps
-// hold a tile's sums in registers over all slabs, so that every slab serves 8 tiles; the next slab is copied asynchronously behind the
-// current one and brought into pairs in place by the threads that copied it.
+// Work of a CTA: its tiles t0 .. t1 in rounds of MV_WARPS / kw tiles; what is left for the last rounds is shared by 2 kw, 4 kw, ...
+// warps a tile, so that no warp waits for the others with nothing to do. Each warp's sums of a tile are joined in shared memory.
+//
+// Where all of A does not fit into shared memory, a cluster of 2, 4 or 8 CTAs shares its tiles: each has a stretch of k, with that
+// stretch of A, for all of them. A round's sums stay in the CTA that made them until the next round is done, when every CTA of the
+// cluster has arrived with its own; then each of them takes a share of the outputs and adds up what the others hold.
+//
+// Where a cluster of 8 does not hold A either, a CTA takes A in slabs: two warps hold a tile's sums in registers over all slabs, so that
+// every slab serves 8 tiles; the next slab is copied asynchronously behind the current one and brought into pairs in place by the
+// threads that copied it.
 template <int kGW, int kNB, typename ST, bool kZeros>
 __global__ void __launch_bounds__(MV_WARPS * 32, 1)
 int4_mma_kernel(const Int4Args p, const MvPlan plan) {
@@ -214,16 +229,25 @@ int4_mma_kernel(const Int4Args p, const MvPlan plan) {
   constexpr int WPG = kGW / 32;  // words of a lane per group of a step
   constexpr int RED_PITCH = 8 * kNB + 1;
   extern __shared__ uint4 dyn_smem[];
+  constexpr int ROUND_SUMS = 4 * MV_TILE * 8 * kNB;  // of a CTA in a cluster: at most four tiles a round
   float* const red = reinterpret_cast<float*>(dyn_smem + MV_RING_BYTES / 16);  // [warp][row of the tile][row of A]
-  uint4* const a_smem = reinterpret_cast<uint4*>(red + MV_WARPS * MV_TILE * RED_PITCH);
+  float* const sums = red + MV_WARPS * MV_TILE * RED_PITCH;                    // cluster: [round mod 2][tile][row of A][row of the tile]
+  uint4* const a_smem = reinterpret_cast<uint4*>(sums + (plan.cluster > 1 ? 2 * ROUND_SUMS : 0));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  const int kw = 1 << plan.kw_log2, RG = MV_WARPS >> plan.kw_log2;
-  const int mk = warp & (kw - 1), rg = warp >> plan.kw_log2;
+  const int rank = plan.cluster > 1 ? (int)cluster_ctarank() : 0;
   const int m0 = blockIdx.y * (8 * kNB);
   const int m_here = min(8 * kNB, p.M - m0);
-  const int steps = (p.K + MV_K - 1) / MV_K;
-  const int t0 = (int)((long long)plan.tiles * blockIdx.x / gridDim.x), t1 = (int)((long long)plan.tiles * (blockIdx.x + 1) / gridDim.x);
+  const int first = plan.cluster > 1 ? rank * plan.slab_steps : 0;  // this CTA's steps
+  const int steps = min((p.K + MV_K - 1) / MV_K, plan.cluster > 1 ? first + plan.slab_steps : 1 << 30);
+  const int crowd = blockIdx.x / plan.cluster, crowds = gridDim.x / plan.cluster;
+  const int t0 = (int)((long long)plan.tiles * crowd / crowds), t1 = (int)((long long)plan.tiles * (crowd + 1) / crowds);
+  // log2 of the warps on each tile in the round that begins at tile b < t1
+  auto round_kw = [&](int b) {
+    const int left = t1 - b, base = plan.kw_log2;
+    if (plan.slabs > 1 || left >= MV_WARPS >> base) return base;
+    return 4 - (31 - __clz(left));
+  };
 
   // The warp's ring of codes: a step is 32 rows of 64 bytes, 16-byte block q of a row at q ^ f with f = the bits of row / 2 in reverse,
   // so that every read below (16, 8 or 4 bytes a lane) meets each bank once.
@@ -231,10 +255,24 @@ int4_mma_kernel(const Int4Args p, const MvPlan plan) {
   const uint32_t f = ((g >> 2) & 1) | (g & 2);  // row / 2 = (g >> 1) mod 4 for all four rows
   const uint32_t put = ring + g * 64 + ((t ^ f) << 4);
 
+  // This warp's next tile and first step in the rounds from the one at `round` (moved on to it) on; tile t1: none.
+  auto after = [&](int& round, int& tile, int& step) {
+    for (; round < t1;) {
+      const int kwl = round_kw(round);
+      tile = round + (warp >> kwl);
+      step = first + (warp & ((1 << kwl) - 1));
+      if (tile < t1 && step < steps) return kwl;
+      round += MV_WARPS >> kwl;
+    }
+    tile = t1;
+    return 0;
+  };
   // The step whose codes are fetched next runs ahead of the one being multiplied by the ring.
-  int far_tile = t0 + rg, far_step = mk;
+  int far_round = t0, far_kw = 0, far_tile = 0, far_step = 0;
   const uint8_t* row[4];  // this lane's share of the fetched tile's rows
   auto far_rows = [&]() {
+    far_kw = after(far_round, far_tile, far_step);
+    if (far_tile >= t1) return;
 #pragma unroll
     for (int r = 0; r < 4; ++r)  // rows past the end repeat the last one and are not written
       row[r] = p.codes + (long long)min(far_tile * MV_TILE + g + 8 * r, p.N - 1) * p.ldq + 16 * t;
@@ -245,11 +283,10 @@ int4_mma_kernel(const Int4Args p, const MvPlan plan) {
       const long long at = bytes ? (long long)far_step * (MV_K / 2) : 0;
 #pragma unroll
       for (int r = 0; r < 4; ++r) cp_async_16(put + slot + r * 512, row[r] + at, bytes);
-      far_step += kw;
+      far_step += 1 << far_kw;
       if (far_step >= steps) {
-        far_tile += RG;
-        far_step = mk;
-        if (far_tile < t1) far_rows();
+        far_round += MV_WARPS >> far_kw;
+        far_rows();
       }
     }
     cp_async_commit();
@@ -263,15 +300,37 @@ int4_mma_kernel(const Int4Args p, const MvPlan plan) {
 
   pdl_launch_dependents();
   pdl_wait_prior_grids();
-  if (far_tile < t1) far_rows();
+  far_rows();
+  Scales sc;
+  if (far_tile < t1) {
+    scale_rows(far_tile);
+    sc.load(p, srow, far_step * MV_K, plan.s_vec);
+  }
 #pragma unroll
   for (int i = 0; i < MV_RING; ++i) fetch(i * MV_STEP_BYTES);
-  Scales sc;
-  if (t0 + rg < t1) {
-    scale_rows(t0 + rg);
-    sc.load(p, srow, mk * MV_K, plan.s_vec);
-  }
-  stage_a(p, plan, a_smem, m0, m_here, 0);
+  stage_a(p, plan, a_smem, m0, m_here, first * MV_K);
+
+  auto write = [&](int tile, int m, int r, float v) {
+    const int n = tile * MV_TILE + r;
+    if (n >= p.N) return;
+    if (p.bias != nullptr) v += p.bias[n];
+    v = activate(v, p.act);
+    const long long at = (m0 + m) * p.ldc + n;
+    if (plan.out_bf16) static_cast<__nv_bfloat16*>(p.C)[at] = __nv_bfloat16(v);
+    else static_cast<float*>(p.C)[at] = v;
+  };
+  // Cluster: this CTA's share of the outputs of a round, once every CTA has arrived with its sums.
+  int held_tile = -1, held_n = 0, held_buf = 0;
+  auto write_held = [&]() {
+    __syncwarp();
+    cluster_wait();
+    for (int e = rank * (MV_WARPS * 32) + threadIdx.x; e < held_n * m_here * MV_TILE; e += plan.cluster * MV_WARPS * 32) {
+      const uint32_t at = smem_u32(sums + held_buf * ROUND_SUMS + e);
+      float v = 0.0f;
+      for (int i = 0; i < plan.cluster; ++i) v += ld_cluster(at, i);
+      write(held_tile + e / (m_here * MV_TILE), e / MV_TILE % m_here, e % MV_TILE, v);
+    }
+  };
 
   // Where a lane finds its blocks of A in a step: two bases, for the even and odd ones among its words, because of the exchange of
   // neighbours in every other eight blocks. Rows of A that do not exist repeat the last one; their sums are not written.
@@ -287,10 +346,13 @@ int4_mma_kernel(const Int4Args p, const MvPlan plan) {
   const int buf_blocks = m_here * plan.pitch;
   uint32_t slot = 0;
   int buf = 0;
-  for (int b0 = t0; b0 < t1; b0 += RG) {
+  for (int b0 = t0, kwl; b0 < t1; b0 += MV_WARPS >> kwl) {
+    kwl = round_kw(b0);
+    const int kw = 1 << kwl, RG = MV_WARPS >> kwl;
+    const int mk = warp & (kw - 1), rg = warp >> kwl;
     const int tile = b0 + rg;
     float acc[kNB][2][4] = {};
-    for (int s0 = 0; s0 < steps; s0 += plan.slab_steps) {
+    for (int s0 = first; s0 < steps; s0 += plan.slab_steps) {
       const int s1 = min(s0 + plan.slab_steps, steps);
       const bool last = s1 == steps && b0 + RG >= t1;
       const int next_k = s1 == steps ? 0 : s1 * MV_K;  // the slab after this one
@@ -308,7 +370,7 @@ int4_mma_kernel(const Int4Args p, const MvPlan plan) {
         cp_async_commit();
       }
       if (tile < t1) {
-        const uint4* a0 = a_smem + buf * buf_blocks + mk * (MV_K / 8);
+        const uint4* a0 = a_smem + buf * buf_blocks + mk * (MV_K / 8);  // s0 + mk: a slab starts at a multiple of kw
         for (int v = s0 + mk; v < s1; v += kw, a0 += kw * (MV_K / 8)) {
           cp_async_wait<MV_RING - 1>();
           __syncwarp();
@@ -335,9 +397,13 @@ int4_mma_kernel(const Int4Args p, const MvPlan plan) {
           const Scales cur = sc;
           if (v + kw < steps) {
             sc.load(p, srow, (v + kw) * MV_K, plan.s_vec);
-          } else if (tile + RG < t1) {
-            scale_rows(tile + RG);
-            sc.load(p, srow, mk * MV_K, plan.s_vec);
+          } else {
+            int round2 = b0 + RG, tile2, step2;
+            after(round2, tile2, step2);
+            if (tile2 < t1) {
+              scale_rows(tile2);
+              sc.load(p, srow, step2 * MV_K, plan.s_vec);
+            }
           }
 #pragma unroll
           for (int j = 0; j < GROUPS; ++j) {
@@ -400,6 +466,7 @@ int4_mma_kernel(const Int4Args p, const MvPlan plan) {
       }
     }
     // The tile's sums over the warps that share it, always in the order of the warps.
+    if (plan.cluster > 1 && held_tile >= 0) write_held();  // and now nobody needs the sums of the round before that any more
     if (tile < t1) {
 #pragma unroll
       for (int nb = 0; nb < kNB; ++nb)
@@ -408,21 +475,32 @@ int4_mma_kernel(const Int4Args p, const MvPlan plan) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             red[(warp * MV_TILE + 16 * mt + g + 8 * (i >> 1)) * RED_PITCH + 8 * nb + 2 * t + (i & 1)] = acc[nb][mt][i];
-      group_barrier(rg, kw);
+      if (kw == 1) __syncwarp();
+      else group_barrier(rg, RG);
+      float* const to = sums + (held_buf ^ 1) * ROUND_SUMS + rg * m_here * MV_TILE;
       for (int e = mk * 32 + lane; e < m_here * MV_TILE; e += 32 * kw) {
         const int m = e / MV_TILE, r = e % MV_TILE;
         float v = 0.0f;
         for (int i = 0; i < kw; ++i) v += red[((rg * kw + i) * MV_TILE + r) * RED_PITCH + m];
-        const int n = tile * MV_TILE + r;
-        if (n >= p.N) continue;
-        if (p.bias != nullptr) v += p.bias[n];
-        v = activate(v, p.act);
-        const long long at = (m0 + m) * p.ldc + n;
-        if (plan.out_bf16) static_cast<__nv_bfloat16*>(p.C)[at] = __nv_bfloat16(v);
-        else static_cast<float*>(p.C)[at] = v;
+        if (plan.cluster > 1) to[e] = v;
+        else write(tile, m, r, v);
       }
-      group_barrier(rg, kw);  // red is free again
+      if (kw == 1) __syncwarp();  // red is free again
+      else group_barrier(rg, RG);
     }
+    if (plan.cluster > 1) {
+      held_tile = b0;
+      held_n = RG;
+      held_buf ^= 1;
+      __syncwarp();
+      cluster_arrive();
+    }
+  }
+  if (plan.cluster > 1) {
+    if (held_tile >= 0) write_held();
+    __syncwarp();
+    cluster_arrive();  // no CTA leaves while its sums are being read
+    cluster_wait();
   }
   cp_async_wait<0>();
 }
@@ -547,16 +625,25 @@ int matvec_mma(const Int4Args& a, bool out_bf16, int sms, cudaStream_t stream) {
   const int steps = (a.K + MV_K - 1) / MV_K;
   const int rows = std::min(a.M, 8 * kNB);
   auto bytes = [&](int n) { return (size_t)rows * (n * (MV_K / 8) + MvPad<kGW>) * 16; };
-  // All of A where it fits, with four warps on a tile, more where a CTA has fewer than four tiles (5 x 50257 x 2048: 24.2 us, 31.3 with
-  // 16 warps, 26.0 with two; 1 x 4096 x 4096 with one tile a CTA: 5.5 with 16 or 4 warps, 8.2 with two); else slabs of 8 steps in two buffers, two warps on a tile.
-  const bool whole = bytes(steps) <= MV_A_BYTES;
+  constexpr int SUMS = MV_WARPS * MV_TILE * (8 * kNB + 1) * 4, HELD = 2 * 4 * MV_TILE * 8 * kNB * 4;
+  const int mblocks = (a.M + 8 * kNB - 1) / (8 * kNB);
+  SX_ENSURE_DYN_SMEM(kern, MV_SMEM);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  // The smallest cluster whose CTAs hold A between them, with four warps on a tile, more where a CTA has fewer than four tiles
+  // (5 x 50257 x 2048: 24.2 us, 31.3 with 16 warps, 26.0 with two; 1 x 4096 x 4096 with one tile a CTA: 5.5 with 16 or 4 warps, 8.2 with
+  // two); else slabs of 8 steps in two buffers, two warps on a tile.
+  plan.cluster = 1;
+  auto fits = [&](int c) { return MV_RING_BYTES + SUMS + (c > 1 ? HELD : 0) + bytes((steps + c - 1) / c) <= MV_SMEM; };
+  while (plan.cluster < MV_CLUSTER_MOST && !fits(plan.cluster)) plan.cluster *= 2;
+  const bool whole = fits(plan.cluster) && sms >= plan.cluster * mblocks;
+  int crowds = std::max(1, sms / mblocks);
   if (whole) {
-    const int each = (plan.tiles + sms - 1) / sms;  // tiles of a CTA
-    while (plan.kw_log2 < 4 && (2 << plan.kw_log2) <= steps && (plan.kw_log2 < 2 || each << plan.kw_log2 < MV_WARPS)) ++plan.kw_log2;
-    plan.slab_steps = steps;
+    plan.slab_steps = (steps + plan.cluster - 1) / plan.cluster;
     plan.slabs = 1;
+    crowds = std::max(1, crowds / plan.cluster);
   } else {
-    plan.kw_log2 = 1;
+    plan.cluster = 1;
     plan.slab_steps = MV_SLAB_STEPS;
     plan.slabs = (steps + MV_SLAB_STEPS - 1) / MV_SLAB_STEPS;
   }
@@ -565,19 +652,41 @@ int matvec_mma(const Int4Args& a, bool out_bf16, int sms, cudaStream_t stream) {
   plan.s_vec = a.group == kGW && a.groups % GROUPS == 0 && reinterpret_cast<uintptr_t>(a.scales) % (GROUPS * sizeof(ST)) == 0 &&
                reinterpret_cast<uintptr_t>(a.zeros) % GROUPS == 0;
   plan.out_bf16 = out_bf16 ? 1 : 0;
-  const size_t smem = MV_RING_BYTES + MV_WARPS * MV_TILE * (8 * kNB + 1) * 4 + bytes(plan.slab_steps) * (whole ? 1 : 2);
-  SX_ENSURE_DYN_SMEM(kern, 227 * 1024);
-  const int mblocks = (a.M + 8 * kNB - 1) / (8 * kNB);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)std::min(plan.tiles, std::max(1, sms / mblocks)), (unsigned)mblocks, 1);
   cfg.blockDim = dim3(MV_WARPS * 32, 1, 1);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = MV_RING_BYTES + SUMS + (plan.cluster > 1 ? HELD : 0) + bytes(plan.slab_steps) * (whole ? 1 : 2);
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 1 : 0;
+  if (plan.cluster > 1) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = plan.cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.numAttrs = 1;
+    // A processing cluster of the GPU may have SMs left over that make no whole cluster.
+    static std::atomic<int> resident[MV_CLUSTER_MOST + 1];
+    int n = resident[plan.cluster].load(std::memory_order_relaxed);
+    if (n == 0) {
+      cfg.gridDim = dim3(plan.cluster, 1, 1);
+      cudaLaunchConfig_t most = cfg;
+      most.dynamicSmemBytes = MV_SMEM;
+      if (cudaOccupancyMaxActiveClusters(&n, kern, &most) != cudaSuccess || n <= 0) return launch_failed(cudaGetLastError(), "cluster size not supported");
+      resident[plan.cluster].store(n, std::memory_order_relaxed);
+    }
+    crowds = std::max(1, std::min(crowds, n / mblocks));
+  }
+  crowds = std::min(crowds, plan.tiles);
+  cfg.gridDim = dim3((unsigned)(crowds * plan.cluster), (unsigned)mblocks, 1);
+  if (whole) {
+    const int each = (plan.tiles + crowds - 1) / crowds;  // tiles of a CTA or cluster
+    while (plan.kw_log2 < 4 && (2 << plan.kw_log2) <= plan.slab_steps && (plan.kw_log2 < 2 || each << plan.kw_log2 < MV_WARPS)) ++plan.kw_log2;
+    if (plan.cluster > 1) plan.kw_log2 = std::max(plan.kw_log2, 2);  // at most four tiles a round
+  } else {
+    plan.kw_log2 = 1;
+  }
+  if (pdl_enabled()) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a, plan);
   if (e != cudaSuccess) return launch_failed(e, "4-bit product launch failed");
   count_launches(1);

@@ -75,6 +75,21 @@ def test_sizes(m, n, k, group, zeros):
     _check(sx.int4_matvec(x, codes, scales, z, group_size=group, out_dtype=F32), x, w)
 
 
+@pytest.mark.parametrize("m,n,k,group,zeros", [
+    (8, 700, 8192, 128, False), (16, 20000, 8192, 64, True), (9, 4736, 5024, 32, True), (16, 33, 16384, 128, False), (29, 5001, 8192, 32, False),
+    (5, 9000, 16416, 32, True), (64, 1500, 12320, 32, True), (16, 300, 20480, 64, True), (3, 2000, 131072, 128, False), (6, 25000, 1056, 96, True),
+])
+def test_rows_of_a_that_do_not_fit_into_shared_memory(m, n, k, group, zeros):
+    """A spread over clusters of 2, 4 and 8 CTAs (stretches of k of unequal length, CTAs with none), and in slabs."""
+    x, codes, scales, z = _case(m, n, k, group, zeros, seed=k + m)
+    w = _dense(codes, scales, z, k, group)
+    y = sx.int4_matvec(x, codes, scales, z, group_size=group)
+    _check(y, x, w)
+    assert torch.equal(y, sx.int4_matvec(x, codes, scales, z, group_size=group))
+    b = torch.randn(n, device=DEV)
+    _check(sx.int4_matvec(x, codes, scales, z, group_size=group, bias=b, out_dtype=F32), x, w, b)
+
+
 @pytest.mark.parametrize("sdt", [BF, F32])
 @pytest.mark.parametrize("odt", [BF, F32])
 def test_types(sdt, odt):
