@@ -74,10 +74,17 @@ __device__ __forceinline__ void group_barrier(int group, int groups) {
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_u32(addr, rank)) : "memory");
+__device__ __forceinline__ float4 ld_cluster(uint32_t addr, uint32_t rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(mapa_u32(addr, rank)) : "memory");
   return v;
+}
+__device__ __forceinline__ void add(float4& a, const float4& b) {
+  a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 r = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&r);
 }
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -172,7 +179,7 @@ struct MvPlan {
   int slab_steps;  // steps whose A is in shared memory at a time
   int slabs;       // 1, or (cluster 1 only) how often A is replaced in a tile's way through k
   int pitch;       // 16-byte blocks from one staged row of A to the next
-  int a_vec, s_vec, out_bf16;
+  int a_vec, s_vec, c_vec, out_bf16;
 };
 
 // A in shared memory: rows of 16-byte blocks of 8 k, each block as the pairs the dequantised words have, (k0,k4) (k1,k5) (k2,k6)
@@ -227,11 +234,12 @@ int4_mma_kernel(const Int4Args p, const MvPlan plan) {
   using Scales = MvScales<kGW, ST, kZeros>;
   constexpr int GROUPS = Scales::GROUPS;
   constexpr int WPG = kGW / 32;  // words of a lane per group of a step
-  constexpr int RED_PITCH = 8 * kNB + 1;
+  constexpr int RED_PITCH = MV_TILE + 4;  // floats from one row of A to the next: the lanes of a store meet every bank once
+  constexpr int RED_WARP = 8 * kNB * RED_PITCH;
   extern __shared__ uint4 dyn_smem[];
   constexpr int ROUND_SUMS = 4 * MV_TILE * 8 * kNB;  // of a CTA in a cluster: at most four tiles a round
-  float* const red = reinterpret_cast<float*>(dyn_smem + MV_RING_BYTES / 16);  // [warp][row of the tile][row of A]
-  float* const sums = red + MV_WARPS * MV_TILE * RED_PITCH;                    // cluster: [round mod 2][tile][row of A][row of the tile]
+  float* const red = reinterpret_cast<float*>(dyn_smem + MV_RING_BYTES / 16);  // [warp][row of A][row of the tile]
+  float* const sums = red + MV_WARPS * RED_WARP;                               // cluster: [round mod 2][tile][row of A][row of the tile]
   uint4* const a_smem = reinterpret_cast<uint4*>(sums + (plan.cluster > 1 ? 2 * ROUND_SUMS : 0));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
@@ -310,25 +318,44 @@ int4_mma_kernel(const Int4Args p, const MvPlan plan) {
   for (int i = 0; i < MV_RING; ++i) fetch(i * MV_STEP_BYTES);
   stage_a(p, plan, a_smem, m0, m_here, first * MV_K);
 
-  auto write = [&](int tile, int m, int r, float v) {
+  auto write = [&](int tile, int m, int r, float4 sum) {  // four outputs of row m, from row r of the tile on
     const int n = tile * MV_TILE + r;
-    if (n >= p.N) return;
-    if (p.bias != nullptr) v += p.bias[n];
-    v = activate(v, p.act);
+    float v[4] = {sum.x, sum.y, sum.z, sum.w};
     const long long at = (m0 + m) * p.ldc + n;
-    if (plan.out_bf16) static_cast<__nv_bfloat16*>(p.C)[at] = __nv_bfloat16(v);
-    else static_cast<float*>(p.C)[at] = v;
+    const bool all = n + 4 <= p.N;
+    if (p.bias != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (all || n + i < p.N) v[i] += p.bias[n + i];
+    }
+    if (p.act != ACT_NONE) {
+#pragma unroll 1
+      for (int i = 0; i < 4; ++i) v[i] = activate(v[i], p.act);
+    }
+    if (all && plan.c_vec) {
+      if (plan.out_bf16) *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.C) + at) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+      else *reinterpret_cast<float4*>(static_cast<float*>(p.C) + at) = make_float4(v[0], v[1], v[2], v[3]);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (n + i >= p.N) break;
+      if (plan.out_bf16) static_cast<__nv_bfloat16*>(p.C)[at + i] = __nv_bfloat16(v[i]);
+      else static_cast<float*>(p.C)[at + i] = v[i];
+    }
   };
   // Cluster: this CTA's share of the outputs of a round, once every CTA has arrived with its sums.
   int held_tile = -1, held_n = 0, held_buf = 0;
   auto write_held = [&]() {
     __syncwarp();
     cluster_wait();
-    for (int e = rank * (MV_WARPS * 32) + threadIdx.x; e < held_n * m_here * MV_TILE; e += plan.cluster * MV_WARPS * 32) {
-      const uint32_t at = smem_u32(sums + held_buf * ROUND_SUMS + e);
-      float v = 0.0f;
-      for (int i = 0; i < plan.cluster; ++i) v += ld_cluster(at, i);
-      write(held_tile + e / (m_here * MV_TILE), e / MV_TILE % m_here, e % MV_TILE, v);
+    for (int e = rank * (MV_WARPS * 32) + threadIdx.x; e < held_n * (8 * kNB) * (MV_TILE / 4); e += plan.cluster * MV_WARPS * 32) {
+      const int m = e / (MV_TILE / 4) % (8 * kNB);
+      if (m >= m_here) continue;
+      const uint32_t at = smem_u32(sums + held_buf * ROUND_SUMS + 4 * e);
+      float4 v = ld_cluster(at, 0);
+      for (int i = 1; i < plan.cluster; ++i) add(v, ld_cluster(at, i));
+      write(held_tile + e / (8 * kNB * (MV_TILE / 4)), m, 4 * e % MV_TILE, v);
     }
   };
 
@@ -474,15 +501,23 @@ int4_mma_kernel(const Int4Args p, const MvPlan plan) {
         for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            red[(warp * MV_TILE + 16 * mt + g + 8 * (i >> 1)) * RED_PITCH + 8 * nb + 2 * t + (i & 1)] = acc[nb][mt][i];
+            red[warp * RED_WARP + (8 * nb + 2 * t + (i & 1)) * RED_PITCH + 16 * mt + g + 8 * (i >> 1)] = acc[nb][mt][i];
       if (kw == 1) __syncwarp();
       else group_barrier(rg, RG);
-      float* const to = sums + (held_buf ^ 1) * ROUND_SUMS + rg * m_here * MV_TILE;
-      for (int e = mk * 32 + lane; e < m_here * MV_TILE; e += 32 * kw) {
-        const int m = e / MV_TILE, r = e % MV_TILE;
-        float v = 0.0f;
-        for (int i = 0; i < kw; ++i) v += red[((rg * kw + i) * MV_TILE + r) * RED_PITCH + m];
-        if (plan.cluster > 1) to[e] = v;
+      const float* const from = red + rg * kw * RED_WARP;
+      for (int e = mk * 32 + lane; e < m_here * (MV_TILE / 4); e += 32 * kw) {
+        const int m = e / (MV_TILE / 4), r = 4 * e % MV_TILE;
+        const float* at = from + m * RED_PITCH + r;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (kw >= 4) {
+          for (int i = 0; i < kw; i += 4) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) add(v, *reinterpret_cast<const float4*>(at + (i + k) * RED_WARP));
+          }
+        } else {
+          for (int i = 0; i < kw; ++i) add(v, *reinterpret_cast<const float4*>(at + i * RED_WARP));
+        }
+        if (plan.cluster > 1) *reinterpret_cast<float4*>(sums + (held_buf ^ 1) * ROUND_SUMS + (rg * 8 * kNB + m) * MV_TILE + r) = v;
         else write(tile, m, r, v);
       }
       if (kw == 1) __syncwarp();  // red is free again
@@ -625,7 +660,7 @@ int matvec_mma(const Int4Args& a, bool out_bf16, int sms, cudaStream_t stream) {
   const int steps = (a.K + MV_K - 1) / MV_K;
   const int rows = std::min(a.M, 8 * kNB);
   auto bytes = [&](int n) { return (size_t)rows * (n * (MV_K / 8) + MvPad<kGW>) * 16; };
-  constexpr int SUMS = MV_WARPS * MV_TILE * (8 * kNB + 1) * 4, HELD = 2 * 4 * MV_TILE * 8 * kNB * 4;
+  constexpr int SUMS = MV_WARPS * (MV_TILE + 4) * 8 * kNB * 4, HELD = 2 * 4 * MV_TILE * 8 * kNB * 4;
   const int mblocks = (a.M + 8 * kNB - 1) / (8 * kNB);
   SX_ENSURE_DYN_SMEM(kern, MV_SMEM);
   cudaLaunchConfig_t cfg = {};
@@ -652,6 +687,7 @@ int matvec_mma(const Int4Args& a, bool out_bf16, int sms, cudaStream_t stream) {
   plan.s_vec = a.group == kGW && a.groups % GROUPS == 0 && reinterpret_cast<uintptr_t>(a.scales) % (GROUPS * sizeof(ST)) == 0 &&
                reinterpret_cast<uintptr_t>(a.zeros) % GROUPS == 0;
   plan.out_bf16 = out_bf16 ? 1 : 0;
+  plan.c_vec = a.ldc % 4 == 0 && reinterpret_cast<uintptr_t>(a.C) % (out_bf16 ? 8 : 16) == 0;
   cfg.blockDim = dim3(MV_WARPS * 32, 1, 1);
   cfg.dynamicSmemBytes = MV_RING_BYTES + SUMS + (plan.cluster > 1 ? HELD : 0) + bytes(plan.slab_steps) * (whole ? 1 : 2);
   cfg.stream = stream;
