@@ -218,8 +218,8 @@ __device__ __forceinline__ void stage_a(const Int4Args& p, const MvPlan& plan, u
   });
 }
 
-// Work of a CTA: its tiles t0 .. t1 in rounds of MV_WARPS / kw tiles; what is left for the last rounds is shared by 2 kw, 4 kw, ...
-// warps a tile, so that no warp waits for the others with nothing to do. Each warp's sums of a tile are joined in shared memory.
+// Work of a CTA: its tiles t0 .. t1 in rounds of MV_WARPS / kw tiles; where half of them or fewer are left for the last round, 2 kw
+// or more warps share each. The warps' sums of a tile are joined in shared memory.
 //
 // Where all of A does not fit into shared memory, a cluster of 2, 4 or 8 CTAs shares its tiles: each has a stretch of k, with that
 // stretch of A, for all of them. A round's sums stay in the CTA that made them until the next round is done, when every CTA of the
@@ -254,7 +254,7 @@ int4_mma_kernel(const Int4Args p, const MvPlan plan) {
   auto round_kw = [&](int b) {
     const int left = t1 - b, base = plan.kw_log2;
     if (plan.slabs > 1 || left >= MV_WARPS >> base) return base;
-    return 4 - (31 - __clz(left));
+    return 4 - (32 - __clz(left - 1));
   };
 
   // The warp's ring of codes: a step is 32 rows of 64 bytes, 16-byte block q of a row at q ^ f with f = the bits of row / 2 in reverse,
@@ -525,7 +525,7 @@ int4_mma_kernel(const Int4Args p, const MvPlan plan) {
     }
     if (plan.cluster > 1) {
       held_tile = b0;
-      held_n = RG;
+      held_n = min(RG, t1 - b0);
       held_buf ^= 1;
       __syncwarp();
       cluster_arrive();
