@@ -52,12 +52,12 @@ struct Int4Args {
 constexpr int MV_WARPS = 16;
 constexpr int MV_TILE = 32;  // rows of W per tile: two m16 tiles share every fragment of A
 constexpr int MV_K = 128;    // k of one step
-constexpr int MV_RING = 3;   // steps of codes in flight per warp, 2 KB each: 96 KB an SM
+constexpr int MV_RING = 2;   // steps of codes in flight per warp, 2 KB each: 64 KB an SM (three steps: within 3 %, but 32 KB less for A)
 constexpr int MV_STEP_BYTES = MV_TILE * MV_K / 2;
 constexpr int MV_RING_BYTES = MV_WARPS * MV_RING * MV_STEP_BYTES;
 constexpr int MV_SMEM = 227 * 1024;
-constexpr int MV_SLAB_STEPS = 8;  // steps of a slab where A does not fit; two of 16 rows fit
 constexpr int MV_CLUSTER_MOST = 8;
+constexpr int MV_CLUSTER_KW = 1;  // log2 of the fewest warps on a tile in a cluster (16 x 28672 x 8192 in groups of 128: 56 us, 62 with 2)
 
 // 16 bytes global -> shared, past L1; `bytes` 0 writes zeros without reading.
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, int bytes) {
@@ -175,9 +175,9 @@ struct MvScales {
 struct MvPlan {
   int tiles;
   int kw_log2;     // warps that share a tile, each with every kw-th step; MV_WARPS / kw tiles are worked on at a time
-  int cluster;     // CTAs that share tiles, each with slab_steps of their steps
-  int slab_steps;  // steps whose A is in shared memory at a time
-  int slabs;       // 1, or (cluster 1 only) how often A is replaced in a tile's way through k
+  int cluster;     // CTAs that share tiles, each with `steps` of their steps
+  int steps;
+  int rows;        // rows of A of a CTA
   int pitch;       // 16-byte blocks from one staged row of A to the next
   int a_vec, s_vec, c_vec, out_bf16;
 };
@@ -191,43 +191,41 @@ __device__ __forceinline__ uint4 pairs_of(const uint4& x) {
   return make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632), __byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632));
 }
 
-// f(block to write, k of it relative to the slab, row of A): this thread's blocks of a slab.
-template <typename F>
-__device__ __forceinline__ void for_blocks(const MvPlan& plan, int rows, F&& f) {
-  const int blocks = plan.slab_steps * (MV_K / 8);
-  for (int m = 0; m < rows; ++m)
-    for (int b = threadIdx.x; b < blocks; b += MV_WARPS * 32) f(m * plan.pitch + (b ^ ((b >> 3) & 1)), 8 * b, m);
-}
-
 __device__ __forceinline__ void stage_a(const Int4Args& p, const MvPlan& plan, uint4* to, int m0, int rows, int k0) {
-  for_blocks(plan, rows, [&](int at, int k, int m) {
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (k0 + k < p.K) {  // K is a multiple of 8: a block is inside or outside
-      const __nv_bfloat16* a = p.A + (long long)(m0 + m) * p.lda + k0 + k;
-      if (plan.a_vec) {
-        x = __ldg(reinterpret_cast<const uint4*>(a));
-      } else {
-        const uint16_t* u = reinterpret_cast<const uint16_t*>(a);
-        x.x = u[0] | (uint32_t(u[1]) << 16);
-        x.y = u[2] | (uint32_t(u[3]) << 16);
-        x.z = u[4] | (uint32_t(u[5]) << 16);
-        x.w = u[6] | (uint32_t(u[7]) << 16);
+  const int blocks = plan.steps * (MV_K / 8);
+  for (int m = 0; m < rows; ++m) {
+    const __nv_bfloat16* row = p.A + (long long)(m0 + m) * p.lda + k0;
+    for (int b = threadIdx.x; b < blocks; b += MV_WARPS * 32) {
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (k0 + 8 * b < p.K) {  // K is a multiple of 8: a block is inside or outside
+        if (plan.a_vec) {
+          x = __ldg(reinterpret_cast<const uint4*>(row + 8 * b));
+        } else {
+          const uint16_t* u = reinterpret_cast<const uint16_t*>(row + 8 * b);
+          x.x = u[0] | (uint32_t(u[1]) << 16);
+          x.y = u[2] | (uint32_t(u[3]) << 16);
+          x.z = u[4] | (uint32_t(u[5]) << 16);
+          x.w = u[6] | (uint32_t(u[7]) << 16);
+        }
       }
+      to[m * plan.pitch + (b ^ ((b >> 3) & 1))] = pairs_of(x);
     }
-    to[at] = pairs_of(x);
-  });
+  }
 }
 
 // Work of a CTA: its tiles t0 .. t1 in rounds of MV_WARPS / kw tiles; where half of them or fewer are left for the last round, 2 kw
 // or more warps share each. The warps' sums of a tile are joined in shared memory.
 //
+// Measured (16 x 28672 x 8192, groups of 64 with zeros): 64 us, 2.0 TB/s; 1 x 28672 x 8192, groups of 128: 34 us, 3.6 TB/s. HBM would
+// take 20 and 18: the ALU, the shared-memory pipe and the issue of instructions are each about half busy, with the four warps a
+// scheduler that 128 registers leave.
+//
 // Where all of A does not fit into shared memory, a cluster of 2, 4 or 8 CTAs shares its tiles: each has a stretch of k, with that
 // stretch of A, for all of them. A round's sums stay in the CTA that made them until the next round is done, when every CTA of the
 // cluster has arrived with its own; then each of them takes a share of the outputs and adds up what the others hold.
 //
-// Where a cluster of 8 does not hold A either, a CTA takes A in slabs: two warps hold a tile's sums in registers over all slabs, so that
-// every slab serves 8 tiles; the next slab is copied asynchronously behind the current one and brought into pairs in place by the
-// threads that copied it.
+// Where a cluster of 8 does not hold A either, fewer rows of A are taken in a pass over W. (A in slabs that every CTA replaces as it
+// goes through k: 81 us for the first case above, the barriers between slabs and the copies of A.)
 template <int kGW, int kNB, typename ST, bool kZeros>
 __global__ void __launch_bounds__(MV_WARPS * 32, 1)
 int4_mma_kernel(const Int4Args p, const MvPlan plan) {
@@ -237,23 +235,23 @@ int4_mma_kernel(const Int4Args p, const MvPlan plan) {
   constexpr int RED_PITCH = MV_TILE + 4;  // floats from one row of A to the next: the lanes of a store meet every bank once
   constexpr int RED_WARP = 8 * kNB * RED_PITCH;
   extern __shared__ uint4 dyn_smem[];
-  constexpr int ROUND_SUMS = 4 * MV_TILE * 8 * kNB;  // of a CTA in a cluster: at most four tiles a round
+  constexpr int ROUND_SUMS = (MV_WARPS >> MV_CLUSTER_KW) * MV_TILE * 8 * kNB;  // of a CTA in a cluster
   float* const red = reinterpret_cast<float*>(dyn_smem + MV_RING_BYTES / 16);  // [warp][row of A][row of the tile]
   float* const sums = red + MV_WARPS * RED_WARP;                               // cluster: [round mod 2][tile][row of A][row of the tile]
   uint4* const a_smem = reinterpret_cast<uint4*>(sums + (plan.cluster > 1 ? 2 * ROUND_SUMS : 0));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int rank = plan.cluster > 1 ? (int)cluster_ctarank() : 0;
-  const int m0 = blockIdx.y * (8 * kNB);
-  const int m_here = min(8 * kNB, p.M - m0);
-  const int first = plan.cluster > 1 ? rank * plan.slab_steps : 0;  // this CTA's steps
-  const int steps = min((p.K + MV_K - 1) / MV_K, plan.cluster > 1 ? first + plan.slab_steps : 1 << 30);
+  const int m0 = blockIdx.y * plan.rows;
+  const int m_here = min(plan.rows, p.M - m0);
+  const int first = rank * plan.steps;  // this CTA's steps
+  const int steps = min((p.K + MV_K - 1) / MV_K, first + plan.steps);
   const int crowd = blockIdx.x / plan.cluster, crowds = gridDim.x / plan.cluster;
   const int t0 = (int)((long long)plan.tiles * crowd / crowds), t1 = (int)((long long)plan.tiles * (crowd + 1) / crowds);
   // log2 of the warps on each tile in the round that begins at tile b < t1
   auto round_kw = [&](int b) {
     const int left = t1 - b, base = plan.kw_log2;
-    if (plan.slabs > 1 || left >= MV_WARPS >> base) return base;
+    if (left >= MV_WARPS >> base) return base;
     return 4 - (32 - __clz(left - 1));
   };
 
@@ -317,6 +315,7 @@ int4_mma_kernel(const Int4Args p, const MvPlan plan) {
 #pragma unroll
   for (int i = 0; i < MV_RING; ++i) fetch(i * MV_STEP_BYTES);
   stage_a(p, plan, a_smem, m0, m_here, first * MV_K);
+  __syncthreads();
 
   auto write = [&](int tile, int m, int r, float4 sum) {  // four outputs of row m, from row r of the tile on
     const int n = tile * MV_TILE + r;
@@ -369,127 +368,96 @@ int4_mma_kernel(const Int4Args p, const MvPlan plan) {
       a_base[nb][i] = min(8 * nb + g, m_here - 1) * plan.pitch + (kGW == 128 ? 4 * t + (i ^ (t >> 1)) : kGW == 64 ? 2 * t + i : t ^ i);
   uint32_t mask = 0x000f000fu, base128 = 0x43004300u;
   asm volatile("" : "+r"(mask), "+r"(base128));
-
-  const int buf_blocks = m_here * plan.pitch;
   uint32_t slot = 0;
-  int buf = 0;
   for (int b0 = t0, kwl; b0 < t1; b0 += MV_WARPS >> kwl) {
     kwl = round_kw(b0);
     const int kw = 1 << kwl, RG = MV_WARPS >> kwl;
     const int mk = warp & (kw - 1), rg = warp >> kwl;
     const int tile = b0 + rg;
     float acc[kNB][2][4] = {};
-    for (int s0 = first; s0 < steps; s0 += plan.slab_steps) {
-      const int s1 = min(s0 + plan.slab_steps, steps);
-      const bool last = s1 == steps && b0 + RG >= t1;
-      const int next_k = s1 == steps ? 0 : s1 * MV_K;  // the slab after this one
-      if (plan.slabs > 1 || b0 == t0) __syncthreads();  // this slab is in place, and nobody reads the one before it
-      if (plan.slabs > 1 && !last) {
-        uint4* to = a_smem + (buf ^ 1) * buf_blocks;
-        if (plan.a_vec) {
-          for_blocks(plan, m_here, [&](int at, int k, int m) {
-            const bool in = next_k + k < p.K;
-            cp_async_16(smem_u32(to + at), p.A + (long long)(m0 + m) * p.lda + (in ? next_k + k : 0), in ? 16 : 0);
-          });
-        } else {
-          stage_a(p, plan, to, m0, m_here, next_k);
-        }
-        cp_async_commit();
-      }
-      if (tile < t1) {
-        const uint4* a0 = a_smem + buf * buf_blocks + mk * (MV_K / 8);  // s0 + mk: a slab starts at a multiple of kw
-        for (int v = s0 + mk; v < s1; v += kw, a0 += kw * (MV_K / 8)) {
-          cp_async_wait<MV_RING - 1>();
-          __syncwarp();
-          uint32_t codes[4][4];
-          const uint32_t base = ring + slot + g * 64;
+    if (tile < t1) {
+      const uint4* a0 = a_smem + mk * (MV_K / 8);
+      for (int v = first + mk; v < steps; v += kw, a0 += kw * (MV_K / 8)) {
+        cp_async_wait<MV_RING - 1>();
+        __syncwarp();
+        uint32_t codes[4][4];
+        const uint32_t base = ring + slot + g * 64;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            if constexpr (kGW == 128) {
-              asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                           : "=r"(codes[r][0]), "=r"(codes[r][1]), "=r"(codes[r][2]), "=r"(codes[r][3])
-                           : "r"(base + ((t ^ f) << 4) + r * 512));
-            } else if constexpr (kGW == 64) {
+        for (int r = 0; r < 4; ++r) {
+          if constexpr (kGW == 128) {
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(codes[r][0]), "=r"(codes[r][1]), "=r"(codes[r][2]), "=r"(codes[r][3])
+                         : "r"(base + ((t ^ f) << 4) + r * 512));
+          } else if constexpr (kGW == 64) {
 #pragma unroll
-              for (int h = 0; h < 2; ++h)
-                asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
-                             : "=r"(codes[r][2 * h]), "=r"(codes[r][2 * h + 1])
-                             : "r"(base + ((((2 * h) | (t >> 1)) ^ f) << 4) + ((t & 1) << 3) + r * 512));
-            } else {
-#pragma unroll
-              for (int h = 0; h < 4; ++h)
-                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(codes[r][h]) : "r"(base + ((h ^ f) << 4) + (t << 2) + r * 512));
-            }
-          }
-          const Scales cur = sc;
-          if (v + kw < steps) {
-            sc.load(p, srow, (v + kw) * MV_K, plan.s_vec);
+            for (int h = 0; h < 2; ++h)
+              asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
+                           : "=r"(codes[r][2 * h]), "=r"(codes[r][2 * h + 1])
+                           : "r"(base + ((((2 * h) | (t >> 1)) ^ f) << 4) + ((t & 1) << 3) + r * 512));
           } else {
-            int round2 = b0 + RG, tile2, step2;
-            after(round2, tile2, step2);
-            if (tile2 < t1) {
-              scale_rows(tile2);
-              sc.load(p, srow, step2 * MV_K, plan.s_vec);
-            }
+#pragma unroll
+            for (int h = 0; h < 4; ++h)
+              asm volatile("ld.shared.u32 %0, [%1];" : "=r"(codes[r][h]) : "r"(base + ((h ^ f) << 4) + (t << 2) + r * 512));
           }
+        }
+        const Scales cur = sc;
+        if (v + kw < steps) {
+          sc.load(p, srow, (v + kw) * MV_K, plan.s_vec);
+        } else {
+          int round2 = b0 + RG, tile2, step2;
+          after(round2, tile2, step2);
+          if (tile2 < t1) {
+            scale_rows(tile2);
+            sc.load(p, srow, step2 * MV_K, plan.s_vec);
+          }
+        }
 #pragma unroll
-          for (int j = 0; j < GROUPS; ++j) {
-            float part[kNB][2][4];
-            uint32_t zero2[4];
+        for (int j = 0; j < GROUPS; ++j) {
+          float part[kNB][2][4];
+          uint32_t zero2[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) zero2[r] = cur.zero2(r, j);
+          for (int r = 0; r < 4; ++r) zero2[r] = cur.zero2(r, j);
 #pragma unroll
-            for (int i = 0; i < WPG; ++i) {
-              const int w = j * WPG + i;
-              uint4 x[kNB];
+          for (int i = 0; i < WPG; ++i) {
+            const int w = j * WPG + i;
+            uint4 x[kNB];
+#pragma unroll
+            for (int nb = 0; nb < kNB; ++nb) {
+              if constexpr (kGW == 128) x[nb] = a0[a_base[nb][i & 1] + (i & 2)];
+              else if constexpr (kGW == 64) x[nb] = a0[a_base[nb][i ^ j] + 8 * j];
+              else x[nb] = a0[a_base[nb][j >> 1] + 4 * j];
+            }
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt) {
+              uint32_t lo[4], hi[4];  // rows g and g + 8 of this m16 tile
+              dequant8(codes[2 * mt][w], zero2[2 * mt], mask, base128, lo);
+              dequant8(codes[2 * mt + 1][w], zero2[2 * mt + 1], mask, base128, hi);
 #pragma unroll
               for (int nb = 0; nb < kNB; ++nb) {
-                if constexpr (kGW == 128) x[nb] = a0[a_base[nb][i & 1] + (i & 2)];
-                else if constexpr (kGW == 64) x[nb] = a0[a_base[nb][i ^ j] + 8 * j];
-                else x[nb] = a0[a_base[nb][j >> 1] + 4 * j];
-              }
-#pragma unroll
-              for (int mt = 0; mt < 2; ++mt) {
-                uint32_t lo[4], hi[4];  // rows g and g + 8 of this m16 tile
-                dequant8(codes[2 * mt][w], zero2[2 * mt], mask, base128, lo);
-                dequant8(codes[2 * mt + 1][w], zero2[2 * mt + 1], mask, base128, hi);
-#pragma unroll
-                for (int nb = 0; nb < kNB; ++nb) {
-                  if (i == 0) mma_bf16_zero(part[nb][mt], lo[0], hi[0], lo[1], hi[1], x[nb].x, x[nb].y);
-                  else mma_bf16(part[nb][mt], lo[0], hi[0], lo[1], hi[1], x[nb].x, x[nb].y);
-                  mma_bf16(part[nb][mt], lo[2], hi[2], lo[3], hi[3], x[nb].z, x[nb].w);
-                }
-              }
-            }
-            // A group that lies past K whole has sums of 0 and repeats a scale, which may be anything: 0 * inf must not count.
-            if (GROUPS == 1 || v * MV_K + j * kGW < p.K) {
-#pragma unroll
-              for (int mt = 0; mt < 2; ++mt) {
-                const float sc0 = cur.scale(2 * mt, j), sc1 = cur.scale(2 * mt + 1, j);
-#pragma unroll
-                for (int nb = 0; nb < kNB; ++nb) {
-                  acc[nb][mt][0] = fmaf(sc0, part[nb][mt][0], acc[nb][mt][0]);
-                  acc[nb][mt][1] = fmaf(sc0, part[nb][mt][1], acc[nb][mt][1]);
-                  acc[nb][mt][2] = fmaf(sc1, part[nb][mt][2], acc[nb][mt][2]);
-                  acc[nb][mt][3] = fmaf(sc1, part[nb][mt][3], acc[nb][mt][3]);
-                }
+                if (i == 0) mma_bf16_zero(part[nb][mt], lo[0], hi[0], lo[1], hi[1], x[nb].x, x[nb].y);
+                else mma_bf16(part[nb][mt], lo[0], hi[0], lo[1], hi[1], x[nb].x, x[nb].y);
+                mma_bf16(part[nb][mt], lo[2], hi[2], lo[3], hi[3], x[nb].z, x[nb].w);
               }
             }
           }
-          __syncwarp();  // every lane has its words: the slot takes the step after the ring's last
-          fetch(slot);
-          slot = slot == (MV_RING - 1) * MV_STEP_BYTES ? 0 : slot + MV_STEP_BYTES;
+          // A group that lies past K whole has sums of 0 and repeats a scale, which may be anything: 0 * inf must not count.
+          if (GROUPS == 1 || v * MV_K + j * kGW < p.K) {
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt) {
+              const float sc0 = cur.scale(2 * mt, j), sc1 = cur.scale(2 * mt + 1, j);
+#pragma unroll
+              for (int nb = 0; nb < kNB; ++nb) {
+                acc[nb][mt][0] = fmaf(sc0, part[nb][mt][0], acc[nb][mt][0]);
+                acc[nb][mt][1] = fmaf(sc0, part[nb][mt][1], acc[nb][mt][1]);
+                acc[nb][mt][2] = fmaf(sc1, part[nb][mt][2], acc[nb][mt][2]);
+                acc[nb][mt][3] = fmaf(sc1, part[nb][mt][3], acc[nb][mt][3]);
+              }
+            }
+          }
         }
-      }
-      if (plan.slabs > 1) {
-        buf ^= 1;
-        if (plan.a_vec && !last) {
-          // The copies of the next slab are older than this slab's fetches, if those were as many as the ring is deep.
-          if (tile < t1 && s1 - s0 >= MV_RING * kw) cp_async_wait<MV_RING - 1>();
-          else cp_async_wait<0>();
-          uint4* to = a_smem + buf * buf_blocks;
-          for_blocks(plan, m_here, [&](int at, int, int) { to[at] = pairs_of(to[at]); });
-        }
+        __syncwarp();  // every lane has its words: the slot takes the step after the ring's last
+        fetch(slot);
+        slot = slot == (MV_RING - 1) * MV_STEP_BYTES ? 0 : slot + MV_STEP_BYTES;
       }
     }
     // The tile's sums over the warps that share it, always in the order of the warps.
@@ -651,45 +619,43 @@ int check_int4(int64_t N, int64_t K, int64_t group, int32_t scale_dtype) {
 bool aligned_to(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 int bytes_of(int32_t dtype) { return dtype == SYMPLEX_DT_F32 ? 4 : 2; }
 
+// Shared memory of a CTA for `rows` rows of A and `steps` steps, alone or in a cluster.
+template <int kGW>
+size_t mv_smem(int rows, int steps, bool cluster) {
+  const int nb = rows > 8 ? 2 : 1;
+  const size_t joined = (size_t)MV_WARPS * (MV_TILE + 4) * 8 * nb * 4, held = cluster ? 2 * (MV_WARPS >> MV_CLUSTER_KW) * MV_TILE * 8 * nb * 4 : 0;
+  return MV_RING_BYTES + joined + held + (size_t)rows * (steps * (MV_K / 8) + MvPad<kGW>) * 16;
+}
+// The smallest cluster whose CTAs hold `rows` rows of A between them; 0: none does.
+template <int kGW>
+int mv_cluster(int rows, int steps) {
+  for (int c = 1; c <= MV_CLUSTER_MOST; c *= 2)
+    if (mv_smem<kGW>(rows, (steps + c - 1) / c, c > 1) <= MV_SMEM) return c;
+  return 0;
+}
+
 template <int kGW, int kNB, typename ST, bool kZeros>
-int matvec_mma(const Int4Args& a, bool out_bf16, int sms, cudaStream_t stream) {
+int matvec_mma(const Int4Args& a, int rows, int cluster, bool out_bf16, int sms, cudaStream_t stream) {
   auto kern = int4_mma_kernel<kGW, kNB, ST, kZeros>;
   constexpr int GROUPS = MV_K / kGW;
-  MvPlan plan{};
-  plan.tiles = (a.N + MV_TILE - 1) / MV_TILE;
-  const int steps = (a.K + MV_K - 1) / MV_K;
-  const int rows = std::min(a.M, 8 * kNB);
-  auto bytes = [&](int n) { return (size_t)rows * (n * (MV_K / 8) + MvPad<kGW>) * 16; };
-  constexpr int SUMS = MV_WARPS * (MV_TILE + 4) * 8 * kNB * 4, HELD = 2 * 4 * MV_TILE * 8 * kNB * 4;
-  const int mblocks = (a.M + 8 * kNB - 1) / (8 * kNB);
+  const int mblocks = (a.M + rows - 1) / rows, steps = (a.K + MV_K - 1) / MV_K;
   SX_ENSURE_DYN_SMEM(kern, MV_SMEM);
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
-  // The smallest cluster whose CTAs hold A between them, with four warps on a tile, more where a CTA has fewer than four tiles
-  // (5 x 50257 x 2048: 24.2 us, 31.3 with 16 warps, 26.0 with two; 1 x 4096 x 4096 with one tile a CTA: 5.5 with 16 or 4 warps, 8.2 with
-  // two); else slabs of 8 steps in two buffers, two warps on a tile.
-  plan.cluster = 1;
-  auto fits = [&](int c) { return MV_RING_BYTES + SUMS + (c > 1 ? HELD : 0) + bytes((steps + c - 1) / c) <= MV_SMEM; };
-  while (plan.cluster < MV_CLUSTER_MOST && !fits(plan.cluster)) plan.cluster *= 2;
-  const bool whole = fits(plan.cluster) && sms >= plan.cluster * mblocks;
-  int crowds = std::max(1, sms / mblocks);
-  if (whole) {
-    plan.slab_steps = (steps + plan.cluster - 1) / plan.cluster;
-    plan.slabs = 1;
-    crowds = std::max(1, crowds / plan.cluster);
-  } else {
-    plan.cluster = 1;
-    plan.slab_steps = MV_SLAB_STEPS;
-    plan.slabs = (steps + MV_SLAB_STEPS - 1) / MV_SLAB_STEPS;
-  }
-  plan.pitch = plan.slab_steps * (MV_K / 8) + MvPad<kGW>;
+  MvPlan plan{};
+  plan.tiles = (a.N + MV_TILE - 1) / MV_TILE;
+  plan.rows = rows;
+  plan.cluster = cluster;
+  plan.steps = (steps + cluster - 1) / cluster;
+  int crowds = std::max(1, sms / mblocks / cluster);
+  plan.pitch = plan.steps * (MV_K / 8) + MvPad<kGW>;
   plan.a_vec = a.lda % 8 == 0 && reinterpret_cast<uintptr_t>(a.A) % 16 == 0;
   plan.s_vec = a.group == kGW && a.groups % GROUPS == 0 && reinterpret_cast<uintptr_t>(a.scales) % (GROUPS * sizeof(ST)) == 0 &&
                reinterpret_cast<uintptr_t>(a.zeros) % GROUPS == 0;
   plan.out_bf16 = out_bf16 ? 1 : 0;
   plan.c_vec = a.ldc % 4 == 0 && reinterpret_cast<uintptr_t>(a.C) % (out_bf16 ? 8 : 16) == 0;
   cfg.blockDim = dim3(MV_WARPS * 32, 1, 1);
-  cfg.dynamicSmemBytes = MV_RING_BYTES + SUMS + (plan.cluster > 1 ? HELD : 0) + bytes(plan.slab_steps) * (whole ? 1 : 2);
+  cfg.dynamicSmemBytes = mv_smem<kGW>(rows, plan.steps, cluster > 1);
   cfg.stream = stream;
   cfg.attrs = attr;
   if (plan.cluster > 1) {
@@ -711,13 +677,12 @@ int matvec_mma(const Int4Args& a, bool out_bf16, int sms, cudaStream_t stream) {
   }
   crowds = std::min(crowds, plan.tiles);
   cfg.gridDim = dim3((unsigned)(crowds * plan.cluster), (unsigned)mblocks, 1);
-  if (whole) {
-    const int each = (plan.tiles + crowds - 1) / crowds;  // tiles of a CTA or cluster
-    while (plan.kw_log2 < 4 && (2 << plan.kw_log2) <= plan.slab_steps && (plan.kw_log2 < 2 || each << plan.kw_log2 < MV_WARPS)) ++plan.kw_log2;
-    if (plan.cluster > 1) plan.kw_log2 = std::max(plan.kw_log2, 2);  // at most four tiles a round
-  } else {
-    plan.kw_log2 = 1;
-  }
+  // Four warps on a tile, more where a CTA has fewer than four tiles (5 x 50257 x 2048: 24.2 us, 31.3 with 16 warps, 26.0 with two;
+  // 1 x 4096 x 4096 with one tile a CTA: 5.5 with 16 or 4 warps, 8.2 with two).
+  const int each = (plan.tiles + crowds - 1) / crowds;  // tiles of a CTA or cluster
+  const int base = cluster > 1 ? MV_CLUSTER_KW : 2;
+  while (plan.kw_log2 < 4 && (2 << plan.kw_log2) <= plan.steps && (plan.kw_log2 < base || each << plan.kw_log2 < MV_WARPS)) ++plan.kw_log2;
+  if (cluster > 1) plan.kw_log2 = std::max(plan.kw_log2, MV_CLUSTER_KW);
   if (pdl_enabled()) {
     attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
@@ -730,10 +695,12 @@ int matvec_mma(const Int4Args& a, bool out_bf16, int sms, cudaStream_t stream) {
 }
 
 template <int kGW, typename ST>
-int matvec_gw(const Int4Args& a, bool out_bf16, int sms, cudaStream_t stream) {
-  if (a.M <= 8)
-    return a.zeros ? matvec_mma<kGW, 1, ST, true>(a, out_bf16, sms, stream) : matvec_mma<kGW, 1, ST, false>(a, out_bf16, sms, stream);
-  return a.zeros ? matvec_mma<kGW, 2, ST, true>(a, out_bf16, sms, stream) : matvec_mma<kGW, 2, ST, false>(a, out_bf16, sms, stream);
+int matvec_gw(const Int4Args& a, int rows, int cluster, bool out_bf16, int sms, cudaStream_t stream) {
+  if (rows <= 8)
+    return a.zeros ? matvec_mma<kGW, 1, ST, true>(a, rows, cluster, out_bf16, sms, stream)
+                   : matvec_mma<kGW, 1, ST, false>(a, rows, cluster, out_bf16, sms, stream);
+  return a.zeros ? matvec_mma<kGW, 2, ST, true>(a, rows, cluster, out_bf16, sms, stream)
+                 : matvec_mma<kGW, 2, ST, false>(a, rows, cluster, out_bf16, sms, stream);
 }
 
 template <typename ST>
@@ -741,9 +708,17 @@ int matvec(const Int4Args& a, bool out_bf16, int sms, cudaStream_t stream) {
   // The fast path reads rows of codes in 16-byte blocks; which of its forms goes by the group.
   const uintptr_t at = reinterpret_cast<uintptr_t>(a.codes) | (uintptr_t)a.ldq;
   if (a.K % 32 == 0 && at % 16 == 0 && (long long)a.N * a.groups < (1ll << 32)) {
-    if (a.group % 128 == 0) return matvec_gw<128, ST>(a, out_bf16, sms, stream);
-    if (a.group % 64 == 0) return matvec_gw<64, ST>(a, out_bf16, sms, stream);
-    return matvec_gw<32, ST>(a, out_bf16, sms, stream);
+    const int steps = (a.K + MV_K - 1) / MV_K, gw = a.group % 128 == 0 ? 128 : a.group % 64 == 0 ? 64 : 32;
+    // Up to 16 rows of A in a pass over W, as even as they go; fewer where even a cluster does not hold them. K is beyond 300000 where not
+    // one fits.
+    const int passes = (a.M + 15) / 16;
+    for (int rows = (a.M + passes - 1) / passes; rows > 0; rows = rows > 8 ? 8 : rows / 2) {
+      const int cluster = gw == 128 ? mv_cluster<128>(rows, steps) : gw == 64 ? mv_cluster<64>(rows, steps) : mv_cluster<32>(rows, steps);
+      if (cluster == 0) continue;
+      if (gw == 128) return matvec_gw<128, ST>(a, rows, cluster, out_bf16, sms, stream);
+      if (gw == 64) return matvec_gw<64, ST>(a, rows, cluster, out_bf16, sms, stream);
+      return matvec_gw<32, ST>(a, rows, cluster, out_bf16, sms, stream);
+    }
   }
   const cudaError_t e = out_bf16 ? launch_kernel_ex(int4_matvec_any_kernel<ST, __nv_bfloat16>, (unsigned)((a.N + 7) / 8), 256, 0, stream, 1,
                                                     pdl_enabled(), a)

@@ -264,7 +264,7 @@ def int4_matvec(x, codes, scales, zeros=None, *, group_size=128, bias=None, acti
     """``act(x @ W.T + bias)`` for a few rows of ``x`` (at most 64), ``W[n, k] = (codes[n, k] - zeros[n, k // group_size]) *
     scales[n, k // group_size]`` held as ``int4_quantize`` lays it out (``symplex_b200_int4_matvec``).
 
-    ``x``: bfloat16 ``[K]`` or ``[M, K]``; ``zeros`` None means 8 everywhere; ``bias``: float32 ``[N]``; ``activation`` as in
+    ``x``: bfloat16 ``[K]`` or ``[M, K]``; ``zeros`` (0 to 15) None means 8 everywhere; ``bias``: float32 ``[N]``; ``activation`` as in
     ``gemm``. ``codes`` may be a view with unit stride in its rows. Returns ``[N]`` / ``[M, N]`` in ``out_dtype`` (bfloat16 or
     float32). More rows than 64 are a product for ``gemm``.
     """
