@@ -57,20 +57,23 @@ def _ptr(t):
 # ----------------------------------------------------------------------------- layer norm
 
 def _norm_checks(who, x, *params):
-    if not x.is_cuda or x.dtype not in _DT:
+    """(columns, dtype of the parameters) of a norm over ``x``."""
+    dtype, shape = x.dtype, x.shape
+    if not x.is_cuda or dtype not in _DT:
         raise ValueError(f"{who} takes float32 or bfloat16 CUDA tensors")
-    if x.dim() == 0 or x.shape[-1] == 0:
-        raise ValueError(f"{who} needs at least one value in the last dimension, got shape {tuple(x.shape)}")
-    dtype = None
+    if not shape or shape[-1] == 0:
+        raise ValueError(f"{who} needs at least one value in the last dimension, got shape {tuple(shape)}")
+    cols, device, found = shape[-1], x.device, None
     for p in params:
         if p is None:
             continue
-        if p.dim() != 1 or p.shape[0] != x.shape[-1] or p.device != x.device:
-            raise ValueError(f"weight and bias must have shape ({x.shape[-1]},) on {x.device}")
-        if p.dtype != x.dtype and p.dtype != torch.float32 or dtype not in (None, p.dtype):
+        if p.shape != (cols,) or p.device != device:
+            raise ValueError(f"weight and bias must have shape ({cols},) on {device}")
+        pdt = p.dtype
+        if pdt != dtype and pdt != torch.float32 or found not in (None, pdt):
             raise ValueError("weight and bias must both have the input's dtype or both be float32")
-        dtype = p.dtype
-    return dtype if dtype is not None else x.dtype
+        found = pdt
+    return cols, found or dtype
 
 
 def layer_norm(x, weight=None, bias=None, *, eps=1e-5, out=None, return_stats=False, stream=None):
@@ -82,7 +85,7 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5, out=None, return_stats=Fa
     Returns ``y``, or ``(y, mean, rstd)`` with ``return_stats`` (float32, shaped like ``x`` without its last dimension):
     what ``layer_norm_backward`` takes.
     """
-    pdt = _norm_checks("layer_norm()", x, weight, bias)
+    cols, pdt = _norm_checks("layer_norm()", x, weight, bias)
     if not eps >= 0:
         raise ValueError("eps must not be negative")
     if out is not None and (out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or
@@ -94,14 +97,13 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5, out=None, return_stats=Fa
         y = out if out is not None else _like(x)
         mean = rstd = None
         if return_stats:
-            mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+            mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
             rstd = torch.empty_like(mean)
         w = weight.contiguous() if weight is not None else None
         b = bias.contiguous() if bias is not None else None
-        cols = x.shape[-1]
         _capi.check(_capi.load().symplex_b200_layer_norm(
             xr.data_ptr(), _ptr(w), _ptr(b), y.data_ptr(), _ptr(mean), _ptr(rstd), x.numel() // cols, cols, ldx,
-            cols if y.is_contiguous() else y.stride(0), _DT[x.dtype], _DT[pdt], eps, s))
+            cols if out is None or y.is_contiguous() else y.stride(0), _DT[x.dtype], _DT[pdt], eps, s))
         return (y, mean, rstd) if return_stats else y
 
     return _run(x.device, stream, call)
@@ -114,28 +116,28 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, *, param_grads=None, str
     ``dweight`` and ``dbias`` have ``weight``'s dtype (``x``'s where there is no weight) and are None unless
     ``param_grads`` (default: whether ``weight`` is given). Their sums over rows are 32-bit, in a fixed order.
     """
-    pdt = _norm_checks("layer_norm_backward()", x, weight)
-    if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
+    cols, pdt = _norm_checks("layer_norm_backward()", x, weight)
+    shape, device = x.shape, x.device
+    if dy.shape != shape or dy.dtype != x.dtype or dy.device != device:
         raise ValueError("dy must match x in shape, dtype and device")
     for t in (mean, rstd):
-        if t.dtype != torch.float32 or t.shape != x.shape[:-1] or t.device != x.device:
-            raise ValueError(f"mean and rstd must be float32 of shape {tuple(x.shape[:-1])} on {x.device}")
+        if t.dtype != torch.float32 or t.shape != shape[:-1] or t.device != device:
+            raise ValueError(f"mean and rstd must be float32 of shape {tuple(shape[:-1])} on {device}")
     if param_grads is None:
         param_grads = weight is not None
 
     def call(s):
         lib = _capi.load()
         (xr, ldx), (dyr, lddy) = _rows(x), _rows(dy)
-        cols = x.shape[-1]
         rows = x.numel() // cols
         dx = _like(x)
         dw = db = ws = None
         size = 0
         if param_grads:
-            dw = torch.empty(cols, dtype=pdt, device=x.device)
+            dw = x.new_empty(cols, dtype=pdt)
             db = torch.empty_like(dw)
             size = lib.symplex_b200_layer_norm_backward_workspace_bytes(rows, cols)
-            ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+            ws = x.new_empty(size, dtype=torch.uint8)
         w = weight.contiguous() if weight is not None else None
         m, r = mean.contiguous(), rstd.contiguous()
         _capi.check(lib.symplex_b200_layer_norm_backward(
@@ -143,24 +145,30 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, *, param_grads=None, str
             lddy, ldx, cols, _DT[x.dtype], _DT[pdt], _ptr(ws), size, s))
         return dx, dw, db
 
-    return _run(x.device, stream, call)
+    return _run(device, stream, call)
 
 
 # ----------------------------------------------------------------------------- softmax cross entropy of a linear head
 
 def _loss_checks(who, x, weight, targets, ignore_index, reduction):
-    if not x.is_cuda or x.dtype not in _DT or x.dim() != 2:
+    """(T, H, V) of a loss."""
+    dtype, shape, device = x.dtype, x.shape, x.device
+    if not x.is_cuda or dtype not in _DT or len(shape) != 2:
         raise ValueError(f"{who} takes a 2-D float32 or bfloat16 CUDA tensor")
-    if weight.dtype != x.dtype or weight.dim() != 2 or weight.shape[1] != x.shape[1] or weight.device != x.device:
-        raise ValueError(f"weight must be {x.dtype} of shape [V, {x.shape[1]}] on {x.device}, got {weight.dtype} {tuple(weight.shape)}")
-    if x.shape[1] == 0 or weight.shape[0] == 0:
+    t, h = shape
+    wshape = weight.shape
+    if weight.dtype != dtype or len(wshape) != 2 or wshape[1] != h or weight.device != device:
+        raise ValueError(f"weight must be {dtype} of shape [V, {h}] on {device}, got {weight.dtype} {tuple(wshape)}")
+    v = wshape[0]
+    if h == 0 or v == 0:
         raise ValueError("the hidden size and the vocabulary must not be empty")
-    if targets.dtype != torch.int64 or targets.shape != x.shape[:1] or targets.device != x.device:
-        raise ValueError(f"targets must be int64 of shape ({x.shape[0]},) on {x.device}")
+    if targets.dtype != torch.int64 or targets.shape != (t,) or targets.device != device:
+        raise ValueError(f"targets must be int64 of shape ({t},) on {device}")
     if reduction not in LOSS_REDUCTIONS:
         raise ValueError(f"reduction must be one of {sorted(LOSS_REDUCTIONS)}, got {reduction!r}")
     if not isinstance(ignore_index, int) or not -2 ** 63 <= ignore_index < 2 ** 63:
         raise ValueError("ignore_index must be a 64-bit integer")
+    return t, h, v
 
 
 def linear_cross_entropy(x, weight, targets, *, ignore_index=-100, reduction="mean", stream=None):
@@ -172,17 +180,15 @@ def linear_cross_entropy(x, weight, targets, *, ignore_index=-100, reduction="me
     rows' log-sum-exp, which the backward pass takes. A target outside ``0..V-1`` gives its row the loss NaN;
     so does an infinity among float32 operands (their products are split into tf32 parts).
     """
-    _loss_checks("linear_cross_entropy()", x, weight, targets, ignore_index, reduction)
+    t, h, v = _loss_checks("linear_cross_entropy()", x, weight, targets, ignore_index, reduction)
 
     def call(s):
         lib = _capi.load()
         (xr, ldx), (w, ldw) = _rows(x), _rows(weight)
-        t, h = x.shape
-        v = weight.shape[0]
-        lse = torch.empty(t, dtype=torch.float32, device=x.device)
-        loss = torch.empty_like(lse) if reduction == "none" else torch.empty((), dtype=torch.float32, device=x.device)
+        lse = x.new_empty(t, dtype=torch.float32)
+        loss = torch.empty_like(lse) if reduction == "none" else lse.new_empty(())
         size = lib.symplex_b200_linear_cross_entropy_workspace_bytes(xr.data_ptr(), w.data_ptr(), t, h, v, ldx, ldw, _DT[x.dtype])
-        ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+        ws = x.new_empty(size, dtype=torch.uint8)
         tg = targets.contiguous()
         _capi.check(lib.symplex_b200_linear_cross_entropy(
             xr.data_ptr(), w.data_ptr(), tg.data_ptr(), loss.data_ptr(), lse.data_ptr(), t, h, v, ldx, ldw, _DT[x.dtype], ignore_index,
@@ -199,9 +205,7 @@ def linear_cross_entropy_backward(dloss, x, weight, targets, lse, *, ignore_inde
     as there. The logits are computed again a piece of the vocabulary at a time. ``dx`` and ``dweight`` have the dtype of ``x``.
     Ignored rows of ``x`` must be finite (their zero gradient meets them in ``dweight``).
     """
-    _loss_checks("linear_cross_entropy_backward()", x, weight, targets, ignore_index, reduction)
-    t, h = x.shape
-    v = weight.shape[0]
+    t, h, v = _loss_checks("linear_cross_entropy_backward()", x, weight, targets, ignore_index, reduction)
     if dloss.dtype != torch.float32 or dloss.device != x.device or \
             (dloss.shape != (t,) if reduction == "none" else dloss.numel() != 1):
         raise ValueError(f"dloss must be float32 on {x.device}: shape ({t},) for 'none', one value otherwise")
@@ -213,7 +217,7 @@ def linear_cross_entropy_backward(dloss, x, weight, targets, lse, *, ignore_inde
         (xr, ldx), (w, ldw) = _rows(x), _rows(weight)
         dx, dw = _like(x), _like(weight)
         size = lib.symplex_b200_linear_cross_entropy_backward_workspace_bytes(xr.data_ptr(), w.data_ptr(), t, h, v, ldx, ldw, _DT[x.dtype])
-        ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+        ws = x.new_empty(size, dtype=torch.uint8)
         tg, ls, dl = targets.contiguous(), lse.contiguous(), dloss.contiguous()
         _capi.check(lib.symplex_b200_linear_cross_entropy_backward(
             dl.data_ptr(), xr.data_ptr(), w.data_ptr(), tg.data_ptr(), ls.data_ptr(), dx.data_ptr(), dw.data_ptr(), t, h, v, ldx, ldw,
@@ -268,31 +272,33 @@ def int4_matvec(x, codes, scales, zeros=None, *, group_size=128, bias=None, acti
     ``gemm``. ``codes`` may be a view with unit stride in its rows. Returns ``[N]`` / ``[M, N]`` in ``out_dtype`` (bfloat16 or
     float32). More rows than 64 are a product for ``gemm``.
     """
-    if not x.is_cuda or x.dtype != torch.bfloat16 or x.dim() not in (1, 2):
+    xshape, device = x.shape, x.device
+    if not x.is_cuda or x.dtype != torch.bfloat16 or len(xshape) not in (1, 2):
         raise ValueError("int4_matvec() takes a 1-D or 2-D bfloat16 CUDA tensor")
-    k = x.shape[-1]
-    m = x.shape[0] if x.dim() == 2 else 1
+    k = xshape[-1]
+    m = xshape[0] if len(xshape) == 2 else 1
     if m > INT4_MAX_ROWS:
         raise ValueError(f"int4_matvec() takes at most {INT4_MAX_ROWS} rows, got {m}: use gemm()")
     if k == 0:
         raise ValueError("K == 0 is not supported")
     groups = _group_count(k, group_size, "int4_matvec()")
-    if codes.dtype != torch.uint8 or codes.dim() != 2 or codes.shape[1] != (k + 1) // 2 or codes.device != x.device:
-        raise ValueError(f"codes must be uint8 of shape [N, {(k + 1) // 2}] on {x.device}, got {codes.dtype} {tuple(codes.shape)}")
-    n = codes.shape[0]
-    if scales.dtype not in _DT or scales.shape != (n, groups) or scales.device != x.device:
-        raise ValueError(f"scales must be float32 or bfloat16 of shape ({n}, {groups}) on {x.device}")
-    if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != (n, groups) or zeros.device != x.device):
-        raise ValueError(f"zeros must be uint8 of shape ({n}, {groups}) on {x.device}")
-    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or bias.device != x.device):
-        raise ValueError(f"bias must be float32 of shape ({n},) on {x.device}")
+    cshape = codes.shape
+    if codes.dtype != torch.uint8 or len(cshape) != 2 or cshape[1] != (k + 1) // 2 or codes.device != device:
+        raise ValueError(f"codes must be uint8 of shape [N, {(k + 1) // 2}] on {device}, got {codes.dtype} {tuple(cshape)}")
+    n = cshape[0]
+    if scales.dtype not in _DT or scales.shape != (n, groups) or scales.device != device:
+        raise ValueError(f"scales must be float32 or bfloat16 of shape ({n}, {groups}) on {device}")
+    if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != (n, groups) or zeros.device != device):
+        raise ValueError(f"zeros must be uint8 of shape ({n}, {groups}) on {device}")
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or bias.device != device):
+        raise ValueError(f"bias must be float32 of shape ({n},) on {device}")
     if activation not in ACTIVATIONS:
         raise ValueError(f"unknown activation {activation!r}; expected one of {sorted(a for a in ACTIVATIONS if a)}")
-    shape = (n,) if x.dim() == 1 else (m, n)
+    shape = (n,) if len(xshape) == 1 else (m, n)
     if out is not None:
-        if out.shape != shape or out.dtype not in _DT or out.device != x.device or not out.is_contiguous() or \
+        if out.shape != shape or out.dtype not in _DT or out.device != device or not out.is_contiguous() or \
                 out_dtype not in (None, out.dtype):
-            raise ValueError(f"out must be a contiguous float32 or bfloat16 tensor of shape {shape} on {x.device}")
+            raise ValueError(f"out must be a contiguous float32 or bfloat16 tensor of shape {shape} on {device}")
         out_dtype = out.dtype
     elif out_dtype is None:
         out_dtype = torch.bfloat16
@@ -300,7 +306,7 @@ def int4_matvec(x, codes, scales, zeros=None, *, group_size=128, bias=None, acti
         raise ValueError("out dtype must be float32 or bfloat16")
 
     def call(s):
-        y = out if out is not None else torch.empty(shape, dtype=out_dtype, device=x.device)
+        y = out if out is not None else x.new_empty(shape, dtype=out_dtype)
         (a, lda), (c, ldq) = _rows(x), _rows(codes)
         sc = scales.contiguous()
         z = zeros.contiguous() if zeros is not None else None
@@ -310,4 +316,4 @@ def int4_matvec(x, codes, scales, zeros=None, *, group_size=128, bias=None, acti
             _DT[sc.dtype], _DT[out_dtype], ACTIVATIONS[activation], s))
         return y
 
-    return _run(x.device, stream, call)
+    return _run(device, stream, call)
