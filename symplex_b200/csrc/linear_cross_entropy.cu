@@ -284,6 +284,9 @@ struct Layout {
   size_t total;
 };
 
+// fp32: columns of a tile of dx.
+int dx_tile(long long H) { return H > 64 ? 128 : 64; }
+
 Layout layout(const Problem& p, bool backward) {
   Layout w{};
   w.hp = up(p.H, 8);
@@ -299,9 +302,10 @@ Layout layout(const Problem& p, bool backward) {
     w.chunks = (int)((nkb + kb - 1) / kb);
   }
   if (backward && !p.bf16) {
-    // dx = G W has T / 128 x H / 64 tiles over the whole piece: cut into parts of 512 columns or more until they fill the SMs
-    const long long tiles = ((p.T + 127) / 128) * ((p.H + 63) / 64);
-    const long long want = std::min<long long>((148 + tiles - 1) / tiles, w.piece / 512);
+    // dx = G W has T / 128 x H / 128 tiles over the whole piece: cut into parts of 512 columns or more, as many as one wave of tiles
+    // takes (509 x 512 x 8192: 160 tiles of 64 columns, two waves, took 71 us of the pass' 183; 144 of 128 columns, one wave: 141 in all)
+    const long long tiles = ((p.T + 127) / 128) * ((p.H + dx_tile(p.H) - 1) / dx_tile(p.H));
+    const long long want = std::min<long long>(148 / tiles, w.piece / 512);
     if (want > 1) {
       w.chunk = up((w.piece + want - 1) / want, 32);
       w.chunks = (int)((w.piece + w.chunk - 1) / w.chunk);
@@ -393,7 +397,7 @@ int readable(bool copy, const void* p, long long rows, long long cols, long long
 
 // fp32: C[M, N] = A B^T + R from operands in {hi, lo} planes, both K contiguous.
 int split_product(const CeCommon& c, const float* A, long long lda, long long plane_a, const float* B, long long ldb, long long plane_b, float* C,
-                  long long ldc, const float* R, long long M, long long N, long long K, cudaStream_t stream, int batch = 1) {
+                  long long ldc, const float* R, long long M, long long N, long long K, cudaStream_t stream, int batch = 1, int bn = 0) {
   TcGemmArgs g{};
   g.M = M; g.N = N; g.K = K;
   g.batch = batch;
@@ -407,7 +411,7 @@ int split_product(const CeCommon& c, const float* A, long long lda, long long pl
   g.num_sms = c.num_sms;
   g.wait_limit_ns = c.wait_limit_ns;
   // the general product's rule: 128-column tiles where they fill the chip
-  g.bn = N > 64 && ((M + 127) / 128) * ((N + 127) / 128) * batch >= c.num_sms ? 128 : 64;
+  g.bn = bn ? bn : N > 64 && ((M + 127) / 128) * ((N + 127) / 128) * batch >= c.num_sms ? 128 : 64;
   const int rc = launch_gemm_tf32x3(g, stream);
   if (rc == SX_ERR_EXEC) return launch_failed(cudaGetLastError(), "loss product launch failed");
   if (rc == SX_OK) count_launches(1);
@@ -519,7 +523,7 @@ int backward(const Problem& p, const CeCommon& dev, const float* dloss, const lo
     CE_LAUNCH(ce_piece_grad_kernel, std::min<long long>(tiles, dev.num_sms * 8LL), 256, (const float*)logits, w.piece, (int)n, v0, targets, lse,
               dloss, (const float*)scale, G, w.chunk, GT, w.tp, n * w.tp, p.T, p.V, p.ignore);
     if (w.chunks > 1) {
-      CE_TRY(split_product(dev, G, w.chunk, p.T * w.chunk, wts, w.chunk, p.H * w.chunk, acc[0], p.H, nullptr, p.T, p.H, w.chunk, stream, chunks));
+      CE_TRY(split_product(dev, G, w.chunk, p.T * w.chunk, wts, w.chunk, p.H * w.chunk, acc[0], p.H, nullptr, p.T, p.H, w.chunk, stream, chunks, dx_tile(p.H)));
       CE_LAUNCH(ce_join_kernel<float>, std::min<long long>((p.T * p.H + 255) / 256, dev.num_sms * 8LL), 256, (const float*)acc[0], chunks, p.T * p.H,
                 (const float*)nullptr, static_cast<float*>(dx), i > 0 ? 1 : 0);
     } else {
