@@ -528,7 +528,8 @@ int symplex_b200_layer_norm(const void* x, const void* weight, const void* bias,
  *   dx = rstd * (g - mean_cols(g) - xh * mean_cols(g * xh)),  dweight = sum_rows dy * xh,  dbias = sum_rows dy.
  * dx (of type dtype, may be dy), dweight and dbias (of type param_dtype) may each be NULL: then they are not computed.
  * The sums over rows are 32-bit and taken in an order that does not change from call to call. rows == 0 sets dweight
- * and dbias to zero. The workspace is used only where dweight or dbias is asked for. */
+ * and dbias to zero. The workspace is used only where dweight or dbias is asked for. The first call on a device must not be
+ * inside a stream capture. */
 size_t symplex_b200_layer_norm_backward_workspace_bytes(int64_t rows, int64_t cols);
 int symplex_b200_layer_norm_backward(const void* dy, const void* x, const float* mean, const float* rstd,
                                      const void* weight, void* dx, void* dweight, void* dbias, int64_t rows,
@@ -582,8 +583,8 @@ int symplex_b200_linear_cross_entropy(const void* x, const void* W, const int64_
  *   dx[T, H] = G . W,  dW[V, H] = G^T . x     (packed, of type dtype)
  * where s[t] is dloss[t] (NONE), dloss[0] (SUM) or dloss[0] / number of counted rows (MEAN), and 0 for ignored rows. The
  * logits are computed again, a piece of the vocabulary at a time; G is held in dtype (BF16: rounded, without the factor all
- * rows share), sums are 32-bit, in an order that does not change from call to call. Rows of x that are ignored still meet G's zeros in the product: they must be finite. A target
- * out of range makes its row of dx and all of dW NaN. T == 0 sets dW to zero. */
+ * rows share), sums are 32-bit, in an order that does not change from call to call. Ignored rows of x may hold anything: they
+ * are taken as 0 (the workspace has a copy of x). A target out of range makes its row of dx and all of dW NaN. T == 0 sets dW to zero. */
 size_t symplex_b200_linear_cross_entropy_backward_workspace_bytes(const void* x, const void* W, int64_t T, int64_t H,
                                                                   int64_t V, int64_t ldx, int64_t ldw, int32_t dtype);
 int symplex_b200_linear_cross_entropy_backward(const float* dloss, const void* x, const void* W, const int64_t* targets,

@@ -169,6 +169,30 @@ ce_scale_kernel(const long long* __restrict__ targets, const float* __restrict__
   if (threadIdx.x == 0) *scale = !mean ? *dloss : n > 0 ? (float)((double)*dloss / (double)n) : 0.0f;
 }
 
+// x with the ignored rows 0, for the backward pass: such a row may hold anything (NaN of a padded sequence), and G's zeros do not keep
+// it out of G^T x. One warp a row; bits of 2 or 4 bytes are copied as they are. 1999 x 768 bf16: 3 us of 465.
+template <typename U>
+__global__ void __launch_bounds__(256)
+ce_counted_rows_kernel(const U* __restrict__ x, long long ldx, int vec, const long long* __restrict__ targets, long long ignore, U* __restrict__ to,
+                       long long ld, long long T, int H) {
+  pdl_launch_dependents();
+  pdl_wait_prior_grids();
+  constexpr int N = 16 / sizeof(U);
+  const int lane = threadIdx.x & 31;
+  for (long long t = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); t < T; t += (long long)gridDim.x * 8) {
+    const bool counted = targets[t] != ignore;
+    const U* from = x + t * ldx;
+    U* row = to + t * ld;
+    int c = 0;
+    if (vec) {
+      for (int i = lane; i < H / N; i += 32)
+        reinterpret_cast<uint4*>(row)[i] = counted ? __ldg(reinterpret_cast<const uint4*>(from) + i) : make_uint4(0, 0, 0, 0);
+      c = H / N * N;
+    }
+    for (c += lane; c < H; c += 32) row[c] = counted ? from[c] : U(0);
+  }
+}
+
 __device__ __forceinline__ float tf32_part(float x) {
   uint32_t r;
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
@@ -317,7 +341,7 @@ Layout layout(const Problem& p, bool backward) {
     off = up256(off + bytes);
     return at;
   };
-  if (p.copy_x()) w.xcopy = take((size_t)p.T * w.hp * 2);
+  if (backward || p.copy_x()) w.xcopy = take((size_t)p.T * w.hp * p.eb);
   if (p.copy_w()) w.wcopy = take((size_t)w.piece * w.hp * 2);
   if (!p.bf16) {
     w.xs = take((size_t)2 * p.T * w.hp * 4);
@@ -460,9 +484,12 @@ int backward(const Problem& p, const CeCommon& dev, const float* dloss, const lo
     scale = reinterpret_cast<float*>(ws + w.scale);
     CE_LAUNCH(ce_scale_kernel, 1, 1024, targets, dloss, scale, p.T, p.ignore, p.reduction == SYMPLEX_LOSS_MEAN ? 1 : 0);
   }
+  const int vec = p.ldx * p.eb % 16 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0;
+  const unsigned copy_ctas = (unsigned)std::min<long long>((p.T + 7) / 8, dev.num_sms * 8LL);
   if (p.bf16) {
-    CeMatrix x;
-    CE_TRY(readable(p.copy_x(), p.x, p.T, p.H, p.ldx, ws + w.xcopy, stream, &x));
+    CE_LAUNCH(ce_counted_rows_kernel<uint16_t>, copy_ctas, 256, static_cast<const uint16_t*>(p.x), p.ldx, vec, targets, p.ignore,
+              reinterpret_cast<uint16_t*>(ws + w.xcopy), w.hp, p.T, (int)p.H);
+    const CeMatrix x{ws + w.xcopy, p.T, p.H, w.hp};
     float* acc = reinterpret_cast<float*>(ws + w.acc);
     for (int i = 0; i < w.pieces; ++i) {
       const long long v0 = i * w.piece, n = std::min(w.piece, p.V - v0);
@@ -503,9 +530,11 @@ int backward(const Problem& p, const CeCommon& dev, const float* dloss, const lo
   auto at = [&](size_t off) { return reinterpret_cast<float*>(ws + off); };
   float *xs = at(w.xs), *xts = at(w.xts), *wsp = at(w.ws), *wts = at(w.wts), *logits = at(w.logits), *G = at(w.G), *GT = at(w.GT);
   float* acc[2] = {at(w.acc), at(w.acc) + p.T * p.H};  // one chunk: accumulators of pieces
-  const float* x = static_cast<const float*>(p.x);
-  CE_TRY(prep(launch_split_tf32(x, p.ldx, 0, xs, (int)p.T, (int)p.H, (int)w.hp, 1, stream)));
-  CE_TRY(prep(launch_split_tf32_transpose(x, p.ldx, 0, xts, (int)p.T, (int)p.H, (int)w.tp, 1, stream)));
+  const float* x = at(w.xcopy);
+  CE_LAUNCH(ce_counted_rows_kernel<uint32_t>, copy_ctas, 256, static_cast<const uint32_t*>(p.x), p.ldx, vec, targets, p.ignore,
+            reinterpret_cast<uint32_t*>(ws + w.xcopy), w.hp, p.T, (int)p.H);
+  CE_TRY(prep(launch_split_tf32(x, w.hp, 0, xs, (int)p.T, (int)p.H, (int)w.hp, 1, stream)));
+  CE_TRY(prep(launch_split_tf32_transpose(x, w.hp, 0, xts, (int)p.T, (int)p.H, (int)w.tp, 1, stream)));
   for (int i = 0; i < w.pieces; ++i) {
     const long long v0 = i * w.piece, n = std::min(w.piece, p.V - v0);
     const float* Wp = static_cast<const float*>(p.W) + v0 * p.ldw;

@@ -203,7 +203,7 @@ def linear_cross_entropy_backward(dloss, x, weight, targets, lse, *, ignore_inde
 
     ``dloss``: float32, one value (``"mean"``, ``"sum"``) or ``[T]`` (``"none"``); ``lse`` from the forward pass; the other arguments
     as there. The logits are computed again a piece of the vocabulary at a time. ``dx`` and ``dweight`` have the dtype of ``x``.
-    Ignored rows of ``x`` must be finite (their zero gradient meets them in ``dweight``).
+    Ignored rows of ``x`` may hold anything; they are taken as 0.
     """
     t, h, v = _loss_checks("linear_cross_entropy_backward()", x, weight, targets, ignore_index, reduction)
     if dloss.dtype != torch.float32 or dloss.device != x.device or \

@@ -56,10 +56,12 @@ def test_workspace_bytes(lib):
             assert w(1, 64, 100, dt) > 0
             # the logits of the whole problem never fit in it
             assert w(8192, 4096, 1 << 17, dt) < 8192 * (1 << 17) * 4
-        # operands that are copied first need room for it
+        # operands that are copied first need room for it (the backward pass has a copy of x whatever its alignment)
         aligned = w(100, 64, 1000, BF16)
-        for bad in (dict(x=258), dict(ldx=65), dict(W=520), dict(ldw=68)):
+        for bad in (dict(W=520), dict(ldw=68)):
             assert w(100, 64, 1000, BF16, **bad) > aligned
+        for bad in (dict(x=258), dict(ldx=65)):
+            assert w(100, 64, 1000, BF16, **bad) > aligned if fn is f else w(100, 64, 1000, BF16, **bad) == aligned
         assert w(100, 64, 1000, BF16, ldx=72, ldw=128) == aligned
 
 

@@ -186,6 +186,29 @@ def test_ignored_rows(dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("t,h,pad", [(40, 64, 0), (300, 100, 0), (257, 33, 3), (500, 128, 8)])
+def test_ignored_rows_may_hold_anything(t, h, pad, dtype):
+    """A padded batch whose padding went wrong upstream: the loss and the gradients are those of the rows that count."""
+    x, w, targets = _inputs(t, h, 700, dtype)
+    skip = targets == -100
+    assert bool(skip.any())
+    x[skip] = 0
+    wide = torch.zeros(t, h + pad, dtype=dtype, device=DEV)
+    bad = wide[:, :h]
+    bad.copy_(x)
+    bad[skip] = float("nan")
+    bad[int(skip.nonzero()[0, 0]), ::2] = float("inf")
+    d = torch.ones((), device=DEV)
+    loss, lse = sx.linear_cross_entropy(bad, w, targets)
+    want, lse0 = sx.linear_cross_entropy(x, w, targets)
+    assert torch.equal(loss, want) and torch.equal(lse[~skip], lse0[~skip])
+    got = sx.linear_cross_entropy_backward(d, bad, w, targets, lse)
+    _check_grads(d, x, w, targets, lse0, *got, "mean")
+    assert all(torch.equal(a, b) for a, b in zip(got, sx.linear_cross_entropy_backward(d, x, w, targets, lse0)))
+    assert not got[0][skip].any()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 def test_targets_out_of_range_are_seen(dtype):
     x, w, targets = _inputs(30, 64, 300, dtype, ignored=0.0)
     targets[4], targets[9] = 300, -1
