@@ -123,3 +123,53 @@ def test_tokens_through_a_4_bit_head(tokens, symmetric):
     _, lse = sx.linear_cross_entropy(y, w.to(BF), targets)
     moved = (2.0 ** -8 + (2 * H + 64) * 2.0 ** -24) * (y.double().abs() @ w.abs().t()).max(1).values + 1e-4
     assert bool(((lse.double() - torch.logsumexp(logits.double(), 1)).abs() <= moved).all())
+
+
+def _far(a, step):
+    """``a`` as a view whose rows are ``step`` elements apart."""
+    flat = torch.empty((a.shape[0] - 1) * step + a.shape[1], dtype=a.dtype, device=DEV)
+    view = torch.as_strided(flat, a.shape, (step, 1))
+    view.copy_(a)
+    return view
+
+
+@pytest.mark.parametrize("shift", [0, 3])
+def test_rows_more_than_4_gb_apart(shift):
+    """Offsets past 32 bits, in elements (1.5 * 2^30 apart, the third row beyond 2^31) and in bytes: the bits of rows that are
+    equally aligned and close together."""
+    def near(a):
+        return _far(a, 2 * H + shift)
+
+    def far(a):
+        return _far(a, 3 * 2 ** 29 + shift)
+
+    def same(a, b):
+        a, b = (v if isinstance(v, tuple) else (v,) for v in (a, b))
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+    x, gain, shift_, head, targets = _model(BF, t=3)
+    targets, head = targets % 3, head[:3]
+    xn = near(x)
+    stats = sx.layer_norm(xn, gain, shift_, return_stats=True)
+    y, mean, rstd = stats
+    xf = far(x)
+    same(sx.layer_norm(xf, gain, shift_, return_stats=True), stats)
+    same(sx.layer_norm_backward(y, xf, mean, rstd, gain), sx.layer_norm_backward(y, xn, mean, rstd, gain))
+    del xf
+    one = torch.ones((), device=DEV)
+    for fx, fh in ((far, near), (near, far)):
+        loss = sx.linear_cross_entropy(near(y), near(head), targets)
+        yf, hf = fx(y), fh(head)
+        same(sx.linear_cross_entropy(yf, hf, targets), loss)
+        same(sx.linear_cross_entropy_backward(one, yf, hf, targets, loss[1]),
+             sx.linear_cross_entropy_backward(one, near(y), near(head), targets, loss[1]))
+        del yf, hf
+    codes, scales, _ = sx.int4_quantize(near(head), 64)
+    same(sx.int4_matvec(far(y), far(codes), scales, group_size=64), sx.int4_matvec(near(y), near(codes), scales, group_size=64))
+
+
+def test_the_current_stream_by_its_handle():
+    m = _model(BF)
+    want = _train_step(*m)
+    got = _train_step(*m, stream=torch.cuda.current_stream().cuda_stream)
+    assert all(torch.equal(got[k], want[k]) for k in want)
