@@ -636,16 +636,18 @@ int out_map(CUtensorMap* out, const void* p, long long rows, long long cols, lon
   return encode_tensor_map_3d(out, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p, dims, strides, box);
 }
 
-// 512-row tiles or 256-row ones: fewer waves x area per tile over the tensor-pipe share each shape reaches on large products
-// (0.875 and 0.80, measured for the general pair kernel). The option "pair_mode" decides here as it does there.
-int row_blocks(long long M, long long N, int num_sms) {
+// The logits' product: one CTA up to 128 tokens; 256-row tiles where K is short, because the epilogue of a 512-row tile, whose two
+// accumulators are all of tensor memory, hides only in part behind the next tile's first half (us, 256 / 512 rows, vocabulary 50257:
+// 2000 x 768 132 / 156, 4096 x 1024 314 / 349, 4096 x 1536 458 / 462, 4096 x 2048 602 / 590, 4096 x 4096 1181 / 1109); else fewer waves x
+// area per tile over the tensor-pipe share each shape reaches (0.80 and 0.84). The option "pair_mode" decides here as it does for products.
+int row_blocks(long long M, long long N, long long K, int num_sms) {
   const int64_t mode = options().pair_mode.load(std::memory_order_relaxed);
   if (mode == 1 || mode == 2) return (int)mode;
   if (M <= 128) return 0;
-  if (M <= 256) return 1;
+  if (M <= 256 || K <= 1536) return 1;
   const long long pairs = num_sms / 2, nt = (N + 255) / 256;
   const long long w1 = ((M + 255) / 256 * nt + pairs - 1) / pairs, w2 = ((M + 511) / 512 * nt + pairs - 1) / pairs;
-  return (double)w2 * 2 / 0.875 <= (double)w1 / 0.80 ? 2 : 1;
+  return (double)w2 * 2 / 0.84 <= (double)w1 / 0.80 ? 2 : 1;
 }
 
 // kMB = 0: columns of a tile, a multiple of `step` of at most 256, so that every CTA's tiles together have as few columns as can be.
@@ -714,8 +716,8 @@ long long ce_piece_of_waves(long long T, long long V, long long most) {
   return best * 256;
 }
 
-int ce_forward_parts(long long T, long long V, int num_sms) {
-  const int mb = row_blocks(T, V, num_sms);
+int ce_forward_parts(long long T, long long V, long long H, int num_sms) {
+  const int mb = row_blocks(T, V, H, num_sms);
   if (mb > 0) return (int)((V + 255) / 256) * mb;
   const int bn = columns_alone(V, 16, num_sms);
   return (int)((V + bn - 1) / bn);
@@ -727,7 +729,7 @@ int ce_forward_parts_most(long long T, long long V) {  // whatever the tile shap
 // The logits' product of either pass: operands, tile shape, and the kernel for it.
 template <int kMode>
 static int launch_logits(const CeCommon& c, const CeMatrix& x, const CeMatrix& W, const CUtensorMap& to, CeKernelParams* p, cudaStream_t stream) {
-  const int mb = row_blocks(x.rows, W.rows, c.num_sms);
+  const int mb = row_blocks(x.rows, W.rows, x.cols, c.num_sms);
   uint32_t a_rows = 128 * mb, b_rows = 128;
   p->job[0] = job_of(x.rows, W.rows, x.cols, mb);
   if (mb == 0) {
@@ -776,23 +778,49 @@ int launch_ce_grad(const CeCommon& c, const CeGrad& a, cudaStream_t stream) {
   return launch_logits<CE_GRAD>(c, a.x, a.W, to, &p, stream);
 }
 
+// The tiles of both products in one shape. Returns how long the busiest pair works, in k-blocks of 256 x 256.
+static double products_plan(long long T, long long H, long long n, int mb, int chunks, int num_sms, CeKernelParams* p) {
+  p->job[0] = job_of(T, H, n, mb);
+  p->job[1] = job_of(n, H, T, mb);
+  // The widest piece (the first one) sets how many accumulators there are; a narrower one may fill fewer of them.
+  const long long nkb = (n + 63) / 64, tkb = (T + 63) / 64;
+  p->job[0].chunk_kb = (int)((nkb + chunks - 1) / chunks);
+  p->job[0].chunks = (int)((nkb + p->job[0].chunk_kb - 1) / p->job[0].chunk_kb);
+  const long long t0 = (long long)p->job[0].m_tiles * p->job[0].n_tiles * p->job[0].chunks, t1 = (long long)p->job[1].m_tiles * p->job[1].n_tiles;
+  const long long pairs = std::min<long long>(t0 + t1, num_sms / 2), full = t0 % pairs;
+  p->first_extra = 0;
+  if (full != 0) {
+    const long long each = (p->job[0].chunk_kb + tkb / 2) / tkb;  // dW tiles that take as long as one of dx
+    p->first_extra = (int)std::min<long long>(t1, each * (pairs - full));
+  }
+  const double tile0 = p->job[0].chunk_kb + 4, tile1 = tkb + 4;  // with the start and end of a tile
+  double most = 0;
+  for (long long i = 0; i < pairs; ++i) {
+    const long long n0 = t0 / pairs + (i < full), rest = t1 - p->first_extra;
+    const long long ahead = i >= full && p->first_extra ? (p->first_extra + pairs - 1 - i) / (pairs - full) : 0;
+    most = std::max(most, n0 * tile0 + (ahead + rest / pairs + (i < rest % pairs)) * tile1);
+  }
+  return most * mb / (mb == 1 ? 0.80 : 0.84);
+}
+
 int launch_ce_products(const CeCommon& c, const CeProducts& a, cudaStream_t stream) {
   const long long T = a.x.rows, H = a.x.cols, n = a.W.rows;
+  CeKernelParams p = common(c);
+  // 256-row or 512-row tiles, whichever get done first (us of a whole backward pass, vocabulary 50257: 8192 x 512 1225 / 1574,
+  // 4096 x 1024 1058 / 1124, 4096 x 2048 1909 / 1872, 8192 x 4096 7226 / 6910).
   const int64_t mode = options().pair_mode.load(std::memory_order_relaxed);
-  const int mb = mode == 1 || mode == 2 ? (int)mode : std::min(T, n) <= 256 ? 1 : 2;
+  int mb = mode == 1 || mode == 2 ? (int)mode : 1;
+  const double time = products_plan(T, H, n, mb, a.chunks, c.num_sms, &p);
+  if (mode != 1 && mode != 2 && std::min(T, n) > 256) {
+    CeKernelParams q = p;
+    if (products_plan(T, H, n, 2, a.chunks, c.num_sms, &q) < time) p = q, mb = 2;
+  }
   CUtensorMap in[4], out[2] = {};
   int rc = map_of(&in[0], a.G, 64, 128 * mb);          // dx: A = G, k = vocabulary
   if (rc == SX_OK) rc = map_of(&in[1], a.W, 64, 64);   //     B = W, MN-major
   if (rc == SX_OK) rc = map_of(&in[2], a.G, 64, 64);   // dW: A = G^T, MN-major, k = tokens
   if (rc == SX_OK) rc = map_of(&in[3], a.x, 64, 64);   //     B = x, MN-major
   if (rc != SX_OK) return rc;
-  CeKernelParams p = common(c);
-  p.job[0] = job_of(T, H, n, mb);
-  p.job[1] = job_of(n, H, T, mb);
-  // The widest piece (the first one) sets how many accumulators there are; a narrower one may fill fewer of them.
-  const long long nkb = (n + 63) / 64;
-  p.job[0].chunk_kb = (int)((nkb + a.chunks - 1) / a.chunks);
-  p.job[0].chunks = (int)((nkb + p.job[0].chunk_kb - 1) / p.job[0].chunk_kb);
   p.scale = a.scale;
   p.dx_acc = a.acc;
   p.dx_add = a.first ? 0 : 1;
@@ -806,11 +834,6 @@ int launch_ce_products(const CeCommon& c, const CeProducts& a, cudaStream_t stre
   }
   const long long t0 = (long long)p.job[0].m_tiles * p.job[0].n_tiles * p.job[0].chunks, t1 = (long long)p.job[1].m_tiles * p.job[1].n_tiles;
   if (t0 + t1 > 0x3fffffffLL) return set_last_error(SX_ERR_INVALID, "the problem has more than 2^30-1 tiles");
-  const long long pairs = std::min<long long>(t0 + t1, c.num_sms / 2);
-  if (t0 % pairs != 0) {
-    const long long tkb = (T + 63) / 64, each = (p.job[0].chunk_kb + tkb / 2) / tkb;  // dW tiles that take as long as one of dx
-    p.first_extra = (int)std::min<long long>(t1, each * (pairs - t0 % pairs));
-  }
   return mb == 2 ? launch<CE_PROD, 2>(in, out, p, t0 + t1, c.num_sms, stream) : launch<CE_PROD, 1>(in, out, p, t0 + t1, c.num_sms, stream);
 }
 

@@ -28,7 +28,7 @@ struct CeForward {
   float* target_logit;
   unsigned* done;  // set to 0
 };
-int ce_forward_parts(long long T, long long V, int num_sms);
+int ce_forward_parts(long long T, long long V, long long H, int num_sms);
 int ce_forward_parts_most(long long T, long long V);  // upper bound over SM counts
 int launch_ce_forward(const CeCommon& c, const CeForward& a, cudaStream_t stream);
 
