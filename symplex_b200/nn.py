@@ -8,6 +8,8 @@ call, so calls can be captured into CUDA graphs and run on several streams at on
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _capi
@@ -48,6 +50,12 @@ def _rows(t):
 def _like(t):
     """A contiguous tensor like ``t`` (``empty_like`` takes half the time of ``empty``, but keeps other strides)."""
     return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(query, *args):
+    """A size query of the library, a function of its arguments alone."""
+    return getattr(_capi.load(), query)(*args)
 
 
 def _ptr(t):
@@ -136,7 +144,7 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, *, param_grads=None, str
         if param_grads:
             dw = x.new_empty(cols, dtype=pdt)
             db = torch.empty_like(dw)
-            size = lib.symplex_b200_layer_norm_backward_workspace_bytes(rows, cols)
+            size = _workspace_bytes("symplex_b200_layer_norm_backward_workspace_bytes", rows, cols)
             ws = x.new_empty(size, dtype=torch.uint8)
         w = weight.contiguous() if weight is not None else None
         m, r = mean.contiguous(), rstd.contiguous()
@@ -187,7 +195,8 @@ def linear_cross_entropy(x, weight, targets, *, ignore_index=-100, reduction="me
         (xr, ldx), (w, ldw) = _rows(x), _rows(weight)
         lse = x.new_empty(t, dtype=torch.float32)
         loss = torch.empty_like(lse) if reduction == "none" else lse.new_empty(())
-        size = lib.symplex_b200_linear_cross_entropy_workspace_bytes(xr.data_ptr(), w.data_ptr(), t, h, v, ldx, ldw, _DT[x.dtype])
+        size = _workspace_bytes("symplex_b200_linear_cross_entropy_workspace_bytes", xr.data_ptr() & 255, w.data_ptr() & 255, t, h, v, ldx,
+                                ldw, _DT[x.dtype])  # of the pointers it looks at the alignment
         ws = x.new_empty(size, dtype=torch.uint8)
         tg = targets.contiguous()
         _capi.check(lib.symplex_b200_linear_cross_entropy(
@@ -216,7 +225,8 @@ def linear_cross_entropy_backward(dloss, x, weight, targets, lse, *, ignore_inde
         lib = _capi.load()
         (xr, ldx), (w, ldw) = _rows(x), _rows(weight)
         dx, dw = _like(x), _like(weight)
-        size = lib.symplex_b200_linear_cross_entropy_backward_workspace_bytes(xr.data_ptr(), w.data_ptr(), t, h, v, ldx, ldw, _DT[x.dtype])
+        size = _workspace_bytes("symplex_b200_linear_cross_entropy_backward_workspace_bytes", xr.data_ptr() & 255, w.data_ptr() & 255, t, h, v, ldx,
+                                ldw, _DT[x.dtype])  # of the pointers it looks at the alignment
         ws = x.new_empty(size, dtype=torch.uint8)
         tg, ls, dl = targets.contiguous(), lse.contiguous(), dloss.contiguous()
         _capi.check(lib.symplex_b200_linear_cross_entropy_backward(
