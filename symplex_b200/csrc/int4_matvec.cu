@@ -4,13 +4,12 @@
 //
 // Bound by HBM: N K / 2 bytes of codes, read once for every 16 rows of A.
 //
-// int4_mma_kernel: the rows of W are the M side of mma.sync m16n8k16, the rows of A (up to 8 per fragment) its N side. A code
-// becomes bf16 exactly - four masked bits under the exponent of 128 read 128 + code, minus (128 + zero) - so the products are
-// exact and each group's sum is scaled once, in fp32. Which k a fragment slot stands for is free as long as both operands agree:
-// a lane takes 8 consecutive k of its row (one 32-bit word), whose nibbles j and j + 4 fall into the halves of one register
-// (pairs (k0,k4), (k1,k5), ...), and the same pairs of A are put together with byte permutes. No shuffle, no shared memory on
-// the way in. 4-bit products are far below what even the warp-level tensor path delivers, so the tcgen05 path has nothing to
-// add here: what has to be fast is the dequantisation, 11 instructions for 8 codes.
+// int4_mma_kernel: the rows of W are the M side of mma.sync m16n8k16, the rows of A (up to 8 per fragment) its N side. A code less
+// its zero becomes bf16 exactly (dequant8 below), so the products are exact and each group's sum is scaled once, in fp32. Which k a
+// fragment slot stands for is free as long as both operands agree: a lane takes 8 consecutive k of its row (one 32-bit word), whose
+// nibbles j and j + 4 fall into the halves of one register (pairs (k0,k4), (k1,k5), ...), and A is laid out in the same pairs.
+// 4-bit products are far below what even the warp-level tensor path delivers, so the tcgen05 path has nothing to add here: what has to
+// be fast is the dequantisation, 9 instructions for 8 codes.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -100,14 +99,25 @@ __device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
   const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-// Eight codes -> four registers (k0,k4), (k1,k5), (k2,k6), (k3,k7) of code - zero; zero2 = (128 + zero) twice. The mask and the
-// exponent are registers: one three-input operation each, where two immediates would take two.
-__device__ __forceinline__ void dequant8(uint32_t w, uint32_t zero2, uint32_t mask, uint32_t base, uint32_t (&out)[4]) {
+__device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
+  const __nv_bfloat162 r = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b),
+                                   *reinterpret_cast<const __nv_bfloat162*>(&c));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+// Eight codes -> four registers (k0,k4), (k1,k5), (k2,k6), (k3,k7) of code - zero, the second and fourth a quarter of it.
+//   0x430q is 128 + q; less zero2 = 128 + zero.
+//   0x00q0 is 16 q 2^-133 (subnormal numbers and the first binade are one run of equal steps), times 2^127 a quarter of q; plus
+//   quarter2 = -zero / 4. All exact. One shift for both pairs of a kind, where the first form alone takes three
+// (16 x 28672 x 8192 in groups of 128: 51.7 us, 54.9 with the first form).
+// The mask and the exponent are registers: one three-input operation each, where two immediates would take two.
+__device__ __forceinline__ void dequant8(uint32_t w, uint32_t zero2, uint32_t quarter2, uint32_t mask, uint32_t base, uint32_t (&out)[4]) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < 2; ++j) {
     uint32_t v;
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(v) : "r"(w >> (4 * j)), "r"(mask), "r"(base));  // (w & mask) | base
-    out[j] = sub_bf16x2(v, zero2);
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(v) : "r"(w), "r"(mask), "r"(base));  // (w & mask) | base
+    out[2 * j] = sub_bf16x2(v, zero2);
+    out[2 * j + 1] = fma_bf16x2(w & 0x00f000f0u, 0x7f007f00u, quarter2);
+    w >>= 8;
   }
 }
 
@@ -187,8 +197,11 @@ struct MvPlan {
 // quarter warp (two rows, four shares of a group) then read eight different bank groups.
 template <int kGW> constexpr int MvPad = kGW == 128 ? 2 : kGW == 64 ? 1 : 4;
 
+// Even k at a quarter, as the odd ones' codes are; a sum's factor of 4 is put back at its end. Exact but for magnitudes below 2^-124.
+__device__ __forceinline__ uint32_t quarter(uint32_t pair) { return fma_bf16x2(pair, 0x3e803e80u, 0x80008000u); }
 __device__ __forceinline__ uint4 pairs_of(const uint4& x) {
-  return make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632), __byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632));
+  return make_uint4(quarter(__byte_perm(x.x, x.z, 0x5410)), __byte_perm(x.x, x.z, 0x7632), quarter(__byte_perm(x.y, x.w, 0x5410)),
+                    __byte_perm(x.y, x.w, 0x7632));
 }
 
 __device__ __forceinline__ void stage_a(const Int4Args& p, const MvPlan& plan, uint4* to, int m0, int rows, int k0) {
@@ -216,7 +229,7 @@ __device__ __forceinline__ void stage_a(const Int4Args& p, const MvPlan& plan, u
 // Work of a CTA: its tiles t0 .. t1 in rounds of MV_WARPS / kw tiles; where half of them or fewer are left for the last round, 2 kw
 // or more warps share each. The warps' sums of a tile are joined in shared memory.
 //
-// Measured (16 x 28672 x 8192, groups of 64 with zeros): 64 us, 2.0 TB/s; 1 x 28672 x 8192, groups of 128: 34 us, 3.6 TB/s. HBM would
+// Measured (16 x 28672 x 8192, groups of 64 with zeros): 64 us, 2.0 TB/s; 1 x 28672 x 8192, groups of 128: 31 us, 3.9 TB/s. HBM would
 // take 20 and 18: the ALU, the shared-memory pipe and the issue of instructions are each about half busy, with the four warps a
 // scheduler that 128 registers leave.
 //
@@ -414,9 +427,12 @@ int4_mma_kernel(const Int4Args p, const MvPlan plan) {
 #pragma unroll
         for (int j = 0; j < GROUPS; ++j) {
           float part[kNB][2][4];
-          uint32_t zero2[4];
+          uint32_t zero2[4], quarter2[4];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) zero2[r] = cur.zero2(r, j);
+          for (int r = 0; r < 4; ++r) {
+            zero2[r] = cur.zero2(r, j);
+            quarter2[r] = kZeros ? fma_bf16x2(zero2[r], 0xbe80be80u, 0x42004200u) : 0xc000c000u;  // 32 - (128 + zero) / 4
+          }
 #pragma unroll
           for (int i = 0; i < WPG; ++i) {
             const int w = j * WPG + i;
@@ -430,8 +446,8 @@ int4_mma_kernel(const Int4Args p, const MvPlan plan) {
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt) {
               uint32_t lo[4], hi[4];  // rows g and g + 8 of this m16 tile
-              dequant8(codes[2 * mt][w], zero2[2 * mt], mask, base128, lo);
-              dequant8(codes[2 * mt + 1][w], zero2[2 * mt + 1], mask, base128, hi);
+              dequant8(codes[2 * mt][w], zero2[2 * mt], quarter2[2 * mt], mask, base128, lo);
+              dequant8(codes[2 * mt + 1][w], zero2[2 * mt + 1], quarter2[2 * mt + 1], mask, base128, hi);
 #pragma unroll
               for (int nb = 0; nb < kNB; ++nb) {
                 if (i == 0) mma_bf16_zero(part[nb][mt], lo[0], hi[0], lo[1], hi[1], x[nb].x, x[nb].y);
@@ -485,6 +501,7 @@ int4_mma_kernel(const Int4Args p, const MvPlan plan) {
         } else {
           for (int i = 0; i < kw; ++i) add(v, *reinterpret_cast<const float4*>(at + i * RED_WARP));
         }
+        v.x *= 4.0f; v.y *= 4.0f; v.z *= 4.0f; v.w *= 4.0f;
         if (plan.cluster > 1) *reinterpret_cast<float4*>(sums + (held_buf ^ 1) * ROUND_SUMS + (rg * 8 * kNB + m) * MV_TILE + r) = v;
         else write(tile, m, r, v);
       }

@@ -90,6 +90,18 @@ def test_rows_of_a_that_do_not_fit_into_shared_memory(m, n, k, group, zeros):
     _check(sx.int4_matvec(x, codes, scales, z, group_size=group, bias=b, out_dtype=F32), x, w, b)
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("e", [100, -100])
+def test_powers_of_two_go_through(group, e):
+    """x 2^e with scales 2^-e is the same product, bit by bit; codes equal to their zero give an exact 0."""
+    x, codes, scales, z = _case(5, 100, 1024, group, True, seed=group)
+    want = sx.int4_matvec(x, codes, scales, z, group_size=group, out_dtype=F32)
+    assert torch.equal(sx.int4_matvec(x * 2.0 ** e, codes, scales * 2.0 ** -e, z, group_size=group, out_dtype=F32), want)
+    z[7] = 5
+    codes[7] = 0x55
+    assert not sx.int4_matvec(x, codes, scales, z, group_size=group)[:, 7].any()
+
+
 @pytest.mark.parametrize("sdt", [BF, F32])
 @pytest.mark.parametrize("odt", [BF, F32])
 def test_types(sdt, odt):
