@@ -265,7 +265,7 @@ int4_mma_kernel(const Int4Args p, const MvPlan plan) {
   auto round_kw = [&](int b) {
     const int left = t1 - b, base = plan.kw_log2;
     if (left >= MV_WARPS >> base) return base;
-    return 4 - (32 - __clz(left - 1));
+    return 4 - (32 - __clz(left - 1));  // the most warps that leave one for every tile
   };
 
   // The warp's ring of codes: a step is 32 rows of 64 bytes, 16-byte block q of a row at q ^ f with f = the bits of row / 2 in reverse,
@@ -694,12 +694,23 @@ int matvec_mma(const Int4Args& a, int rows, int cluster, bool out_bf16, int sms,
   }
   crowds = std::min(crowds, plan.tiles);
   cfg.gridDim = dim3((unsigned)(crowds * plan.cluster), (unsigned)mblocks, 1);
-  // Four warps on a tile, more where a CTA has fewer than four tiles (5 x 50257 x 2048: 24.2 us, 31.3 with 16 warps, 26.0 with two;
-  // 1 x 4096 x 4096 with one tile a CTA: 5.5 with 16 or 4 warps, 8.2 with two).
-  const int each = (plan.tiles + crowds - 1) / crowds;  // tiles of a CTA or cluster
-  const int base = cluster > 1 ? MV_CLUSTER_KW : 2;
-  while (plan.kw_log2 < 4 && (2 << plan.kw_log2) <= plan.steps && (plan.kw_log2 < base || each << plan.kw_log2 < MV_WARPS)) ++plan.kw_log2;
-  if (cluster > 1) plan.kw_log2 = std::max(plan.kw_log2, MV_CLUSTER_KW);
+  // Warps on a tile: those with which the rounds of a CTA (or cluster) take the fewest steps, two counted for joining the sums
+  // (5 x 50257 x 2048: 23.0 us with two, 23.2 with four, 30 with 16; 1 x 28672 x 8192: 31 with four, 33 with two).
+  const int each = plan.tiles / crowds;
+  double least = 1e30;
+  for (int kwl = cluster > 1 ? MV_CLUSTER_KW : 0; kwl <= 4; ++kwl) {
+    double cost = 0;
+    for (int n : {each, each + (plan.tiles % crowds ? 1 : 0)}) {
+      const int whole = n / (MV_WARPS >> kwl), left = n % (MV_WARPS >> kwl);
+      cost += whole * (double)((plan.steps + (1 << kwl) - 1) / (1 << kwl) + 2);
+      if (left > 0) {
+        int kw = 1 << kwl;
+        while (MV_WARPS / (2 * kw) >= left) kw *= 2;
+        cost += (plan.steps + kw - 1) / kw + 2;
+      }
+    }
+    if (cost < least) least = cost, plan.kw_log2 = kwl;
+  }
   if (pdl_enabled()) {
     attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
