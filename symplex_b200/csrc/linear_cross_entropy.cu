@@ -170,26 +170,24 @@ ce_scale_kernel(const long long* __restrict__ targets, const float* __restrict__
 }
 
 // x with the ignored rows 0, for the backward pass: such a row may hold anything (NaN of a padded sequence), and G's zeros do not keep
-// it out of G^T x. One warp a row; bits of 2 or 4 bytes are copied as they are. 1999 x 768 bf16: 3 us of 465.
-template <typename U>
+// it out of G^T x. One warp a row, bf16 (fp32 does it where it splits x). 1999 x 768 bf16: 3 us of 460.
 __global__ void __launch_bounds__(256)
-ce_counted_rows_kernel(const U* __restrict__ x, long long ldx, int vec, const long long* __restrict__ targets, long long ignore, U* __restrict__ to,
-                       long long ld, long long T, int H) {
+ce_counted_rows_kernel(const uint16_t* __restrict__ x, long long ldx, int vec, const long long* __restrict__ targets, long long ignore,
+                       uint16_t* __restrict__ to, long long ld, long long T, int H) {
   pdl_launch_dependents();
   pdl_wait_prior_grids();
-  constexpr int N = 16 / sizeof(U);
   const int lane = threadIdx.x & 31;
   for (long long t = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); t < T; t += (long long)gridDim.x * 8) {
     const bool counted = targets[t] != ignore;
-    const U* from = x + t * ldx;
-    U* row = to + t * ld;
+    const uint16_t* from = x + t * ldx;
+    uint16_t* row = to + t * ld;
     int c = 0;
     if (vec) {
-      for (int i = lane; i < H / N; i += 32)
+      for (int i = lane; i < H / 8; i += 32)
         reinterpret_cast<uint4*>(row)[i] = counted ? __ldg(reinterpret_cast<const uint4*>(from) + i) : make_uint4(0, 0, 0, 0);
-      c = H / N * N;
+      c = H / 8 * 8;
     }
-    for (c += lane; c < H; c += 32) row[c] = counted ? from[c] : U(0);
+    for (c += lane; c < H; c += 32) row[c] = counted ? from[c] : 0;
   }
 }
 
@@ -201,49 +199,138 @@ __device__ __forceinline__ float tf32_part(float x) {
 
 // fp32: G and its transpose from a piece of logits, both as the {hi, lo} tf32 planes the products read (hi = tf32(g), lo =
 // tf32(g - hi)): G in parts of `chunk` columns (a multiple of 32), [part][2][rows][chunk], the columns of the last part past the
-// piece 0; G^T [2][cols][ldt], planes plane_t values apart. 32 x 32 tiles, the transpose through shared memory.
+// piece 0; G^T [2][cols][ldt], planes plane_t values apart. Tiles of 32 rows x 128 columns, four values a thread at a time, the transpose
+// through shared memory. 509 x 8192: 16 us (32 x 32 tiles, single values: 25).
+constexpr int GT_PITCH = 33;
 __global__ void __launch_bounds__(256)
 ce_piece_grad_kernel(const float* __restrict__ L, long long ld, int cols, long long v0, const long long* __restrict__ targets,
                      const float* __restrict__ lse, const float* __restrict__ dloss, const float* __restrict__ scale,
-                     float* __restrict__ G, long long chunk, float* __restrict__ GT, long long ldt, long long plane_t,
+                     float* __restrict__ G, int chunk, float* __restrict__ GT, long long ldt, long long plane_t,
                      long long rows, long long V, long long ignore) {
-  __shared__ float tile[32][33];
+  __shared__ float tile[128 * GT_PITCH];
   pdl_launch_dependents();
   pdl_wait_prior_grids();
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
-  const long long padded = (cols + chunk - 1) / chunk * chunk;
-  const long long row_tiles = (rows + 31) / 32, tiles = row_tiles * (padded / 32);
+  const int padded = (cols + chunk - 1) / chunk * chunk;  // columns of all parts
+  const long long row_tiles = (rows + 31) / 32, tiles = row_tiles * ((padded + 127) / 128);
   for (long long i = blockIdx.x; i < tiles; i += gridDim.x) {
     const long long r0 = i % row_tiles * 32;
-    const long long c0 = i / row_tiles * 32, part = c0 / chunk;
-    float* const g_part = G + part * 2 * rows * chunk + (c0 - part * chunk);
+    const int c0 = int(i / row_tiles) * 128, c = c0 + 4 * x;  // this thread's four columns: in one part, chunk is a multiple of 32
+    const int part = c / chunk;
+    float* const g_part = G + (long long)part * 2 * rows * chunk + (c - part * chunk);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const long long r = r0 + y + 8 * j;
-      const long long c = c0 + x;
-      float g = 0.0f;
-      if (r < rows) {
+      float g[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (r < rows && c < padded) {
         const long long at = targets[r];
-        if (c < cols && at != ignore) {
+        if (c < cols && at != ignore) {  // a piece's rows are a multiple of 8 values apart: four of them are there
           const float s = scale != nullptr ? *scale : dloss[r];
-          g = (exp2f((L[r * ld + c] - lse[r]) * LOG2E) - (at == v0 + c ? 1.0f : 0.0f)) * s;
-          if (at < 0 || at >= V) g = __int_as_float(0x7fc00000);
+          const float l = lse[r];
+          const float4 v = *reinterpret_cast<const float4*>(L + r * ld + c);
+          const float w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (c + k >= cols) continue;
+            g[k] = (exp2f((w[k] - l) * LOG2E) - (at == v0 + c + k ? 1.0f : 0.0f)) * s;
+            if (at < 0 || at >= V) g[k] = __int_as_float(0x7fc00000);
+          }
         }
-        const float hi = tf32_part(g);
-        g_part[r * chunk + x] = hi;
-        g_part[(rows + r) * chunk + x] = tf32_part(g - hi);
+        float hi[4], lo[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          hi[k] = tf32_part(g[k]);
+          lo[k] = tf32_part(g[k] - hi[k]);
+        }
+        *reinterpret_cast<float4*>(g_part + r * chunk) = make_float4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<float4*>(g_part + (rows + r) * chunk) = make_float4(lo[0], lo[1], lo[2], lo[3]);
       }
-      tile[y + 8 * j][x] = g;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) tile[(4 * x + k) * GT_PITCH + y + 8 * j] = g[k];
+    }
+    __syncthreads();
+    // four rows of one column: 8 neighbouring threads write its 128 bytes
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int e = threadIdx.x + 256 * j, ct = e >> 3, rt = (e & 7) * 4;
+      const long long r = r0 + rt;
+      if (r < rows && c0 + ct < cols) {  // rows of G^T are padded to a multiple of 8 values, with the zeros of rows past the last
+        float hi[4], lo[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float g = tile[ct * GT_PITCH + rt + k];
+          hi[k] = tf32_part(g);
+          lo[k] = tf32_part(g - hi[k]);
+        }
+        float* const to = GT + (long long)(c0 + ct) * ldt + r;
+        *reinterpret_cast<float4*>(to) = make_float4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<float4*>(to + plane_t) = make_float4(lo[0], lo[1], lo[2], lo[3]);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// An fp32 operand that is read in both orders, as {hi, lo} planes: `to` [2][rows][ld_to] and `trans` in parts of `chunk` rows,
+// [part][2][cols][chunk], 0 past the last row. With targets, rows to be ignored are 0 whatever they hold. Tiles as above. Reading W once
+// instead of once for each order: 14 us against 23 of the 509 x 512 x 8192 backward pass.
+__global__ void __launch_bounds__(256)
+ce_split_both_kernel(const float* __restrict__ in, long long ld, int vec, long long rows, int cols, const long long* __restrict__ targets,
+                     long long ignore, float* __restrict__ to, long long ld_to, float* __restrict__ trans, long long chunk) {
+  __shared__ float tile[128 * GT_PITCH];
+  pdl_launch_dependents();
+  pdl_wait_prior_grids();
+  const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const long long padded = (rows + chunk - 1) / chunk * chunk;
+  const long long row_tiles = (padded + 31) / 32, tiles = row_tiles * ((cols + 127) / 128);
+  for (long long i = blockIdx.x; i < tiles; i += gridDim.x) {
+    const long long r0 = i % row_tiles * 32;
+    const int c0 = int(i / row_tiles) * 128, c = c0 + 4 * x;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const long long r = r0 + y + 8 * j;
+      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (r < rows && c < ld_to) {
+        if (targets == nullptr || targets[r] != ignore) {
+          const float* from = in + r * ld + c;
+          if (vec && c + 4 <= cols) {
+            const float4 w = __ldg(reinterpret_cast<const float4*>(from));
+            v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (c + k < cols) v[k] = __ldg(from + k);
+          }
+        }
+        float hi[4], lo[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          hi[k] = tf32_part(v[k]);
+          lo[k] = tf32_part(v[k] - hi[k]);
+        }
+        *reinterpret_cast<float4*>(to + r * ld_to + c) = make_float4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<float4*>(to + (rows + r) * ld_to + c) = make_float4(lo[0], lo[1], lo[2], lo[3]);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) tile[(4 * x + k) * GT_PITCH + y + 8 * j] = v[k];
     }
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const long long c = c0 + y + 8 * j;
-      const long long r = r0 + x;
-      if (r < rows && c < cols) {
-        const float g = tile[x][y + 8 * j], hi = tf32_part(g);
-        GT[c * ldt + r] = hi;
-        GT[plane_t + c * ldt + r] = tf32_part(g - hi);
+      const int e = threadIdx.x + 256 * j, ct = e >> 3, rt = (e & 7) * 4;
+      const long long r = r0 + rt;
+      if (r < padded && c0 + ct < cols) {  // four rows are in one part: chunk is a multiple of 8
+        const long long part = r / chunk;
+        float hi[4], lo[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float v = tile[ct * GT_PITCH + rt + k];
+          hi[k] = tf32_part(v);
+          lo[k] = tf32_part(v - hi[k]);
+        }
+        float* const at = trans + ((part * 2) * cols + c0 + ct) * chunk + (r - part * chunk);
+        *reinterpret_cast<float4*>(at) = make_float4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<float4*>(at + cols * chunk) = make_float4(lo[0], lo[1], lo[2], lo[3]);
       }
     }
     __syncthreads();
@@ -327,7 +414,7 @@ Layout layout(const Problem& p, bool backward) {
   }
   if (backward && !p.bf16) {
     // dx = G W has T / 128 x H / 128 tiles over the whole piece: cut into parts of 512 columns or more, as many as one wave of tiles
-    // takes (509 x 512 x 8192: 160 tiles of 64 columns, two waves, took 71 us of the pass' 183; 144 of 128 columns, one wave: 141 in all)
+    // takes (509 x 512 x 8192: 160 tiles of 64 columns, two waves, took 71 us of the pass' 183; 144 of 128 columns, one wave: 141 in all; 126 with the passes since)
     const long long tiles = ((p.T + 127) / 128) * ((p.H + dx_tile(p.H) - 1) / dx_tile(p.H));
     const long long want = std::min<long long>(148 / tiles, w.piece / 512);
     if (want > 1) {
@@ -341,7 +428,7 @@ Layout layout(const Problem& p, bool backward) {
     off = up256(off + bytes);
     return at;
   };
-  if (backward || p.copy_x()) w.xcopy = take((size_t)p.T * w.hp * p.eb);
+  if (backward ? p.bf16 : p.copy_x()) w.xcopy = take((size_t)p.T * w.hp * 2);
   if (p.copy_w()) w.wcopy = take((size_t)w.piece * w.hp * 2);
   if (!p.bf16) {
     w.xs = take((size_t)2 * p.T * w.hp * 4);
@@ -484,11 +571,10 @@ int backward(const Problem& p, const CeCommon& dev, const float* dloss, const lo
     scale = reinterpret_cast<float*>(ws + w.scale);
     CE_LAUNCH(ce_scale_kernel, 1, 1024, targets, dloss, scale, p.T, p.ignore, p.reduction == SYMPLEX_LOSS_MEAN ? 1 : 0);
   }
-  const int vec = p.ldx * p.eb % 16 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0;
-  const unsigned copy_ctas = (unsigned)std::min<long long>((p.T + 7) / 8, dev.num_sms * 8LL);
   if (p.bf16) {
-    CE_LAUNCH(ce_counted_rows_kernel<uint16_t>, copy_ctas, 256, static_cast<const uint16_t*>(p.x), p.ldx, vec, targets, p.ignore,
-              reinterpret_cast<uint16_t*>(ws + w.xcopy), w.hp, p.T, (int)p.H);
+    const int vec = p.ldx % 8 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0;
+    CE_LAUNCH(ce_counted_rows_kernel, std::min<long long>((p.T + 7) / 8, dev.num_sms * 8LL), 256, static_cast<const uint16_t*>(p.x), p.ldx, vec, targets,
+              p.ignore, reinterpret_cast<uint16_t*>(ws + w.xcopy), w.hp, p.T, (int)p.H);
     const CeMatrix x{ws + w.xcopy, p.T, p.H, w.hp};
     float* acc = reinterpret_cast<float*>(ws + w.acc);
     for (int i = 0; i < w.pieces; ++i) {
@@ -530,27 +616,23 @@ int backward(const Problem& p, const CeCommon& dev, const float* dloss, const lo
   auto at = [&](size_t off) { return reinterpret_cast<float*>(ws + off); };
   float *xs = at(w.xs), *xts = at(w.xts), *wsp = at(w.ws), *wts = at(w.wts), *logits = at(w.logits), *G = at(w.G), *GT = at(w.GT);
   float* acc[2] = {at(w.acc), at(w.acc) + p.T * p.H};  // one chunk: accumulators of pieces
-  const float* x = at(w.xcopy);
-  CE_LAUNCH(ce_counted_rows_kernel<uint32_t>, copy_ctas, 256, static_cast<const uint32_t*>(p.x), p.ldx, vec, targets, p.ignore,
-            reinterpret_cast<uint32_t*>(ws + w.xcopy), w.hp, p.T, (int)p.H);
-  CE_TRY(prep(launch_split_tf32(x, w.hp, 0, xs, (int)p.T, (int)p.H, (int)w.hp, 1, stream)));
-  CE_TRY(prep(launch_split_tf32_transpose(x, w.hp, 0, xts, (int)p.T, (int)p.H, (int)w.tp, 1, stream)));
+  auto split_both = [&](const float* in, long long ld, long long rows, const long long* tg, float* to, float* trans, long long chunk) -> int {
+    const int v = ld % 4 == 0 && reinterpret_cast<uintptr_t>(in) % 16 == 0;
+    const long long tiles = ((rows + chunk - 1) / chunk * chunk + 31) / 32 * ((p.H + 127) / 128);
+    CE_LAUNCH(ce_split_both_kernel, std::min<long long>(tiles, dev.num_sms * 8LL), 256, in, ld, v, rows, (int)p.H, tg, p.ignore, to, w.hp, trans, chunk);
+    return SX_OK;
+  };
+  CE_TRY(split_both(static_cast<const float*>(p.x), p.ldx, p.T, targets, xs, xts, w.tp));
   for (int i = 0; i < w.pieces; ++i) {
     const long long v0 = i * w.piece, n = std::min(w.piece, p.V - v0);
     const float* Wp = static_cast<const float*>(p.W) + v0 * p.ldw;
-    CE_TRY(prep(launch_split_tf32(Wp, p.ldw, 0, wsp, (int)n, (int)p.H, (int)w.hp, 1, stream)));
+    // W in both orders; W^T, for dx, in parts of the vocabulary
+    const int chunks = (int)((n + w.chunk - 1) / w.chunk);
+    CE_TRY(split_both(Wp, p.ldw, n, nullptr, wsp, wts, w.chunk));
     CE_TRY(split_product(dev, xs, w.hp, p.T * w.hp, wsp, w.hp, n * w.hp, logits, w.piece, nullptr, p.T, n, p.H, stream));
-    // dx: the piece in parts of the vocabulary, their planes one after the other (rows of W past the piece are 0)
-    const int chunks = (int)((n + w.chunk - 1) / w.chunk), whole = (int)(n / w.chunk);
-    const long long part_w = 2 * p.H * w.chunk;
-    if (whole > 0)
-      CE_TRY(prep(launch_split_tf32_transpose(Wp, p.ldw, w.chunk * p.ldw, wts, (int)w.chunk, (int)p.H, (int)w.chunk, whole, stream)));
-    if (whole < chunks)
-      CE_TRY(prep(launch_split_tf32_transpose(Wp + whole * w.chunk * p.ldw, p.ldw, 0, wts + whole * part_w, (int)(n - whole * w.chunk), (int)p.H,
-                                              (int)w.chunk, 1, stream)));
-    const long long tiles = (p.T + 31) / 32 * (chunks * w.chunk / 32 + 1);
+    const long long tiles = (p.T + 31) / 32 * ((chunks * w.chunk + 127) / 128);
     CE_LAUNCH(ce_piece_grad_kernel, std::min<long long>(tiles, dev.num_sms * 8LL), 256, (const float*)logits, w.piece, (int)n, v0, targets, lse,
-              dloss, (const float*)scale, G, w.chunk, GT, w.tp, n * w.tp, p.T, p.V, p.ignore);
+              dloss, (const float*)scale, G, (int)w.chunk, GT, w.tp, n * w.tp, p.T, p.V, p.ignore);
     if (w.chunks > 1) {
       CE_TRY(split_product(dev, G, w.chunk, p.T * w.chunk, wts, w.chunk, p.H * w.chunk, acc[0], p.H, nullptr, p.T, p.H, w.chunk, stream, chunks, dx_tile(p.H)));
       CE_LAUNCH(ce_join_kernel<float>, std::min<long long>((p.T * p.H + 255) / 256, dev.num_sms * 8LL), 256, (const float*)acc[0], chunks, p.T * p.H,
