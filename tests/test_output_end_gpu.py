@@ -173,3 +173,28 @@ def test_the_current_stream_by_its_handle():
     want = _train_step(*m)
     got = _train_step(*m, stream=torch.cuda.current_stream().cuda_stream)
     assert all(torch.equal(got[k], want[k]) for k in want)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_two_graphs_at_once(dtype):
+    """Two captured steps, replayed side by side again and again: neither has the other's scratch."""
+    models = [_model(dtype, seed=k) for k in (3, 4)]
+    want = [_train_step(*m) for m in models]
+    codes = [sx.int4_quantize(m[3], 64)[:2] for m in models]
+    logits = [sx.int4_matvec(w["y"][:9].to(BF), *c, group_size=64) for w, c in zip(want, codes)]
+    torch.cuda.synchronize()
+    graphs, got = [], []
+    for m, w, c in zip(models, want, codes):
+        graph = torch.cuda.CUDAGraph()
+        few = w["y"][:9].to(BF)
+        with torch.cuda.graph(graph):
+            got.append((_train_step(*m), sx.int4_matvec(few, *c, group_size=64), few))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(20):
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    for w, l, (g, l2, _) in zip(want, logits, got):
+        assert all(torch.equal(g[k], w[k]) for k in w) and torch.equal(l, l2)
