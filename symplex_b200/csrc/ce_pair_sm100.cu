@@ -161,6 +161,16 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// 16 columns of this warp's 32 rows, a row a lane; waits for them.
+__device__ __forceinline__ void tmem_get_32x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+               "tcgen05.wait::ld.sync.aligned;"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                 "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(taddr)
+               : "memory");
+}
+
 // 32 values of one row into a 128-byte-swizzled staging tile of 32 rows x 128 bytes, one row per lane (the layout of a
 // SWIZZLE_128B tensor map): bf16 fills four of the eight 16-byte chunks from `chunk` on, fp32 all eight.
 __device__ __forceinline__ void stage_bf16(const float (&v)[32], uint8_t* tile, int lane, int chunk) {
@@ -174,8 +184,16 @@ __device__ __forceinline__ void stage_f32(const float (&v)[32], uint8_t* tile, i
     *reinterpret_cast<float4*>(tile + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
 }
 
-template <int kMode, int kMB>
-__global__ void __launch_bounds__(CeCfg<kMB>::THREADS, 1)
+// The accumulators round every sum towards 0: a logit loses about 2^-26 of itself for each 16 k, and the loss, which all logits move the
+// same way, 2e-10 H of itself (measured: 8e-7 at H = 4096, 1.6e-6 at 8192; with 3000 words, whose loss is smaller, 1.1e-6 and 2.6e-6).
+// kSegments (CE_LSE, kMB 0 and 1): k in segments of 512, each from zero into the next accumulator; twice the epilogue warps, half of a
+// tile's columns each, add them up in registers with rounded sums. 1e-7 at any H.
+constexpr int CE_SEGMENT = 8;  // k-blocks
+template <int kMB, bool kSegments>
+constexpr int CE_EPI_WARPS = kSegments ? 8 : CeCfg<kMB>::EPI_WARPS;
+
+template <int kMode, int kMB, bool kSegments>
+__global__ void __launch_bounds__(64 + 32 * CE_EPI_WARPS<kMB, kSegments>, 1)
 ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmB0,
                const __grid_constant__ CUtensorMap tmA1, const __grid_constant__ CUtensorMap tmB1,
                const __grid_constant__ CUtensorMap out0, const __grid_constant__ CUtensorMap out1,
@@ -212,7 +230,7 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&acc_full[a], 1);
-      mbar_init(&acc_empty[a], kGroup * Cfg::EPI_WARPS);  // every epilogue warp of both CTAs
+      mbar_init(&acc_empty[a], kGroup * CE_EPI_WARPS<kMB, kSegments>);  // every epilogue warp of both CTAs
     }
     abort_flag = 0;
     fence_mbar_init();
@@ -333,18 +351,22 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
           else umma_commit(bar);
         };
         if constexpr (kMB <= 1) {
-          if (!mbar_wait<true>(&acc_empty[slot], acc_phase ^ 1, &abort_flag, wait_ns)) break;
-          tc_fence_after_sync();
-          for (int kb = 0; kb < nk; ++kb) {
-            if (!mbar_wait(&full_bar[stage], phase, &abort_flag, wait_ns)) { ok = false; break; }
+          const int length = kSegments ? CE_SEGMENT : nk;
+          for (int k0 = 0; ok && k0 < nk; k0 += length) {
+            if (!mbar_wait<true>(&acc_empty[slot], acc_phase ^ 1, &abort_flag, wait_ns)) { ok = false; break; }
             tc_fence_after_sync();
-            issue(slot, 0, stage, kb != 0 ? 1u : 0u);
-            commit(&empty_bar[stage]);
-            advance(stage, phase);
+            for (int kb = k0; kb < min(k0 + length, nk); ++kb) {
+              if (!mbar_wait(&full_bar[stage], phase, &abort_flag, wait_ns)) { ok = false; break; }
+              tc_fence_after_sync();
+              issue(slot, 0, stage, kb != k0 ? 1u : 0u);
+              commit(&empty_bar[stage]);
+              advance(stage, phase);
+            }
+            if (!ok) break;
+            commit(&acc_full[slot]);
+            if (++slot == 2) { slot = 0; acc_phase ^= 1; }
           }
           if (!ok) break;
-          commit(&acc_full[slot]);
-          if (++slot == 2) { slot = 0; acc_phase ^= 1; }
         } else {
           // The tile's two row blocks share every B stage; the first and last SKEW k-blocks are issued block-major, so block 0
           // is done 4 SKEW MMAs early and the next tile starts on it while block 1 is still being drained.
@@ -397,9 +419,10 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
   } else {
     // ------------------------------------------------------------ epilogue (both CTAs)
     const int q = warp & 3;  // TMEM lane quarter this warp may read
-    const int half = kMB <= 1 ? 0 : (warp - 2) >> 2;
+    const int half = kMB <= 1 && !kSegments ? 0 : (warp - 2) >> 2;
     constexpr int kBlocks = kMB == 2 ? 2 : 1;
-    constexpr int STRIPS = (BN / 32) / kBlocks;  // 32-column strips per warp and accumulator
+    constexpr int kHalves = kMB == 2 || kSegments ? 2 : 1;
+    constexpr int STRIPS = (BN / 32) / kHalves;  // 32-column strips per warp and accumulator
     uint8_t* staging = tiles + (kPair ? STAGES * STAGE_BYTES : Cfg::DYN_SMEM - 1024 - Cfg::EPI_WARPS * Cfg::STAGING_BYTES) + (warp - 2) * Cfg::STAGING_BYTES;
     int slot = 0;
     uint32_t acc_phase = 0;
@@ -432,9 +455,72 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
             }
           }
         }
+        float m = -INFINITY, s = 0.0f;
+        // One strip of logits into the row's part.
+        auto lse_strip = [&](float (&v)[32], int cb) {
+          if (cb + 32 > n_end) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (cb + j >= n_end) v[j] = -INFINITY;
+          }
+          const int a = at - cb;
+          if (a >= 0 && a < 32) {
+            float l = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) l = a == j ? v[j] : l;
+            p.target_logit[row] = l;
+          }
+          float top = v[0];
+#pragma unroll
+          for (int j = 1; j < 32; ++j) top = fmaxf(top, v[j]);  // a NaN is passed over here and meets the sum below
+          const float nm = fmaxf(m, top);
+          if (nm == -INFINITY) {  // no mass so far: -inf - -inf must not become NaN, a NaN must stay one
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (v[j] != v[j]) s = v[j];
+          } else {
+            float add = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) add += ex2((v[j] - nm) * CE_LOG2E);
+            s = fmaf(s, ex2((m - nm) * CE_LOG2E), add);
+            m = nm;
+          }
+        };
+        if constexpr (kSegments) {
+          float l[STRIPS][32];
+#pragma unroll
+          for (int c = 0; c < STRIPS; ++c)
+#pragma unroll
+            for (int j = 0; j < 32; ++j) l[c][j] = 0.0f;
+          for (int k0 = 0; ok && k0 < t.kb; k0 += CE_SEGMENT) {
+            if (!mbar_wait(&acc_full[slot], acc_phase, &abort_flag, wait_ns)) { ok = false; break; }
+            tc_fence_after_sync();
+#pragma unroll
+            for (int c = 0; c < 2 * STRIPS; ++c) {
+              uint32_t r[16];
+              tmem_get_32x16(tmem_base + (uint32_t(q * 32) << 16) + slot * BN + half * STRIPS * 32 + c * 16, r);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) l[c / 2][c % 2 * 16 + j] += __uint_as_float(r[j]);
+            }
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) {
+              if constexpr (kPair) mbar_arrive_cluster(mapa_u32(smem_u32(&acc_empty[slot]), 0));
+              else mbar_arrive(&acc_empty[slot]);
+            }
+            if (++slot == 2) { slot = 0; acc_phase ^= 1; }
+          }
+          if (!ok) break;
+#pragma unroll
+          for (int c = 0; c < STRIPS; ++c) {
+            const int cb = t.n0 + (half * STRIPS + c) * 32;
+            if (cb < n_end) lse_strip(l[c], cb);
+          }
+          if (row_ok) p.part[((long long)(kPair ? t.n0 / BN : t.n0 / p.bn) * 2 + half) * job.M + row] = make_float2(m, s);
+          continue;
+        }
         if (!mbar_wait(&acc_full[slot], acc_phase, &abort_flag, wait_ns)) { ok = false; break; }
         tc_fence_after_sync();
-        float m = -INFINITY, s = 0.0f;
 #pragma unroll 1
         for (int c = half * STRIPS; c < (half + 1) * STRIPS; c += 2) {
           uint32_t r0[32], r1[32];
@@ -451,33 +537,7 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
             auto strip = [&](const uint32_t (&r)[32], int cb) {
 #pragma unroll
               for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-              if (cb + 32 > n_end) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                  if (cb + j >= n_end) v[j] = -INFINITY;
-              }
-              const int a = at - cb;
-              if (a >= 0 && a < 32) {
-                float l = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 32; ++j) l = a == j ? v[j] : l;
-                p.target_logit[row] = l;
-              }
-              float top = v[0];
-#pragma unroll
-              for (int j = 1; j < 32; ++j) top = fmaxf(top, v[j]);  // a NaN is passed over here and meets the sum below
-              const float nm = fmaxf(m, top);
-              if (nm == -INFINITY) {  // no mass so far: -inf - -inf must not become NaN, a NaN must stay one
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                  if (v[j] != v[j]) s = v[j];
-              } else {
-                float add = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 32; ++j) add += ex2((v[j] - nm) * CE_LOG2E);
-                s = fmaf(s, ex2((m - nm) * CE_LOG2E), add);
-                m = nm;
-              }
+              lse_strip(v, cb);
             };
             strip(r0, col0);
             if (second) strip(r1, col0 + 32);
@@ -598,7 +658,8 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
           if (row_ok) p.part[(long long)(kPair ? t.n0 / BN * kMB + half : t.n0 / p.bn) * job.M + row] = make_float2(m, s);
         }
       }
-      if constexpr (kMB <= 1) {
+      if constexpr (kSegments) {
+      } else if constexpr (kMB <= 1) {
         if (++slot == 2) { slot = 0; acc_phase ^= 1; }
       } else {
         acc_phase ^= 1;
@@ -651,10 +712,10 @@ int row_blocks(long long M, long long N, long long K, int num_sms) {
 }
 
 // kMB = 0: columns of a tile, a multiple of `step` of at most 256, so that every CTA's tiles together have as few columns as can be.
-int columns_alone(long long N, int step, int num_sms) {
+int columns_alone(long long N, int step, int least_bn, int num_sms) {
   int best = 256;
   long long least = 1LL << 62;
-  for (int bn = 256; bn >= 32; bn -= step) {
+  for (int bn = 256; bn >= least_bn; bn -= step) {
     const long long tiles = (N + bn - 1) / bn, each = (tiles + num_sms - 1) / num_sms * bn;
     if (each < least) least = each, best = bn;
   }
@@ -673,14 +734,15 @@ CeJob job_of(long long M, long long N, long long K, int mb) {
   return j;
 }
 
-template <int kMode, int kMB>
+template <int kMode, int kMB, bool kSegments = false>
 int launch(const CUtensorMap (&in)[4], const CUtensorMap (&out)[2], const CeKernelParams& p, long long tiles, int num_sms, cudaStream_t stream) {
   using Cfg = CeCfg<kMB>;
-  auto kern = ce_pair_kernel<kMode, kMB>;
+  auto kern = ce_pair_kernel<kMode, kMB, kSegments>;
+  constexpr int THREADS = 64 + 32 * CE_EPI_WARPS<kMB, kSegments>;
   SX_ENSURE_DYN_SMEM(kern, Cfg::DYN_SMEM);
   constexpr int kGroup = kMB > 0 ? 2 : 1;
   const unsigned groups = (unsigned)std::min<long long>(tiles, num_sms / kGroup);
-  const cudaError_t e = launch_kernel_ex(kern, kGroup * groups, Cfg::THREADS, Cfg::DYN_SMEM, stream, kGroup, pdl_enabled(), in[0], in[1], in[2], in[3],
+  const cudaError_t e = launch_kernel_ex(kern, kGroup * groups, THREADS, Cfg::DYN_SMEM, stream, kGroup, pdl_enabled(), in[0], in[1], in[2], in[3],
                                          out[0], out[1], p);
   if (e != cudaSuccess) return launch_failed(e, "loss kernel launch failed");
   count_launches(1);
@@ -716,25 +778,36 @@ long long ce_piece_of_waves(long long T, long long V, long long most) {
   return best * 256;
 }
 
-int ce_forward_parts(long long T, long long V, long long H, int num_sms) {
+// The forward pass in segments where its error would be near 1e-6: up to 128 tokens from 2048 values on (1 x 4096 x 65536 101 us, 95
+// without), pairs where the sum is longer than 4096 or the vocabulary is small (8192 x 4096 x 50257 would take 2305 us instead of 2164).
+static bool in_segments(long long T, long long V, long long H) { return H > 4096 || (H > 2048 && (T <= 128 || V < 16384)); }
+static int forward_row_blocks(long long T, long long V, long long H, int num_sms) {
   const int mb = row_blocks(T, V, H, num_sms);
-  if (mb > 0) return (int)((V + 255) / 256) * mb;
-  const int bn = columns_alone(V, 16, num_sms);
-  return (int)((V + bn - 1) / bn);
+  return in_segments(T, V, H) ? std::min(mb, 1) : mb;
+}
+static int forward_columns_alone(long long V, long long T, long long H, int num_sms) { return columns_alone(V, 16, in_segments(T, V, H) ? 64 : 32, num_sms); }
+
+int ce_forward_parts(long long T, long long V, long long H, int num_sms) {
+  const int mb = forward_row_blocks(T, V, H, num_sms), halves = in_segments(T, V, H) ? 2 : 1;
+  if (mb > 0) return (int)((V + 255) / 256) * (halves == 2 ? 2 : mb);
+  const int bn = forward_columns_alone(V, T, H, num_sms);
+  return (int)((V + bn - 1) / bn) * halves;
 }
 int ce_forward_parts_most(long long T, long long V) {  // whatever the tile shape
-  return (int)std::max((V + 255) / 256 * 2, T <= 128 ? (V + 31) / 32 : 0);
+  return (int)std::max((V + 255) / 256 * 2, T <= 128 ? (V + 63) / 64 * 2 : 0);
 }
 
 // The logits' product of either pass: operands, tile shape, and the kernel for it.
 template <int kMode>
 static int launch_logits(const CeCommon& c, const CeMatrix& x, const CeMatrix& W, const CUtensorMap& to, CeKernelParams* p, cudaStream_t stream) {
-  const int mb = row_blocks(x.rows, W.rows, x.cols, c.num_sms);
+  const bool segments = kMode == CE_LSE && in_segments(x.rows, W.rows, x.cols);
+  const int mb = kMode == CE_LSE ? forward_row_blocks(x.rows, W.rows, x.cols, c.num_sms) : row_blocks(x.rows, W.rows, x.cols, c.num_sms);
   uint32_t a_rows = 128 * mb, b_rows = 128;
   p->job[0] = job_of(x.rows, W.rows, x.cols, mb);
   if (mb == 0) {
     a_rows = (uint32_t)(x.rows + 15) / 16 * 16;
-    b_rows = (uint32_t)columns_alone(W.rows, kMode == CE_GRAD ? 64 : 16, c.num_sms);  // G leaves in blocks of 64 columns
+    // G leaves in blocks of 64 columns
+    b_rows = (uint32_t)(kMode == CE_GRAD ? columns_alone(W.rows, 64, 64, c.num_sms) : forward_columns_alone(W.rows, x.rows, x.cols, c.num_sms));
     p->bn = (int)b_rows;
     p->a_bytes = (int)a_rows * 128;
     p->stages = std::min(CeCfg<0>::STAGES, CeCfg<0>::STAGE_ROOM / (p->a_bytes + p->bn * 128));
@@ -747,6 +820,10 @@ static int launch_logits(const CeCommon& c, const CeMatrix& x, const CeMatrix& W
   if (rc != SX_OK) return rc;
   const long long tiles = (long long)p->job[0].m_tiles * p->job[0].n_tiles;
   if (tiles > 0x7fffffffLL) return set_last_error(SX_ERR_INVALID, "the problem has more than 2^31-1 tiles");
+  if constexpr (kMode == CE_LSE) {
+    if (segments)
+      return mb == 0 ? launch<CE_LSE, 0, true>(in, out, *p, tiles, c.num_sms, stream) : launch<CE_LSE, 1, true>(in, out, *p, tiles, c.num_sms, stream);
+  }
   switch (mb) {
     case 0: return launch<kMode, 0>(in, out, *p, tiles, c.num_sms, stream);
     case 1: return launch<kMode, 1>(in, out, *p, tiles, c.num_sms, stream);

@@ -132,6 +132,24 @@ def test_few_tokens(t, h, v):
     _both(t, h, v, BF, "none" if t % 2 else "mean", seed=t)
 
 
+@pytest.mark.parametrize("t,h,v", [(5, 1032, 300), (128, 2048, 5000), (1, 4096, 9001), (37, 8192, 3000), (130, 4104, 700), (300, 6144, 5001), (600, 8192, 3000)])
+def test_long_products_round_in_segments(t, h, v):
+    """An accumulator that rounds towards 0 loses half a unit in the last place of its running sum per instruction (16 k) on
+    average, always the same way. A segment of 512 is 32 instructions; while its sum runs from 0 to s, that is at most
+    1/2 2^-23 s (1 + ... + 32) / 32 = 9.8e-7 s, and all segments together 9.8e-7 of a logit; lse moves by the mean of that over
+    its logits, which are no larger than it is (here: most of the mass is on the target's). One sum over 8192 loses 16 times as much.
+    (Up to H = 2048 it is one sum, 3.9e-6 by this estimate, which takes every unit at its largest; it is held to 1e-6 too.)
+    """
+    x, w, targets = _inputs(t, h, v, BF, seed=h, sharp=3.0)
+    loss, lse = sx.linear_cross_entropy(x, w, targets, reduction="none")
+    sx.sync_status()
+    _check_loss(x, w, targets, loss, lse, "none")
+    ref = torch.logsumexp(x.double() @ w.double().t(), 1)
+    assert float((lse.double() - ref).norm() / ref.norm()) < 1e-6
+    d = torch.ones(t, device=DEV)
+    _check_grads(d, x, w, targets, lse, *sx.linear_cross_entropy_backward(d, x, w, targets, lse, reduction="none"), "none")
+
+
 @pytest.mark.parametrize("shape", [1, 2])
 @pytest.mark.parametrize("t,h,v", [(40, 64, 700), (600, 200, 3001), (1100, 512, 9000)])
 def test_both_tile_shapes(t, h, v, shape):
