@@ -86,6 +86,7 @@ struct CeKernelParams {
   const float* lse;
   const float* dloss;
   const float* scale;
+  int lo;           // CE_GRAD: G's rounding errors are written too, through out1
   int dx_add;       // CE_PROD: job 0 adds to what the accumulators hold
   const float* dx_acc;
   int dx_bf16;      // CE_PROD: job 0 writes bf16 dx (last piece, one chunk), else the fp32 accumulators
@@ -556,21 +557,31 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
                 for (int j = 0; j < 32; ++j) v[j] = 0.0f;
               }
             };
-            strip(r0, col0);
-            if (stored && lane == 0) bulk_wait_group_read<0>();  // the previous block has left the staging tile
-            __syncwarp();
-            stage_bf16(v, staging, lane, 0);
-            if (second) {
-              strip(r1, col0 + 32);
-              stage_bf16(v, staging, lane, 4);
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              tma_store_3d(&out0, staging, col0, row0, 0);
-              bulk_commit_group();
-            }
-            stored = true;
+            auto put = [&](const CUtensorMap* to, bool lo) {
+              auto rest = [&]() {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] -= float(__nv_bfloat16(v[j]));
+              };
+              strip(r0, col0);
+              if (lo) rest();
+              if (stored && lane == 0) bulk_wait_group_read<0>();  // the previous block has left the staging tile
+              __syncwarp();
+              stage_bf16(v, staging, lane, 0);
+              if (second) {
+                strip(r1, col0 + 32);
+                if (lo) rest();
+                stage_bf16(v, staging, lane, 4);
+              }
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                tma_store_3d(to, staging, col0, row0, 0);
+                bulk_commit_group();
+              }
+              stored = true;
+            };
+            put(&out0, false);
+            if (kMB == 0 && p.lo) put(&out1, true);
           } else {
             const bool f32 = t.job == 0 && !p.dx_bf16;
             const CUtensorMap* om = t.job == 0 ? &out0 : &out1;
@@ -799,9 +810,9 @@ int ce_forward_parts_most(long long T, long long V) {  // whatever the tile shap
 
 // The logits' product of either pass: operands, tile shape, and the kernel for it.
 template <int kMode>
-static int launch_logits(const CeCommon& c, const CeMatrix& x, const CeMatrix& W, const CUtensorMap& to, CeKernelParams* p, cudaStream_t stream) {
+static int launch_logits(const CeCommon& c, const CeMatrix& x, const CeMatrix& W, const CUtensorMap (&out)[2], CeKernelParams* p, cudaStream_t stream) {
   const bool segments = kMode == CE_LSE && in_segments(x.rows, W.rows, x.cols);
-  const int mb = kMode == CE_LSE ? forward_row_blocks(x.rows, W.rows, x.cols, c.num_sms) : row_blocks(x.rows, W.rows, x.cols, c.num_sms);
+  const int mb = kMode == CE_LSE ? forward_row_blocks(x.rows, W.rows, x.cols, c.num_sms) : p->lo ? 0 : row_blocks(x.rows, W.rows, x.cols, c.num_sms);
   uint32_t a_rows = 128 * mb, b_rows = 128;
   p->job[0] = job_of(x.rows, W.rows, x.cols, mb);
   if (mb == 0) {
@@ -814,7 +825,6 @@ static int launch_logits(const CeCommon& c, const CeMatrix& x, const CeMatrix& W
     p->job[0].n_tiles = (int)((W.rows + p->bn - 1) / p->bn);
   }
   CUtensorMap in[4] = {};
-  const CUtensorMap out[2] = {to, CUtensorMap{}};
   int rc = map_of(&in[0], x, 64, a_rows);
   if (rc == SX_OK) rc = map_of(&in[1], W, 64, b_rows);
   if (rc != SX_OK) return rc;
@@ -838,14 +848,16 @@ int launch_ce_forward(const CeCommon& c, const CeForward& a, cudaStream_t stream
   p.part = a.part;
   p.target_logit = a.target_logit;
   p.done = a.done;
-  return launch_logits<CE_LSE>(c, a.x, a.W, CUtensorMap{}, &p, stream);
+  return launch_logits<CE_LSE>(c, a.x, a.W, {CUtensorMap{}, CUtensorMap{}}, &p, stream);
 }
 
 int launch_ce_grad(const CeCommon& c, const CeGrad& a, cudaStream_t stream) {
-  CUtensorMap to{};
-  const int rc = out_map(&to, a.G, a.x.rows, a.W.rows, a.ldg, false);
+  CUtensorMap to[2] = {};
+  int rc = out_map(&to[0], a.G, a.x.rows, a.W.rows, a.ldg, false);
+  if (rc == SX_OK && a.lo) rc = out_map(&to[1], static_cast<const uint16_t*>(a.G) + a.x.rows * a.ldg, a.x.rows, a.W.rows, a.ldg, false);
   if (rc != SX_OK) return rc;
   CeKernelParams p = common(c);
+  p.lo = a.lo ? 1 : 0;
   p.targets = a.targets;
   p.lse = a.lse;
   p.dloss = a.dloss;
@@ -901,7 +913,7 @@ int launch_ce_products(const CeCommon& c, const CeProducts& a, cudaStream_t stre
   p.scale = a.scale;
   p.dx_acc = a.acc;
   p.dx_add = a.first ? 0 : 1;
-  p.dx_bf16 = a.chunks == 1 && a.last;
+  p.dx_bf16 = a.chunks == 1 && a.last && a.dx != nullptr;
   p.out[0] = p.dx_bf16 ? a.dx : a.acc;
   p.out[1] = a.dW;
   for (int j = 0; j < 2; ++j) {

@@ -37,6 +37,7 @@ struct CeGrad {
   CeMatrix x, W;  // [T, H], the piece of W: [n, H]
   void* G;        // bf16 [T, ldg], ldg a multiple of 8, 16-byte aligned
   long long ldg;
+  bool lo;  // T <= 128 only: G's rounding errors follow in another T rows, bf16 as well
   const long long* targets;
   const float* lse;
   const float* dloss;  // per row, or null
@@ -46,7 +47,7 @@ int launch_ce_grad(const CeCommon& c, const CeGrad& a, cudaStream_t stream);
 
 // dx (+)= G W and dW = G^T x of one piece, times *scale where scale is not null. dx goes to `chunks` fp32 accumulators [T, H] in a row
 // (its k, the vocabulary, cut into as many parts), to which pieces after the first one add. With one chunk the last piece writes
-// bf16 dx = (acc + G W) * scale instead; with several, launch_ce_join does it in the end.
+// bf16 dx = (acc + G W) * scale instead where dx is given; else the accumulators are joined afterwards.
 struct CeProducts {
   CeMatrix G, x, W;  // [T, n], [T, H], [n, H]
   float* acc;

@@ -173,21 +173,23 @@ ce_scale_kernel(const long long* __restrict__ targets, const float* __restrict__
 // it out of G^T x. One warp a row, bf16 (fp32 does it where it splits x). 1999 x 768 bf16: 3 us of 460.
 __global__ void __launch_bounds__(256)
 ce_counted_rows_kernel(const uint16_t* __restrict__ x, long long ldx, int vec, const long long* __restrict__ targets, long long ignore,
-                       uint16_t* __restrict__ to, long long ld, long long T, int H) {
+                       uint16_t* __restrict__ to, long long ld, long long T, int H, int copies) {
   pdl_launch_dependents();
   pdl_wait_prior_grids();
   const int lane = threadIdx.x & 31;
   for (long long t = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); t < T; t += (long long)gridDim.x * 8) {
     const bool counted = targets[t] != ignore;
     const uint16_t* from = x + t * ldx;
-    uint16_t* row = to + t * ld;
-    int c = 0;
-    if (vec) {
-      for (int i = lane; i < H / 8; i += 32)
-        reinterpret_cast<uint4*>(row)[i] = counted ? __ldg(reinterpret_cast<const uint4*>(from) + i) : make_uint4(0, 0, 0, 0);
-      c = H / 8 * 8;
+    for (int k = 0; k < copies; ++k) {
+      uint16_t* row = to + (k * T + t) * ld;
+      int c = 0;
+      if (vec) {
+        for (int i = lane; i < H / 8; i += 32)
+          reinterpret_cast<uint4*>(row)[i] = counted ? __ldg(reinterpret_cast<const uint4*>(from) + i) : make_uint4(0, 0, 0, 0);
+        c = H / 8 * 8;
+      }
+      for (c += lane; c < H; c += 32) row[c] = counted ? from[c] : 0;
     }
-    for (c += lane; c < H; c += 32) row[c] = counted ? from[c] : 0;
   }
 }
 
@@ -364,6 +366,13 @@ struct Problem {
   long long ignore;
   int reduction;
 
+  // bf16 backward, few tokens: G in two bf16 parts. A row of G holds one large entry, the target's, whose rounding moves the whole row
+  // of dx and the target's row of dW; over many tokens that adds a fifth to the results' own rounding, over one it may be as large as
+  // that (error of the gradients of one token 2.6e-3, 1.6e-3 in two parts). The second part is T more rows of G (and of x), for which a
+  // tile has room: 1 x 2048 x 32768 120 us either way; 100 x 1024 x 32768 would take 85 us instead of 73.
+  bool two_parts() const { return bf16 && T <= 64; }
+  long long g_rows() const { return two_parts() ? 2 * T : T; }
+
   // bf16 operands that TMA cannot read in place go through a padded copy.
   bool copy(const void* p, long long ld) const { return bf16 && (ld % 8 != 0 || reinterpret_cast<uintptr_t>(p) % 16 != 0); }
   bool copy_x() const { return copy(x, ldx); }
@@ -409,7 +418,7 @@ Layout layout(const Problem& p, bool backward) {
   w.chunk = up(w.piece, 32);
   if (backward && p.bf16) {
     // counted as the kernel cuts them: parts of as many k-blocks each, the last one shorter
-    const long long nkb = (std::min(w.piece, p.V) + 63) / 64, c = ce_dx_chunks(p.T, p.H, std::min(w.piece, p.V)), kb = (nkb + c - 1) / c;
+    const long long nkb = (std::min(w.piece, p.V) + 63) / 64, c = ce_dx_chunks(p.g_rows(), p.H, std::min(w.piece, p.V)), kb = (nkb + c - 1) / c;
     w.chunks = (int)((nkb + kb - 1) / kb);
   }
   if (backward && !p.bf16) {
@@ -428,7 +437,7 @@ Layout layout(const Problem& p, bool backward) {
     off = up256(off + bytes);
     return at;
   };
-  if (backward ? p.bf16 : p.copy_x()) w.xcopy = take((size_t)p.T * w.hp * 2);
+  if (backward ? p.bf16 : p.copy_x()) w.xcopy = take((size_t)(backward ? p.g_rows() : p.T) * w.hp * 2);
   if (p.copy_w()) w.wcopy = take((size_t)w.piece * w.hp * 2);
   if (!p.bf16) {
     w.xs = take((size_t)2 * p.T * w.hp * 4);
@@ -443,8 +452,8 @@ Layout layout(const Problem& p, bool backward) {
   } else {
     w.scale = take(4);
     const long long cols = p.bf16 ? w.piece : w.chunks * w.chunk;
-    w.G = take((size_t)p.T * cols * (p.bf16 ? 2 : 8));
-    if (w.chunks > 1) w.acc = take((size_t)w.chunks * p.T * p.H * 4);
+    w.G = take((size_t)p.g_rows() * cols * (p.bf16 ? 2 : 8));
+    if (w.chunks > 1 || p.two_parts()) w.acc = take((size_t)w.chunks * p.g_rows() * p.H * 4);
     else if (w.pieces > 1) w.acc = take((size_t)p.T * p.H * 4 * (p.bf16 ? 1 : 2));  // fp32: from one accumulator into the other
     if (!p.bf16) {
       w.xts = take((size_t)2 * p.H * w.tp * 4);
@@ -574,8 +583,8 @@ int backward(const Problem& p, const CeCommon& dev, const float* dloss, const lo
   if (p.bf16) {
     const int vec = p.ldx % 8 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0;
     CE_LAUNCH(ce_counted_rows_kernel, std::min<long long>((p.T + 7) / 8, dev.num_sms * 8LL), 256, static_cast<const uint16_t*>(p.x), p.ldx, vec, targets,
-              p.ignore, reinterpret_cast<uint16_t*>(ws + w.xcopy), w.hp, p.T, (int)p.H);
-    const CeMatrix x{ws + w.xcopy, p.T, p.H, w.hp};
+              p.ignore, reinterpret_cast<uint16_t*>(ws + w.xcopy), w.hp, p.T, (int)p.H, p.two_parts() ? 2 : 1);
+    const CeMatrix x{ws + w.xcopy, p.T, p.H, w.hp}, xs{ws + w.xcopy, p.g_rows(), p.H, w.hp};
     float* acc = reinterpret_cast<float*>(ws + w.acc);
     for (int i = 0; i < w.pieces; ++i) {
       const long long v0 = i * w.piece, n = std::min(w.piece, p.V - v0);
@@ -586,6 +595,7 @@ int backward(const Problem& p, const CeCommon& dev, const float* dloss, const lo
       g.W = Wp;
       g.G = ws + w.G;
       g.ldg = w.piece;
+      g.lo = p.two_parts();
       g.targets = targets;
       g.lse = lse;
       g.dloss = per_row ? dloss : nullptr;
@@ -596,20 +606,20 @@ int backward(const Problem& p, const CeCommon& dev, const float* dloss, const lo
       // One factor for all rows is left out of G, where rounding it would move every large entry (the targets', close to
       // -factor) the same way, and multiplied into the results' fp32 sums instead.
       CeProducts d{};
-      d.G = CeMatrix{ws + w.G, p.T, n, w.piece};
-      d.x = x;
+      d.G = CeMatrix{ws + w.G, p.g_rows(), n, w.piece};
+      d.x = xs;
       d.W = Wp;
       d.acc = acc;
       d.chunks = w.chunks;
       d.first = i == 0;
       d.last = i == w.pieces - 1;
-      d.dx = dx;
+      d.dx = p.two_parts() ? nullptr : dx;
       d.dW = static_cast<uint8_t*>(dW) + (size_t)v0 * p.H * 2;
       d.scale = scale;
       CE_TRY(launch_ce_products(dev, d, stream));
     }
-    if (w.chunks > 1)
-      CE_LAUNCH(ce_join_kernel<__nv_bfloat16>, std::min<long long>((p.T * p.H + 255) / 256, dev.num_sms * 8LL), 256, (const float*)acc, w.chunks,
+    if (w.chunks > 1 || p.two_parts())  // [chunk][part of G][T][H]
+      CE_LAUNCH(ce_join_kernel<__nv_bfloat16>, std::min<long long>((p.T * p.H + 255) / 256, dev.num_sms * 8LL), 256, (const float*)acc, w.chunks * (p.two_parts() ? 2 : 1),
                 p.T * p.H, (const float*)scale, static_cast<__nv_bfloat16*>(dx), 0);
     return SX_OK;
   }

@@ -150,6 +150,25 @@ def test_long_products_round_in_segments(t, h, v):
     _check_grads(d, x, w, targets, lse, *sx.linear_cross_entropy_backward(d, x, w, targets, lse, reduction="none"), "none")
 
 
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("t,h,v", [(1, 64, 33), (1, 512, 3000), (2, 256, 1000), (5, 1000, 5001), (33, 136, 700), (64, 512, 9000)])
+def test_few_tokens_gradients_are_rounded_once(t, h, v, reduction):
+    """G in two bf16 parts is off by 2^-17: beside it the results' own rounding is all there is. A value whose rounding G's error turns
+    over (it lies within 2^-17 of a tie: one in 2^8) is off by a whole step instead of half, 3.7 times the mean square: under 1 %
+    of the norm; the chains' bound of _check_grads is 2^-13 at these sizes at the most."""
+    x, w, targets = _inputs(t, h, v, BF, seed=7 * t + v, ignored=0.0)
+    _, lse = sx.linear_cross_entropy(x, w, targets)
+    d = torch.full((t,) if reduction == "none" else (), 0.7, device=DEV)
+    got = sx.linear_cross_entropy_backward(d, x, w, targets, lse, reduction=reduction)
+    sx.sync_status()
+    p = torch.exp(x.double() @ w.double().t() - lse.double()[:, None])
+    p[torch.arange(t, device=DEV), targets] -= 1
+    g = p * (d.double() if reduction == "none" else d.double() / t).reshape(-1, 1)
+    for a, ref in zip(got, (g @ w.double(), g.t() @ x.double())):
+        rounding = (ref.to(BF).double() - ref).norm()
+        assert float((a.double() - ref).norm()) <= 1.02 * float(rounding) + 2.0 ** -13 * float(ref.norm())
+
+
 @pytest.mark.parametrize("shape", [1, 2])
 @pytest.mark.parametrize("t,h,v", [(40, 64, 700), (600, 200, 3001), (1100, 512, 9000)])
 def test_both_tile_shapes(t, h, v, shape):
