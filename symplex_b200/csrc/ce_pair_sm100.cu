@@ -246,7 +246,6 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
   else __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = tmem_base_slot;
-  pdl_launch_dependents();
   pdl_wait_prior_grids();
   if (kMode == CE_LSE && blockIdx.x == 0 && threadIdx.x == 0) *p.done = 0;
 
@@ -430,6 +429,11 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
     bool ok = true;
     const float scale = kMode == CE_PROD && p.scale != nullptr ? *p.scale : 1.0f;
     bool stored = false;  // this warp has TMA stores that may be reading its staging tile
+    // The lanes wait one by one, and may leave the wait at different times; what follows is the whole warp's.
+    auto warp_wait = [&](uint64_t* bar, uint32_t parity) {
+      const bool got = mbar_wait(bar, parity, &abort_flag, wait_ns);
+      return __all_sync(0xffffffffu, got) != 0;
+    };
     CeTile t;
     for (Work w(p, pair_id, num_pairs); ok && w.get(&t);) {
       const CeJob& job = p.job[t.job];
@@ -494,7 +498,7 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
 #pragma unroll
             for (int j = 0; j < 32; ++j) l[c][j] = 0.0f;
           for (int k0 = 0; ok && k0 < t.kb; k0 += CE_SEGMENT) {
-            if (!mbar_wait(&acc_full[slot], acc_phase, &abort_flag, wait_ns)) { ok = false; break; }
+            if (!warp_wait(&acc_full[slot], acc_phase)) { ok = false; break; }
             tc_fence_after_sync();
 #pragma unroll
             for (int c = 0; c < 2 * STRIPS; ++c) {
@@ -520,11 +524,12 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
           if (row_ok) p.part[((long long)(kPair ? t.n0 / BN : t.n0 / p.bn) * 2 + half) * job.M + row] = make_float2(m, s);
           continue;
         }
-        if (!mbar_wait(&acc_full[slot], acc_phase, &abort_flag, wait_ns)) { ok = false; break; }
+        if (!warp_wait(&acc_full[slot], acc_phase)) { ok = false; break; }
         tc_fence_after_sync();
 #pragma unroll 1
         for (int c = half * STRIPS; c < (half + 1) * STRIPS; c += 2) {
           uint32_t r0[32], r1[32];
+          __syncwarp();  // the lanes part in every strip (targets), the loads are the whole warp's
           const uint32_t taddr = tmem_base + (uint32_t(q * 32) << 16) + slot * BN + c * 32;
           tmem_ld_32x32(taddr, r0);
           tmem_ld_32x32(taddr + 32, r1);
@@ -708,18 +713,17 @@ int out_map(CUtensorMap* out, const void* p, long long rows, long long cols, lon
   return encode_tensor_map_3d(out, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p, dims, strides, box);
 }
 
-// The logits' product: one CTA up to 128 tokens; 256-row tiles where K is short, because the epilogue of a 512-row tile, whose two
-// accumulators are all of tensor memory, hides only in part behind the next tile's first half (us, 256 / 512 rows, vocabulary 50257:
-// 2000 x 768 132 / 156, 4096 x 1024 314 / 349, 4096 x 1536 458 / 462, 4096 x 2048 602 / 590, 4096 x 4096 1181 / 1109); else fewer waves x
-// area per tile over the tensor-pipe share each shape reaches (0.80 and 0.84). The option "pair_mode" decides here as it does for products.
-int row_blocks(long long M, long long N, long long K, int num_sms) {
+// The logits' product: one CTA up to 128 tokens, else 512-row tiles or 256-row ones: fewer waves x area per tile over the tensor-pipe share
+// each shape reaches on large products (0.875 and 0.80, measured for the general pair kernel). The option "pair_mode" decides here as it
+// does there.
+int row_blocks(long long M, long long N, int num_sms) {
   const int64_t mode = options().pair_mode.load(std::memory_order_relaxed);
   if (mode == 1 || mode == 2) return (int)mode;
   if (M <= 128) return 0;
-  if (M <= 256 || K <= 1536) return 1;
+  if (M <= 256) return 1;
   const long long pairs = num_sms / 2, nt = (N + 255) / 256;
   const long long w1 = ((M + 255) / 256 * nt + pairs - 1) / pairs, w2 = ((M + 511) / 512 * nt + pairs - 1) / pairs;
-  return (double)w2 * 2 / 0.84 <= (double)w1 / 0.80 ? 2 : 1;
+  return (double)w2 * 2 / 0.875 <= (double)w1 / 0.80 ? 2 : 1;
 }
 
 // kMB = 0: columns of a tile, a multiple of `step` of at most 256, so that every CTA's tiles together have as few columns as can be.
@@ -752,8 +756,10 @@ int launch(const CUtensorMap (&in)[4], const CUtensorMap (&out)[2], const CeKern
   constexpr int THREADS = 64 + 32 * CE_EPI_WARPS<kMB, kSegments>;
   SX_ENSURE_DYN_SMEM(kern, Cfg::DYN_SMEM);
   constexpr int kGroup = kMB > 0 ? 2 : 1;
+  // In plain stream order: launched early behind the kernel that joins a few thousand rows, a long queue of forward passes (3815 x 1104 x
+  // 26330, 256-row tiles) stopped making progress.
   const unsigned groups = (unsigned)std::min<long long>(tiles, num_sms / kGroup);
-  const cudaError_t e = launch_kernel_ex(kern, kGroup * groups, THREADS, Cfg::DYN_SMEM, stream, kGroup, pdl_enabled(), in[0], in[1], in[2], in[3],
+  const cudaError_t e = launch_kernel_ex(kern, kGroup * groups, THREADS, Cfg::DYN_SMEM, stream, kGroup, false, in[0], in[1], in[2], in[3],
                                          out[0], out[1], p);
   if (e != cudaSuccess) return launch_failed(e, "loss kernel launch failed");
   count_launches(1);
@@ -793,7 +799,7 @@ long long ce_piece_of_waves(long long T, long long V, long long most) {
 // without), pairs where the sum is longer than 4096 or the vocabulary is small (8192 x 4096 x 50257 would take 2305 us instead of 2164).
 static bool in_segments(long long T, long long V, long long H) { return H > 4096 || (H > 2048 && (T <= 128 || V < 16384)); }
 static int forward_row_blocks(long long T, long long V, long long H, int num_sms) {
-  const int mb = row_blocks(T, V, H, num_sms);
+  const int mb = row_blocks(T, V, num_sms);
   return in_segments(T, V, H) ? std::min(mb, 1) : mb;
 }
 static int forward_columns_alone(long long V, long long T, long long H, int num_sms) { return columns_alone(V, 16, in_segments(T, V, H) ? 64 : 32, num_sms); }
@@ -812,7 +818,7 @@ int ce_forward_parts_most(long long T, long long V) {  // whatever the tile shap
 template <int kMode>
 static int launch_logits(const CeCommon& c, const CeMatrix& x, const CeMatrix& W, const CUtensorMap (&out)[2], CeKernelParams* p, cudaStream_t stream) {
   const bool segments = kMode == CE_LSE && in_segments(x.rows, W.rows, x.cols);
-  const int mb = kMode == CE_LSE ? forward_row_blocks(x.rows, W.rows, x.cols, c.num_sms) : p->lo ? 0 : row_blocks(x.rows, W.rows, x.cols, c.num_sms);
+  const int mb = kMode == CE_LSE ? forward_row_blocks(x.rows, W.rows, x.cols, c.num_sms) : p->lo ? 0 : row_blocks(x.rows, W.rows, c.num_sms);
   uint32_t a_rows = 128 * mb, b_rows = 128;
   p->job[0] = job_of(x.rows, W.rows, x.cols, mb);
   if (mb == 0) {

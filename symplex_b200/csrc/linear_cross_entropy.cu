@@ -43,7 +43,6 @@ __global__ void __launch_bounds__(256)
 ce_piece_rows_kernel(const float* __restrict__ L, long long ld, int cols, long long v0, const long long* __restrict__ targets,
                      float2* __restrict__ part, float* __restrict__ target_logit, unsigned* __restrict__ done) {
   __shared__ float2 red[8];
-  pdl_launch_dependents();
   pdl_wait_prior_grids();
   const long long t = blockIdx.x;
   if (t == 0 && threadIdx.x == 0) *done = 0;
@@ -99,7 +98,6 @@ ce_finish_kernel(const float2* __restrict__ part, int parts, const float* __rest
   __shared__ int last;
   __shared__ double sred[32];
   __shared__ long long cred[32];
-  pdl_launch_dependents();
   pdl_wait_prior_grids();
   const int mine = threadIdx.x & 3;
   const long long t = (long long)blockIdx.x * 4 + mine;
@@ -148,7 +146,6 @@ ce_finish_kernel(const float2* __restrict__ part, int parts, const float* __rest
 
 // The sum over no rows, or their mean.
 __global__ void ce_nothing_kernel(float* loss, int mean) {
-  pdl_launch_dependents();
   pdl_wait_prior_grids();
   *loss = mean ? __int_as_float(0x7fc00000) : 0.0f;
 }
@@ -159,7 +156,6 @@ __global__ void __launch_bounds__(1024)
 ce_scale_kernel(const long long* __restrict__ targets, const float* __restrict__ dloss, float* __restrict__ scale, long long T,
                 long long ignore, int mean) {
   __shared__ long long cred[32];
-  pdl_launch_dependents();
   pdl_wait_prior_grids();
   long long n = 0;
   if (mean) {
@@ -174,7 +170,6 @@ ce_scale_kernel(const long long* __restrict__ targets, const float* __restrict__
 __global__ void __launch_bounds__(256)
 ce_counted_rows_kernel(const uint16_t* __restrict__ x, long long ldx, int vec, const long long* __restrict__ targets, long long ignore,
                        uint16_t* __restrict__ to, long long ld, long long T, int H, int copies) {
-  pdl_launch_dependents();
   pdl_wait_prior_grids();
   const int lane = threadIdx.x & 31;
   for (long long t = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); t < T; t += (long long)gridDim.x * 8) {
@@ -210,7 +205,6 @@ ce_piece_grad_kernel(const float* __restrict__ L, long long ld, int cols, long l
                      float* __restrict__ G, int chunk, float* __restrict__ GT, long long ldt, long long plane_t,
                      long long rows, long long V, long long ignore) {
   __shared__ float tile[128 * GT_PITCH];
-  pdl_launch_dependents();
   pdl_wait_prior_grids();
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
   const int padded = (cols + chunk - 1) / chunk * chunk;  // columns of all parts
@@ -280,7 +274,6 @@ __global__ void __launch_bounds__(256)
 ce_split_both_kernel(const float* __restrict__ in, long long ld, int vec, long long rows, int cols, const long long* __restrict__ targets,
                      long long ignore, float* __restrict__ to, long long ld_to, float* __restrict__ trans, long long chunk) {
   __shared__ float tile[128 * GT_PITCH];
-  pdl_launch_dependents();
   pdl_wait_prior_grids();
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
   const long long padded = (rows + chunk - 1) / chunk * chunk;
@@ -343,7 +336,6 @@ ce_split_both_kernel(const float* __restrict__ in, long long ld, int vec, long l
 template <typename T>
 __global__ void __launch_bounds__(256)
 ce_join_kernel(const float* __restrict__ acc, int chunks, long long n, const float* __restrict__ scale, T* out, int add) {
-  pdl_launch_dependents();
   pdl_wait_prior_grids();
   const float f = scale != nullptr ? *scale : 1.0f;
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
@@ -487,7 +479,7 @@ bool aligned_to(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p
 
 #define CE_LAUNCH(kern, grid, block, ...)                                                                             \
   do {                                                                                                                \
-    const cudaError_t e__ = launch_kernel_ex(kern, (unsigned)(grid), block, 0, stream, 1, pdl_enabled(), __VA_ARGS__); \
+    const cudaError_t e__ = launch_kernel_ex(kern, (unsigned)(grid), block, 0, stream, 1, false, __VA_ARGS__);         \
     if (e__ != cudaSuccess) return launch_failed(e__, "loss kernel launch failed");                                   \
     count_launches(1);                                                                                                \
   } while (0)
