@@ -387,6 +387,15 @@ def test_two_streams_at_once():
         assert all(torch.equal(a, b) for one in got[k] for a, b in zip(want[k], one))
 
 
+def test_a_long_queue_of_passes():
+    x, w, targets = _inputs(3815, 1104, 26330, BF)
+    want, lse = sx.linear_cross_entropy(x, w, targets, reduction="sum")
+    torch.cuda.synchronize()
+    got = [sx.linear_cross_entropy(x, w, targets, reduction="sum")[0] for _ in range(400)]
+    sx.sync_status()
+    assert all(torch.equal(v, want) for v in got)
+
+
 def test_refusals():
     x, w, targets = _inputs(8, 64, 100, BF)
     loss, lse = sx.linear_cross_entropy(x, w, targets)
