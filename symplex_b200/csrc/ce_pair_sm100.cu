@@ -49,7 +49,7 @@ struct CeCfg {
 
 // At most 128 tokens. A pair's tile would be filled up to 256 rows with nothing, and its MMAs then take as long as W's rows take to
 // arrive (512 cycles for 16 KB per SM, 9 TB/s with no pause): one CTA has half the rows to multiply (1 x 4096 x 65536: 150 us on
-// pairs, 94 us alone, 5.7 TB/s; 61 x 1024 x 50257: 32 and 25 us). Columns of a tile, rows of A that
+// pairs, 94 us alone, 5.7 TB/s; 37 x 1024 x 50257: 32 and 25 us, each launched behind the call before). Columns of a tile, rows of A that
 // are copied and stages are set at launch: the tiles share the vocabulary out evenly, and the stages fill shared memory. The MMA
 // reads 128 rows of A from a stage whatever was copied; the rows behind the copied ones are other data, and nobody reads their sums.
 template <>

@@ -711,7 +711,7 @@ int matvec_mma(const Int4Args& a, int rows, int cluster, bool out_bf16, int sms,
     }
     if (cost < least) least = cost, plan.kw_log2 = kwl;
   }
-  if (pdl_enabled()) {
+  if (pdl_enabled() && cluster == 1) {  // clusters start in plain stream order (a microsecond of 40 or more)
     attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
     ++cfg.numAttrs;
