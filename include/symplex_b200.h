@@ -581,8 +581,9 @@ int symplex_b200_linear_cross_entropy(const void* x, const void* W, const int64_
 
 /* Its gradients: with p = exp(l - lse) and G[t][v] = (p[t][v] - [v == targets[t]]) * s[t],
  *   dx[T, H] = G . W,  dW[V, H] = G^T . x     (packed, of type dtype)
- * where s[t] is dloss[t] (NONE), dloss[0] (SUM) or dloss[0] / number of counted rows (MEAN), and 0 for ignored rows. The
- * logits are computed again, a piece of the vocabulary at a time; G is held in dtype (BF16: rounded, without the factor all
+ * where s[t] is dloss[t] (NONE), dloss[0] (SUM) or dloss[0] / number of counted rows (MEAN), and 0 for ignored rows. lse is the
+ * forward pass' for the same T, H, V and dtype: both passes then sum (and round) a logit alike, which p - 1 of a row that is sure
+ * of its target depends on. The logits are computed again, a piece of the vocabulary at a time; G is held in dtype (BF16: rounded, without the factor all
  * rows share; in two parts up to 64 tokens), sums are 32-bit, in an order that does not change from call to call. Ignored rows of x may hold anything: they
  * are taken as 0 (the workspace has a copy of x). A target out of range makes its row of dx and all of dW NaN. T == 0 sets dW to zero. */
 size_t symplex_b200_linear_cross_entropy_backward_workspace_bytes(const void* x, const void* W, int64_t T, int64_t H,

@@ -41,10 +41,7 @@ struct CeCfg {
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int STAGES = kMB == 1 ? 6 : 4;
   static constexpr int EPI_WARPS = 4 * kMB;
-  static constexpr int THREADS = 64 + 32 * EPI_WARPS;
   static constexpr int TMEM_COLS = 512;
-  static constexpr int STAGING_BYTES = 32 * 128;
-  static constexpr int DYN_SMEM = STAGES * STAGE_BYTES + EPI_WARPS * STAGING_BYTES + 1024;
 };
 
 // At most 128 tokens. A pair's tile would be filled up to 256 rows with nothing, and its MMAs then take as long as W's rows take to
@@ -60,11 +57,7 @@ struct CeCfg<0> {
   static constexpr int BK = 64;
   static constexpr int STAGES = 12;  // at most
   static constexpr int EPI_WARPS = 4;
-  static constexpr int THREADS = 64 + 32 * EPI_WARPS;
   static constexpr int TMEM_COLS = 512;
-  static constexpr int STAGING_BYTES = 32 * 128;
-  static constexpr int STAGE_ROOM = 200 * 1024;
-  static constexpr int DYN_SMEM = STAGE_ROOM + EPI_WARPS * STAGING_BYTES + 1024;
 };
 
 // One product: tiles of [M, N] over K.
@@ -172,26 +165,39 @@ __device__ __forceinline__ void tmem_get_32x16(uint32_t taddr, uint32_t (&r)[16]
                : "memory");
 }
 
-// 32 values of one row into a 128-byte-swizzled staging tile of 32 rows x 128 bytes, one row per lane (the layout of a
-// SWIZZLE_128B tensor map): bf16 fills four of the eight 16-byte chunks from `chunk` on, fp32 all eight.
+// 16-byte chunk `chunk` (of 8) of a lane's row of a 128-byte-swizzled staging tile of 32 rows x 128 bytes, one row per lane (the layout
+// of a SWIZZLE_128B tensor map).
+__device__ __forceinline__ uint8_t* staged_at(uint8_t* tile, int lane, int chunk) { return tile + lane * 128 + ((chunk ^ (lane & 7)) << 4); }
+// 32 values of one row: bf16 fills four chunks from `chunk` on, fp32 all eight.
 __device__ __forceinline__ void stage_bf16(const float (&v)[32], uint8_t* tile, int lane, int chunk) {
 #pragma unroll
-  for (int c = 0; c < 4; ++c)
-    *reinterpret_cast<uint4*>(tile + lane * 128 + (((chunk + c) ^ (lane & 7)) << 4)) = EpilogueCtx<__nv_bfloat16>::pack8_bf16(v + 8 * c);
+  for (int c = 0; c < 4; ++c) *reinterpret_cast<uint4*>(staged_at(tile, lane, chunk + c)) = EpilogueCtx<__nv_bfloat16>::pack8_bf16(v + 8 * c);
 }
 __device__ __forceinline__ void stage_f32(const float (&v)[32], uint8_t* tile, int lane) {
 #pragma unroll
   for (int c = 0; c < 8; ++c)
-    *reinterpret_cast<float4*>(tile + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+    *reinterpret_cast<float4*>(staged_at(tile, lane, c)) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
 }
 
 // The accumulators round every sum towards 0: a logit loses about 2^-26 of itself for each 16 k, and the loss, which all logits move the
 // same way, 2e-10 H of itself (measured: 8e-7 at H = 4096, 1.6e-6 at 8192; with 3000 words, whose loss is smaller, 1.1e-6 and 2.6e-6).
-// kSegments (CE_LSE, kMB 0 and 1): k in segments of 512, each from zero into the next accumulator; twice the epilogue warps, half of a
-// tile's columns each, add them up in registers with rounded sums. 1e-7 at any H.
+// Where all products of a logit have one sign (a row that is sure of its target) it is ten times as much.
+// kSegments (CE_LSE and CE_GRAD, kMB 0 and 1): k in segments of 512, each from zero into the next accumulator; twice the epilogue warps,
+// half of a tile's columns each, add them up in registers with rounded sums. 1e-7 at any H. Both passes of a problem take the same form:
+// the target's entry of G is exp(l - lse) - 1, of which an l with the bias beside an lse without it leaves nothing right where 1 - p is
+// small (T = 2100, H = 4104, rows of 1 - p = 1e-5 to 1e-3: G off by 3e-4, by 1e-6 in the same form).
 constexpr int CE_SEGMENT = 8;  // k-blocks
 template <int kMB, bool kSegments>
 constexpr int CE_EPI_WARPS = kSegments ? 8 : CeCfg<kMB>::EPI_WARPS;
+// Shared memory: operand stages, then a staging tile of 32 x 128 bytes for each epilogue warp that writes through one.
+constexpr int CE_STAGING_BYTES = 32 * 128;
+template <int kMode, int kMB, bool kSegments>
+__host__ __device__ constexpr int ce_stage_room() {
+  if constexpr (kMB > 0) return CeCfg<kMB>::STAGES * CeCfg<kMB>::STAGE_BYTES;
+  else return (kMode == CE_GRAD && kSegments ? 192 : 200) * 1024;
+}
+template <int kMode, int kMB, bool kSegments>
+constexpr int CE_DYN_SMEM = ce_stage_room<kMode, kMB, kSegments>() + (kMode == CE_LSE ? 0 : CE_EPI_WARPS<kMB, kSegments> * CE_STAGING_BYTES) + 1024;
 
 template <int kMode, int kMB, bool kSegments>
 __global__ void __launch_bounds__(64 + 32 * CE_EPI_WARPS<kMB, kSegments>, 1)
@@ -423,7 +429,7 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
     constexpr int kBlocks = kMB == 2 ? 2 : 1;
     constexpr int kHalves = kMB == 2 || kSegments ? 2 : 1;
     constexpr int STRIPS = (BN / 32) / kHalves;  // 32-column strips per warp and accumulator
-    uint8_t* staging = tiles + (kPair ? STAGES * STAGE_BYTES : Cfg::DYN_SMEM - 1024 - Cfg::EPI_WARPS * Cfg::STAGING_BYTES) + (warp - 2) * Cfg::STAGING_BYTES;
+    uint8_t* staging = tiles + ce_stage_room<kMode, kMB, kSegments>() + (warp - 2) * CE_STAGING_BYTES;
     int slot = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
@@ -491,6 +497,46 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
             m = nm;
           }
         };
+        // CE_GRAD: two strips of logits (bits of floats) -> a block of 64 columns of G.
+        auto grad_block = [&](const uint32_t (&a0)[32], const uint32_t (&a1)[32], int col0) {
+          const bool second = col0 + 32 < n_end;
+          auto put = [&](const CUtensorMap* to, bool lo) {
+            auto entry = [&](uint32_t bits, float minus) {
+              float g = (ex2((__uint_as_float(bits) - lse) * CE_LOG2E) - minus) * rs;
+              if (lo) g -= float(__nv_bfloat16(g));
+              return counted ? g : 0.0f;
+            };
+            auto strip = [&](const uint32_t (&r)[32], int cb, int chunk) {
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {  // eight values at a time: the segmented form has 128 logits in registers
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = entry(r[8 * c + j], 0.0f);
+                *reinterpret_cast<uint4*>(staged_at(staging, lane, chunk + c)) = EpilogueCtx<__nv_bfloat16>::pack8_bf16(v);
+              }
+              const int a = at - cb;
+              if (a >= 0 && a < 32) {
+                uint32_t l = 0;
+#pragma unroll
+                for (int j = 0; j < 32; ++j) l = a == j ? r[j] : l;
+                *reinterpret_cast<__nv_bfloat16*>(staged_at(staging, lane, chunk + (a >> 3)) + 2 * (a & 7)) = __nv_bfloat16(entry(l, 1.0f));
+              }
+            };
+            if (stored && lane == 0) bulk_wait_group_read<0>();  // the previous block has left the staging tile
+            __syncwarp();
+            strip(a0, col0, 0);
+            if (second) strip(a1, col0 + 32, 4);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_3d(to, staging, col0, row0, 0);
+              bulk_commit_group();
+            }
+            stored = true;
+          };
+          put(&out0, false);
+          if (kMB == 0 && p.lo) put(&out1, true);
+        };
         if constexpr (kSegments) {
           float l[STRIPS][32];
 #pragma unroll
@@ -516,12 +562,24 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
             if (++slot == 2) { slot = 0; acc_phase ^= 1; }
           }
           if (!ok) break;
+          if constexpr (kMode == CE_LSE) {
 #pragma unroll
-          for (int c = 0; c < STRIPS; ++c) {
-            const int cb = t.n0 + (half * STRIPS + c) * 32;
-            if (cb < n_end) lse_strip(l[c], cb);
+            for (int c = 0; c < STRIPS; ++c) {
+              const int cb = t.n0 + (half * STRIPS + c) * 32;
+              if (cb < n_end) lse_strip(l[c], cb);
+            }
+            if (row_ok) p.part[((long long)(kPair ? t.n0 / BN : t.n0 / p.bn) * 2 + half) * job.M + row] = make_float2(m, s);
+          } else {
+#pragma unroll
+            for (int c = 0; c < STRIPS; c += 2) {
+              const int cb = t.n0 + (half * STRIPS + c) * 32;
+              if (cb >= n_end) continue;
+              uint32_t a0[32], a1[32];
+#pragma unroll
+              for (int j = 0; j < 32; ++j) a0[j] = __float_as_uint(l[c][j]), a1[j] = __float_as_uint(l[c + 1][j]);
+              grad_block(a0, a1, cb);
+            }
           }
-          if (row_ok) p.part[((long long)(kPair ? t.n0 / BN : t.n0 / p.bn) * 2 + half) * job.M + row] = make_float2(m, s);
           continue;
         }
         if (!warp_wait(&acc_full[slot], acc_phase)) { ok = false; break; }
@@ -548,45 +606,7 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
             strip(r0, col0);
             if (second) strip(r1, col0 + 32);
           } else if constexpr (kMode == CE_GRAD) {
-            auto strip = [&](const uint32_t (&r)[32], int cb) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = ex2((__uint_as_float(r[j]) - lse) * CE_LOG2E) * rs;
-              const int a = at - cb;
-              if (a >= 0 && a < 32) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                  if (a == j) v[j] = (ex2((__uint_as_float(r[j]) - lse) * CE_LOG2E) - 1.0f) * rs;
-              }
-              if (!counted) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = 0.0f;
-              }
-            };
-            auto put = [&](const CUtensorMap* to, bool lo) {
-              auto rest = [&]() {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] -= float(__nv_bfloat16(v[j]));
-              };
-              strip(r0, col0);
-              if (lo) rest();
-              if (stored && lane == 0) bulk_wait_group_read<0>();  // the previous block has left the staging tile
-              __syncwarp();
-              stage_bf16(v, staging, lane, 0);
-              if (second) {
-                strip(r1, col0 + 32);
-                if (lo) rest();
-                stage_bf16(v, staging, lane, 4);
-              }
-              fence_proxy_async_smem();
-              __syncwarp();
-              if (lane == 0) {
-                tma_store_3d(to, staging, col0, row0, 0);
-                bulk_commit_group();
-              }
-              stored = true;
-            };
-            put(&out0, false);
-            if (kMB == 0 && p.lo) put(&out1, true);
+            grad_block(r0, r1, col0);
           } else {
             const bool f32 = t.job == 0 && !p.dx_bf16;
             const CUtensorMap* om = t.job == 0 ? &out0 : &out1;
@@ -751,15 +771,15 @@ CeJob job_of(long long M, long long N, long long K, int mb) {
 
 template <int kMode, int kMB, bool kSegments = false>
 int launch(const CUtensorMap (&in)[4], const CUtensorMap (&out)[2], const CeKernelParams& p, long long tiles, int num_sms, cudaStream_t stream) {
-  using Cfg = CeCfg<kMB>;
   auto kern = ce_pair_kernel<kMode, kMB, kSegments>;
   constexpr int THREADS = 64 + 32 * CE_EPI_WARPS<kMB, kSegments>;
-  SX_ENSURE_DYN_SMEM(kern, Cfg::DYN_SMEM);
+  constexpr int DYN_SMEM = CE_DYN_SMEM<kMode, kMB, kSegments>;
+  SX_ENSURE_DYN_SMEM(kern, DYN_SMEM);
   constexpr int kGroup = kMB > 0 ? 2 : 1;
   // In plain stream order: launched early behind the kernel that joins a few thousand rows, a long queue of forward passes (3815 x 1104 x
   // 26330, 256-row tiles) stopped making progress.
   const unsigned groups = (unsigned)std::min<long long>(tiles, num_sms / kGroup);
-  const cudaError_t e = launch_kernel_ex(kern, kGroup * groups, THREADS, Cfg::DYN_SMEM, stream, kGroup, false, in[0], in[1], in[2], in[3],
+  const cudaError_t e = launch_kernel_ex(kern, kGroup * groups, THREADS, DYN_SMEM, stream, kGroup, false, in[0], in[1], in[2], in[3],
                                          out[0], out[1], p);
   if (e != cudaSuccess) return launch_failed(e, "loss kernel launch failed");
   count_launches(1);
@@ -795,8 +815,10 @@ long long ce_piece_of_waves(long long T, long long V, long long most) {
   return best * 256;
 }
 
-// The forward pass in segments where its error would be near 1e-6: up to 128 tokens from 2048 values on (1 x 4096 x 65536 101 us, 95
+// Logits in segments where the error of one sum would be near 1e-6: up to 128 tokens from 2048 values on (1 x 4096 x 65536 101 us, 95
 // without), pairs where the sum is longer than 4096 or the vocabulary is small (8192 x 4096 x 50257 would take 2305 us instead of 2164).
+// The gradient's logits with them: 2048 x 8192 x 32000 2250 us for the whole pass (2130 without), 300 x 8192 x 8000 192 (188),
+// 3 x 8192 x 8205 159 (152).
 static bool in_segments(long long T, long long V, long long H) { return H > 4096 || (H > 2048 && (T <= 128 || V < 16384)); }
 static int forward_row_blocks(long long T, long long V, long long H, int num_sms) {
   const int mb = row_blocks(T, V, num_sms);
@@ -817,8 +839,9 @@ int ce_forward_parts_most(long long T, long long V) {  // whatever the tile shap
 // The logits' product of either pass: operands, tile shape, and the kernel for it.
 template <int kMode>
 static int launch_logits(const CeCommon& c, const CeMatrix& x, const CeMatrix& W, const CUtensorMap (&out)[2], CeKernelParams* p, cudaStream_t stream) {
-  const bool segments = kMode == CE_LSE && in_segments(x.rows, W.rows, x.cols);
-  const int mb = kMode == CE_LSE ? forward_row_blocks(x.rows, W.rows, x.cols, c.num_sms) : p->lo ? 0 : row_blocks(x.rows, W.rows, c.num_sms);
+  const bool segments = in_segments(x.rows, p->V, x.cols);  // by the whole vocabulary: the same for both passes
+  int mb = p->lo ? 0 : row_blocks(x.rows, W.rows, c.num_sms);
+  if (segments) mb = std::min(mb, 1);
   uint32_t a_rows = 128 * mb, b_rows = 128;
   p->job[0] = job_of(x.rows, W.rows, x.cols, mb);
   if (mb == 0) {
@@ -827,7 +850,8 @@ static int launch_logits(const CeCommon& c, const CeMatrix& x, const CeMatrix& W
     b_rows = (uint32_t)(kMode == CE_GRAD ? columns_alone(W.rows, 64, 64, c.num_sms) : forward_columns_alone(W.rows, x.rows, x.cols, c.num_sms));
     p->bn = (int)b_rows;
     p->a_bytes = (int)a_rows * 128;
-    p->stages = std::min(CeCfg<0>::STAGES, CeCfg<0>::STAGE_ROOM / (p->a_bytes + p->bn * 128));
+    const int room = segments ? ce_stage_room<kMode, 0, true>() : ce_stage_room<kMode, 0, false>();
+    p->stages = std::min(CeCfg<0>::STAGES, room / (p->a_bytes + p->bn * 128));
     p->job[0].n_tiles = (int)((W.rows + p->bn - 1) / p->bn);
   }
   CUtensorMap in[4] = {};
@@ -836,10 +860,7 @@ static int launch_logits(const CeCommon& c, const CeMatrix& x, const CeMatrix& W
   if (rc != SX_OK) return rc;
   const long long tiles = (long long)p->job[0].m_tiles * p->job[0].n_tiles;
   if (tiles > 0x7fffffffLL) return set_last_error(SX_ERR_INVALID, "the problem has more than 2^31-1 tiles");
-  if constexpr (kMode == CE_LSE) {
-    if (segments)
-      return mb == 0 ? launch<CE_LSE, 0, true>(in, out, *p, tiles, c.num_sms, stream) : launch<CE_LSE, 1, true>(in, out, *p, tiles, c.num_sms, stream);
-  }
+  if (segments) return mb == 0 ? launch<kMode, 0, true>(in, out, *p, tiles, c.num_sms, stream) : launch<kMode, 1, true>(in, out, *p, tiles, c.num_sms, stream);
   switch (mb) {
     case 0: return launch<kMode, 0>(in, out, *p, tiles, c.num_sms, stream);
     case 1: return launch<kMode, 1>(in, out, *p, tiles, c.num_sms, stream);

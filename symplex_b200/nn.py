@@ -210,8 +210,8 @@ def linear_cross_entropy(x, weight, targets, *, ignore_index=-100, reduction="me
 def linear_cross_entropy_backward(dloss, x, weight, targets, lse, *, ignore_index=-100, reduction="mean", stream=None):
     """Gradients ``(dx, dweight)`` of ``linear_cross_entropy`` (``symplex_b200_linear_cross_entropy_backward``).
 
-    ``dloss``: float32, one value (``"mean"``, ``"sum"``) or ``[T]`` (``"none"``); ``lse`` from the forward pass; the other arguments
-    as there. The logits are computed again a piece of the vocabulary at a time. ``dx`` and ``dweight`` have the dtype of ``x``.
+    ``dloss``: float32, one value (``"mean"``, ``"sum"``) or ``[T]`` (``"none"``); ``lse`` from the forward pass over the same rows (both
+    passes round a logit alike, which rows that are sure of their target depend on); the other arguments as there. The logits are computed again a piece of the vocabulary at a time. ``dx`` and ``dweight`` have the dtype of ``x``.
     Ignored rows of ``x`` may hold anything; they are taken as 0.
     """
     t, h, v = _loss_checks("linear_cross_entropy_backward()", x, weight, targets, ignore_index, reduction)
