@@ -820,25 +820,17 @@ long long ce_piece_of_waves(long long T, long long V, long long most) {
 // The gradient's logits with them: 2048 x 8192 x 32000 2250 us for the whole pass (2130 without), 300 x 8192 x 8000 192 (188),
 // 3 x 8192 x 8205 159 (152).
 static bool in_segments(long long T, long long V, long long H) { return H > 4096 || (H > 2048 && (T <= 128 || V < 16384)); }
-static int forward_row_blocks(long long T, long long V, long long H, int num_sms) {
-  const int mb = row_blocks(T, V, num_sms);
-  return in_segments(T, V, H) ? std::min(mb, 1) : mb;
-}
 static int forward_columns_alone(long long V, long long T, long long H, int num_sms) { return columns_alone(V, 16, in_segments(T, V, H) ? 64 : 32, num_sms); }
 
-int ce_forward_parts(long long T, long long V, long long H, int num_sms) {
-  const int mb = forward_row_blocks(T, V, H, num_sms), halves = in_segments(T, V, H) ? 2 : 1;
-  if (mb > 0) return (int)((V + 255) / 256) * (halves == 2 ? 2 : mb);
-  const int bn = forward_columns_alone(V, T, H, num_sms);
-  return (int)((V + bn - 1) / bn) * halves;
-}
 int ce_forward_parts_most(long long T, long long V) {  // whatever the tile shape
   return (int)std::max((V + 255) / 256 * 2, T <= 128 ? (V + 63) / 64 * 2 : 0);
 }
 
-// The logits' product of either pass: operands, tile shape, and the kernel for it.
+// The logits' product of either pass: operands, tile shape (chosen here alone, by one look at the options), and the kernel for it. `parts`:
+// how many parts the forward pass writes of a row.
 template <int kMode>
-static int launch_logits(const CeCommon& c, const CeMatrix& x, const CeMatrix& W, const CUtensorMap (&out)[2], CeKernelParams* p, cudaStream_t stream) {
+static int launch_logits(const CeCommon& c, const CeMatrix& x, const CeMatrix& W, const CUtensorMap (&out)[2], CeKernelParams* p, cudaStream_t stream,
+                         int* parts) {
   const bool segments = in_segments(x.rows, p->V, x.cols);  // by the whole vocabulary: the same for both passes
   int mb = p->lo ? 0 : row_blocks(x.rows, W.rows, c.num_sms);
   if (segments) mb = std::min(mb, 1);
@@ -854,6 +846,7 @@ static int launch_logits(const CeCommon& c, const CeMatrix& x, const CeMatrix& W
     p->stages = std::min(CeCfg<0>::STAGES, room / (p->a_bytes + p->bn * 128));
     p->job[0].n_tiles = (int)((W.rows + p->bn - 1) / p->bn);
   }
+  if constexpr (kMode == CE_LSE) *parts = p->job[0].n_tiles * (segments ? 2 : std::max(mb, 1));
   CUtensorMap in[4] = {};
   int rc = map_of(&in[0], x, 64, a_rows);
   if (rc == SX_OK) rc = map_of(&in[1], W, 64, b_rows);
@@ -868,14 +861,14 @@ static int launch_logits(const CeCommon& c, const CeMatrix& x, const CeMatrix& W
   }
 }
 
-int launch_ce_forward(const CeCommon& c, const CeForward& a, cudaStream_t stream) {
+int launch_ce_forward(const CeCommon& c, const CeForward& a, cudaStream_t stream, int* parts) {
   CeKernelParams p = common(c);
   p.targets = a.targets;
   p.V = a.W.rows;
   p.part = a.part;
   p.target_logit = a.target_logit;
   p.done = a.done;
-  return launch_logits<CE_LSE>(c, a.x, a.W, {CUtensorMap{}, CUtensorMap{}}, &p, stream);
+  return launch_logits<CE_LSE>(c, a.x, a.W, {CUtensorMap{}, CUtensorMap{}}, &p, stream, parts);
 }
 
 int launch_ce_grad(const CeCommon& c, const CeGrad& a, cudaStream_t stream) {
@@ -891,7 +884,7 @@ int launch_ce_grad(const CeCommon& c, const CeGrad& a, cudaStream_t stream) {
   p.v0 = a.v0;
   p.V = a.V;
   p.ignore = a.ignore;
-  return launch_logits<CE_GRAD>(c, a.x, a.W, to, &p, stream);
+  return launch_logits<CE_GRAD>(c, a.x, a.W, to, &p, stream, nullptr);
 }
 
 // The tiles of both products in one shape. Returns how long the busiest pair works, in k-blocks of 256 x 256.

@@ -545,8 +545,7 @@ int forward(const Problem& p, const CeCommon& dev, const long long* targets, flo
     f.part = part;
     f.target_logit = target_logit;
     f.done = done;
-    parts = ce_forward_parts(p.T, p.V, p.H, dev.num_sms);
-    CE_TRY(launch_ce_forward(dev, f, stream));
+    CE_TRY(launch_ce_forward(dev, f, stream, &parts));
   } else {
     float *xs = reinterpret_cast<float*>(ws + w.xs), *wsp = reinterpret_cast<float*>(ws + w.ws), *logits = reinterpret_cast<float*>(ws + w.logits);
     CE_TRY(prep(launch_split_tf32(static_cast<const float*>(p.x), p.ldx, 0, xs, (int)p.T, (int)p.H, (int)w.hp, 1, stream)));
