@@ -519,7 +519,8 @@ int symplex_b200_gemm_plan(const symplex_gemm_desc* desc, int num_sms, symplex_g
  * mean squared deviation. x and y have element type dtype (SYMPLEX_DT_F32 / SYMPLEX_DT_BF16) and leading dimensions
  * ldx, ldy in elements (0 = cols); weight and bias have param_dtype (either dtype or SYMPLEX_DT_F32) and may be NULL
  * (1 and 0), as may mean and rstd (float[rows], the statistics the backward pass takes). Statistics and arithmetic are
- * 32-bit, y is rounded once. y may be x. rows == 0 is a no-op. */
+ * 32-bit, y is rounded once. y may be x (with ldy == ldx); any other overlap of y with an input is refused. rows == 0 is a
+ * no-op. */
 int symplex_b200_layer_norm(const void* x, const void* weight, const void* bias, void* y, float* mean, float* rstd,
                             int64_t rows, int64_t cols, int64_t ldx, int64_t ldy, int32_t dtype, int32_t param_dtype,
                             double eps, void* stream);
@@ -545,7 +546,7 @@ int symplex_b200_layer_norm_backward(const void* dy, const void* x, const float*
 /* C[M, N] = act(A[M, K] . W^T + bias) for a few rows of A (M <= SYMPLEX_B200_INT4_MAX_M): the product of single tokens,
  * bound by reading the codes. A is bf16 with leading dimension lda, C has out_dtype (F32 / BF16) and leading dimension ldc
  * (elements, 0 = packed), bias is fp32[N] or NULL, activation one of SYMPLEX_ACT_*. code - zero enters the product as the
- * whole number it is, sums are 32-bit, the scale is applied to each group's sum. */
+ * whole number it is, sums are 32-bit, the scale is applied to each group's sum. C must not overlap an input (refused). */
 #define SYMPLEX_B200_INT4_MAX_M 64
 int symplex_b200_int4_matvec(const void* A, const uint8_t* codes, const void* scales, const uint8_t* zeros,
                              const float* bias, void* C, int64_t M, int64_t N, int64_t K, int64_t group, int64_t lda,

@@ -16,6 +16,7 @@
 #include <atomic>
 
 #include "../../include/symplex_b200.h"
+#include "byte_rows.h"
 #include "epilogue.cuh"
 #include "host_api.h"
 #include "sm100_ptx.cuh"
@@ -811,6 +812,11 @@ int symplex_b200_int4_matvec(const void* A, const uint8_t* codes, const void* sc
   a.act = activation;
   int sms = 0;
   if ((rc = current_device_sms(&sms)) != SX_OK) return rc;
+  const ByteRows out{C, M, N * bytes_of(out_dtype), a.ldc * bytes_of(out_dtype)};
+  const long long sums = N * a.groups;
+  if (share_bytes(out, {A, M, K * 2, a.lda * 2}) || share_bytes(out, {codes, N, (K + 1) / 2, a.ldq}) ||
+      share_bytes(out, one_row(scales, sums * bytes_of(scale_dtype))) || share_bytes(out, one_row(zeros, sums)) || share_bytes(out, one_row(bias, N * 4)))
+    return fail_fmt(SX_ERR_INVALID, "C overlaps an operand, which other columns of the product still read");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool out_bf16 = out_dtype == SYMPLEX_DT_BF16;
   return scale_dtype == SYMPLEX_DT_F32 ? matvec<float>(a, out_bf16, sms, st) : matvec<__nv_bfloat16>(a, out_bf16, sms, st);

@@ -19,6 +19,7 @@
 #include <type_traits>
 
 #include "../../include/symplex_b200.h"
+#include "byte_rows.h"
 #include "gemm_params.h"
 #include "host_api.h"
 #include "sm100_ptx.cuh"
@@ -1017,6 +1018,12 @@ int symplex_b200_layer_norm(const void* x, const void* weight, const void* bias,
     return fail_fmt(SX_ERR_INVALID, "a pointer is not aligned to its element type");
   int sms = 0;
   if ((rc = current_device_sms(&sms)) != SX_OK) return rc;
+  const long long eb = dtype == SYMPLEX_DT_F32 ? 4 : 2, params = cols * (param_dtype == SYMPLEX_DT_F32 ? 4 : 2);
+  const ByteRows out{y, rows, cols * eb, s.ldy * eb};
+  const bool in_place = x == y && (s.ldx == s.ldy || rows == 1);
+  if ((!in_place && share_bytes(out, {x, rows, cols * eb, s.ldx * eb})) || share_bytes(out, one_row(weight, params)) ||
+      share_bytes(out, one_row(bias, params)))
+    return fail_fmt(SX_ERR_INVALID, "y overlaps x (and is not x itself), weight or bias");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == SYMPLEX_DT_F32) return forward<float, float>(x, weight, bias, y, mean, rstd, s, (float)eps, sms, st);
   if (param_dtype == SYMPLEX_DT_F32)

@@ -58,6 +58,13 @@ def _workspace_bytes(query, *args):
     return getattr(_capi.load(), query)(*args)
 
 
+def _check(code):
+    """Arguments that the library refuses are the caller's, like those refused here."""
+    if code == _capi.ERR_INVALID:
+        raise ValueError(_capi.last_error())
+    _capi.check(code)
+
+
 def _ptr(t):
     return t.data_ptr() if t is not None else None
 
@@ -89,7 +96,7 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5, out=None, return_stats=Fa
 
     ``x``: float32 or bfloat16 of any shape; a 2-D view with unit stride in its rows is read in place, other strides
     through a copy. ``weight`` and ``bias``: ``[cols]`` of ``x``'s dtype or float32, or None. ``out``: contiguous (or 2-D
-    with unit stride in its rows), may be ``x``. Statistics are computed in 32 bits, the result is rounded once.
+    with unit stride in its rows), may be ``x`` but not overlap it otherwise. Statistics are computed in 32 bits, the result is rounded once.
     Returns ``y``, or ``(y, mean, rstd)`` with ``return_stats`` (float32, shaped like ``x`` without its last dimension):
     what ``layer_norm_backward`` takes.
     """
@@ -109,7 +116,7 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5, out=None, return_stats=Fa
             rstd = torch.empty_like(mean)
         w = weight.contiguous() if weight is not None else None
         b = bias.contiguous() if bias is not None else None
-        _capi.check(_capi.load().symplex_b200_layer_norm(
+        _check(_capi.load().symplex_b200_layer_norm(
             xr.data_ptr(), _ptr(w), _ptr(b), y.data_ptr(), _ptr(mean), _ptr(rstd), x.numel() // cols, cols, ldx,
             cols if out is None or y.is_contiguous() else y.stride(0), _DT[x.dtype], _DT[pdt], eps, s))
         return (y, mean, rstd) if return_stats else y
@@ -148,7 +155,7 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, *, param_grads=None, str
             ws = x.new_empty(size, dtype=torch.uint8)
         w = weight.contiguous() if weight is not None else None
         m, r = mean.contiguous(), rstd.contiguous()
-        _capi.check(lib.symplex_b200_layer_norm_backward(
+        _check(lib.symplex_b200_layer_norm_backward(
             dyr.data_ptr(), xr.data_ptr(), m.data_ptr(), r.data_ptr(), _ptr(w), dx.data_ptr(), _ptr(dw), _ptr(db), rows, cols,
             lddy, ldx, cols, _DT[x.dtype], _DT[pdt], _ptr(ws), size, s))
         return dx, dw, db
@@ -199,7 +206,7 @@ def linear_cross_entropy(x, weight, targets, *, ignore_index=-100, reduction="me
                                 ldw, _DT[x.dtype])  # of the pointers it looks at the alignment
         ws = x.new_empty(size, dtype=torch.uint8)
         tg = targets.contiguous()
-        _capi.check(lib.symplex_b200_linear_cross_entropy(
+        _check(lib.symplex_b200_linear_cross_entropy(
             xr.data_ptr(), w.data_ptr(), tg.data_ptr(), loss.data_ptr(), lse.data_ptr(), t, h, v, ldx, ldw, _DT[x.dtype], ignore_index,
             LOSS_REDUCTIONS[reduction], ws.data_ptr(), size, s))
         return loss, lse
@@ -229,7 +236,7 @@ def linear_cross_entropy_backward(dloss, x, weight, targets, lse, *, ignore_inde
                                 ldw, _DT[x.dtype])  # of the pointers it looks at the alignment
         ws = x.new_empty(size, dtype=torch.uint8)
         tg, ls, dl = targets.contiguous(), lse.contiguous(), dloss.contiguous()
-        _capi.check(lib.symplex_b200_linear_cross_entropy_backward(
+        _check(lib.symplex_b200_linear_cross_entropy_backward(
             dl.data_ptr(), xr.data_ptr(), w.data_ptr(), tg.data_ptr(), ls.data_ptr(), dx.data_ptr(), dw.data_ptr(), t, h, v, ldx, ldw,
             _DT[x.dtype], ignore_index, LOSS_REDUCTIONS[reduction], ws.data_ptr(), size, s))
         return dx, dw
@@ -266,7 +273,7 @@ def int4_quantize(weight, group_size=128, *, symmetric=True, scale_dtype=torch.b
         codes = torch.empty(n, (k + 1) // 2, dtype=torch.uint8, device=weight.device)
         scales = torch.empty(n, groups, dtype=scale_dtype, device=weight.device)
         zeros = None if symmetric else torch.empty(n, groups, dtype=torch.uint8, device=weight.device)
-        _capi.check(_capi.load().symplex_b200_int4_quantize(w.data_ptr(), codes.data_ptr(), scales.data_ptr(), _ptr(zeros), n, k,
+        _check(_capi.load().symplex_b200_int4_quantize(w.data_ptr(), codes.data_ptr(), scales.data_ptr(), _ptr(zeros), n, k,
                                                             group_size, ldw, _DT[weight.dtype], _DT[scale_dtype], s))
         return codes, scales, zeros
 
@@ -280,7 +287,7 @@ def int4_matvec(x, codes, scales, zeros=None, *, group_size=128, bias=None, acti
 
     ``x``: bfloat16 ``[K]`` or ``[M, K]``; ``zeros`` (0 to 15) None means 8 everywhere; ``bias``: float32 ``[N]``; ``activation`` as in
     ``gemm``. ``codes`` may be a view with unit stride in its rows. Returns ``[N]`` / ``[M, N]`` in ``out_dtype`` (bfloat16 or
-    float32). More rows than 64 are a product for ``gemm``.
+    float32); ``out`` must not overlap an operand. More rows than 64 are a product for ``gemm``.
     """
     xshape, device = x.shape, x.device
     if not x.is_cuda or x.dtype != torch.bfloat16 or len(xshape) not in (1, 2):
@@ -321,7 +328,7 @@ def int4_matvec(x, codes, scales, zeros=None, *, group_size=128, bias=None, acti
         sc = scales.contiguous()
         z = zeros.contiguous() if zeros is not None else None
         b = bias.contiguous() if bias is not None else None
-        _capi.check(_capi.load().symplex_b200_int4_matvec(
+        _check(_capi.load().symplex_b200_int4_matvec(
             a.data_ptr(), c.data_ptr(), sc.data_ptr(), _ptr(z), _ptr(b), y.data_ptr(), m, n, k, group_size, lda, ldq, n,
             _DT[sc.dtype], _DT[out_dtype], ACTIVATIONS[activation], s))
         return y
