@@ -17,6 +17,7 @@ library or a B200 is missing.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 
 import numpy as np
 
@@ -24,19 +25,25 @@ from . import _capi
 from ._capi import (ACT_GELU, ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_SILU, ACT_TANH, ACTIVATIONS, COL_MAJOR, DT_BF16,
                     DT_F32, ROW_MAJOR, GemmDesc, SymplexB200Error)
 
+# live in the nn sub-module, which imports torch
+_NN = ("layer_norm", "layer_norm_backward", "linear_cross_entropy", "linear_cross_entropy_backward", "int4_quantize", "int4_matvec")
+
 __all__ = [
     "matmul_jit", "matmul_tiled", "matmul", "fused_matmul_bias_relu", "gemm", "gemm_host", "make_desc",
     "cuda_available", "launch_count", "SymplexB200Error", "fused_elementwise",
-    "layer_norm", "layer_norm_backward", "linear_cross_entropy", "linear_cross_entropy_backward", "int4_quantize", "int4_matvec",
 ]
-
-# live in the nn sub-module, which imports torch
-_NN = ("layer_norm", "layer_norm_backward", "linear_cross_entropy", "linear_cross_entropy_backward", "int4_quantize", "int4_matvec")
+if importlib.util.find_spec("torch") is not None:  # found, not imported: a star import works without it
+    __all__ += _NN
 
 
 def __getattr__(name):
     if name in _NN:
-        from . import nn
+        try:
+            from . import nn
+        except ModuleNotFoundError as e:
+            if e.name != "torch":
+                raise
+            raise AttributeError(f"{__name__}.{name} needs torch, which is not installed") from e
         for n in _NN:
             globals()[n] = getattr(nn, n)
         return globals()[name]
