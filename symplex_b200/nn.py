@@ -4,7 +4,9 @@
 Like ``gemm`` they are asynchronous on ``stream`` (a raw handle; default: torch's current stream of the tensors' device)
 and raise ``ValueError`` for arguments they do not take. Forward and backward passes are functions of their own; nothing
 is recorded between them. What they allocate (results and scratch) comes from torch's allocator on the stream of the
-call, so calls can be captured into CUDA graphs and run on several streams at once.
+call, so calls can be captured into CUDA graphs and run on several streams at once. On a ``stream`` that is not the current one the
+operands are named to the allocator (``record_stream``) and may be dropped behind the call; that they are ready on that stream, and
+that it is done before another one takes the results, is the caller's to see to.
 """
 from __future__ import annotations
 
@@ -27,14 +29,21 @@ _DT = {torch.float32: DT_F32, torch.bfloat16: DT_BF16}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _run(device, stream, fn):
-    """``fn(raw_stream)`` with ``device`` current and, where a stream is given, torch's allocations on that stream."""
+def _run(device, stream, fn, *operands):
+    """``fn(raw_stream)`` with ``device`` current and, where a stream is given, torch's allocations on that stream and the ``operands``
+    kept from being handed out again before it has read them."""
     if stream is None:
         if device.index == torch.cuda.current_device():
             return fn(_raw_stream(device.index))
         with torch.cuda.device(device):
             return fn(_raw_stream(device.index))
-    with torch.cuda.device(device), torch.cuda.stream(torch.cuda.ExternalStream(stream, device)):
+    other = stream != _raw_stream(device.index)
+    s = torch.cuda.ExternalStream(stream, device)
+    with torch.cuda.device(device), torch.cuda.stream(s):
+        if other:
+            for t in operands:
+                if t is not None:
+                    t.record_stream(s)
         return fn(stream)
 
 
@@ -121,7 +130,7 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5, out=None, return_stats=Fa
             cols if out is None or y.is_contiguous() else y.stride(0), _DT[x.dtype], _DT[pdt], eps, s))
         return (y, mean, rstd) if return_stats else y
 
-    return _run(x.device, stream, call)
+    return _run(x.device, stream, call, x, weight, bias, out)
 
 
 def layer_norm_backward(dy, x, mean, rstd, weight=None, *, param_grads=None, stream=None):
@@ -160,7 +169,7 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, *, param_grads=None, str
             lddy, ldx, cols, _DT[x.dtype], _DT[pdt], _ptr(ws), size, s))
         return dx, dw, db
 
-    return _run(device, stream, call)
+    return _run(device, stream, call, dy, x, mean, rstd, weight)
 
 
 # ----------------------------------------------------------------------------- softmax cross entropy of a linear head
@@ -211,7 +220,7 @@ def linear_cross_entropy(x, weight, targets, *, ignore_index=-100, reduction="me
             LOSS_REDUCTIONS[reduction], ws.data_ptr(), size, s))
         return loss, lse
 
-    return _run(x.device, stream, call)
+    return _run(x.device, stream, call, x, weight, targets)
 
 
 def linear_cross_entropy_backward(dloss, x, weight, targets, lse, *, ignore_index=-100, reduction="mean", stream=None):
@@ -241,7 +250,7 @@ def linear_cross_entropy_backward(dloss, x, weight, targets, lse, *, ignore_inde
             _DT[x.dtype], ignore_index, LOSS_REDUCTIONS[reduction], ws.data_ptr(), size, s))
         return dx, dw
 
-    return _run(x.device, stream, call)
+    return _run(x.device, stream, call, dloss, x, weight, targets, lse)
 
 
 # ----------------------------------------------------------------------------- products with 4-bit weights
@@ -277,7 +286,7 @@ def int4_quantize(weight, group_size=128, *, symmetric=True, scale_dtype=torch.b
                                                             group_size, ldw, _DT[weight.dtype], _DT[scale_dtype], s))
         return codes, scales, zeros
 
-    return _run(weight.device, stream, call)
+    return _run(weight.device, stream, call, weight)
 
 
 def int4_matvec(x, codes, scales, zeros=None, *, group_size=128, bias=None, activation=None, out=None, out_dtype=None,
@@ -333,4 +342,4 @@ def int4_matvec(x, codes, scales, zeros=None, *, group_size=128, bias=None, acti
             _DT[sc.dtype], _DT[out_dtype], ACTIVATIONS[activation], s))
         return y
 
-    return _run(device, stream, call)
+    return _run(device, stream, call, x, codes, scales, zeros, bias, out)
