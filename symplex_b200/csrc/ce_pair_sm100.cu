@@ -157,6 +157,7 @@ __device__ __forceinline__ float ex2(float x) {
 
 // 16 columns of this warp's 32 rows, a row a lane; waits for them.
 __device__ __forceinline__ void tmem_get_32x16(uint32_t taddr, uint32_t (&r)[16]) {
+  __syncwarp();
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
                "tcgen05.wait::ld.sync.aligned;"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
@@ -435,11 +436,6 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
     bool ok = true;
     const float scale = kMode == CE_PROD && p.scale != nullptr ? *p.scale : 1.0f;
     bool stored = false;  // this warp has TMA stores that may be reading its staging tile
-    // The lanes wait one by one, and may leave the wait at different times; what follows is the whole warp's.
-    auto warp_wait = [&](uint64_t* bar, uint32_t parity) {
-      const bool got = mbar_wait(bar, parity, &abort_flag, wait_ns);
-      return __all_sync(0xffffffffu, got) != 0;
-    };
     CeTile t;
     for (Work w(p, pair_id, num_pairs); ok && w.get(&t);) {
       const CeJob& job = p.job[t.job];
@@ -544,7 +540,7 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
 #pragma unroll
             for (int j = 0; j < 32; ++j) l[c][j] = 0.0f;
           for (int k0 = 0; ok && k0 < t.kb; k0 += CE_SEGMENT) {
-            if (!warp_wait(&acc_full[slot], acc_phase)) { ok = false; break; }
+            if (!mbar_wait_warp(&acc_full[slot], acc_phase, &abort_flag, wait_ns)) { ok = false; break; }
             tc_fence_after_sync();
 #pragma unroll
             for (int c = 0; c < 2 * STRIPS; ++c) {
@@ -582,12 +578,11 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
           }
           continue;
         }
-        if (!warp_wait(&acc_full[slot], acc_phase)) { ok = false; break; }
+        if (!mbar_wait_warp(&acc_full[slot], acc_phase, &abort_flag, wait_ns)) { ok = false; break; }
         tc_fence_after_sync();
 #pragma unroll 1
         for (int c = half * STRIPS; c < (half + 1) * STRIPS; c += 2) {
           uint32_t r0[32], r1[32];
-          __syncwarp();  // the lanes part in every strip (targets), the loads are the whole warp's
           const uint32_t taddr = tmem_base + (uint32_t(q * 32) << 16) + slot * BN + c * 32;
           tmem_ld_32x32(taddr, r0);
           tmem_ld_32x32(taddr + 32, r1);

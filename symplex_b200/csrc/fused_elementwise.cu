@@ -517,7 +517,7 @@ fused_elementwise_ring_kernel(const __grid_constant__ FeKernelArgs<T, MAXOPS> P)
     int stage = 0;
     uint32_t phase = 0;
     for (long long c = blockIdx.x; c < nchunks; c += gridDim.x) {
-      if (!mbar_wait(&full_bar[stage], phase, &abort_flag)) break;
+      if (!mbar_wait_warp(&full_bar[stage], phase, &abort_flag)) break;
       RingLoader<T, U> ld;
       ld.base = ring + (size_t)stage * ni * CHUNK + tid * VE;
       ld.stride = CHUNK;

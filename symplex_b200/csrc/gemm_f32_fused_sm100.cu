@@ -235,7 +235,7 @@ gemm_f32_fused_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         if (it % Cfg::CONV_GROUPS != group) continue;
         const int stage = it % STAGES;
         const uint32_t phase = (uint32_t)(it / STAGES) & 1u;
-        if (!mbar_wait(&raw_full[stage], phase, &abort_flag)) { ok = false; break; }
+        if (!mbar_wait_warp(&raw_full[stage], phase, &abort_flag)) { ok = false; break; }
         uint8_t* base = tiles + stage * Cfg::STAGE_BYTES;
 #pragma unroll
         for (int i = 0; i < 1024 / CT; ++i) {  // A: 1024 16-byte chunks, position-wise
@@ -292,7 +292,7 @@ gemm_f32_fused_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
 #pragma unroll
       for (int j = 0; j < BN; ++j) sum[j] = 0.0f;
       for (int ch = 0; ch < nchunks; ++ch) {
-        if (!mbar_wait(&main_full[macc], mphase, &abort_flag)) { ok = false; break; }
+        if (!mbar_wait_warp(&main_full[macc], mphase, &abort_flag)) { ok = false; break; }
         tc_fence_after_sync();
 #pragma unroll
         for (int c = 0; c < BN / 32; ++c) {
@@ -308,7 +308,7 @@ gemm_f32_fused_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         if (++macc == 2) { macc = 0; mphase ^= 1; }
       }
       if (!ok) break;
-      if (!mbar_wait(&corr_full[cacc], cphase, &abort_flag)) break;
+      if (!mbar_wait_warp(&corr_full[cacc], cphase, &abort_flag)) break;
       tc_fence_after_sync();
 #pragma unroll
       for (int c = 0; c < BN / 32; ++c) {
@@ -329,7 +329,7 @@ gemm_f32_fused_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         float* part = reinterpret_cast<float*>(tiles + STAGES * Cfg::STAGE_BYTES);
         const int prow = q * 32 + lane;
         if (rank != 0) {
-          if (!mbar_wait<true>(&part_empty[q], xphase ^ 1, &abort_flag)) break;  // leader has read the previous one
+          if (!mbar_wait_warp<true>(&part_empty[q], xphase ^ 1, &abort_flag)) break;  // leader has read the previous one
 #pragma unroll
           for (int g = 0; g < BN / 4; ++g)
             *reinterpret_cast<float4*>(part + (g * BM + prow) * 4) =
@@ -341,7 +341,7 @@ gemm_f32_fused_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         }
         bool got = true;
         for (int r = 1; r < kSplit; ++r)
-          if (!mbar_wait<true>(&part_full[r - 1][q], xphase, &abort_flag)) { got = false; break; }
+          if (!mbar_wait_warp<true>(&part_full[r - 1][q], xphase, &abort_flag)) { got = false; break; }
         if (got) {
           // Remote (distributed shared memory) loads take on the order of 100 ns each: a round issues the loads
           // of all peers for a group of columns before the first add, so 12 (8 for two CTAs) are in flight per

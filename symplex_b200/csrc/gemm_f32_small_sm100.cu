@@ -227,8 +227,8 @@ gemm_f32_small_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       for (int kb = 0; kb < nkb; ++kb, ++it) {
         if (it % Cfg::CONV_GROUPS != group) continue;
         const int rs = it % RS, os = it % OS;
-        if (!mbar_wait(&raw_full[rs], (uint32_t)(it / RS) & 1u, &abort_flag)) { ok = false; break; }
-        if (!mbar_wait(&op_empty[os], ((uint32_t)(it / OS) & 1u) ^ 1u, &abort_flag)) { ok = false; break; }
+        if (!mbar_wait_warp(&raw_full[rs], (uint32_t)(it / RS) & 1u, &abort_flag)) { ok = false; break; }
+        if (!mbar_wait_warp(&op_empty[os], ((uint32_t)(it / OS) & 1u) ^ 1u, &abort_flag)) { ok = false; break; }
         const uint8_t* raw = tiles + rs * Cfg::RAW_BYTES;
         uint8_t* op = tiles + Cfg::OP_BASE + os * Cfg::OP_BYTES;
         // Read the whole raw stage into registers first and hand it back to the producer at once: the next
@@ -306,7 +306,7 @@ gemm_f32_small_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
 #pragma unroll
       for (int j = 0; j < PN; ++j) sum[j] = 0.0f;
       for (int ch = 0; ch < nchunks; ++ch) {
-        if (!mbar_wait(&main_full[macc], mphase, &abort_flag)) { ok = false; break; }
+        if (!mbar_wait_warp(&main_full[macc], mphase, &abort_flag)) { ok = false; break; }
         tc_fence_after_sync();
 #pragma unroll
         for (int c = 0; c < PN / 32; ++c) {
@@ -322,7 +322,7 @@ gemm_f32_small_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         if (++macc == 2) { macc = 0; mphase ^= 1; }
       }
       if (!ok) break;
-      if (!mbar_wait(&corr_full[cacc], cphase, &abort_flag)) break;
+      if (!mbar_wait_warp(&corr_full[cacc], cphase, &abort_flag)) break;
       tc_fence_after_sync();
 #pragma unroll
       for (int c = 0; c < PN / 32; ++c) {

@@ -425,7 +425,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 #pragma unroll 1
       for (int blk = 0; blk < kMB; ++blk) {
         if constexpr (kMB == 2) slot = blk;
-        if (!mbar_wait(&acc_full[slot], acc_phase, &abort_flag, wait_ns)) { ok = false; break; }
+        if (!mbar_wait_warp(&acc_full[slot], acc_phase, &abort_flag, wait_ns)) { ok = false; break; }
         tc_fence_after_sync();
         const int row0 = tc.m0 + int(cta_rank) * Cfg::ROWS + blk * 128 + q * 32;  // this warp's first row
         const int row = row0 + lane;

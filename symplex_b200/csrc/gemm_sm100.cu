@@ -193,7 +193,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
     uint32_t acc_phase = 0;
     for (int t = blockIdx.x; t < total_tiles; t += gridDim.x) {
       const TileCoord tc = tile_coord<BM, BN>(p, t);
-      if (!mbar_wait(&acc_full[acc], acc_phase, &abort_flag, p.wait_limit_ns)) break;
+      if (!mbar_wait_warp(&acc_full[acc], acc_phase, &abort_flag, p.wait_limit_ns)) break;
       tc_fence_after_sync();
       const int row = tc.m0 + q * 32 + lane;
       const bool row_ok = row < p.M;

@@ -197,7 +197,7 @@ gemm_tf32x3_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
 #pragma unroll
       for (int j = 0; j < BN; ++j) sum[j] = 0.0f;
       for (int ch = 0; ch < nchunks; ++ch) {
-        if (!mbar_wait(&main_full[macc], mphase, &abort_flag)) { ok = false; break; }
+        if (!mbar_wait_warp(&main_full[macc], mphase, &abort_flag)) { ok = false; break; }
         tc_fence_after_sync();
 #pragma unroll
         for (int c = 0; c < BN / 32; ++c) {
@@ -213,7 +213,7 @@ gemm_tf32x3_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         if (++macc == 2) { macc = 0; mphase ^= 1; }
       }
       if (!ok) break;
-      if (!mbar_wait(&corr_full[cacc], cphase, &abort_flag)) break;
+      if (!mbar_wait_warp(&corr_full[cacc], cphase, &abort_flag)) break;
       tc_fence_after_sync();
 #pragma unroll
       for (int c = 0; c < BN / 32; ++c) {

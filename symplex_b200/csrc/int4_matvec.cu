@@ -72,8 +72,14 @@ __device__ __forceinline__ void cp_async_wait() {
 __device__ __forceinline__ void group_barrier(int group, int groups) {
   asm volatile("bar.sync %0, %1;" ::"r"(groups + group), "r"(32 * MV_WARPS / groups) : "memory");
 }
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive() {
+  __syncwarp();  // both barriers are the whole warp's
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 __device__ __forceinline__ float4 ld_cluster(uint32_t addr, uint32_t rank) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(mapa_u32(addr, rank)) : "memory");
@@ -360,7 +366,6 @@ int4_mma_kernel(const Int4Args p, const MvPlan plan) {
   // Cluster: this CTA's share of the outputs of a round, once every CTA has arrived with its sums.
   int held_tile = -1, held_n = 0, held_buf = 0;
   auto write_held = [&]() {
-    __syncwarp();
     cluster_wait();
     for (int e = rank * (MV_WARPS * 32) + threadIdx.x; e < held_n * (8 * kNB) * (MV_TILE / 4); e += plan.cluster * MV_WARPS * 32) {
       const int m = e / (MV_TILE / 4) % (8 * kNB);
@@ -513,13 +518,11 @@ int4_mma_kernel(const Int4Args p, const MvPlan plan) {
       held_tile = b0;
       held_n = min(RG, t1 - b0);
       held_buf ^= 1;
-      __syncwarp();
       cluster_arrive();
     }
   }
   if (plan.cluster > 1) {
     if (held_tile >= 0) write_held();
-    __syncwarp();
     cluster_arrive();  // no CTA leaves while its sums are being read
     cluster_wait();
   }

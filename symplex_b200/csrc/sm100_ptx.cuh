@@ -37,7 +37,11 @@ __device__ __forceinline__ uint32_t mapa_u32(uint32_t addr, uint32_t rank) {
   return r;
 }
 
+// Instructions marked .aligned are the whole warp's: all 32 lanes have to execute them together, and what happens where they do not is
+// undefined, with no limit on how long it takes. Lanes that waited in a loop, branched on their row or left a one-lane section need not be
+// together again by themselves, so the helpers below bring them together first (one instruction).
 __device__ __forceinline__ void cluster_sync_all() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -141,6 +145,15 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
       }
     }
   }
+}
+
+// The same wait of a whole warp (all 32 lanes call it), with one answer for all of them: the lanes poll one by one, and one that runs out
+// of time may stand beside one that has just seen the barrier flip.
+template <bool kClusterAcquire = false>
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                               uint64_t limit_ns = WAIT_LIMIT_NS) {
+  const bool got = mbar_wait<kClusterAcquire>(bar, parity, abort_flag, limit_ns);
+  return __all_sync(0xffffffffu, got) != 0;
 }
 
 // ---------------------------------------------------------------- flags and counters (exchange between GPUs)
@@ -317,6 +330,7 @@ __device__ __forceinline__ void bulk_wait_group() {
 // ---------------------------------------------------------------- tcgen05
 template <int kCtaGroup>
 __device__ __forceinline__ void tmem_alloc(uint32_t* smem_result, uint32_t ncols) {
+  __syncwarp();
   if constexpr (kCtaGroup == 1)
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_result)),
                  "r"(ncols)
@@ -335,6 +349,7 @@ __device__ __forceinline__ void tmem_relinquish() {
 }
 template <int kCtaGroup>
 __device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
+  __syncwarp();
   if constexpr (kCtaGroup == 1)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
   else
@@ -394,6 +409,7 @@ __device__ __forceinline__ void umma_commit_pair(uint64_t* bar, uint16_t cta_mas
 // 32 lanes x 32 columns of 32-bit: thread i of the warp receives TMEM lane (base lane + i),
 // columns [col, col+32). A warp may only touch lanes 32*(warp_id % 4) .. +31.
 __device__ __forceinline__ void tmem_ld_32x32(uint32_t taddr, uint32_t (&r)[32]) {
+  __syncwarp();
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
       "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
@@ -405,6 +421,7 @@ __device__ __forceinline__ void tmem_ld_32x32(uint32_t taddr, uint32_t (&r)[32])
       : "r"(taddr)
       : "memory");
 }
+// Directly behind the loads: the lanes are still together.
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // ---------------------------------------------------------------- descriptors
