@@ -771,8 +771,8 @@ int launch(const CUtensorMap (&in)[4], const CUtensorMap (&out)[2], const CeKern
   constexpr int DYN_SMEM = CE_DYN_SMEM<kMode, kMB, kSegments>;
   SX_ENSURE_DYN_SMEM(kern, DYN_SMEM);
   constexpr int kGroup = kMB > 0 ? 2 : 1;
-  // In plain stream order: launched early behind the kernel that joins a few thousand rows, a long queue of forward passes (3815 x 1104 x
-  // 26330, 256-row tiles) stopped making progress.
+  // In plain stream order, not as a programmatic dependent: one of two things that a hang of unknown cause had in common (2 us more for
+  // the smallest calls).
   const unsigned groups = (unsigned)std::min<long long>(tiles, num_sms / kGroup);
   const cudaError_t e = launch_kernel_ex(kern, kGroup * groups, THREADS, DYN_SMEM, stream, kGroup, false, in[0], in[1], in[2], in[3],
                                          out[0], out[1], p);
@@ -815,6 +815,20 @@ long long ce_piece_of_waves(long long T, long long V, long long most) {
 // The gradient's logits with them: 2048 x 8192 x 32000 2250 us for the whole pass (2130 without), 300 x 8192 x 8000 192 (188),
 // 3 x 8192 x 8205 159 (152).
 static bool in_segments(long long T, long long V, long long H) { return H > 4096 || (H > 2048 && (T <= 128 || V < 16384)); }
+
+// Tile rows and the form of the sums, of the forward pass. 256-row tiles run in segments whatever the length: one form for them, whose
+// epilogue reads a whole accumulator before the lanes' branches (3816 x 1104 x 26330 196 us, 172 as one sum; 200 x 768 x 50257 32, 29;
+// 2000 x 256 x 30000, where 512-row tiles are taken, 59, 65).
+struct LogitsForm {
+  int mb;
+  bool segments;
+};
+static LogitsForm forward_form(long long T, long long V, long long H, int num_sms) {
+  int mb = row_blocks(T, V, num_sms);
+  const bool segments = in_segments(T, V, H);
+  if (segments) mb = std::min(mb, 1);
+  return {mb, segments || mb == 1};
+}
 static int forward_columns_alone(long long V, long long T, long long H, int num_sms) { return columns_alone(V, 16, in_segments(T, V, H) ? 64 : 32, num_sms); }
 
 int ce_forward_parts_most(long long T, long long V) {  // whatever the tile shape
@@ -826,9 +840,14 @@ int ce_forward_parts_most(long long T, long long V) {  // whatever the tile shap
 template <int kMode>
 static int launch_logits(const CeCommon& c, const CeMatrix& x, const CeMatrix& W, const CUtensorMap (&out)[2], CeKernelParams* p, cudaStream_t stream,
                          int* parts) {
-  const bool segments = in_segments(x.rows, p->V, x.cols);  // by the whole vocabulary: the same for both passes
-  int mb = p->lo ? 0 : row_blocks(x.rows, W.rows, c.num_sms);
-  if (segments) mb = std::min(mb, 1);
+  const LogitsForm form = forward_form(x.rows, p->V, x.cols, c.num_sms);
+  // The gradient's tiles go by the piece at hand, its sums by the forward pass. One segment is the same sum in either form.
+  const bool segments = form.segments && (kMode == CE_LSE || x.cols > CE_SEGMENT * 64);
+  int mb = form.mb;
+  if constexpr (kMode == CE_GRAD) {
+    mb = p->lo ? 0 : row_blocks(x.rows, W.rows, c.num_sms);
+    if (segments) mb = std::min(mb, 1);
+  }
   uint32_t a_rows = 128 * mb, b_rows = 128;
   p->job[0] = job_of(x.rows, W.rows, x.cols, mb);
   if (mb == 0) {
@@ -849,11 +868,11 @@ static int launch_logits(const CeCommon& c, const CeMatrix& x, const CeMatrix& W
   const long long tiles = (long long)p->job[0].m_tiles * p->job[0].n_tiles;
   if (tiles > 0x7fffffffLL) return set_last_error(SX_ERR_INVALID, "the problem has more than 2^31-1 tiles");
   if (segments) return mb == 0 ? launch<kMode, 0, true>(in, out, *p, tiles, c.num_sms, stream) : launch<kMode, 1, true>(in, out, *p, tiles, c.num_sms, stream);
-  switch (mb) {
-    case 0: return launch<kMode, 0>(in, out, *p, tiles, c.num_sms, stream);
-    case 1: return launch<kMode, 1>(in, out, *p, tiles, c.num_sms, stream);
-    default: return launch<kMode, 2>(in, out, *p, tiles, c.num_sms, stream);
+  if (mb == 0) return launch<kMode, 0>(in, out, *p, tiles, c.num_sms, stream);
+  if constexpr (kMode == CE_GRAD) {
+    if (mb == 1) return launch<kMode, 1>(in, out, *p, tiles, c.num_sms, stream);
   }
+  return launch<kMode, 2>(in, out, *p, tiles, c.num_sms, stream);
 }
 
 int launch_ce_forward(const CeCommon& c, const CeForward& a, cudaStream_t stream, int* parts) {
