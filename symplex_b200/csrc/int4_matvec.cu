@@ -684,15 +684,20 @@ int matvec_mma(const Int4Args& a, int rows, int cluster, bool out_bf16, int sms,
     attr[0].val.clusterDim.x = plan.cluster;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.numAttrs = 1;
-    // A processing cluster of the GPU may have SMs left over that make no whole cluster.
-    static std::atomic<int> resident[MV_CLUSTER_MOST + 1];
-    int n = resident[plan.cluster].load(std::memory_order_relaxed);
+    // A processing cluster of the GPU may have SMs left over that make no whole cluster; each device has its own.
+    constexpr int DEVICES = 16;  // current_device_sms takes no more
+    static std::atomic<int> resident[DEVICES][MV_CLUSTER_MOST + 1];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || dev < 0 || dev >= DEVICES) return launch_failed(e, "device of a 4-bit product");
+    int n = resident[dev][plan.cluster].load(std::memory_order_relaxed);
     if (n == 0) {
       cfg.gridDim = dim3(plan.cluster, 1, 1);
       cudaLaunchConfig_t most = cfg;
       most.dynamicSmemBytes = MV_SMEM;
-      if (cudaOccupancyMaxActiveClusters(&n, kern, &most) != cudaSuccess || n <= 0) return launch_failed(cudaGetLastError(), "cluster size not supported");
-      resident[plan.cluster].store(n, std::memory_order_relaxed);
+      e = cudaOccupancyMaxActiveClusters(&n, kern, &most);
+      if (e != cudaSuccess || n <= 0) return launch_failed(e, "cluster size not supported");
+      resident[dev][plan.cluster].store(n, std::memory_order_relaxed);
     }
     crowds = std::max(1, std::min(crowds, n / mblocks));
   }
