@@ -296,7 +296,8 @@ def int4_matvec(x, codes, scales, zeros=None, *, group_size=128, bias=None, acti
 
     ``x``: bfloat16 ``[K]`` or ``[M, K]``; ``zeros`` (0 to 15) None means 8 everywhere; ``bias``: float32 ``[N]``; ``activation`` as in
     ``gemm``. ``codes`` may be a view with unit stride in its rows. Returns ``[N]`` / ``[M, N]`` in ``out_dtype`` (bfloat16 or
-    float32); ``out`` must not overlap an operand. More rows than 64 are a product for ``gemm``.
+    float32); ``out`` must not overlap an operand. More rows are passed in parts of at most 64 (``gemm`` takes
+    no codes).
     """
     xshape, device = x.shape, x.device
     if not x.is_cuda or x.dtype != torch.bfloat16 or len(xshape) not in (1, 2):
@@ -304,7 +305,7 @@ def int4_matvec(x, codes, scales, zeros=None, *, group_size=128, bias=None, acti
     k = xshape[-1]
     m = xshape[0] if len(xshape) == 2 else 1
     if m > INT4_MAX_ROWS:
-        raise ValueError(f"int4_matvec() takes at most {INT4_MAX_ROWS} rows, got {m}: use gemm()")
+        raise ValueError(f"int4_matvec() takes at most {INT4_MAX_ROWS} rows a call, got {m}: pass them in parts")
     if k == 0:
         raise ValueError("K == 0 is not supported")
     groups = _group_count(k, group_size, "int4_matvec()")
