@@ -253,7 +253,6 @@ ce_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__
   else __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = tmem_base_slot;
-  pdl_wait_prior_grids();
   if (kMode == CE_LSE && blockIdx.x == 0 && threadIdx.x == 0) *p.done = 0;
 
   if (warp == 0) {

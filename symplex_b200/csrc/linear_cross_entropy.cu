@@ -43,7 +43,6 @@ __global__ void __launch_bounds__(256)
 ce_piece_rows_kernel(const float* __restrict__ L, long long ld, int cols, long long v0, const long long* __restrict__ targets,
                      float2* __restrict__ part, float* __restrict__ target_logit, unsigned* __restrict__ done) {
   __shared__ float2 red[8];
-  pdl_wait_prior_grids();
   const long long t = blockIdx.x;
   if (t == 0 && threadIdx.x == 0) *done = 0;
   const float* row = L + t * ld;
@@ -98,7 +97,6 @@ ce_finish_kernel(const float2* __restrict__ part, int parts, const float* __rest
   __shared__ int last;
   __shared__ double sred[32];
   __shared__ long long cred[32];
-  pdl_wait_prior_grids();
   const int mine = threadIdx.x & 3;
   const long long t = (long long)blockIdx.x * 4 + mine;
   RowPart r{-INFINITY, 0.0f};
@@ -146,7 +144,6 @@ ce_finish_kernel(const float2* __restrict__ part, int parts, const float* __rest
 
 // The sum over no rows, or their mean.
 __global__ void ce_nothing_kernel(float* loss, int mean) {
-  pdl_wait_prior_grids();
   *loss = mean ? __int_as_float(0x7fc00000) : 0.0f;
 }
 
@@ -156,7 +153,6 @@ __global__ void __launch_bounds__(1024)
 ce_scale_kernel(const long long* __restrict__ targets, const float* __restrict__ dloss, float* __restrict__ scale, long long T,
                 long long ignore, int mean) {
   __shared__ long long cred[32];
-  pdl_wait_prior_grids();
   long long n = 0;
   if (mean) {
     for (long long t = threadIdx.x; t < T; t += 1024) n += targets[t] != ignore ? 1 : 0;
@@ -166,11 +162,10 @@ ce_scale_kernel(const long long* __restrict__ targets, const float* __restrict__
 }
 
 // x with the ignored rows 0, for the backward pass: such a row may hold anything (NaN of a padded sequence), and G's zeros do not keep
-// it out of G^T x. One warp a row, bf16 (fp32 does it where it splits x). 1999 x 768 bf16: 3 us of 460.
+// it out of G^T x. One warp a row, bf16 (fp32 does it where it splits x). 1999 x 768 bf16: 3 us of 440.
 __global__ void __launch_bounds__(256)
 ce_counted_rows_kernel(const uint16_t* __restrict__ x, long long ldx, int vec, const long long* __restrict__ targets, long long ignore,
                        uint16_t* __restrict__ to, long long ld, long long T, int H, int copies) {
-  pdl_wait_prior_grids();
   const int lane = threadIdx.x & 31;
   for (long long t = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); t < T; t += (long long)gridDim.x * 8) {
     const bool counted = targets[t] != ignore;
@@ -205,7 +200,6 @@ ce_piece_grad_kernel(const float* __restrict__ L, long long ld, int cols, long l
                      float* __restrict__ G, int chunk, float* __restrict__ GT, long long ldt, long long plane_t,
                      long long rows, long long V, long long ignore) {
   __shared__ float tile[128 * GT_PITCH];
-  pdl_wait_prior_grids();
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
   const int padded = (cols + chunk - 1) / chunk * chunk;  // columns of all parts
   const long long row_tiles = (rows + 31) / 32, tiles = row_tiles * ((padded + 127) / 128);
@@ -274,7 +268,6 @@ __global__ void __launch_bounds__(256)
 ce_split_both_kernel(const float* __restrict__ in, long long ld, int vec, long long rows, int cols, const long long* __restrict__ targets,
                      long long ignore, float* __restrict__ to, long long ld_to, float* __restrict__ trans, long long chunk) {
   __shared__ float tile[128 * GT_PITCH];
-  pdl_wait_prior_grids();
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
   const long long padded = (rows + chunk - 1) / chunk * chunk;
   const long long row_tiles = (padded + 31) / 32, tiles = row_tiles * ((cols + 127) / 128);
@@ -336,7 +329,6 @@ ce_split_both_kernel(const float* __restrict__ in, long long ld, int vec, long l
 template <typename T>
 __global__ void __launch_bounds__(256)
 ce_join_kernel(const float* __restrict__ acc, int chunks, long long n, const float* __restrict__ scale, T* out, int add) {
-  pdl_wait_prior_grids();
   const float f = scale != nullptr ? *scale : 1.0f;
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
     float v = 0.0f;
@@ -477,6 +469,7 @@ int check_workspace(size_t need, const void* ws, size_t bytes) {
 
 bool aligned_to(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
+// In plain stream order, like the tensor-core kernels of these passes: none of them has a griddepcontrol.wait.
 #define CE_LAUNCH(kern, grid, block, ...)                                                                             \
   do {                                                                                                                \
     const cudaError_t e__ = launch_kernel_ex(kern, (unsigned)(grid), block, 0, stream, 1, false, __VA_ARGS__);         \
