@@ -15,6 +15,11 @@ inline bool share_bytes(const ByteRows& a, const ByteRows& b) {
   const uintptr_t pa = reinterpret_cast<uintptr_t>(a.p), pb = reinterpret_cast<uintptr_t>(b.p);
   if (a.rows <= 0 || b.rows <= 0 || a.bytes <= 0 || b.bytes <= 0) return false;
   if (pa + (a.rows - 1) * a.stride + a.bytes <= pb || pb + (b.rows - 1) * b.stride + b.bytes <= pa) return false;
+  if (a.stride == b.stride) {  // two views of one buffer: the same for every pair of rows
+    if (pb < pa) return share_bytes(b, a);
+    const long long q = (long long)(pb - pa) / a.stride, r = (long long)(pb - pa) % a.stride;
+    return (q < a.rows && r < a.bytes) || (q + 1 < a.rows && r + b.bytes > a.stride);
+  }
   for (long long i = 0, j = 0; i < a.rows && j < b.rows;) {
     const uintptr_t ra = pa + i * a.stride, rb = pb + j * b.stride;
     if (ra < rb + b.bytes && rb < ra + a.bytes) return true;

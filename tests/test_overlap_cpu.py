@@ -4,6 +4,7 @@ import os
 import random
 import shutil
 import subprocess
+import time
 
 import pytest
 
@@ -31,15 +32,27 @@ def _addresses(p, rows, width, stride):
     return {p + i * stride + k for i in range(rows) for k in range(width)}
 
 
-def test_against_sets(share):
+@pytest.mark.parametrize("one_stride", [False, True])
+def test_against_sets(share, one_stride):
     rng = random.Random(0)
     seen = [0, 0]
     for _ in range(20000):
         a, b = ((rng.randrange(64, 160), rng.randrange(0, 5), w := rng.randrange(0, 9), w + rng.choice([0, 0, 1, 4, 13, 40])) for _ in range(2))
+        if one_stride:
+            a, b = a[:3] + (max(a[3], b[3]),), b[:3] + (max(a[3], b[3]),)
         want = bool(_addresses(*a) & _addresses(*b))
         assert bool(share.share(*a, *b)) == want, (a, b)
         seen[want] += 1
     assert min(seen) > 2000
+
+
+def test_views_of_a_long_buffer_are_told_apart_at_once(share):
+    """Two halves of the same rows: not one look at each of a billion of them on every call."""
+    start = time.perf_counter()
+    for _ in range(1000):
+        assert not share.share(1 << 20, 1 << 30, 256, 512, (1 << 20) + 256, 1 << 30, 256, 512)
+        assert share.share(1 << 20, 1 << 30, 256, 512, (1 << 20) + 254, 1 << 30, 256, 512)
+    assert time.perf_counter() - start < 1
 
 
 def test_nothing_shares_with_a_missing_operand(share):
