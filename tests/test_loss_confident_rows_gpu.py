@@ -26,6 +26,7 @@ BF, F32 = torch.bfloat16, torch.float32
     (300, 8192, 3000, BF), (200, 4104, 20011, BF), (700, 6144, 20000, BF), (900, 4096, 5000, BF),                    # pairs, in segments
     (200, 2048, 3000, BF), (300, 4096, 20000, BF), (40, 1000, 3000, BF), (1300, 512, 17000, BF),                     # one sum
     (300, 1024, 20011, BF), (200, 768, 9000, BF), (256, 2048, 30000, BF), (1100, 1104, 17000, BF),                   # 256-row tiles
+    (1300, 2048, 17000, BF), (4096, 2048, 21500, BF),  # 512-row tiles, one sum (the last piece of the second: 256-row ones)
     (2100, 4104, 40000, BF),                                                                                         # pieces of the vocabulary
     (100, 4096, 2000, F32), (300, 1000, 5000, F32),
 ])
