@@ -46,7 +46,7 @@ struct CeCfg {
 
 // At most 128 tokens. A pair's tile would be filled up to 256 rows with nothing, and its MMAs then take as long as W's rows take to
 // arrive (512 cycles for 16 KB per SM, 9 TB/s with no pause): one CTA has half the rows to multiply (1 x 4096 x 65536: 150 us on
-// pairs, 94 us alone, 5.7 TB/s; 37 x 1024 x 50257: 32 and 25 us, each launched behind the call before). Columns of a tile, rows of A that
+// pairs, 94 us alone, 5.7 TB/s; 37 x 1024 x 50257: 32 and 25 us, 26 since the kernels start in plain stream order). Columns of a tile, rows of A that
 // are copied and stages are set at launch: the tiles share the vocabulary out evenly, and the stages fill shared memory. The MMA
 // reads 128 rows of A from a stage whatever was copied; the rows behind the copied ones are other data, and nobody reads their sums.
 template <>
@@ -182,7 +182,7 @@ __device__ __forceinline__ void stage_f32(const float (&v)[32], uint8_t* tile, i
 
 // The accumulators round every sum towards 0: a logit loses about 2^-26 of itself for each 16 k, and the loss, which all logits move the
 // same way, 2e-10 H of itself (measured: 8e-7 at H = 4096, 1.6e-6 at 8192; with 3000 words, whose loss is smaller, 1.1e-6 and 2.6e-6).
-// Where all products of a logit have one sign (a row that is sure of its target) it is ten times as much.
+// Where all products of a logit have one sign (a row that is sure of its target) it is 6e-6 at 2048 and 1.5e-5 at 4096 (segments: 1.1e-6).
 // kSegments (CE_LSE and CE_GRAD, kMB 0 and 1): k in segments of 512, each from zero into the next accumulator; twice the epilogue warps,
 // half of a tile's columns each, add them up in registers with rounded sums. 1e-7 at any H. Both passes of a problem take the same form:
 // the target's entry of G is exp(l - lse) - 1, of which an l with the bias beside an lse without it leaves nothing right where 1 - p is
