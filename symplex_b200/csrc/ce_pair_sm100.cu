@@ -18,6 +18,7 @@
 #include <algorithm>
 
 #include "ce_params.h"
+#include "ce_tiles.h"
 #include "epilogue.cuh"
 #include "gemm_params.h"
 #include "host_api.h"
@@ -187,7 +188,6 @@ __device__ __forceinline__ void stage_f32(const float (&v)[32], uint8_t* tile, i
 // half of a tile's columns each, add them up in registers with rounded sums. 1e-7 at any H. Both passes of a problem take the same form:
 // the target's entry of G is exp(l - lse) - 1, of which an l with the bias beside an lse without it leaves nothing right where 1 - p is
 // small (T = 2100, H = 4104, rows of 1 - p = 1e-5 to 1e-3: G off by 3e-4, by 1e-6 in the same form).
-constexpr int CE_SEGMENT = 8;  // k-blocks
 template <int kMB, bool kSegments>
 constexpr int CE_EPI_WARPS = kSegments ? 8 : CeCfg<kMB>::EPI_WARPS;
 // Shared memory: operand stages, then a staging tile of 32 x 128 bytes for each epilogue warp that writes through one.
@@ -727,30 +727,6 @@ int out_map(CUtensorMap* out, const void* p, long long rows, long long cols, lon
   return encode_tensor_map_3d(out, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p, dims, strides, box);
 }
 
-// The logits' product: one CTA up to 128 tokens, else 512-row tiles or 256-row ones: fewer waves x area per tile over the tensor-pipe share
-// each shape reaches on large products (0.875 and 0.80, measured for the general pair kernel). The option "pair_mode" decides here as it
-// does there.
-int row_blocks(long long M, long long N, int num_sms) {
-  const int64_t mode = options().pair_mode.load(std::memory_order_relaxed);
-  if (mode == 1 || mode == 2) return (int)mode;
-  if (M <= 128) return 0;
-  if (M <= 256) return 1;
-  const long long pairs = num_sms / 2, nt = (N + 255) / 256;
-  const long long w1 = ((M + 255) / 256 * nt + pairs - 1) / pairs, w2 = ((M + 511) / 512 * nt + pairs - 1) / pairs;
-  return (double)w2 * 2 / 0.875 <= (double)w1 / 0.80 ? 2 : 1;
-}
-
-// kMB = 0: columns of a tile, a multiple of `step` of at most 256, so that every CTA's tiles together have as few columns as can be.
-int columns_alone(long long N, int step, int least_bn, int num_sms) {
-  int best = 256;
-  long long least = 1LL << 62;
-  for (int bn = 256; bn >= least_bn; bn -= step) {
-    const long long tiles = (N + bn - 1) / bn, each = (tiles + num_sms - 1) / num_sms * bn;
-    if (each < least) least = each, best = bn;
-  }
-  return best;
-}
-
 CeJob job_of(long long M, long long N, long long K, int mb) {
   CeJob j;
   j.M = (int)M; j.N = (int)N; j.K = (int)K;
@@ -809,57 +785,27 @@ long long ce_piece_of_waves(long long T, long long V, long long most) {
   return best * 256;
 }
 
-// Logits in segments where the error of one sum would be near 1e-6: up to 128 tokens from 2048 values on (1 x 4096 x 65536 101 us, 95
-// without), pairs where the sum is longer than 4096 or the vocabulary is small (8192 x 4096 x 50257 would take 2305 us instead of 2164).
-// The gradient's logits with them: 2048 x 8192 x 32000 2250 us for the whole pass (2130 without), 300 x 8192 x 8000 192 (188),
-// 3 x 8192 x 8205 159 (152).
-static bool in_segments(long long T, long long V, long long H) { return H > 4096 || (H > 2048 && (T <= 128 || V < 16384)); }
-
-// Tile rows and the form of the sums, of the forward pass. 256-row tiles run in segments whatever the length: one form for them, whose
-// epilogue reads a whole accumulator before the lanes' branches (3816 x 1104 x 26330 196 us, 172 as one sum; 200 x 768 x 50257 32, 29;
-// 2000 x 256 x 30000, where 512-row tiles are taken, 59, 65).
-struct LogitsForm {
-  int mb;
-  bool segments;
-};
-static LogitsForm forward_form(long long T, long long V, long long H, int num_sms) {
-  int mb = row_blocks(T, V, num_sms);
-  const bool segments = in_segments(T, V, H);
-  if (segments) mb = std::min(mb, 1);
-  return {mb, segments || mb == 1};
-}
-static int forward_columns_alone(long long V, long long T, long long H, int num_sms) { return columns_alone(V, 16, in_segments(T, V, H) ? 64 : 32, num_sms); }
-
-int ce_forward_parts_most(long long T, long long V) {  // whatever the tile shape
-  return (int)std::max((V + 255) / 256 * 2, T <= 128 ? (V + 63) / 64 * 2 : 0);
-}
-
 // The logits' product of either pass: operands, tile shape (chosen here alone, by one look at the options), and the kernel for it. `parts`:
 // how many parts the forward pass writes of a row.
 template <int kMode>
 static int launch_logits(const CeCommon& c, const CeMatrix& x, const CeMatrix& W, const CUtensorMap (&out)[2], CeKernelParams* p, cudaStream_t stream,
                          int* parts) {
-  const LogitsForm form = forward_form(x.rows, p->V, x.cols, c.num_sms);
-  // The gradient's tiles go by the piece at hand, its sums by the forward pass. One segment is the same sum in either form.
-  const bool segments = form.segments && (kMode == CE_LSE || x.cols > CE_SEGMENT * 64);
-  int mb = form.mb;
-  if constexpr (kMode == CE_GRAD) {
-    mb = p->lo ? 0 : row_blocks(x.rows, W.rows, c.num_sms);
-    if (segments) mb = std::min(mb, 1);
-  }
+  const CeTiles tiling = kMode == CE_LSE ? ce_forward_tiles(x.rows, W.rows, x.cols, c.num_sms, (int)options().pair_mode.load(std::memory_order_relaxed))
+                                         : ce_gradient_tiles(x.rows, p->V, x.cols, W.rows, p->lo != 0, c.num_sms, (int)options().pair_mode.load(std::memory_order_relaxed));
+  const int mb = tiling.mb;
+  const bool segments = tiling.segments;
   uint32_t a_rows = 128 * mb, b_rows = 128;
   p->job[0] = job_of(x.rows, W.rows, x.cols, mb);
   if (mb == 0) {
     a_rows = (uint32_t)(x.rows + 15) / 16 * 16;
-    // G leaves in blocks of 64 columns
-    b_rows = (uint32_t)(kMode == CE_GRAD ? columns_alone(W.rows, 64, 64, c.num_sms) : forward_columns_alone(W.rows, x.rows, x.cols, c.num_sms));
-    p->bn = (int)b_rows;
+    b_rows = (uint32_t)tiling.bn;
+    p->bn = tiling.bn;
     p->a_bytes = (int)a_rows * 128;
     const int room = segments ? ce_stage_room<kMode, 0, true>() : ce_stage_room<kMode, 0, false>();
     p->stages = std::min(CeCfg<0>::STAGES, room / (p->a_bytes + p->bn * 128));
     p->job[0].n_tiles = (int)((W.rows + p->bn - 1) / p->bn);
   }
-  if constexpr (kMode == CE_LSE) *parts = p->job[0].n_tiles * (segments ? 2 : std::max(mb, 1));
+  if constexpr (kMode == CE_LSE) *parts = ce_parts(tiling, W.rows);
   CUtensorMap in[4] = {};
   int rc = map_of(&in[0], x, 64, a_rows);
   if (rc == SX_OK) rc = map_of(&in[1], W, 64, b_rows);

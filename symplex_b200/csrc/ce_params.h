@@ -24,11 +24,10 @@ struct CeCommon {
 struct CeForward {
   CeMatrix x, W;  // [T, H], [V, H]
   const long long* targets;
-  float2* part;  // [parts][T], room for ce_forward_parts_most
+  float2* part;  // [parts][T], room for ce_parts_most
   float* target_logit;
   unsigned* done;  // set to 0
 };
-int ce_forward_parts_most(long long T, long long V);  // upper bound over tile shapes and SM counts
 int launch_ce_forward(const CeCommon& c, const CeForward& a, cudaStream_t stream, int* parts);  // parts: those that it writes
 
 // G[t][v] = (exp(x W^T - lse) - [v0 + v = target]) * (dloss ? dloss[t] : 1), 0 in ignored rows, NaN where the target is none.

@@ -18,6 +18,7 @@
 
 #include "../../include/symplex_b200.h"
 #include "ce_params.h"
+#include "ce_tiles.h"
 #include "host_api.h"
 #include "sm100_ptx.cuh"
 
@@ -397,7 +398,7 @@ Layout layout(const Problem& p, bool backward) {
   w.tp = up(p.T, 8);
   w.piece = piece_columns(p, backward);
   w.pieces = (int)((p.V + w.piece - 1) / w.piece);
-  w.parts = p.bf16 ? ce_forward_parts_most(p.T, p.V) : w.pieces;
+  w.parts = p.bf16 ? ce_parts_most(p.T, p.V) : w.pieces;
   w.chunks = 1;
   w.chunk = up(w.piece, 32);
   if (backward && p.bf16) {
