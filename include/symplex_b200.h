@@ -545,7 +545,7 @@ int symplex_b200_layer_norm_backward(const void* dy, const void* x, const float*
 
 /* C[M, N] = act(A[M, K] . W^T + bias) for a few rows of A (M <= SYMPLEX_B200_INT4_MAX_M): the product of single tokens,
  * bound by reading the codes. A is bf16 with leading dimension lda, C has out_dtype (F32 / BF16) and leading dimension ldc
- * (elements, 0 = packed), bias is fp32[N] or NULL, activation one of SYMPLEX_ACT_*. code - zero enters the product as the
+ * (elements, 0 = packed), bias is fp32[N] or NULL, activation one of SYMPLEX_ACT_* (each keeps NaN). code - zero enters the product as the
  * whole number it is, sums are 32-bit, the scale is applied to each group's sum. C must not overlap an input (refused). */
 #define SYMPLEX_B200_INT4_MAX_M 64
 int symplex_b200_int4_matvec(const void* A, const uint8_t* codes, const void* scales, const uint8_t* zeros,

@@ -27,7 +27,7 @@ namespace {
 // One value of the activation set with the accurate device functions.
 __device__ __forceinline__ float activate(float x, int act) {
   switch (act) {
-    case ACT_RELU: return fmaxf(x, 0.0f);
+    case ACT_RELU: return x > 0.0f || x != x ? x : 0.0f;  // a NaN stays one (fmaxf would answer 0)
     case ACT_GELU: return 0.5f * x * (1.0f + tanhf(0.7978845608028654f * (x + 0.044715f * x * x * x)));
     case ACT_SIGMOID: return 1.0f / (1.0f + expf(-x));
     case ACT_TANH: return tanhf(x);

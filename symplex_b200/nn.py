@@ -295,7 +295,7 @@ def int4_matvec(x, codes, scales, zeros=None, *, group_size=128, bias=None, acti
     scales[n, k // group_size]`` held as ``int4_quantize`` lays it out (``symplex_b200_int4_matvec``).
 
     ``x``: bfloat16 ``[K]`` or ``[M, K]``; ``zeros`` (0 to 15) None means 8 everywhere; ``bias``: float32 ``[N]``; ``activation`` as in
-    ``gemm``. ``codes`` may be a view with unit stride in its rows. Returns ``[N]`` / ``[M, N]`` in ``out_dtype`` (bfloat16 or
+    ``gemm`` (the relu of NaN is NaN here). ``codes`` may be a view with unit stride in its rows. Returns ``[N]`` / ``[M, N]`` in ``out_dtype`` (bfloat16 or
     float32); ``out`` must not overlap an operand. More rows are passed in parts of at most 64 (``gemm`` takes
     no codes).
     """
